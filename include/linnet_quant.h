@@ -467,6 +467,88 @@ LNQ_API LnqStatus lnq_mxfp4_experts(const void* x, int64_t x_row_stride, int64_t
 LNQ_API LnqStatus lnq_mxfp4_experts_plan(int64_t rows, int64_t chosen, int64_t num_experts,
                                          int64_t out_features, int64_t in_features, int32_t* pass);
 
+/* MXFP4 made and read (the OCP microscaling format): x [rows, in] of `dtype` (bf16, f16 or
+ * f32), contiguous, in blocks of 32. A block's scale byte is floor(log2 of its largest
+ * magnitude) - 2 + 127, at least 0; its values over 2^(byte - 127) are rounded to E2M1, ties
+ * to the even code, past 6 to 6. A block with an infinity or a NaN gets the byte 255 (E8M0's
+ * NaN) and codes of 0. Layout as above: blocks [rows, in/32, 16], scales [rows, in/32].
+ * x and blocks 16-byte aligned; in % 32 == 0. No counterpart in the reference, which reads
+ * MXFP4 checkpoints and makes none. */
+LNQ_API LnqStatus lnq_mxfp4_quantize(const void* x, uint8_t* blocks, uint8_t* scales, int64_t rows,
+                                     int64_t in_features, int32_t dtype, void* stream);
+
+/* out[rows, in] of `dtype` (bf16, f16 or f32): each code's value times 2^(scale - 127),
+ * rounded once; a scale byte of 255 gives NaN. blocks and out 16-byte aligned. Replaces:
+ * `dequantize_mxfp4` (stdlib/quant.linnet:334-341). */
+LNQ_API LnqStatus lnq_mxfp4_dequantize(const uint8_t* blocks, const uint8_t* scales, void* out,
+                                       int64_t rows, int64_t in_features, int32_t dtype, void* stream);
+
+/* Rows of activations as lnq_mxfp4_mm reads them: lnq_mxfp4_quantize's rounding of x [rows,
+ * in] (rows x_stride elements apart, a multiple of 8), the codes in q [rows, in/2], the scales
+ * as tiles: [units][padded][4] bytes, unit u holding blocks 4u .. 4u + 3 (128 inputs) of every
+ * row, units = ceil(in / 128), padded = rows rounded up to a multiple of 4 (rows past the last
+ * and blocks past `in` hold 0). x, q and scales 16-byte aligned. No counterpart in the
+ * reference. */
+LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, uint8_t* scales,
+                                 int64_t rows, int64_t in_features, int32_t dtype, void* stream);
+
+/* A weight's scales as stored, [count, out, in/32], as tiles: [count][units][padded][4] bytes
+ * (units, padded as lnq_mxfp4_rows has them, of `out` rows). Made once, as the weight is
+ * loaded. tiles 16-byte aligned. */
+LNQ_API LnqStatus lnq_mxfp4_scale_tiles(const uint8_t* scales, uint8_t* tiles, int64_t count,
+                                        int64_t out_features, int64_t in_features, void* stream);
+
+/* y[rows, out] = x[rows, in] @ W^T (+ bias[out]) for few rows: x, bias and y of `dtype` (bf16 or
+ * f16), x's rows x_stride elements apart (a multiple of 8, below 2^23), the weight's blocks
+ * [out, in/32, 16] and scales [out, in/32] read as stored. Summed in f32, the bias added there,
+ * rounded once. A scale byte of 255 gives NaN. rows <= 65535, in <= 65536, out <= 4194240, in %
+ * 32 == 0; each 32 rows read the weight again. x and blocks 16-byte aligned. */
+LNQ_API LnqStatus lnq_mxfp4_linear(const void* x, int64_t x_stride, const uint8_t* blocks,
+                                   const uint8_t* scales, const void* bias, void* y, int64_t rows,
+                                   int64_t out_features, int64_t in_features, int32_t dtype, void* stream);
+
+/* The same with x rounded too: q and x_scale as lnq_mxfp4_rows writes them, the weight's blocks
+ * as stored and its scales as tiles (lnq_mxfp4_scale_tiles), multiplied on the block-scaled
+ * MFMA (exact products, f32 sums), bias added in f32, rounded once to `dtype` (bf16 or f16).
+ * NaN where a row's or an output's block has the scale 255. rows, out <= 2^27, in <= 2^22, in %
+ * 32 == 0; operands 16-byte aligned, y 8-byte. */
+LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const uint8_t* blocks,
+                               const uint8_t* tiles, const void* bias, void* y, int64_t rows,
+                               int64_t out_features, int64_t in_features, int32_t dtype, void* stream);
+
+/* lnq_mxfp4_experts with x rounded to MXFP4: y[r, k, :] = x[r (, k)] @ W[experts[r, k]]^T, the
+ * pairs of each expert multiplied together. q and x_scale hold `rows` rows (shared: every
+ * chosen expert of a row reads it) or rows * chosen; blocks [E, out, in/32, 16] as stored,
+ * tiles [E] scale tiles each. An expert index outside 0 .. num_experts - 1 gives zeros.
+ * workspace (16-byte aligned, at least lnq_mxfp4_experts_workspace bytes) holds the lists of
+ * the pairs, written by the call: calls that overlap on one workspace race. num_experts <=
+ * 2048, rows * chosen and out <= 2^27, x's codes below 2 GiB. */
+LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t num_experts, int64_t* bytes);
+LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale, const uint8_t* blocks,
+                                       const uint8_t* tiles, const int64_t* experts, void* y,
+                                       int64_t rows, int64_t chosen, int64_t num_experts,
+                                       int64_t out_features, int64_t in_features, int32_t shared,
+                                       int32_t dtype, void* workspace, int64_t workspace_bytes,
+                                       void* stream);
+
+/* The experts that each row of a router's logits [rows, num_experts] (bf16, f16 or f32; rows
+ * `stride` elements apart) chooses, and their weights; experts [rows, top] int64 and weights
+ * [rows, top] f32, by falling choice.
+ * Scores are a softmax over the experts or a sigmoid of each; the choice goes by score + bias
+ * (f32 [num_experts]; NULL: by the logits, which order as the scores do), in 64 bits, equal ones
+ * by the lower index. With groups > 1 (equal runs of experts, at most 64) only the group_top
+ * groups with the largest sum of their group_best (1 or 2) best choices are chosen from (a group
+ * with fewer counts -inf; by the scores' sum without a bias). Weights are the chosen experts'
+ * scores, without the bias, over their sum if `renormalize` (0 where that is 0), times `scale`.
+ * An expert with a logit of -inf, or a choice of -inf or NaN, is never chosen; places left over
+ * hold -1 and weight 0. A row with a NaN logit (or +inf, for softmax): -1 and NaN throughout.
+ * num_experts <= 1024, top <= 64 and at most what the kept groups hold. The reference runs a
+ * router as framework ops. */
+LNQ_API LnqStatus lnq_expert_route(const void* logits, int64_t stride, const float* bias, int64_t* experts,
+                                   float* weights, int64_t rows, int64_t num_experts, int64_t top,
+                                   int64_t groups, int64_t group_top, int64_t group_best, int32_t softmax,
+                                   int32_t renormalize, double scale, int32_t dtype, void* stream);
+
 /* ------------------------------------------------------------------------- NF4
  * std.quant::Nf4Linear (stdlib/quant.linnet:177-215): codes [out, in/2] bytes of
  * QLoRA's 4-bit NormalFloat, the first input of a pair in the low nibble, and

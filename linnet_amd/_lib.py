@@ -66,6 +66,16 @@ SIGNATURES: dict[str, list[object]] = {
     "lnq_mm8_block": [_p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i32, _p],
     "lnq_mxfp4_experts": [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _p],
     "lnq_mxfp4_experts_plan": [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i32)],
+    "lnq_mxfp4_quantize": [_p, _p, _p, _i64, _i64, _i32, _p],
+    "lnq_mxfp4_dequantize": [_p, _p, _p, _i64, _i64, _i32, _p],
+    "lnq_mxfp4_rows": [_p, _i64, _p, _p, _i64, _i64, _i32, _p],
+    "lnq_mxfp4_scale_tiles": [_p, _p, _i64, _i64, _i64, _p],
+    "lnq_mxfp4_linear": [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p],
+    "lnq_mxfp4_mm": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p],
+    "lnq_mxfp4_experts_workspace": [_i64, _i64, ctypes.POINTER(_i64)],
+    "lnq_mxfp4_experts_mm": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _p, _i64, _p],
+    "lnq_expert_route": [_p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, ctypes.c_double,
+                         _i32, _p],
     "lnq_nf4_dequant": [_p, _p, _p, _i64, _i64, _i64, _i32, _p],
     "lnq_nf4_linear": [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _p],
     "lnq_nf4_linear_plan": [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i32)],

@@ -1,0 +1,291 @@
+// Rounding to MXFP4 (OCP microscaling: 32 values share an E8M0 scale, E2M1 elements) and
+// back, and the scale layout of the MXFP4 x MXFP4 product (mxfp4_mm.hip).
+//
+// A block of 32 values with largest magnitude m: the scale byte is s = floor(log2 m) - 2 +
+// 127 (E2M1's largest exponent is 2), at least 0, and each value is x / 2^(s - 127) rounded
+// to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, ties to the even code,
+// past 6 to 6. floor(log2 m) is m's f32 exponent field; the division by a power of two is
+// exact in f32, so the one rounding is the conversion's (v_cvt_scalef32_pk_fp4_f32 with a
+// scale of 1). A block that holds an infinity or a NaN gets s = 255, E8M0's NaN, and codes
+// of 0: every reader of it gives NaN.
+//
+// Bound by HBM: 2 or 4 bytes a value read, 17/32 written (back: the reverse). Four lanes
+// take a block, 8 values each: a wave's loads are whole kilobytes.
+#include "common.hpp"
+
+namespace lnq {
+
+namespace mxr {
+constexpr int THREADS = 256;
+constexpr int ROWS = 32;   // rows of a workgroup of the row-rounding kernel: 128 bytes of scales a unit
+constexpr int SPAN = 512;  // inputs of a row that a wave takes: 8 a lane
+
+// 8 values as loaded.
+template <int DT>
+struct Raw {
+  u32x4 v;
+};
+template <>
+struct Raw<LNQ_F32> {
+  f32x4 a, b;
+};
+
+template <int DT>
+__device__ inline Raw<DT> load8(const typename Elem<DT>::storage* p) {
+  Raw<DT> r;
+  if constexpr (DT == LNQ_F32) {
+    r.a = *reinterpret_cast<const f32x4*>(p);
+    r.b = *reinterpret_cast<const f32x4*>(p + 4);
+  } else {
+    r.v = *reinterpret_cast<const u32x4*>(p);
+  }
+  return r;
+}
+
+template <int DT>
+__device__ inline void widen8(const Raw<DT>& r, float (&v)[8]) {
+  if constexpr (DT == LNQ_F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = r.a[e], v[4 + e] = r.b[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t d = r.v[e];
+      v[2 * e] = Elem<DT>::to_f32(static_cast<uint16_t>(d & 0xffffu));
+      v[2 * e + 1] = Elem<DT>::to_f32(static_cast<uint16_t>(d >> 16));
+    }
+  }
+}
+
+// This lane's 8 values of a block whose other values the lanes of its quad (l & ~3 .. l | 3)
+// hold: the scale byte (the same in all four) and the 8 codes, element 0 lowest.
+__device__ inline uint32_t round8(const float (&v)[8], uint32_t& byte) {
+  uint32_t top = 0;  // magnitudes order as their bits
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1, 64)));
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2, 64)));
+  const uint32_t exponent = top >> 23;
+  if (exponent == 255) {
+    byte = 255;
+    return 0;
+  }
+  byte = max(exponent, 2u) - 2u;
+  const float inverse = __builtin_bit_cast(float, (254u - byte) << 23);  // 2^(127 - byte), byte <= 252
+  uint32_t word = 0;
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0] * inverse, v[1] * inverse, 1.0f, 0);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2] * inverse, v[3] * inverse, 1.0f, 1);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4] * inverse, v[5] * inverse, 1.0f, 2);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6] * inverse, v[7] * inverse, 1.0f, 3);
+  return word;
+}
+
+// 2^(byte - 127); 255 is NaN.
+__device__ inline float scale_of(uint32_t byte) {
+  const uint32_t bits = byte == 255 ? 0x7fc00000u : byte == 0 ? 0x00400000u : byte << 23;
+  return __builtin_bit_cast(float, bits);
+}
+}  // namespace mxr
+
+// Blocks one after another, as a checkpoint stores them: thread i of the grid takes values
+// 8 i .. 8 i + 7 of all, UNROLL of them a grid apart.
+template <int DT>
+__global__ __launch_bounds__(mxr::THREADS) void mxfp4_quantize_kernel(const typename Elem<DT>::storage* __restrict__ x,
+                                                                      uint32_t* __restrict__ codes,
+                                                                      uint8_t* __restrict__ scales, int64_t eights) {
+  using namespace mxr;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+  if (i >= eights) return;  // eights % 4 == 0: whole quads
+  float v[8];
+  widen8<DT>(load8<DT>(x + i * 8), v);
+  uint32_t byte;
+  codes[i] = round8(v, byte);
+  if ((threadIdx.x & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(byte);
+}
+
+// Rows for the product: codes [rows, K / 2] as above, scales [units][padded][4] bytes, a
+// unit being 128 inputs (4 blocks) and `padded` rows rounded up to a multiple of 4. A
+// workgroup takes 32 rows by 512 inputs, so the scales leave in runs of 128 bytes.
+template <int DT>
+__global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename Elem<DT>::storage* __restrict__ x,
+                                                                  int64_t x_stride, uint32_t* __restrict__ codes,
+                                                                  uint32_t* __restrict__ scales, int rows, int padded,
+                                                                  int K) {
+  using namespace mxr;
+  constexpr int PER_WAVE = ROWS / (THREADS / 64);
+  __shared__ uint32_t unit[SPAN / 128][ROWS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r0 = blockIdx.x * ROWS, k = blockIdx.y * SPAN + lane * 8;
+  const bool in = k < K;
+#pragma unroll
+  for (int i = 0; i < PER_WAVE; ++i) {
+    const int r = wave * PER_WAVE + i;
+    uint32_t byte = 0;
+    if (r0 + r < rows && in) {
+      float v[8];
+      widen8<DT>(load8<DT>(x + (r0 + r) * x_stride + k), v);
+      codes[(static_cast<int64_t>(r0 + r) * K + k) >> 3] = round8(v, byte);
+    }
+    // The four blocks of a unit, 16 lanes: block b's byte at bits 8 b.
+    uint32_t word = byte << (8 * ((lane >> 2) & 3));
+    word |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(word), 4, 64));
+    word |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(word), 8, 64));
+    if ((lane & 15) == 0) unit[lane >> 4][r] = word;
+  }
+  __syncthreads();
+  const int u = threadIdx.x / ROWS, r = threadIdx.x % ROWS;
+  const int at = blockIdx.y * (SPAN / 128) + u;
+  if (u < SPAN / 128 && at * 128 < K && r0 + r < padded) scales[static_cast<int64_t>(at) * padded + r0 + r] = unit[u][r];
+}
+
+template <int DT>
+__global__ __launch_bounds__(mxr::THREADS) void mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes,
+                                                                        const uint8_t* __restrict__ scales,
+                                                                        typename Elem<DT>::storage* __restrict__ out,
+                                                                        int64_t eights) {
+  using namespace mxr;
+  using E = Elem<DT>;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+  if (i >= eights) return;
+  const uint32_t w = codes[i];
+  const float s = scale_of(scales[i >> 2]);
+  const f32x2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1),
+                      __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3)};
+  if constexpr (DT == LNQ_F32) {
+    *reinterpret_cast<f32x4*>(out + i * 8) = f32x4{p[0][0] * s, p[0][1] * s, p[1][0] * s, p[1][1] * s};
+    *reinterpret_cast<f32x4*>(out + i * 8 + 4) = f32x4{p[2][0] * s, p[2][1] * s, p[3][0] * s, p[3][1] * s};
+  } else {
+    u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] = static_cast<uint32_t>(E::from_f32(p[e][0] * s)) | (static_cast<uint32_t>(E::from_f32(p[e][1] * s)) << 16);
+    *reinterpret_cast<u32x4*>(out + i * 8) = o;
+  }
+}
+
+// Scales as stored, [count, N, groups], laid out for the product: [count][units][padded][4].
+__global__ __launch_bounds__(mxr::THREADS) void mxfp4_scale_tiles_kernel(const uint8_t* __restrict__ scales,
+                                                                         uint32_t* __restrict__ tiles, int N, int padded,
+                                                                         int groups, int units) {
+  const int n = blockIdx.x * mxr::THREADS + threadIdx.x;
+  if (n >= padded) return;
+  const int u = blockIdx.y, e = blockIdx.z;
+  uint32_t word = 0;
+  if (n < N) {
+    const uint8_t* from = scales + (static_cast<int64_t>(e) * N + n) * groups + 4 * u;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      if (4 * u + b < groups) word |= static_cast<uint32_t>(from[b]) << (8 * b);
+  }
+  tiles[(static_cast<int64_t>(e) * units + u) * padded + n] = word;
+}
+
+}  // namespace lnq
+
+using namespace lnq;
+
+namespace {
+
+LnqStatus check_rounding(const char* what, int64_t rows, int64_t in_features, int32_t dtype) {
+  LNQ_REQUIRE(dtype == LNQ_BF16 || dtype == LNQ_F16 || dtype == LNQ_F32, "%s: dtype %d is not bf16, f16 or f32", what, dtype);
+  LNQ_REQUIRE(rows >= 0 && in_features >= 0 && in_features % 32 == 0, "%s: bad shape rows=%lld in=%lld (in %% 32 == 0)", what,
+              static_cast<long long>(rows), static_cast<long long>(in_features));
+  LNQ_REQUIRE(in_features <= INT32_MAX && rows <= INT32_MAX, "%s: sizes exceed 2^31", what);
+  return LNQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+LNQ_API LnqStatus lnq_mxfp4_quantize(const void* x, uint8_t* blocks, uint8_t* scales, int64_t rows, int64_t in_features,
+                                     int32_t dtype, void* stream) {
+  if (const LnqStatus st = check_rounding("lnq_mxfp4_quantize", rows, in_features, dtype)) return st;
+  if (rows == 0 || in_features == 0) {
+    clear_error();
+    return LNQ_OK;
+  }
+  LNQ_REQUIRE(x && blocks && scales, "lnq_mxfp4_quantize: null pointer");
+  LNQ_REQUIRE(aligned(x, 16) && aligned(blocks, 16), "lnq_mxfp4_quantize: x and blocks must be 16-byte aligned");
+  const int64_t eights = rows * (in_features / 8), grid = (eights + mxr::THREADS - 1) / mxr::THREADS;
+  LNQ_REQUIRE(grid <= INT32_MAX, "lnq_mxfp4_quantize: too large");
+#define LNQ_MXQ(DT)                                                                                          \
+  hipLaunchKernelGGL((mxfp4_quantize_kernel<DT>), dim3(static_cast<unsigned>(grid)), dim3(mxr::THREADS), 0,  \
+                     static_cast<hipStream_t>(stream), static_cast<const typename Elem<DT>::storage*>(x),    \
+                     reinterpret_cast<uint32_t*>(blocks), scales, eights)
+  if (dtype == LNQ_BF16) LNQ_MXQ(LNQ_BF16);
+  else if (dtype == LNQ_F16) LNQ_MXQ(LNQ_F16);
+  else LNQ_MXQ(LNQ_F32);
+#undef LNQ_MXQ
+  return launched("mxfp4_quantize");
+}
+
+LNQ_API LnqStatus lnq_mxfp4_dequantize(const uint8_t* blocks, const uint8_t* scales, void* out, int64_t rows,
+                                       int64_t in_features, int32_t dtype, void* stream) {
+  if (const LnqStatus st = check_rounding("lnq_mxfp4_dequantize", rows, in_features, dtype)) return st;
+  if (rows == 0 || in_features == 0) {
+    clear_error();
+    return LNQ_OK;
+  }
+  LNQ_REQUIRE(blocks && scales && out, "lnq_mxfp4_dequantize: null pointer");
+  LNQ_REQUIRE(aligned(blocks, 16) && aligned(out, 16), "lnq_mxfp4_dequantize: blocks and out must be 16-byte aligned");
+  const int64_t eights = rows * (in_features / 8), grid = (eights + mxr::THREADS - 1) / mxr::THREADS;
+  LNQ_REQUIRE(grid <= INT32_MAX, "lnq_mxfp4_dequantize: too large");
+#define LNQ_MXD(DT)                                                                                           \
+  hipLaunchKernelGGL((mxfp4_dequantize_kernel<DT>), dim3(static_cast<unsigned>(grid)), dim3(mxr::THREADS), 0, \
+                     static_cast<hipStream_t>(stream), reinterpret_cast<const uint32_t*>(blocks), scales,     \
+                     static_cast<typename Elem<DT>::storage*>(out), eights)
+  if (dtype == LNQ_BF16) LNQ_MXD(LNQ_BF16);
+  else if (dtype == LNQ_F16) LNQ_MXD(LNQ_F16);
+  else LNQ_MXD(LNQ_F32);
+#undef LNQ_MXD
+  return launched("mxfp4_dequantize");
+}
+
+LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, uint8_t* scales, int64_t rows,
+                                 int64_t in_features, int32_t dtype, void* stream) {
+  if (const LnqStatus st = check_rounding("lnq_mxfp4_rows", rows, in_features, dtype)) return st;
+  if (rows == 0 || in_features == 0) {
+    clear_error();
+    return LNQ_OK;
+  }
+  LNQ_REQUIRE(x && q && scales, "lnq_mxfp4_rows: null pointer");
+  LNQ_REQUIRE(x_stride >= 0 && x_stride % 8 == 0 && aligned(x, 16) && aligned(q, 16) && aligned(scales, 16),
+              "lnq_mxfp4_rows: x (with its row stride), q and scales must be 16-byte aligned");
+  const dim3 grid(static_cast<unsigned>((rows + mxr::ROWS - 1) / mxr::ROWS),
+                  static_cast<unsigned>((in_features + mxr::SPAN - 1) / mxr::SPAN));
+  LNQ_REQUIRE(grid.y <= 65535, "lnq_mxfp4_rows: in too large");
+  const int R = static_cast<int>(rows), P = (R + 3) / 4 * 4, K = static_cast<int>(in_features);
+#define LNQ_MXW(DT)                                                                                                     \
+  hipLaunchKernelGGL((mxfp4_rows_kernel<DT>), grid, dim3(mxr::THREADS), 0, static_cast<hipStream_t>(stream),            \
+                     static_cast<const typename Elem<DT>::storage*>(x), x_stride, reinterpret_cast<uint32_t*>(q),       \
+                     reinterpret_cast<uint32_t*>(scales), R, P, K)
+  if (dtype == LNQ_BF16) LNQ_MXW(LNQ_BF16);
+  else if (dtype == LNQ_F16) LNQ_MXW(LNQ_F16);
+  else LNQ_MXW(LNQ_F32);
+#undef LNQ_MXW
+  return launched("mxfp4_rows");
+}
+
+LNQ_API LnqStatus lnq_mxfp4_scale_tiles(const uint8_t* scales, uint8_t* tiles, int64_t count, int64_t out_features,
+                                        int64_t in_features, void* stream) {
+  LNQ_REQUIRE(count >= 0 && out_features >= 0 && in_features >= 0 && in_features % 32 == 0,
+              "lnq_mxfp4_scale_tiles: bad shape count=%lld out=%lld in=%lld (in %% 32 == 0)", static_cast<long long>(count),
+              static_cast<long long>(out_features), static_cast<long long>(in_features));
+  if (count == 0 || out_features == 0 || in_features == 0) {
+    clear_error();
+    return LNQ_OK;
+  }
+  LNQ_REQUIRE(scales && tiles, "lnq_mxfp4_scale_tiles: null pointer");
+  LNQ_REQUIRE(aligned(tiles, 16), "lnq_mxfp4_scale_tiles: tiles must be 16-byte aligned");
+  LNQ_REQUIRE(count <= 65535 && in_features <= 128 * 65535 && out_features <= INT32_MAX - 4, "lnq_mxfp4_scale_tiles: too large");
+  const int N = static_cast<int>(out_features), padded = (N + 3) / 4 * 4, groups = static_cast<int>(in_features / 32);
+  const int units = (groups + 3) / 4;
+  const dim3 grid(static_cast<unsigned>((padded + mxr::THREADS - 1) / mxr::THREADS), static_cast<unsigned>(units),
+                  static_cast<unsigned>(count));
+  hipLaunchKernelGGL(mxfp4_scale_tiles_kernel, grid, dim3(mxr::THREADS), 0, static_cast<hipStream_t>(stream), scales,
+                     reinterpret_cast<uint32_t*>(tiles), N, padded, groups, units);
+  return launched("mxfp4_scale_tiles");
+}
+
+}  // extern "C"

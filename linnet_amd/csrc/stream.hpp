@@ -2,7 +2,7 @@
 // for 1..32 rows of x a workgroup: the weight streamed once from HBM in its own bytes,
 // widened in registers and multiplied on MFMA (16x16x32). Used by lnq_int4_linear
 // (groups and widths the one-workgroup-per-CU GEMVs do not take), lnq_w8a16,
-// lnq_nf4_linear and lnq_mxfp4_experts.
+// lnq_nf4_linear, lnq_mxfp4_linear and lnq_mxfp4_experts.
 //
 // Bound: HBM (the weight's bytes), then the CU's memory pipeline, which also moves x (every
 // workgroup reads all the x its rows meet), then VALU issue (widening: about 200
@@ -201,8 +201,8 @@ inline int scale_lds(int f, bool per_row, bool blocks, int rows, int cols, int r
 // rows 0 .. 4 XI - 1), and `put(m, n, v)` for every output (m < 16 MT, n < n_end; m may
 // lie past the rows that exist). XI: instructions that move a step's x (4 rows each).
 // GPS: groups a step (0: one scale a row). NW: the workgroup's waves, which
-// all call it.
-template <int NW, int DT, int F, int GPS, int MT, int XI, int NT, int KIND, class RowOf, class Put>
+// all call it. NANS (FP4): a scale byte of 255 is E8M0's NaN, and not 2^128.
+template <int NW, int DT, int F, int GPS, int MT, int XI, int NT, int KIND, bool NANS = false, class RowOf, class Put>
 __device__ inline void product(const Args& a, int n0, int n_end, const uint16_t* xbase, uint32_t xbytes, uint16_t* X0, uint16_t* X1,
                                uint8_t* SC, RowOf row_of, Put put) {
   using E = Elem<DT>;
@@ -435,6 +435,9 @@ __device__ inline void product(const Args& a, int n0, int n_end, const uint16_t*
               const uint32_t v = *reinterpret_cast<const uint16_t*>(SC + sat[T] + 2 * cc);
               sf = E::to_f32(static_cast<uint16_t>(in ? v : 0u));
               off = E::MAGIC_VALUE + static_cast<float>(SC[zat[T] + cc]);
+            } else if constexpr (F == FP4 && NANS) {
+              const uint32_t v = SC[sat[T] + cc];
+              sf = __builtin_bit_cast(float, v == 255 ? 0x7fc00000u : max(v << 23, 0x00400000u));
             } else if constexpr (F == FP4) {
               e = static_cast<int>(SC[sat[T] + cc]) - 127;
             } else {
@@ -448,7 +451,7 @@ __device__ inline void product(const Args& a, int n0, int n_end, const uint16_t*
               for (int t = g * TPG; t < (g + 1) * TPG; ++t) p = mfma16x16x32<DT>(xa[h][mt][t], b[t], p);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                if constexpr (F == FP4) acc[mt][T][r] += ldexpf(p[r], e);
+                if constexpr (F == FP4 && !NANS) acc[mt][T][r] += ldexpf(p[r], e);
                 else if constexpr (XS) acc[mt][T][r] = fmaf(sf, fmaf(-off, cx[h][mt][g][r], p[r]), acc[mt][T][r]);
                 else acc[mt][T][r] = fmaf(sf, p[r], acc[mt][T][r]);
               }
@@ -552,7 +555,7 @@ __global__ __launch_bounds__(64 * WAVES) void dense_kernel(Args a) {
   const int live = min(a.M - m0, 16 * MT);
   const uint16_t* x = a.x + static_cast<int64_t>(m0) * a.x_stride;
   const uint32_t xbytes = static_cast<uint32_t>(((live - 1) * a.x_stride + a.K) * 2);
-  product<WAVES, DT, F, GPS, MT, XI, NT, KIND>(
+  product<WAVES, DT, F, GPS, MT, XI, NT, KIND, F == FP4>(
       a, n0, n_end, x, xbytes, X0, X1, SC, [&](int i) -> int { return i < live ? i * a.x_stride : -1; },
       [&](int m, int n, float v) {
         if (m < live) {

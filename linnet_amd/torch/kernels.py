@@ -576,6 +576,226 @@ def mxfp4_experts(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, e
     return y
 
 
+_ANY = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _mxfp4_operands(what: str, blocks: torch.Tensor, scales: torch.Tensor) -> int:
+    """In of MXFP4 tensors: blocks [..., G, 16] and scales [..., G], both uint8."""
+    if blocks.dim() < 2 or blocks.shape[-1] != 16 or blocks.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise LinnetError(f"{what}: blocks are [..., G, 16] and scales [..., G], both uint8")
+    if scales.shape != blocks.shape[:-1]:
+        raise LinnetError(f"{what}: blocks {tuple(blocks.shape)} and scales {tuple(scales.shape)}")
+    return blocks.shape[-2] * 32
+
+
+def _mxfp4_tiles(what: str, tiles: torch.Tensor, lead: tuple[int, ...], rows: int, in_features: int) -> None:
+    shape = (*lead, -(-in_features // 128), -(-rows // 4) * 4, 4)
+    if tiles.dtype != torch.uint8 or tuple(tiles.shape) != shape:
+        raise LinnetError(f"{what}: scale tiles are {list(shape)} uint8, got {list(tiles.shape)} {tiles.dtype}")
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """`t` contiguous and 16-byte aligned (a copy where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """`x` [..., In] (bf16, f16 or f32) rounded to MXFP4, `(blocks [..., In/32, 16] u8, scales
+    [..., In/32] u8)` as checkpoints store it: every 32 values share the scale 2^(s - 127), s -
+    127 the exponent of their largest magnitude less 2 (at least -127), and are rounded to E2M1,
+    ties to the even code, past 6 to 6 (the OCP microscaling format's conversion). A block with
+    an infinity or a NaN gets s = 255, which every reader but `mxfp4_experts` takes as NaN."""
+    device = _on_gpu("mxfp4_quantize", x)
+    if x.dim() == 0 or x.shape[-1] % 32:
+        raise LinnetError(f"mxfp4_quantize: x is [..., In] with In % 32 == 0, got {tuple(x.shape)}")
+    code = _code(x.dtype, "mxfp4_quantize", _ANY)
+    depth = x.shape[-1]
+    x = _aligned(x)
+    blocks = torch.empty(*x.shape[:-1], depth // 32, 16, dtype=torch.uint8, device=device)
+    scales = torch.empty(*x.shape[:-1], depth // 32, dtype=torch.uint8, device=device)
+    with _on(device):
+        _lib.call("lnq_mxfp4_quantize", _ptr(x), _ptr(blocks), _ptr(scales), x.numel() // max(depth, 1), depth, code,
+                  _stream(device))
+    return blocks, scales
+
+
+def mxfp4_dequantize(blocks: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """MXFP4 `blocks` [..., G, 16] and `scales` [..., G] as values [..., 32 G] of `dtype` (bf16,
+    f16 or f32), rounded once (`dequantize_mxfp4`, `stdlib/quant.linnet:334-341`); a scale of 255
+    gives NaN."""
+    device = _on_gpu("mxfp4_dequantize", blocks, scales)
+    depth = _mxfp4_operands("mxfp4_dequantize", blocks, scales)
+    code = _code(dtype, "mxfp4_dequantize", _ANY)
+    blocks, scales = _aligned(blocks), scales.contiguous()
+    out = torch.empty(*blocks.shape[:-2], depth, dtype=dtype, device=device)
+    with _on(device):
+        _lib.call("lnq_mxfp4_dequantize", _ptr(blocks), _ptr(scales), _ptr(out), out.numel() // max(depth, 1), depth, code,
+                  _stream(device))
+    return out
+
+
+def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Each row of `x` [rows, In] (bf16, f16 or f32) rounded to MXFP4 as `mxfp4_quantize` does, laid
+    out for `mxfp4_mm`: `(q [rows, In/2] u8, scales [ceil(In/128), rows rounded up to 4, 4] u8)`,
+    a row's four scales of 128 inputs together ("scale tiles")."""
+    device = _on_gpu("mxfp4_rows", x)
+    if x.dim() != 2 or x.shape[1] % 32:
+        raise LinnetError(f"mxfp4_rows: x is [rows, In] with In % 32 == 0, got {tuple(x.shape)}")
+    rows, depth = x.shape
+    code = _code(x.dtype, "mxfp4_rows", _ANY)
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = _aligned(x)
+    q = torch.empty(rows, depth // 2, dtype=torch.uint8, device=device)
+    scales = torch.empty(-(-depth // 128), -(-rows // 4) * 4, 4, dtype=torch.uint8, device=device)
+    with _on(device):
+        _lib.call("lnq_mxfp4_rows", _ptr(x), x.stride(0), _ptr(q), _ptr(scales), rows, depth, code, _stream(device))
+    return q, scales
+
+
+def mxfp4_scale_tiles(scales: torch.Tensor, in_features: int) -> torch.Tensor:
+    """A weight's scales as stored ([Out, In/32], or [E, Out, In/32] for experts) as the scale tiles
+    that `mxfp4_mm` / `mxfp4_experts_mm` read ([(E,) ceil(In/128), Out rounded up to 4, 4]);
+    made once, when the weight is loaded."""
+    device = _on_gpu("mxfp4_scale_tiles", scales)
+    if scales.dtype != torch.uint8 or scales.dim() not in (2, 3) or in_features != 32 * scales.shape[-1]:
+        raise LinnetError(f"mxfp4_scale_tiles: scales are [(E,) Out, {in_features} / 32] uint8, got "
+                          f"{tuple(scales.shape)} {scales.dtype}")
+    out_features = scales.shape[-2]
+    scales = scales.contiguous()
+    tiles = torch.empty(*scales.shape[:-2], -(-in_features // 128), -(-out_features // 4) * 4, 4, dtype=torch.uint8,
+                        device=device)
+    with _on(device):
+        _lib.call("lnq_mxfp4_scale_tiles", _ptr(scales), _ptr(tiles), scales.shape[0] if scales.dim() == 3 else 1,
+                  out_features, in_features, _stream(device))
+    return tiles
+
+
+def _mxfp4_bias(what: str, bias: torch.Tensor | None, dtype: torch.dtype, out_features: int) -> torch.Tensor | None:
+    if bias is None:
+        return None
+    if bias.dtype != dtype or bias.shape != (out_features,):
+        raise LinnetError(f"{what}: bias is [{out_features}] {dtype}, got {tuple(bias.shape)} {bias.dtype}")
+    return bias.contiguous()
+
+
+def mxfp4_w4a16(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """`F.linear(x, W, bias)` for few rows `x` [rows, In] (bf16 or f16) and the MXFP4 weight as
+    stored (`blocks` [Out, In/32, 16], `scales` [Out, In/32]), widened in registers, x unrounded;
+    summed in f32 with the bias, rounded once. Each 32 rows read the weight again."""
+    device = _on_gpu("mxfp4_w4a16", x, blocks, scales, bias)
+    depth = _mxfp4_operands("mxfp4_w4a16", blocks, scales)
+    if x.dim() != 2 or blocks.dim() != 3 or x.shape[1] != depth:
+        raise LinnetError(f"mxfp4_w4a16: x {tuple(x.shape)} against blocks {tuple(blocks.shape)}")
+    code = _code(x.dtype, "mxfp4_w4a16")
+    rows, out_features = x.shape[0], blocks.shape[0]
+    bias = _mxfp4_bias("mxfp4_w4a16", bias, x.dtype, out_features)
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16 or x.stride(0) < depth or x.stride(0) >= 1 << 23:
+        x = _aligned(x)
+    blocks, scales = _aligned(blocks), scales.contiguous()
+    y = torch.empty(rows, out_features, dtype=x.dtype, device=device)
+    with _on(device):
+        _lib.call("lnq_mxfp4_linear", _ptr(x), max(x.stride(0), depth), _ptr(blocks), _ptr(scales), _ptr(bias), _ptr(y), rows,
+                  out_features, depth, code, _stream(device))
+    return y
+
+
+def mxfp4_mm(q: torch.Tensor, x_scale: torch.Tensor, blocks: torch.Tensor, tiles: torch.Tensor, dtype: torch.dtype,
+             bias: torch.Tensor | None = None) -> torch.Tensor:
+    """`x @ W.T (+ bias)` in `dtype` (bf16 or f16) for rows rounded by `mxfp4_rows` (`q`, `x_scale`)
+    and an MXFP4 weight (`blocks` [Out, In/32, 16] as stored, `tiles` of `mxfp4_scale_tiles`) on
+    gfx950's block-scaled MFMA: exact products, f32 sums, the bias added in f32, rounded once."""
+    device = _on_gpu("mxfp4_mm", q, x_scale, blocks, tiles, bias)
+    if blocks.dim() != 3 or blocks.shape[2] != 16 or blocks.dtype != torch.uint8 or q.dim() != 2 or q.dtype != torch.uint8:
+        raise LinnetError("mxfp4_mm: q is [rows, In/2] and blocks [Out, In/32, 16], both uint8")
+    out_features, depth = blocks.shape[0], blocks.shape[1] * 32
+    rows = q.shape[0]
+    if q.shape[1] * 2 != depth:
+        raise LinnetError(f"mxfp4_mm: q {tuple(q.shape)} against blocks {tuple(blocks.shape)}")
+    _mxfp4_tiles("mxfp4_mm", x_scale, (), rows, depth)
+    _mxfp4_tiles("mxfp4_mm", tiles, (), out_features, depth)
+    code = _code(dtype, "mxfp4_mm")
+    bias = _mxfp4_bias("mxfp4_mm", bias, dtype, out_features)
+    q, x_scale, blocks, tiles = _aligned(q), _aligned(x_scale), _aligned(blocks), _aligned(tiles)
+    y = torch.empty(rows, out_features, dtype=dtype, device=device)
+    with _on(device):
+        _lib.call("lnq_mxfp4_mm", _ptr(q), _ptr(x_scale), _ptr(blocks), _ptr(tiles), _ptr(bias), _ptr(y), rows, out_features,
+                  depth, code, _stream(device))
+    return y
+
+
+MXFP4_MM_EXPERTS = 2048  # experts that `mxfp4_experts_mm` takes at most
+
+
+def mxfp4_experts_mm(q: torch.Tensor, x_scale: torch.Tensor, blocks: torch.Tensor, tiles: torch.Tensor,
+                     experts: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """`mxfp4_experts` of rows rounded to MXFP4: `y[r, k] = x[r (, k)] @ W[experts[r, k]].T` in
+    `dtype`, each expert's pairs multiplied together on the block-scaled MFMA. `q` and `x_scale`
+    (`mxfp4_rows`) hold R rows (every chosen expert of a row reads it) or R * K, one a pair; with
+    K = 1 the two are the same. `blocks` [E, Out, In/32, 16] as stored, `tiles` of
+    `mxfp4_scale_tiles`. An expert outside 0 .. E - 1 gives zeros."""
+    device = _on_gpu("mxfp4_experts_mm", q, x_scale, blocks, tiles, experts)
+    if blocks.dim() != 4 or blocks.shape[3] != 16 or blocks.dtype != torch.uint8 or q.dim() != 2 or q.dtype != torch.uint8:
+        raise LinnetError("mxfp4_experts_mm: q is [rows, In/2] and blocks [E, Out, In/32, 16], both uint8")
+    count, out_features, groups, _ = blocks.shape
+    if experts.dim() != 2 or experts.is_floating_point():
+        raise LinnetError(f"mxfp4_experts_mm: experts are integers [R, K], got {tuple(experts.shape)} {experts.dtype}")
+    rows, chosen = experts.shape
+    if q.shape[0] not in (rows, rows * chosen) or q.shape[1] != groups * 16:
+        raise LinnetError(f"mxfp4_experts_mm: q {tuple(q.shape)} against experts {tuple(experts.shape)} and blocks "
+                          f"{tuple(blocks.shape)}")
+    _mxfp4_tiles("mxfp4_experts_mm", x_scale, (), q.shape[0], groups * 32)
+    _mxfp4_tiles("mxfp4_experts_mm", tiles, (count,), out_features, groups * 32)
+    code = _code(dtype, "mxfp4_experts_mm")
+    q, x_scale, blocks, tiles = _aligned(q), _aligned(x_scale), _aligned(blocks), _aligned(tiles)
+    ids = experts.to(torch.int64).contiguous()
+    y = torch.empty(rows, chosen, out_features, dtype=dtype, device=device)
+    need = ctypes.c_int64(0)
+    with _on(device):
+        _lib.call("lnq_mxfp4_experts_workspace", rows * chosen, count, ctypes.byref(need))
+        space = torch.empty(need.value, dtype=torch.uint8, device=device)
+        _lib.call("lnq_mxfp4_experts_mm", _ptr(q), _ptr(x_scale), _ptr(blocks), _ptr(tiles), _ptr(ids), _ptr(y), rows, chosen,
+                  count, out_features, groups * 32, int(q.shape[0] == rows), code, _ptr(space), need.value, _stream(device))
+    return y
+
+
+def expert_route(logits: torch.Tensor, top: int, bias: torch.Tensor | None = None, score: str = "softmax", groups: int = 1,
+                 group_top: int = 1, group_best: int = 2, renormalize: bool = True,
+                 scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """The experts a router chooses: `(experts [..., top] int64, weights [..., top] f32)` of `logits`
+    [..., E] (bf16, f16 or f32), by falling choice. Scores are a "softmax" over the experts or each
+    logit's "sigmoid"; the choice goes by score + `bias` ([E] f32; without one by the logits), in
+    64 bits, equal ones by the lower index. With `groups` > 1 (equal runs of experts) only the
+    `group_top` groups whose `group_best` (1 or 2) best choices sum highest are chosen from. The
+    weights are the chosen experts' scores (without the bias), over their sum if `renormalize`,
+    times `scale`. An expert whose logit is -inf, or whose choice is -inf or NaN, is never chosen;
+    a place left over holds -1 with weight 0, which the experts' products take as zeros. A row with
+    a NaN logit (or +inf under softmax) gets -1 and NaN. E <= 1024, top <= 64, groups <= 64."""
+    device = _on_gpu("expert_route", logits, bias)
+    if logits.dim() == 0:
+        raise LinnetError("expert_route: logits are [..., E]")
+    if top < 1:
+        raise LinnetError(f"expert_route: {top} choices a row")
+    if score not in ("softmax", "sigmoid"):
+        raise LinnetError(f"expert_route: score is softmax or sigmoid, not {score}")
+    count = logits.shape[-1]
+    code = _code(logits.dtype, "expert_route", _ANY)
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape != (count,):
+            raise LinnetError(f"expert_route: bias is [{count}] float32, got {tuple(bias.shape)} {bias.dtype}")
+        bias = bias.contiguous()
+    lead = logits.shape[:-1]
+    flat = logits if logits.dim() == 2 else logits.reshape(-1, count)
+    if flat.stride(1) != 1 and count > 1:
+        flat = flat.contiguous()
+    experts = torch.empty(*lead, top, dtype=torch.int64, device=device)
+    weights = torch.empty(*lead, top, dtype=torch.float32, device=device)
+    with _on(device):
+        _lib.call("lnq_expert_route", _ptr(flat), flat.stride(0), _ptr(bias), _ptr(experts), _ptr(weights), flat.shape[0], count,
+                  top, groups, group_top, group_best, int(score == "softmax"), int(renormalize), scale, code, _stream(device))
+    return experts, weights
+
+
 # ------------------------------------------------------------------------ 8-bit
 
 

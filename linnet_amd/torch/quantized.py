@@ -33,6 +33,7 @@ Fp8Operands = tuple[torch.Tensor, torch.Tensor, torch.Tensor, int, int]
 Fp8BlockOperands = tuple[torch.Tensor, torch.Tensor, torch.Tensor, int, int, int]
 Int8Operands = tuple[torch.Tensor, torch.Tensor, int, int]
 Int8GroupOperands = tuple[torch.Tensor, torch.Tensor, int, int]
+Mxfp4Operands = tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, int]
 
 
 def _gpu(weight: torch.Tensor) -> None:
@@ -173,3 +174,70 @@ def int8_group_linear(x: torch.Tensor, operands: Int8GroupOperands, bias: torch.
     else:
         y = functional.linear(flat, kernels.dequantize8(weight, scale, False, group, 1, flat.dtype))
     return _finish(x, y, bias)
+
+
+# Widest MXFP4 layer that the few-row kernel and the 4-bit product take.
+_MXFP4_IN, _MXFP4_OUT = 65536, 65535 * 64
+
+
+def mxfp4_operands(blocks: torch.Tensor, scales: torch.Tensor, rounded: int) -> Mxfp4Operands:
+    """An MXFP4 layer's weight as stored, `blocks` [Out, In/32, 16] and `scales` [Out, In/32] u8
+    (`kernels.mxfp4_quantize`; gpt-oss's expert layout for one weight), with, where `rounded`, the
+    scales laid out for the 4-bit product too."""
+    _gpu(blocks)
+    if blocks.dim() != 3 or tuple(scales.shape) != tuple(blocks.shape[:2]):
+        raise LinnetError(f"mxfp4_operands: blocks [Out, In/32, 16] and scales [Out, In/32], got {tuple(blocks.shape)} and "
+                          f"{tuple(scales.shape)}")
+    blocks, scales = blocks.contiguous(), scales.contiguous()
+    tiles = kernels.mxfp4_scale_tiles(scales, blocks.shape[1] * 32) if rounded else None
+    return blocks, scales, tiles, rounded
+
+
+def mxfp4_linear(x: torch.Tensor, operands: Mxfp4Operands, bias: torch.Tensor | None) -> torch.Tensor:
+    """`x W^T (+ bias)` for an MXFP4 weight, as the 8-bit layers dispatch: past `FEW_ROWS` rows with
+    `rounded`, x rounded to MXFP4 (`mxfp4_rows`) and the two multiplied in 4 bits; else up to
+    `TILED_ROWS` rows the weight widened in registers, and past those dequantized for the call.
+    bf16 and f16; the bias is added in f32, before the one rounding."""
+    blocks, scales, tiles, rounded = operands
+    out_features, in_features = blocks.shape[0], blocks.shape[1] * 32
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    rows = flat.shape[0]
+    if flat.dtype in _HALF and 0 < in_features <= _MXFP4_IN and out_features <= _MXFP4_OUT:
+        if rounded and tiles is not None and rows > FEW_ROWS:
+            q, row_scales = kernels.mxfp4_rows(flat)
+            y = kernels.mxfp4_mm(q, row_scales, blocks, tiles, flat.dtype, bias)
+            return _finish(x, y, None)
+        if rows <= TILED_ROWS:
+            return _finish(x, kernels.mxfp4_w4a16(flat, blocks, scales, bias), None)
+    return _finish(x, functional.linear(flat, kernels.mxfp4_dequantize(blocks, scales, flat.dtype), bias), None)
+
+
+def mxfp4_experts_operands(blocks: torch.Tensor, scales: torch.Tensor, rounded: int) -> Mxfp4Operands:
+    """The experts of an MXFP4 mixture as stored, `blocks` [E, Out, In/32, 16] and `scales` [E, Out,
+    In/32] u8, with, where `rounded`, the scales laid out for the 4-bit product too."""
+    _gpu(blocks)
+    if blocks.dim() != 4 or tuple(scales.shape) != tuple(blocks.shape[:3]):
+        raise LinnetError(f"mxfp4_experts_operands: blocks [E, Out, In/32, 16] and scales [E, Out, In/32], got "
+                          f"{tuple(blocks.shape)} and {tuple(scales.shape)}")
+    blocks, scales = blocks.contiguous(), scales.contiguous()
+    tiles = kernels.mxfp4_scale_tiles(scales, blocks.shape[2] * 32) if rounded else None
+    return blocks, scales, tiles, rounded
+
+
+def mxfp4_experts_linear(x: torch.Tensor, operands: Mxfp4Operands, experts: torch.Tensor) -> torch.Tensor:
+    """`y[r, k] = x[r (, k)] W[experts[r, k]]^T` [R, K, Out] for `experts` [R, K] (`kernels.expert_route`'s
+    choice) and `x` [R, In], which the chosen experts of a row share, or [R, K, In]: past
+    `FEW_ROWS` rows with `rounded`, x rounded to MXFP4 and each expert's pairs multiplied together
+    in 4 bits; else `kernels.mxfp4_experts`. An expert outside 0 .. E - 1 gives zeros."""
+    blocks, scales, tiles, rounded = operands
+    if experts.dim() != 2 or x.dim() not in (2, 3) or tuple(x.shape[:-1]) != tuple(experts.shape[: x.dim() - 1]):
+        raise LinnetError(f"mxfp4_experts_linear: x [R, In] or [R, K, In] and experts [R, K], got {tuple(x.shape)} and "
+                          f"{tuple(experts.shape)}")
+    rows, chosen = experts.shape
+    x_rows = rows if x.dim() == 2 else rows * chosen
+    if (rounded and tiles is not None and rows > FEW_ROWS and x.dtype in _HALF and blocks.shape[0] <= kernels.MXFP4_MM_EXPERTS
+            and x_rows * x.shape[-1] < 1 << 32):
+        q, row_scales = kernels.mxfp4_rows(x.reshape(x_rows, x.shape[-1]))
+        return kernels.mxfp4_experts_mm(q, row_scales, blocks, tiles, experts, x.dtype)
+    shared = x[:, None, :].expand(rows, chosen, x.shape[1]) if x.dim() == 2 else x
+    return kernels.mxfp4_experts(shared, blocks, scales, experts)

@@ -17,6 +17,7 @@ Modules:
 - `oracle.linear`  -- the reference's CPU linear paths (torch on the CPU, as
   the reference itself runs them) and fp64 products for tolerances (plain,
   8-bit rows, block-scaled FP8, MXFP4 experts).
+- `oracle.route`   -- a mixture's router, row by row in fp64.
 
 Parity pins (what fixes each function independently of its own formula) are
 listed in each function's docstring and exercised in `tests/test_oracle.py`.

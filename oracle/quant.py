@@ -382,6 +382,30 @@ def dequantize_mxfp4(blocks: np.ndarray, scales: np.ndarray) -> np.ndarray:
     return (values * factor[..., None]).reshape(*b.shape[:-2], b.shape[-2] * 32)
 
 
+def quantize_mxfp4(x: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """`x` [..., In] rounded to MXFP4 in f64: blocks [..., G, 16] bytes and E8M0 scales [..., G].
+    A block's scale exponent is floor(log2 max|x|) - 2, at least -127 (the OCP microscaling
+    format's conversion); each value is the nearest E2M1 one after the division, a midpoint to
+    the even code, past 6 to 6. A block with an infinity or a NaN: scale 255, codes 0.
+
+    Pin: a search over the 16 values for the nearest and the format's worked exponents
+    (tests/test_mxfp4_host.py::test_mxfp4_rounding_by_search)."""
+    v = np.asarray(x, dtype=np.float64)
+    v = v.reshape(*v.shape[:-1], v.shape[-1] // 32, 32)
+    fine = np.isfinite(v).all(-1)
+    v = np.where(fine[..., None], v, 0.0)
+    exponent = np.frexp(np.abs(v).max(-1))[1] - 3
+    exponent = np.where(np.abs(v).max(-1) == 0, -127, np.maximum(exponent, -127))
+    a = np.ldexp(np.abs(v), -exponent[..., None])
+    code = np.zeros(a.shape, dtype=np.uint8)
+    for i, middle in enumerate((0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)):
+        code += (a >= middle) if i % 2 else (a > middle)
+    code |= np.signbit(v).astype(np.uint8) << 3
+    code = np.where(fine[..., None], code, 0).astype(np.uint8)
+    scales = np.where(fine, exponent + 127, 255).astype(np.uint8)
+    return code[..., 0::2] | (code[..., 1::2] << 4), scales
+
+
 # ------------------------------------------------------------------------ NF4
 
 # QLoRA's NormalFloat-4 values by code, as bitsandbytes' map holds them (the

@@ -1,0 +1,475 @@
+"""MXFP4 made and multiplied on the GPU: rounding to MXFP4 and back bit for bit against the
+oracle, the 4-bit x 4-bit product, the linear layer and the experts of a prompt against f64
+products of the exact values.
+
+Tolerance of a product: the MFMA's products are exact and its f32 sum of K terms errs by at
+most K ulps of the terms' magnitudes whatever its order (2^-23 each, rounded or cut), then one
+rounding: |got - want| <= K 2^-23 sum|x w| + half a step of the type (bf16 2^-8, f16 2^-11
+relative, f16 2^-25 absolute below its normal range), the latter of a value that the former
+has moved."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from linnet_amd import LinnetError, _lib
+from linnet_amd.torch import kernels, quantized
+from oracle import quant
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _values(rng: np.random.Generator, *shape: int, spread: int = 3) -> np.ndarray:
+    """Values whose blocks have scales of their own."""
+    v = rng.standard_normal(shape).astype(np.float32)
+    return v * np.exp2(rng.integers(-spread, spread + 1, (*shape[:-1], shape[-1] // 32))).astype(np.float32).repeat(32, -1)
+
+
+def _weight(rng: np.random.Generator, *shape: int) -> tuple[torch.Tensor, torch.Tensor, np.ndarray]:
+    """(blocks, scales on the GPU, values) of a random weight [..., Out, In]: every code, scales a few steps apart."""
+    *lead, depth = shape
+    blocks = rng.integers(0, 256, (*lead, depth // 32, 16)).astype(np.uint8)
+    scales = rng.integers(120, 127, (*lead, depth // 32)).astype(np.uint8)
+    return torch.from_numpy(blocks).to(DEV), torch.from_numpy(scales).to(DEV), quant.dequantize_mxfp4(blocks, scales)
+
+
+def _rounded(x: torch.Tensor) -> np.ndarray:
+    return quant.dequantize_mxfp4(*quant.quantize_mxfp4(x.float().cpu().numpy())).astype(np.float64)
+
+
+def _check(got: torch.Tensor, x: np.ndarray, w: np.ndarray, bias: torch.Tensor | None = None) -> None:
+    assert got.dtype in HALF
+    x, w = x.astype(np.float64), w.astype(np.float64)
+    want, terms = x @ w.T, np.abs(x) @ np.abs(w).T
+    if bias is not None:
+        b = bias.double().cpu().numpy()
+        want, terms = want + b, terms + np.abs(b)
+    sums = (x.shape[-1] + 1) * 2.0 ** -23 * terms
+    half = HALF[got.dtype]
+    bound = sums + half * (np.abs(want) + sums) + (2.0 ** -25 if got.dtype == torch.float16 else 0.0)
+    g = got.double().cpu().numpy()
+    off = np.abs(g - want)
+    assert np.isfinite(g).all()
+    assert (off <= bound).all(), f"{int((off > bound).sum())} of {off.size} past the bound, worst {float((off / bound).max()):.3g}"
+
+
+# ------------------------------------------------------------------ rounding
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(32,), (1, 64), (3, 5, 96), (33, 2880), (7, 4096), (0, 64), (4, 0)])
+def test_quantize_is_the_oracles(dtype: torch.dtype, shape: tuple[int, ...]) -> None:
+    print(f"quantize {shape} {dtype}", flush=True)
+    rng = np.random.default_rng(sum(shape))
+    x = torch.from_numpy(_values(rng, *shape)).to(dtype)
+    blocks, scales = kernels.mxfp4_quantize(x.to(DEV))
+    assert blocks.shape == (*shape[:-1], shape[-1] // 32, 16) and scales.shape == (*shape[:-1], shape[-1] // 32)
+    if x.numel():
+        want_blocks, want_scales = quant.quantize_mxfp4(x.float().numpy())
+        assert np.array_equal(scales.cpu().numpy(), want_scales)
+        assert np.array_equal(blocks.cpu().numpy(), want_blocks)
+    back = kernels.mxfp4_dequantize(blocks, scales, dtype)
+    want = quant.dequantize_mxfp4(blocks.cpu().numpy(), scales.cpu().numpy()).reshape(shape)
+    assert back.dtype == dtype and torch.equal(back.cpu(), torch.from_numpy(want).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_at_every_border(dtype: torch.dtype) -> None:
+    """Midpoints, their neighbours in the type, zeros of both signs, the smallest and largest
+    magnitudes, at scales over the type's whole range."""
+    print(f"borders {dtype}", flush=True)
+    top = torch.finfo(dtype)
+    points = torch.tensor([0.0, 0.25, 0.5, 0.75, 1.0, 1.25, 1.5, 1.75, 2.0, 2.5, 3.0, 3.5, 4.0, 5.0, 6.0, 7.0], dtype=dtype)
+    bits = points.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    points = torch.cat([points, (bits + 1).view(dtype), (bits - (bits > 0).to(bits.dtype)).view(dtype), points + top.eps])
+    points = torch.cat([points, -points]).view(4, 32)
+    points[:, 0] = 7.75  # the largest: a scale of 1 before the factor below
+    low = {torch.float32: -148, torch.bfloat16: -132, torch.float16: -23}[dtype]
+    high = {torch.float32: 125, torch.bfloat16: 125, torch.float16: 13}[dtype]
+    rows = [(points.double() * 2.0 ** e).to(dtype) for e in range(low, high + 1)]
+    rows += [torch.zeros(1, 32, dtype=dtype), -torch.zeros(1, 32, dtype=dtype),
+             torch.full((1, 32), top.max, dtype=dtype), torch.full((1, 32), -top.smallest_normal, dtype=dtype),
+             torch.full((1, 32), top.smallest_normal * top.eps, dtype=dtype)]
+    x = torch.cat(rows)
+    assert torch.isfinite(x).all()
+    blocks, scales = kernels.mxfp4_quantize(x.to(DEV))
+    want_blocks, want_scales = quant.quantize_mxfp4(x.float().numpy())
+    assert np.array_equal(scales.cpu().numpy(), want_scales)
+    assert np.array_equal(blocks.cpu().numpy(), want_blocks)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_blocks_that_are_not_finite(dtype: torch.dtype) -> None:
+    print(f"not finite {dtype}", flush=True)
+    x = torch.from_numpy(_values(np.random.default_rng(1), 4, 128)).to(dtype)
+    x[0, 5], x[1, 40], x[2, 127] = float("nan"), float("inf"), float("-inf")
+    blocks, scales = kernels.mxfp4_quantize(x.to(DEV))
+    want_blocks, want_scales = quant.quantize_mxfp4(x.float().numpy())
+    assert np.array_equal(scales.cpu().numpy(), want_scales) and (want_scales == 255).sum() == 3
+    assert np.array_equal(blocks.cpu().numpy(), want_blocks)
+    back = kernels.mxfp4_dequantize(blocks, scales, dtype).view(4, 4, 32).cpu()
+    assert torch.equal(back.isnan().all(-1), torch.from_numpy(want_scales == 255))
+    assert torch.equal(back.isnan().any(-1), torch.from_numpy(want_scales == 255))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_dequantize_every_code_and_scale(dtype: torch.dtype) -> None:
+    print(f"dequantize {dtype}", flush=True)
+    codes = np.arange(256, dtype=np.uint8)[None].repeat(256, 0).reshape(256, 16, 16)
+    scales = np.arange(256, dtype=np.uint8)[:, None].repeat(16, 1)
+    got = kernels.mxfp4_dequantize(torch.from_numpy(codes).to(DEV), torch.from_numpy(scales).to(DEV), dtype).cpu()
+    values = np.stack([quant.FP4_VALUES[codes & 15], quant.FP4_VALUES[codes >> 4]], -1).reshape(256, 512).astype(np.float64)
+    want = torch.from_numpy(values * np.exp2(np.arange(256.0) - 127)[:, None]).to(torch.float32).to(dtype)
+    assert torch.equal(got[:255], want[:255]) and got[255].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize(("rows", "depth"), [(1, 32), (2, 96), (4, 128), (33, 2880), (64, 544), (131, 512), (3, 4128), (0, 64)])
+def test_rows_are_quantize_in_tiles(rows: int, depth: int, dtype: torch.dtype) -> None:
+    print(f"rows {rows} x {depth} {dtype}", flush=True)
+    wide = torch.from_numpy(_values(np.random.default_rng(rows + depth), rows, depth + 32)).to(dtype).to(DEV)
+    for x in (wide[:, 32:], wide[:, :depth].contiguous()):  # strided rows, packed ones
+        q, tiles = kernels.mxfp4_rows(x)
+        blocks, scales = kernels.mxfp4_quantize(x)
+        assert torch.equal(q, blocks.view(rows, depth // 2))
+        padded, units = -(-rows // 4) * 4, -(-depth // 128)
+        assert tiles.shape == (units, padded, 4)
+        want = torch.zeros(padded, units * 4, dtype=torch.uint8, device=DEV)
+        want[:rows, : depth // 32] = scales
+        assert torch.equal(tiles, want.view(padded, units, 4).permute(1, 0, 2))
+        # A weight's scales, laid out once, hold the same.
+        assert torch.equal(kernels.mxfp4_scale_tiles(scales, depth), tiles)
+
+
+def test_scale_tiles_of_experts() -> None:
+    scales = torch.randint(0, 256, (5, 70, 9), dtype=torch.uint8, device=DEV)
+    tiles = kernels.mxfp4_scale_tiles(scales, 288)
+    assert tiles.shape == (5, 3, 72, 4)
+    for e in range(5):
+        assert torch.equal(tiles[e], kernels.mxfp4_scale_tiles(scales[e], 288))
+
+
+# ------------------------------------------------------------------ products
+
+SIZES = [(1, 1, 32), (3, 7, 96), (33, 64, 128), (64, 100, 160), (65, 257, 256), (129, 130, 288), (300, 513, 544),
+         (40, 96, 2880), (257, 300, 1056)]
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize(("rows", "out", "depth"), SIZES)
+def test_mm(rows: int, out: int, depth: int, dtype: torch.dtype, bias: bool) -> None:
+    print(f"mm {rows} x {depth} -> {out} {dtype} bias={bias}", flush=True)
+    rng = np.random.default_rng(rows * 7 + out + depth)
+    x = torch.from_numpy(_values(rng, rows, depth)).to(dtype).to(DEV)
+    blocks, scales, w = _weight(rng, out, depth)
+    b = torch.from_numpy(rng.standard_normal(out).astype(np.float32)).to(dtype).to(DEV) if bias else None
+    q, row_scales = kernels.mxfp4_rows(x)
+    y = kernels.mxfp4_mm(q, row_scales, blocks, kernels.mxfp4_scale_tiles(scales, depth), dtype, b)
+    assert y.shape == (rows, out)
+    _check(y, _rounded(x), w, b)
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize(("rows", "out", "depth"), [(1, 1, 32), (1, 4096, 4096), (2, 100, 96), (4, 300, 2880), (8, 65, 544),
+                                                    (16, 1000, 1056), (17, 33, 288), (32, 257, 160), (64, 96, 128)])
+def test_w4a16(rows: int, out: int, depth: int, dtype: torch.dtype, bias: bool) -> None:
+    print(f"w4a16 {rows} x {depth} -> {out} {dtype} bias={bias}", flush=True)
+    rng = np.random.default_rng(rows * 7 + out + depth)
+    wide = torch.from_numpy(_values(rng, rows, depth + 32)).to(dtype).to(DEV)
+    blocks, scales, w = _weight(rng, out, depth)
+    b = torch.from_numpy(rng.standard_normal(out).astype(np.float32)).to(dtype).to(DEV) if bias else None
+    for x in (wide[:, :depth], wide[:, 32:].contiguous()):
+        _check(kernels.mxfp4_w4a16(x, blocks, scales, b), x.float().cpu().numpy(), w, b)
+
+
+def test_scales_that_are_nan_reach_every_output_of_theirs() -> None:
+    """A row's or an output's block with the scale 255 makes that row's or output's values NaN
+    and no others, in both products."""
+    rng = np.random.default_rng(5)
+    rows, out, depth = 40, 72, 288
+    x = torch.from_numpy(_values(rng, rows, depth)).to(torch.bfloat16)
+    x[3, 287], x[17, 0] = float("inf"), float("nan")
+    blocks, scales, w = _weight(rng, out, depth)
+    scales[5, 8] = 255
+    scales[70, 0] = 255
+    want = torch.zeros(rows, out, dtype=torch.bool)
+    want[[3, 17]] = True
+    want[:, [5, 70]] = True
+    operands = quantized.mxfp4_operands(blocks, scales, 1)
+    y = quantized.mxfp4_linear(x.to(DEV), operands, None)
+    assert torch.equal(y.isnan().cpu(), want) and y[~want].isfinite().all()
+    few = quantized.mxfp4_linear(x[:20].to(DEV), operands, None)
+    assert torch.equal(few.isnan().cpu()[:3], want[:3]) and few[:3][~want[:3]].isfinite().all()
+    widened = quantized.mxfp4_linear(x[:3].float().to(DEV), operands, None)
+    assert torch.equal(widened.isnan().cpu(), want[:3])
+
+
+@pytest.mark.parametrize("scale", [0, 1, 60, 200])
+def test_extreme_scales(scale: int) -> None:
+    """Products far from 1: scale bytes at and near the ends, still in bf16's range."""
+    rng = np.random.default_rng(scale)
+    blocks, _, _ = _weight(rng, 40, 160)
+    scales = torch.full((40, 5), scale, dtype=torch.uint8, device=DEV)
+    w = quant.dequantize_mxfp4(blocks.cpu().numpy(), scales.cpu().numpy())
+    # x such that the products are about 1: its own block scales are at the other end.
+    power = min(127 - scale, 120)
+    x = (torch.from_numpy(_values(rng, 40, 160, spread=0)).double() * 2.0 ** power).to(torch.bfloat16).to(DEV)
+    operands = quantized.mxfp4_operands(blocks, scales, 1)
+    _check(quantized.mxfp4_linear(x, operands, None), _rounded(x), w)
+    _check(quantized.mxfp4_linear(x[:9], operands, None), x[:9].float().cpu().numpy(), w)
+
+
+def test_nothing_behind_the_last_row_is_read_into_the_sums_or_written() -> None:
+    """q, scales and y inside larger buffers: NaN scales and full codes behind the rows change no
+    output, and what lies behind y stays."""
+    rng = np.random.default_rng(9)
+    for rows, out, depth in [(33, 50, 160), (65, 130, 96), (130, 70, 2880), (300, 260, 288)]:
+        x = torch.from_numpy(_values(rng, rows, depth)).to(torch.bfloat16).to(DEV)
+        blocks, scales, _ = _weight(rng, out, depth)
+        q, row_scales = kernels.mxfp4_rows(x)
+        tiles = kernels.mxfp4_scale_tiles(scales, depth)
+        want = kernels.mxfp4_mm(q, row_scales, blocks, tiles, torch.bfloat16)
+
+        def behind(t: torch.Tensor) -> torch.Tensor:
+            room = torch.full((t.numel() + (1 << 16),), 255, dtype=torch.uint8, device=DEV)
+            room[: t.numel()] = t.reshape(-1)
+            return room
+
+        row_scales = row_scales.clone()
+        row_scales[:, rows:] = 255
+        tiles = tiles.clone()
+        tiles[:, out:] = 255
+        held = [behind(t) for t in (q, row_scales, blocks, tiles)]
+        y = torch.full((rows * out + 4096,), 3.0, dtype=torch.bfloat16, device=DEV)
+        _lib.call("lnq_mxfp4_mm", *(t.data_ptr() for t in held), None, y.data_ptr(), rows, out, depth, _lib.BF16,
+                  torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(y[: rows * out].view(rows, out), want)
+        assert (y[rows * out:] == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+def test_linear_takes_the_documented_product(dtype: torch.dtype) -> None:
+    rng = np.random.default_rng(3)
+    blocks, scales, w = _weight(rng, 96, 288)
+    bias = torch.from_numpy(rng.standard_normal(96).astype(np.float32)).to(dtype).to(DEV)
+    for rounded in (0, 1):
+        operands = quantized.mxfp4_operands(blocks, scales, rounded)
+        for rows in (0, 1, 32, 33, 64, 65, 200):
+            print(f"linear rounded={rounded} rows={rows} {dtype}", flush=True)
+            x = torch.from_numpy(_values(rng, rows, 288)).to(dtype).to(DEV)
+            y = quantized.mxfp4_linear(x, operands, bias)
+            assert y.shape == (rows, 96) and y.dtype == dtype
+            values = _rounded(x) if rounded and rows > 32 else x.float().cpu().numpy()
+            if rows:
+                _check(y, values, w, bias)
+    x = torch.from_numpy(_values(rng, 2, 3, 288)).to(dtype).to(DEV)
+    y = quantized.mxfp4_linear(x, operands, None)
+    assert y.shape == (2, 3, 96)
+    _check(y.view(6, 96), x.view(6, 288).float().cpu().numpy(), w)
+    wide = quantized.mxfp4_linear(x.float(), operands, None)
+    assert wide.dtype == torch.float32
+    torch.testing.assert_close(wide.cpu().double().view(6, 96), torch.from_numpy(x.view(6, 288).double().cpu().numpy() @ w.T.astype(np.float64)),
+                               rtol=288 * 2.0 ** -24, atol=288 * 2.0 ** -23 * float(np.abs(w).max() * x.abs().max().item() * 288))
+
+
+# ------------------------------------------------------------------ experts
+
+
+def _experts(rng: np.random.Generator, kind: str, rows: int, chosen: int, count: int) -> np.ndarray:
+    if kind == "spread":
+        return np.stack([rng.permutation(count)[:chosen] if chosen <= count else rng.integers(0, count, chosen) for _ in range(rows)])
+    if kind == "one":
+        return np.full((rows, chosen), count - 1)
+    if kind == "ends":  # choices that are no expert among the others
+        e = rng.integers(-2, count + 2, (rows, chosen))
+        e[0, 0], e[-1, -1] = -(2 ** 40), 2 ** 40
+        return e
+    return np.full((rows, chosen), -1)
+
+
+@pytest.mark.parametrize("kind", ["spread", "one", "ends", "none"])
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize(("rows", "chosen", "count", "out", "depth"), [
+    (1, 1, 1, 1, 32), (33, 4, 8, 70, 96), (40, 2, 5, 128, 288), (70, 1, 3, 33, 160), (257, 4, 4, 64, 128),
+    (300, 3, 40, 36, 64), (64, 8, 2, 200, 544)])
+def test_experts_mm(rows: int, chosen: int, count: int, out: int, depth: int, dtype: torch.dtype, kind: str) -> None:
+    print(f"experts {kind} rows={rows} chosen={chosen} E={count} {depth} -> {out} {dtype}", flush=True)
+    rng = np.random.default_rng(rows + chosen + count + out)
+    blocks, scales, w = _weight(rng, count, out, depth)
+    tiles = kernels.mxfp4_scale_tiles(scales, depth)
+    experts = _experts(rng, kind, rows, chosen, count).astype(np.int64)
+    ids = torch.from_numpy(experts).to(DEV)
+    for shared in (True, False):
+        x = torch.from_numpy(_values(rng, rows if shared else rows * chosen, depth)).to(dtype).to(DEV)
+        q, row_scales = kernels.mxfp4_rows(x)
+        y = kernels.mxfp4_experts_mm(q, row_scales, blocks, tiles, ids, dtype)
+        assert y.shape == (rows, chosen, out)
+        values = _rounded(x)
+        for e in range(count):
+            r, k = np.nonzero(experts == e)
+            if r.size:
+                _check(y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)], values[r if shared else r * chosen + k], w[e])
+        r, k = np.nonzero((experts < 0) | (experts >= count))
+        assert not y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)].any()
+
+
+def test_experts_linear_takes_the_documented_product() -> None:
+    rng = np.random.default_rng(11)
+    count, out, depth = 6, 96, 160
+    blocks, scales, w = _weight(rng, count, out, depth)
+    for rounded in (0, 1):
+        operands = quantized.mxfp4_experts_operands(blocks, scales, rounded)
+        for rows in (1, 32, 33, 100):
+            experts = torch.from_numpy(_experts(rng, "spread", rows, 2, count)).to(DEV)
+            for shape in ((rows, depth), (rows, 2, depth)):
+                print(f"experts_linear rounded={rounded} {shape}", flush=True)
+                x = torch.from_numpy(_values(rng, *shape)).to(torch.bfloat16).to(DEV)
+                y = quantized.mxfp4_experts_linear(x, operands, experts)
+                values = _rounded(x) if rounded and rows > 32 else x.double().cpu().numpy()
+                pairs = values if len(shape) == 3 else values[:, None].repeat(2, 1)
+                for e in range(count):
+                    r, k = np.nonzero(experts.cpu().numpy() == e)
+                    if r.size:
+                        _check(y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)], pairs[r, k], w[e])
+
+
+# ------------------------------------------------------------------ refusals, streams, graphs
+
+
+def test_refusals() -> None:
+    u8 = lambda *shape: torch.zeros(*shape, dtype=torch.uint8, device=DEV)  # noqa: E731
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device=DEV)
+    for call, message in [
+        (lambda: kernels.mxfp4_quantize(torch.zeros(4, 40, device=DEV)), "In % 32"),
+        (lambda: kernels.mxfp4_quantize(torch.zeros(4, 64, dtype=torch.float64, device=DEV)), "dtype"),
+        (lambda: kernels.mxfp4_dequantize(u8(4, 2, 15), u8(4, 2), torch.float32), "16"),
+        (lambda: kernels.mxfp4_dequantize(u8(4, 2, 16), u8(4, 3), torch.float32), "scales"),
+        (lambda: kernels.mxfp4_rows(torch.zeros(4, 2, 64, device=DEV)), "rows, In"),
+        (lambda: kernels.mxfp4_scale_tiles(u8(4, 2), 96), "scales are"),
+        (lambda: kernels.mxfp4_w4a16(x, u8(8, 3, 16), u8(8, 3)), "against"),
+        (lambda: kernels.mxfp4_w4a16(x.float(), u8(8, 2, 16), u8(8, 2)), "dtype"),
+        (lambda: kernels.mxfp4_w4a16(x, u8(8, 2, 16), u8(8, 2), torch.zeros(8, device=DEV)), "bias"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 3, 16), u8(1, 8, 4), torch.bfloat16), "against"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 8, 4), u8(8, 2, 16), u8(1, 8, 4), torch.bfloat16), "scale tiles"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(2, 8, 4), torch.bfloat16), "scale tiles"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(1, 8, 4), torch.float32), "dtype"),
+        (lambda: kernels.mxfp4_experts_mm(u8(5, 32), u8(1, 8, 4), u8(2, 8, 2, 16), u8(2, 1, 8, 4),
+                                          torch.zeros(4, 2, dtype=torch.int64, device=DEV), torch.bfloat16), "against"),
+        (lambda: kernels.mxfp4_experts_mm(u8(4, 32), u8(1, 4, 4), u8(2, 8, 2, 16), u8(2, 1, 8, 4),
+                                          torch.zeros(4, 2, device=DEV), torch.bfloat16), "integers"),
+        (lambda: quantized.mxfp4_operands(u8(2, 8, 2, 16), u8(2, 8, 2), 1), "blocks"),
+        (lambda: quantized.mxfp4_experts_operands(u8(8, 2, 16), u8(8, 2), 1), "blocks"),
+        (lambda: quantized.mxfp4_experts_linear(x, quantized.mxfp4_experts_operands(u8(2, 8, 2, 16), u8(2, 8, 2), 1),
+                                                torch.zeros(5, 2, dtype=torch.int64, device=DEV)), "experts"),
+    ]:
+        with pytest.raises(LinnetError, match=message):
+            call()
+
+
+def test_workspace_is_checked() -> None:
+    need = ctypes.c_int64(0)
+    _lib.call("lnq_mxfp4_experts_workspace", 64, 8, ctypes.byref(need))
+    with pytest.raises(LinnetError, match="workspace"):
+        _lib.call("lnq_mxfp4_experts_mm", *[4096] * 6, 16, 4, 8, 64, 64, 1, _lib.BF16, 4096, need.value - 1, None)
+
+
+def _mixture(x: torch.Tensor, router: torch.Tensor, gate_up: tuple, down: tuple) -> torch.Tensor:
+    """A mixture's layer as a program strings the calls together."""
+    experts, weights = kernels.expert_route(x @ router, 2)
+    h = quantized.mxfp4_experts_linear(x, gate_up, experts)
+    g, u = h.chunk(2, dim=-1)
+    h = (torch.nn.functional.silu(g.float()) * u.float()).to(x.dtype)
+    y = quantized.mxfp4_experts_linear(h, down, experts)
+    return (y.float() * weights[..., None]).sum(1).to(x.dtype)
+
+
+def _mixture_case(rows: int):
+    rng = np.random.default_rng(rows)
+    hidden, inner, count = 96, 64, 6
+    gate_up = _weight(rng, count, 2 * inner, hidden)
+    down = _weight(rng, count, hidden, inner)
+    x = torch.from_numpy(rng.standard_normal((rows, hidden)).astype(np.float32)).to(torch.bfloat16).to(DEV)
+    router = torch.from_numpy(rng.standard_normal((hidden, count)).astype(np.float32)).to(torch.bfloat16).to(DEV)
+    return x, router, gate_up, down
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+def test_a_mixture_layer_end_to_end(rows: int) -> None:
+    """Router, gate | up experts, SiLU, down experts and the weighted sum, against the same in f64
+    from each stage's own inputs (so that a stage's rounding is not another's error)."""
+    print(f"mixture rows={rows}", flush=True)
+    x, router, gate_up, down = _mixture_case(rows)
+    up_ops = quantized.mxfp4_experts_operands(*gate_up[:2], 1)
+    down_ops = quantized.mxfp4_experts_operands(*down[:2], 1)
+    got = _mixture(x, router, up_ops, down_ops)
+    experts, weights = kernels.expert_route(x @ router, 2)
+    logits = (x @ router).double()
+    assert torch.equal(experts, torch.sort(logits, dim=-1, descending=True, stable=True).indices[:, :2])
+    torch.testing.assert_close(weights.double(), torch.softmax(logits.gather(1, experts), -1), rtol=2e-7, atol=0)
+    h = quantized.mxfp4_experts_linear(x, up_ops, experts)
+    g, u = h.chunk(2, dim=-1)
+    h = (torch.nn.functional.silu(g.float()) * u.float()).to(x.dtype)
+    v = _rounded(h) if rows > 32 else h.double().cpu().numpy()
+    ids = experts.cpu().numpy()
+    pair = np.einsum("rki,rkoi->rko", v, down[2].astype(np.float64)[ids])
+    terms = np.einsum("rki,rkoi->rko", np.abs(v), np.abs(down[2]).astype(np.float64)[ids])
+    wk = weights.double().cpu().numpy()[..., None]
+    want = (pair * wk).sum(1)
+    # Each pair's product is rounded to bf16 (half a step of it and of its sum's error), the sum once more.
+    bound = (wk * (2.0 ** -8 * np.abs(pair) + 64 * 2.0 ** -23 * terms)).sum(1) * 1.02 + 2.0 ** -8 * np.abs(want) * 1.02
+    assert (np.abs(got.double().cpu().numpy() - want) <= bound).all()
+
+
+def test_captured_and_replayed() -> None:
+    """The layer's calls in a graph, replayed on new inputs with eager work between, against the
+    eager calls; two graphs side by side keep their own workspaces."""
+    graphs = []
+    for rows in (70, 40):
+        x, router, gate_up, down = _mixture_case(rows)
+        ops = [quantized.mxfp4_experts_operands(*w[:2], 1) for w in (gate_up, down)]
+        linear = quantized.mxfp4_operands(gate_up[0][0], gate_up[1][0], 1)
+
+        def layer(x=x, router=router, ops=ops, linear=linear):
+            return _mixture(x, router, *ops), quantized.mxfp4_linear(x, linear, None)
+
+        layer()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layer()
+        graphs.append((graph, x, layer, out))
+    for i in range(3):
+        for graph, x, layer, out in graphs:
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16))
+        for graph, *_ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, x, layer, out in graphs:
+            for got, want in zip(out, layer()):
+                assert torch.equal(got, want)
+
+
+def test_two_streams_at_once() -> None:
+    cases = [_mixture_case(rows) for rows in (90, 50)]
+    layers = [(c[0], c[1], *(quantized.mxfp4_experts_operands(*w[:2], 1) for w in c[2:])) for c in cases]
+    want = [_mixture(*layer) for layer in layers]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got: list[list[torch.Tensor]] = [[], []]
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(_mixture(*layers[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y in got[i]:
+            assert torch.equal(y, want[i])
