@@ -14,15 +14,22 @@
 // weight of 0 (the experts' products give zeros for it). A row with a NaN logit (or +inf under
 // softmax) has no scores: its experts are -1, its weights NaN.
 //
-// A wave takes a row, lane l the experts l S .. l S + S - 1.
+// A wave takes a row: with G groups rounded up to a power of two, 64 / G lanes hold a group, S
+// experts a lane, so that experts rise with the lane and its slot. Bound by VALU issue, not by
+// the row's bytes: so
+// * a group's two best are a butterfly over its lanes, and its rank among the groups a count;
+// * a choice is the wave's largest f32 key, the choice rounded once (order survives rounding):
+//   six DPP maxima. Only where several lanes hold that key, which differ in 64 bits, are
+//   those compared.
 #include "common.hpp"
 
 namespace lnq {
 
 namespace route {
 constexpr int THREADS = 256;
-constexpr int MAX_TOP = 64;      // a lane holds a choice
-constexpr int MAX_SLOTS = 16;    // experts of a lane
+constexpr int MAX_TOP = 64;    // a lane holds a choice
+constexpr int MAX_COUNT = 1024;
+constexpr int MAX_SLOTS = 32;  // experts of a lane: 1024 in 33 groups leave a lane a group of 31
 }  // namespace route
 
 struct RouteArgs {
@@ -31,33 +38,72 @@ struct RouteArgs {
   float* weights;
   int64_t stride;  // logits from row to row
   int rows, count, top, groups, group_top, group_best;
+  int size, lanes;  // experts and lanes of a group
   int softmax, renormalize;
   double scale;
 };
 
-__device__ inline double shfl_double(double v, int from) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = static_cast<uint32_t>(__shfl(static_cast<int>(b & 0xffffffffu), from, 64));
-  const uint32_t hi = static_cast<uint32_t>(__shfl(static_cast<int>(b >> 32), from, 64));
+// `v` of another lane by a DPP control (lanes without a partner: `old`).
+template <int CTRL>
+__device__ inline float dpp(float old, float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v), CTRL,
+                                                               0xf, 0xf, false));
+}
+
+template <int CTRL>
+__device__ inline double dpp(double old, double v) {
+  const uint64_t o = __builtin_bit_cast(uint64_t, old), b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(o), static_cast<int>(b), CTRL, 0xf, 0xf, false));
+  const uint32_t hi =
+      static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(o >> 32), static_cast<int>(b >> 32), CTRL, 0xf, 0xf, false));
   return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
 }
 
-__device__ inline double shfl_xor_double(double v, int mask) { return shfl_double(v, (threadIdx.x & 63) ^ mask); }
-
-// The largest v of the wave and the lowest index that has it, in every lane.
-__device__ inline void wave_best(double& v, int& at) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double w = shfl_xor_double(v, off);
-    const int o = __shfl_xor(at, off, 64);
-    if (w > v || (w == v && o < at)) v = w, at = o;
-  }
+__device__ inline float lane_of(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
-__device__ inline double wave_sum_double(double v) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) v += shfl_xor_double(v, off);
-  return v;
+__device__ inline double lane_of(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b), lane));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane));
+  return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
+}
+
+// The wave's largest value: within rows of 16 lanes (row_shr 1, 2, 4, 8), then over the rows
+// (row_bcast 15, 31); lane 63 ends with it.
+template <class T>
+__device__ inline T wave_top(T v) {
+  auto larger = [](T a, T b) { return a > b ? a : b; };
+  v = larger(v, dpp<0x111>(v, v));
+  v = larger(v, dpp<0x112>(v, v));
+  v = larger(v, dpp<0x114>(v, v));
+  v = larger(v, dpp<0x118>(v, v));
+  v = larger(v, dpp<0x142>(v, v));
+  v = larger(v, dpp<0x143>(v, v));
+  return lane_of(v, 63);
+}
+
+// The wave's sum: that of each row of 16 lanes in its last lane, the four added.
+__device__ inline double wave_total(double v) {
+  v += dpp<0x111>(0.0, v);
+  v += dpp<0x112>(0.0, v);
+  v += dpp<0x114>(0.0, v);
+  v += dpp<0x118>(0.0, v);
+  return (lane_of(v, 15) + lane_of(v, 31)) + (lane_of(v, 47) + lane_of(v, 63));
+}
+
+// The partner's value in the butterfly step over `d` lanes, where every lane of a run of d
+// holds the same (quad_perm, then mirrors of 8 and 16 lanes).
+__device__ inline double across(double v, int d) {
+  if (d == 1) return dpp<0xb1>(v, v);
+  if (d == 2) return dpp<0x4e>(v, v);
+  if (d == 4) return dpp<0x141>(v, v);
+  if (d == 8) return dpp<0x140>(v, v);
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = static_cast<uint32_t>(__shfl_xor(static_cast<int>(b), d, 64));
+  const uint32_t hi = static_cast<uint32_t>(__shfl_xor(static_cast<int>(b >> 32), d, 64));
+  return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
 }
 
 template <int DT, int S>
@@ -65,19 +111,21 @@ __global__ __launch_bounds__(route::THREADS) void expert_route_kernel(const type
                                                                       RouteArgs a) {
   using E = Elem<DT>;
   const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * (route::THREADS / 64) + (threadIdx.x >> 6);
+  const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * (route::THREADS / 64) + (threadIdx.x >> 6));
   if (row >= a.rows) return;  // the whole wave
   const double none = -__builtin_huge_val();
+  const float nothing = -__builtin_huge_valf();
   const typename E::storage* from = logits + row * a.stride;
-  float l[S];
-  double top = none;
+  const int group = lane / a.lanes, place = (lane - group * a.lanes) * S;
+  const int e0 = group * a.size + place;  // this lane's first expert
+  const int held = group < a.groups ? min(S, a.size - place) : 0;
+  float l[S], most = nothing;
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < S; ++i) {
-    const int e = lane * S + i;
-    l[i] = e < a.count ? E::to_f32(from[e]) : -__builtin_huge_valf();
+    l[i] = i < held ? E::to_f32(from[e0 + i]) : nothing;
     bad = bad || l[i] != l[i] || (a.softmax && l[i] == __builtin_huge_valf());
-    top = fmax(top, static_cast<double>(l[i]));
+    most = fmaxf(most, l[i]);
   }
   int64_t* const experts = a.experts + static_cast<int64_t>(row) * a.top;
   float* const weights = a.weights + static_cast<int64_t>(row) * a.top;
@@ -85,89 +133,101 @@ __global__ __launch_bounds__(route::THREADS) void expert_route_kernel(const type
     if (lane < a.top) experts[lane] = -1, weights[lane] = __builtin_nanf("");
     return;
   }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) top = fmax(top, shfl_xor_double(top, off));
 
-  double s[S], c[S], sum = 0;
-#pragma unroll
-  for (int i = 0; i < S; ++i) {
-    const double v = l[i];
-    if (v == none) s[i] = 0;
-    else if (a.softmax) s[i] = exp(v - top);
-    else s[i] = 1 / (1 + exp(-v));
-    sum += s[i];
-  }
+  double s[S];
   if (a.softmax) {
-    sum = wave_sum_double(sum);
+    const double top = wave_top(most);
+    double sum = 0;
 #pragma unroll
-    for (int i = 0; i < S; ++i) s[i] = sum > 0 ? s[i] / sum : 0;
+    for (int i = 0; i < S; ++i) {
+      s[i] = l[i] == nothing ? 0 : exp(l[i] - top);
+      sum += s[i];
+    }
+    sum = wave_total(sum);
+    const double part = sum > 0 ? 1 / sum : 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i) s[i] *= part;
+  } else {
+#pragma unroll
+    for (int i = 0; i < S; ++i) s[i] = l[i] == nothing ? 0 : 1 / (1 + exp(-static_cast<double>(l[i])));
   }
+  // The choices and their keys.
+  const bool biased = a.bias != nullptr;
+  double c[S];
+  float key[S];
 #pragma unroll
   for (int i = 0; i < S; ++i) {
     c[i] = l[i];
-    if (a.bias != nullptr && c[i] != none) {
-      c[i] = s[i] + static_cast<double>(a.bias[min(lane * S + i, a.count - 1)]);
+    if (biased && i < held && l[i] != nothing) {
+      c[i] = s[i] + static_cast<double>(a.bias[e0 + i]);
       if (c[i] != c[i]) c[i] = none;
     }
+    key[i] = static_cast<float>(c[i]);
   }
-
-  // The value of slot i of the lane that holds expert `at`, in every lane.
-  auto pick = [&](const double (&v)[S], int at) -> double {
-    double mine = 0;
-#pragma unroll
-    for (int i = 0; i < S; ++i)
-      if (at % S == i) mine = v[i];
-    return shfl_double(mine, at / S);
-  };
-  // The best expert that `in` lets through: its choice and index (none: `none`).
-  auto best = [&](auto in, int& at) -> double {
-    double v = none;
-    at = INT32_MAX;
-#pragma unroll
-    for (int i = 0; i < S; ++i) {
-      const int e = lane * S + i;
-      if (in(e) && c[i] > v) v = c[i], at = e;
-    }
-    wave_best(v, at);
-    return v;
-  };
 
   if (a.groups > 1) {
-    const int size = a.count / a.groups;
-    double score = none;  // lane g: group g's
-    for (int g = 0; g < a.groups; ++g) {
-      int at, second;
-      double v = best([&](int e) { return e / size == g; }, at);
-      if (a.group_best == 2 && v != none) {
-        const double w = best([&](int e) { return e / size == g && e != at; }, second);
-        if (w == none) v = none;
-        else v = a.bias != nullptr ? v + w : pick(s, at) + pick(s, second);
-      }
-      if (lane == g) score = v;
-    }
-    uint64_t kept = 0;
-    for (int i = 0; i < a.group_top; ++i) {
-      double v = (kept >> lane) & 1 || lane >= a.groups ? none : score;
-      int at = (kept >> lane) & 1 || lane >= a.groups ? INT32_MAX : lane;
-      wave_best(v, at);
-      kept |= uint64_t{1} << at;
-    }
+    // The two best of the group; without a bias their scores, which rise with the logits.
+    double v = none, w = none;
 #pragma unroll
-    for (int i = 0; i < S; ++i)
-      if (!((kept >> ((lane * S + i) / size & 63)) & 1)) c[i] = none;
+    for (int i = 0; i < S; ++i) {
+      const double q = c[i] == none || biased || a.group_best == 1 ? c[i] : s[i];
+      w = fmax(w, fmin(v, q));
+      v = fmax(v, q);
+    }
+    for (int d = 1; d < a.lanes; d *= 2) {
+      const double v2 = across(v, d), w2 = across(w, d);
+      w = fmax(fmax(w, w2), fmin(v, v2));
+      v = fmax(v, v2);
+    }
+    if (a.group_best == 2) v = w == none ? none : v + w;
+    int rank = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      const double other = lane_of(v, g * a.lanes);
+      rank += other > v || (other == v && g < group);
+    }
+    if (rank >= a.group_top) {
+#pragma unroll
+      for (int i = 0; i < S; ++i) key[i] = nothing;
+    }
   }
 
+  // This lane's best: its key, choice, score and expert (the first slot of the largest choice).
+  float best;
+  double best_c, best_s;
+  int best_e;
+  auto look = [&]() {
+    best = nothing, best_c = none, best_s = 0, best_e = -1;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const bool better = key[i] > best || (key[i] == best && key[i] != nothing && c[i] > best_c);
+      best = better ? key[i] : best;
+      best_c = better ? c[i] : best_c;
+      best_s = better ? s[i] : best_s;
+      best_e = better ? i : best_e;
+    }
+  };
+  look();
   int mine = -1;
   double weight = 0, total = 0;
   for (int i = 0; i < a.top; ++i) {
-    int at;
-    if (best([](int) { return true; }, at) == none) break;
-    const double v = pick(s, at);
+    const float top = wave_top(best);
+    if (top == nothing) break;
+    uint64_t mask = __ballot(best == top);
+    if (biased && (mask & (mask - 1))) {
+      const double first = wave_top(best == top ? best_c : none);
+      mask = __ballot(best == top && best_c == first);
+    }
+    const int owner = __builtin_ctzll(mask);
+    const double v = lane_of(best_s, owner);
+    const int at = __builtin_amdgcn_readlane(e0 + best_e, owner);
     total += v;
     if (lane == i) mine = at, weight = v;
+    if (lane == owner) {
 #pragma unroll
-    for (int j = 0; j < S; ++j)
-      if (lane * S + j == at) c[j] = none;
+      for (int j = 0; j < S; ++j)
+        if (j == best_e) key[j] = nothing;
+      look();
+    }
   }
   if (a.renormalize) weight = total > 0 ? weight / total : 0;
   if (lane < a.top) experts[lane] = mine, weights[lane] = static_cast<float>(weight * a.scale);
@@ -185,9 +245,9 @@ LNQ_API LnqStatus lnq_expert_route(const void* logits, int64_t stride, const flo
                                    void* stream) {
   LNQ_REQUIRE(dtype == LNQ_BF16 || dtype == LNQ_F16 || dtype == LNQ_F32, "lnq_expert_route: dtype %d is not bf16, f16 or f32",
               dtype);
-  LNQ_REQUIRE(rows >= 0 && rows <= INT32_MAX && num_experts > 0 && num_experts <= 64 * route::MAX_SLOTS,
+  LNQ_REQUIRE(rows >= 0 && rows <= INT32_MAX && num_experts > 0 && num_experts <= route::MAX_COUNT,
               "lnq_expert_route: %lld rows of %lld experts (1 to %d)", static_cast<long long>(rows),
-              static_cast<long long>(num_experts), 64 * route::MAX_SLOTS);
+              static_cast<long long>(num_experts), route::MAX_COUNT);
   LNQ_REQUIRE(groups > 0 && groups <= 64 && num_experts % groups == 0 && group_top > 0 && group_top <= groups &&
                   (group_best == 1 || group_best == 2),
               "lnq_expert_route: %lld experts in %lld groups (1 to 64, of equal size), %lld kept by their best %lld (1 or 2)",
@@ -213,11 +273,15 @@ LNQ_API LnqStatus lnq_expert_route(const void* logits, int64_t stride, const flo
   a.groups = static_cast<int>(groups);
   a.group_top = static_cast<int>(group_top);
   a.group_best = static_cast<int>(group_best);
+  a.size = a.count / a.groups;
+  int wide = 1;
+  while (wide < a.groups) wide *= 2;
+  a.lanes = 64 / wide;
   a.softmax = softmax != 0;
   a.renormalize = renormalize != 0;
   a.scale = scale;
   const dim3 grid((a.rows + route::THREADS / 64 - 1) / (route::THREADS / 64));
-  const int slots = (a.count + 63) / 64;
+  const int slots = (a.size + a.lanes - 1) / a.lanes;  // at most 31: 1024 / 33 with a lane a group
 #define LNQ_ROUTE(DT, S)                                                                                \
   hipLaunchKernelGGL((expert_route_kernel<DT, S>), grid, dim3(route::THREADS), 0,                       \
                      static_cast<hipStream_t>(stream), static_cast<const typename Elem<DT>::storage*>(logits), a)
@@ -227,7 +291,8 @@ LNQ_API LnqStatus lnq_expert_route(const void* logits, int64_t stride, const flo
     else if (slots <= 2) LNQ_ROUTE(DT, 2);     \
     else if (slots <= 4) LNQ_ROUTE(DT, 4);     \
     else if (slots <= 8) LNQ_ROUTE(DT, 8);     \
-    else LNQ_ROUTE(DT, 16);                    \
+    else if (slots <= 16) LNQ_ROUTE(DT, 16);   \
+    else LNQ_ROUTE(DT, 32);                    \
   } while (0)
   if (dtype == LNQ_BF16) LNQ_ROUTE_S(LNQ_BF16);
   else if (dtype == LNQ_F16) LNQ_ROUTE_S(LNQ_F16);
