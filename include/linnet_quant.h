@@ -485,16 +485,15 @@ LNQ_API LnqStatus lnq_mxfp4_dequantize(const uint8_t* blocks, const uint8_t* sca
 
 /* Rows of activations as lnq_mxfp4_mm reads them: lnq_mxfp4_quantize's rounding of x [rows,
  * in] (rows x_stride elements apart, a multiple of 8), the codes in q [rows, in/2], the scales
- * as tiles: [units][padded][4] bytes, unit u holding blocks 4u .. 4u + 3 (128 inputs) of every
- * row, units = ceil(in / 128), padded = rows rounded up to a multiple of 4 (rows past the last
- * and blocks past `in` hold 0). x, q and scales 16-byte aligned. No counterpart in the
- * reference. */
+ * as scale tiles: [units][padded][4] bytes, unit u holding blocks 4u .. 4u + 3 (128 inputs) of
+ * every row, units = ceil(in / 128), padded = rows rounded up to a multiple of 128; row r lies at
+ * place (r - r % 128) + 4 (r % 32) + r / 32 % 4 (places of no row and blocks past `in` hold 0).
+ * x, q and scales 16-byte aligned. No counterpart in the reference. */
 LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, uint8_t* scales,
                                  int64_t rows, int64_t in_features, int32_t dtype, void* stream);
 
-/* A weight's scales as stored, [count, out, in/32], as tiles: [count][units][padded][4] bytes
- * (units, padded as lnq_mxfp4_rows has them, of `out` rows). Made once, as the weight is
- * loaded. tiles 16-byte aligned. */
+/* A weight's scales as stored, [count, out, in/32], as scale tiles (of `out` rows), one after
+ * another. Made once, as the weight is loaded. tiles 16-byte aligned. */
 LNQ_API LnqStatus lnq_mxfp4_scale_tiles(const uint8_t* scales, uint8_t* tiles, int64_t count,
                                         int64_t out_features, int64_t in_features, void* stream);
 
@@ -522,7 +521,7 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
  * tiles [E] scale tiles each. An expert index outside 0 .. num_experts - 1 gives zeros.
  * workspace (16-byte aligned, at least lnq_mxfp4_experts_workspace bytes) holds the lists of
  * the pairs, written by the call: calls that overlap on one workspace race. num_experts <=
- * 2048, rows * chosen and out <= 2^27, x's codes below 2 GiB. */
+ * 2048, rows * chosen <= 2^26, out <= 2^27, x's codes below 2 GiB. */
 LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t num_experts, int64_t* bytes);
 LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale, const uint8_t* blocks,
                                        const uint8_t* tiles, const int64_t* experts, void* y,

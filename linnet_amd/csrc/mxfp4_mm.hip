@@ -2,11 +2,10 @@
 // for the experts of a mixture: the (row, choice) pairs of each expert against its weight.
 //
 // Operands: codes [rows, K / 2] bytes, two E2M1 values each, a row's 32-value blocks in a
-// row; scales [units][padded][4] E8M0 bytes, a unit being 128 inputs (4 blocks) of every row
-// and `padded` the rows rounded up to a multiple of 4 (mxfp4_round.hip writes both so). The
-// MFMA (v_mfma_scale_f32_32x32x64_f8f6f4, 131072 operations in 32 cycles) takes a lane's 32
-// codes and their scale byte and adds the exact products of 64 inputs in f32; the sum is
-// rounded once, after the bias.
+// row; scales as scale tiles (mx4.hpp; mxfp4_round.hip writes both so). The MFMA
+// (v_mfma_scale_f32_32x32x64_f8f6f4, 131072 operations in 32 cycles) takes a lane's 32 codes and
+// their scale byte and adds the exact products of 64 inputs in f32; the sum is rounded once,
+// after the bias.
 //
 // A workgroup owns BM rows by BN columns, its waves WM x WN of them in 32 x 32 MFMA tiles.
 // 256 inputs (128 bytes a row) a step: codes and scales move to LDS by buffer_load ... lds,
@@ -15,44 +14,15 @@
 // / 32) once, bytes 0 and 2 are those of its halves of the unit's two MFMAs, named by the
 // instruction's operand selects.
 #include <algorithm>
+#include <cstdlib>
 
-#include "eight_bit.hpp"
+#include "mx4.hpp"
 
 namespace lnq {
 
 namespace mx4 {
-constexpr int BKB = 128;                        // bytes of a row a step
-constexpr int BK = 2 * BKB;                     // inputs a step
-constexpr uint32_t NOWHERE = 0x80000000u;       // an offset past every buffer (each below 2 GiB): reads zeros
-constexpr int MAX_EXPERTS = 2048;               // of the pair lists' LDS
 constexpr int LIST_THREADS = 1024;
-
-struct Args {
-  const uint8_t* q;      // x's codes
-  const uint32_t* xs;    // and scales [units][xp]
-  const uint8_t* w;
-  const uint32_t* ws;    // [units][wp]
-  const uint16_t* bias;
-  uint16_t* y;
-  int M, N, K, xp, wp;
-  // Experts: tile t's (expert, first place in `order`, pairs) in table, -1 for none.
-  const int* order;
-  const i32x4* table;
-  int tiles, count, chosen;  // chosen: pairs that share a row of x, 1 for none
-  int64_t w_step, ws_step;   // from an expert's weight / scales to the next one's
-};
-
-// 16 or 4 bytes a lane from `at` of a buffer to LDS, lane l's at to + 16 l (4 l). (Called in a
-// kernel template with arguments of known types the builtin makes the host's pass drop the
-// kernel's stub without a word.)
-__device__ inline void load16(__amdgpu_buffer_rsrc_t r, uint8_t* to, uint32_t at) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)to, 16, at, 0, 0, 0);
 }
-
-__device__ inline void load4(__amdgpu_buffer_rsrc_t r, uint8_t* to, uint32_t at) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)to, 4, at, 0, 0, 0);
-}
-}  // namespace mx4
 
 template <int DT, int BM, int BN, int WM, int WN, int S, bool EXPERTS>
 __global__ __launch_bounds__(64 * WM * WN, 1) void mx4_kernel(mx4::Args a) {
@@ -79,13 +49,16 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx4_kernel(mx4::Args a) {
   const uint8_t* w = a.w;
   const uint32_t* ws = a.ws;
   if constexpr (EXPERTS) {
-    const int t = static_cast<int>(blockIdx.x % a.tiles);
-    tn = static_cast<int>(blockIdx.x / a.tiles);
-    const i32x4 entry = a.table[t];
+    // Expert by expert, its tiles of rows together for each run of columns.
+    const int at = xcd_tile(blockIdx.x, a.used[0] * tiles_n);
+    if (at < 0) return;
+    const i32x4 any = a.table[at / tiles_n];
+    const int many = __builtin_amdgcn_readfirstlane(any.z) >> 9, tile0 = __builtin_amdgcn_readfirstlane(any.w);
+    tn = (at - tile0 * tiles_n) / many;
+    const i32x4 entry = a.table[tile0 + (at - tile0 * tiles_n) % many];
     const int e = __builtin_amdgcn_readfirstlane(entry.x);
     first = __builtin_amdgcn_readfirstlane(entry.y);
-    live = __builtin_amdgcn_readfirstlane(entry.z);
-    if (e < 0) return;
+    live = __builtin_amdgcn_readfirstlane(entry.z) & 511;
     const int n0 = tn * BN;
     if (e >= a.count) {  // pairs whose choice is no expert: zeros
       const int width = min(BN, a.N - n0);
@@ -142,7 +115,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx4_kernel(mx4::Args a) {
     const int rows = is_x ? BM : BN, p = is_x ? a.xp : a.wp;
     const int unit = d / rows, r = d % rows;
     const int row = is_x ? x_row(r) : (n0 + r < a.N ? n0 + r : -1);
-    soff_g[i] = row < 0 ? NOWHERE : (static_cast<uint32_t>(unit) * p + row) * 4u;
+    soff_g[i] = row < 0 ? NOWHERE : (static_cast<uint32_t>(unit) * p + scale_place(row)) * 4u;
   }
   const uint8_t* const qb = EXPERTS ? a.q : a.q + static_cast<int64_t>(m0) * row_bytes;
   const uint32_t q_bytes = EXPERTS ? static_cast<uint32_t>(a.M) * row_bytes : static_cast<uint32_t>(live) * row_bytes;
@@ -214,11 +187,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx4_kernel(mx4::Args a) {
     }
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      i32x8 af[FA], bf[FB];
-      auto fetch = [&](i32x8& o, uint32_t at) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(st + at);
-        o = i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
-      };
+      i32x4 af[FA], bf[FB];
+      auto fetch = [&](i32x4& o, uint32_t at) { o = *reinterpret_cast<const i32x4*>(st + at); };
 #pragma unroll
       for (int i = 0; i < FA; ++i) fetch(af[i], aoff[kk] + i * 32 * BKB);
 #pragma unroll
@@ -226,15 +196,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx4_kernel(mx4::Args a) {
 #pragma unroll
       for (int i = 0; i < FA; ++i)
 #pragma unroll
-        for (int j = 0; j < FB; ++j) {
+        for (int j = 0; j < FB; ++j)
           // The weight is the MFMA's A operand: a lane then holds 4 outputs of a row together.
-          if (kk & 1)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bf[j], af[i], acc[i][j], 4, 4, 2, sb[j][kk >> 1], 2,
-                                                                        sa[i][kk >> 1]);
-          else
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bf[j], af[i], acc[i][j], 4, 4, 0, sb[j][kk >> 1], 0,
-                                                                        sa[i][kk >> 1]);
-        }
+          acc[i][j] = mma(kk & 1, bf[j], af[i], acc[i][j], sb[j][kk >> 1], sa[i][kk >> 1]);
     }
   };
 
@@ -292,10 +256,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx4_kernel(mx4::Args a) {
 
 // The pairs of each expert, in order: workgroup e counts every expert's pairs, which tells it
 // where its own begin in `order` and in the tile table, then lists them. Workgroup `count`
-// lists the pairs whose choice is no expert and ends the table with -1.
+// lists the pairs whose choice is no expert and writes how many tiles there are.
 __global__ __launch_bounds__(mx4::LIST_THREADS) void expert_lists_kernel(const int64_t* __restrict__ experts, int pairs,
-                                                                         int count, int bm, int tiles,
-                                                                         int* __restrict__ order, i32x4* __restrict__ table) {
+                                                                         int count, int bm,
+                                                                         int* __restrict__ order, i32x4* __restrict__ table,
+                                                                         int* __restrict__ used) {
   using namespace mx4;
   constexpr int WAVES = LIST_THREADS / 64;
   __shared__ int number[MAX_EXPERTS + 1];
@@ -328,9 +293,9 @@ __global__ __launch_bounds__(mx4::LIST_THREADS) void expert_lists_kernel(const i
 #pragma unroll
   for (int v = 0; v < WAVES; ++v) first += part[0][v], tile += part[1][v], all += part[2][v];
   const int mine = number[e];
-  for (int i = tid; i * bm < mine; i += LIST_THREADS) table[tile + i] = i32x4{e, first + i * bm, min(bm, mine - i * bm), 0};
-  if (e == count)
-    for (int i = all + tid; i < tiles; i += LIST_THREADS) table[i] = i32x4{-1, 0, 0, 0};
+  for (int i = tid; i * bm < mine; i += LIST_THREADS) 
+    table[tile + i] = i32x4{e, first + i * bm, min(bm, mine - i * bm) + 512 * ((mine + bm - 1) / bm), tile};
+  if (e == count && tid == 0) used[0] = all;
   if (mine == 0) return;
   int at = first;
   for (int p0 = 0; p0 < pairs; p0 += LIST_THREADS) {
@@ -380,7 +345,7 @@ static Plan experts_plan(int64_t pairs, int64_t count) {
   p.bm = tile_rows(static_cast<double>(pairs) / static_cast<double>(count));
   p.tiles = static_cast<int>(pairs / p.bm + std::min(pairs, count + 1));
   p.order_bytes = (pairs * 4 + 15) / 16 * 16;
-  p.bytes = p.order_bytes + static_cast<int64_t>(p.tiles) * 16;
+  p.bytes = p.order_bytes + static_cast<int64_t>(p.tiles) * 16 + 16;
   return p;
 }
 
@@ -418,10 +383,11 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
   a.M = static_cast<int>(rows);
   a.N = static_cast<int>(out_features);
   a.K = static_cast<int>(in_features);
-  a.xp = (a.M + 3) / 4 * 4;
-  a.wp = (a.N + 3) / 4 * 4;
+  a.xp = mx4::padded_rows(a.M);
+  a.wp = mx4::padded_rows(a.N);
   LNQ_REQUIRE((rows + 31) / 32 * ((out_features + 63) / 64) <= INT32_MAX, "lnq_mxfp4_mm: too large");
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (getenv("MXL")) return mx4::launch_large(a, false, dtype, s);
   const int bm = mx4::tile_rows(static_cast<double>(rows));
   if (dtype == LNQ_BF16) mx4::launch<LNQ_BF16, false>(a, bm, s);
   else mx4::launch<LNQ_F16, false>(a, bm, s);
@@ -430,7 +396,7 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
 
 LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t num_experts, int64_t* bytes) {
   LNQ_REQUIRE(bytes != nullptr, "lnq_mxfp4_experts_workspace: null pointer");
-  LNQ_REQUIRE(pairs >= 0 && pairs <= (1 << 27) && num_experts > 0 && num_experts <= mx4::MAX_EXPERTS,
+  LNQ_REQUIRE(pairs >= 0 && pairs <= (1 << 26) && num_experts > 0 && num_experts <= mx4::MAX_EXPERTS,
               "lnq_mxfp4_experts_workspace: %lld pairs of %lld experts (1 to %d)", static_cast<long long>(pairs),
               static_cast<long long>(num_experts), mx4::MAX_EXPERTS);
   *bytes = pairs == 0 ? 0 : mx4::experts_plan(pairs, num_experts).bytes;
@@ -448,9 +414,9 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
               "lnq_mxfp4_experts_mm: bad shape rows=%lld chosen=%lld experts=%lld (1 to %d) out=%lld in=%lld (in %% 32 == 0)",
               static_cast<long long>(rows), static_cast<long long>(chosen), static_cast<long long>(num_experts),
               mx4::MAX_EXPERTS, static_cast<long long>(out_features), static_cast<long long>(in_features));
-  LNQ_REQUIRE(rows <= (1 << 27) && chosen <= (1 << 27) && rows * chosen <= (1 << 27) && out_features <= (1 << 27) &&
+  LNQ_REQUIRE(rows <= (1 << 27) && chosen <= (1 << 27) && rows * chosen <= (1 << 26) && out_features <= (1 << 27) &&
                   in_features <= (1 << 22),
-              "lnq_mxfp4_experts_mm: past 2^27 pairs or outputs, or 2^22 inputs");
+              "lnq_mxfp4_experts_mm: past 2^26 pairs, 2^27 outputs or 2^22 inputs");
   if (rows == 0 || chosen == 0 || out_features == 0) {
     clear_error();
     return LNQ_OK;
@@ -473,12 +439,13 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   a.M = static_cast<int>(x_rows);
   a.N = static_cast<int>(out_features);
   a.K = static_cast<int>(in_features);
-  a.xp = (a.M + 3) / 4 * 4;
-  a.wp = (a.N + 3) / 4 * 4;
+  a.xp = mx4::padded_rows(a.M);
+  a.wp = mx4::padded_rows(a.N);
   LNQ_REQUIRE(static_cast<int64_t>(plan.tiles) * ((out_features + 63) / 64) <= INT32_MAX,
               "lnq_mxfp4_experts_mm: too large");
   a.order = static_cast<const int*>(workspace);
   a.table = reinterpret_cast<const i32x4*>(static_cast<const uint8_t*>(workspace) + plan.order_bytes);
+  a.used = reinterpret_cast<const int*>(a.table + plan.tiles);
   a.tiles = plan.tiles;
   a.count = static_cast<int>(num_experts);
   a.chosen = shared ? static_cast<int>(chosen) : 1;
@@ -486,7 +453,7 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   a.ws_step = (in_features + 127) / 128 * a.wp;
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(expert_lists_kernel, dim3(a.count + 1), dim3(mx4::LIST_THREADS), 0, s, experts, static_cast<int>(pairs),
-                     a.count, plan.bm, plan.tiles, const_cast<int*>(a.order), const_cast<i32x4*>(a.table));
+                     a.count, plan.bm, const_cast<int*>(a.order), const_cast<i32x4*>(a.table), const_cast<int*>(a.used));
   if (const LnqStatus st = launched("expert_lists")) return st;
   if (dtype == LNQ_BF16) mx4::launch<LNQ_BF16, true>(a, plan.bm, s);
   else mx4::launch<LNQ_F16, true>(a, plan.bm, s);

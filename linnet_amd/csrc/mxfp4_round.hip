@@ -11,14 +11,14 @@
 //
 // Bound by HBM: 2 or 4 bytes a value read, 17/32 written (back: the reverse). Four lanes
 // take a block, 8 values each: a wave's loads are whole kilobytes.
-#include "common.hpp"
+#include "mx4.hpp"
 
 namespace lnq {
 
 namespace mxr {
 constexpr int THREADS = 256;
-constexpr int ROWS = 32;   // rows of a workgroup of the row-rounding kernel: 128 bytes of scales a unit
-constexpr int SPAN = 512;  // inputs of a row that a wave takes: 8 a lane
+constexpr int ROWS = 128;  // rows of a workgroup of the row-rounding kernel: a whole scale tile
+constexpr int UNIT = 128;  // by the inputs of a unit
 
 // 8 values as loaded.
 template <int DT>
@@ -103,39 +103,37 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_quantize_kernel(const type
   if ((threadIdx.x & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(byte);
 }
 
-// Rows for the product: codes [rows, K / 2] as above, scales [units][padded][4] bytes, a
-// unit being 128 inputs (4 blocks) and `padded` rows rounded up to a multiple of 4. A
-// workgroup takes 32 rows by 512 inputs, so the scales leave in runs of 128 bytes.
+// Rows for the product: codes [rows, K / 2] as above, scales as scale tiles (mx4.hpp). A
+// workgroup takes 128 rows by 128 inputs, 16 lanes a row, so that its scales, whose places
+// lie strewn, leave as 512 bytes in a run.
 template <int DT>
 __global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename Elem<DT>::storage* __restrict__ x,
                                                                   int64_t x_stride, uint32_t* __restrict__ codes,
                                                                   uint32_t* __restrict__ scales, int rows, int padded,
                                                                   int K) {
   using namespace mxr;
-  constexpr int PER_WAVE = ROWS / (THREADS / 64);
-  __shared__ uint32_t unit[SPAN / 128][ROWS];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r0 = blockIdx.x * ROWS, k = blockIdx.y * SPAN + lane * 8;
+  constexpr int A_PASS = THREADS / 16;  // rows
+  __shared__ uint32_t unit[ROWS];
+  const int lane = threadIdx.x & 63;
+  const int r0 = blockIdx.x * ROWS, k = blockIdx.y * UNIT + (threadIdx.x & 15) * 8;
   const bool in = k < K;
 #pragma unroll
-  for (int i = 0; i < PER_WAVE; ++i) {
-    const int r = wave * PER_WAVE + i;
+  for (int i = 0; i < ROWS / A_PASS; ++i) {
+    const int r = i * A_PASS + (threadIdx.x >> 4);
     uint32_t byte = 0;
     if (r0 + r < rows && in) {
       float v[8];
       widen8<DT>(load8<DT>(x + (r0 + r) * x_stride + k), v);
       codes[(static_cast<int64_t>(r0 + r) * K + k) >> 3] = round8(v, byte);
     }
-    // The four blocks of a unit, 16 lanes: block b's byte at bits 8 b.
+    // The four blocks of the unit, 16 lanes: block b's byte at bits 8 b.
     uint32_t word = byte << (8 * ((lane >> 2) & 3));
     word |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(word), 4, 64));
     word |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(word), 8, 64));
-    if ((lane & 15) == 0) unit[lane >> 4][r] = word;
+    if ((lane & 15) == 0) unit[mx4::scale_place(r)] = word;
   }
   __syncthreads();
-  const int u = threadIdx.x / ROWS, r = threadIdx.x % ROWS;
-  const int at = blockIdx.y * (SPAN / 128) + u;
-  if (u < SPAN / 128 && at * 128 < K && r0 + r < padded) scales[static_cast<int64_t>(at) * padded + r0 + r] = unit[u][r];
+  if (threadIdx.x < ROWS) scales[static_cast<int64_t>(blockIdx.y) * padded + r0 + threadIdx.x] = unit[threadIdx.x];
 }
 
 template <int DT>
@@ -163,7 +161,7 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_dequantize_kernel(const ui
   }
 }
 
-// Scales as stored, [count, N, groups], laid out for the product: [count][units][padded][4].
+// Scales as stored, [count, N, groups], as scale tiles.
 __global__ __launch_bounds__(mxr::THREADS) void mxfp4_scale_tiles_kernel(const uint8_t* __restrict__ scales,
                                                                          uint32_t* __restrict__ tiles, int N, int padded,
                                                                          int groups, int units) {
@@ -177,7 +175,7 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_scale_tiles_kernel(const u
     for (int b = 0; b < 4; ++b)
       if (4 * u + b < groups) word |= static_cast<uint32_t>(from[b]) << (8 * b);
   }
-  tiles[(static_cast<int64_t>(e) * units + u) * padded + n] = word;
+  tiles[(static_cast<int64_t>(e) * units + u) * padded + mx4::scale_place(n)] = word;
 }
 
 }  // namespace lnq
@@ -190,7 +188,7 @@ LnqStatus check_rounding(const char* what, int64_t rows, int64_t in_features, in
   LNQ_REQUIRE(dtype == LNQ_BF16 || dtype == LNQ_F16 || dtype == LNQ_F32, "%s: dtype %d is not bf16, f16 or f32", what, dtype);
   LNQ_REQUIRE(rows >= 0 && in_features >= 0 && in_features % 32 == 0, "%s: bad shape rows=%lld in=%lld (in %% 32 == 0)", what,
               static_cast<long long>(rows), static_cast<long long>(in_features));
-  LNQ_REQUIRE(in_features <= INT32_MAX && rows <= INT32_MAX, "%s: sizes exceed 2^31", what);
+  LNQ_REQUIRE(in_features <= INT32_MAX && rows <= INT32_MAX - 128, "%s: sizes exceed 2^31", what);
   return LNQ_OK;
 }
 
@@ -253,9 +251,9 @@ LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, ui
   LNQ_REQUIRE(x_stride >= 0 && x_stride % 8 == 0 && aligned(x, 16) && aligned(q, 16) && aligned(scales, 16),
               "lnq_mxfp4_rows: x (with its row stride), q and scales must be 16-byte aligned");
   const dim3 grid(static_cast<unsigned>((rows + mxr::ROWS - 1) / mxr::ROWS),
-                  static_cast<unsigned>((in_features + mxr::SPAN - 1) / mxr::SPAN));
+                  static_cast<unsigned>((in_features + mxr::UNIT - 1) / mxr::UNIT));
   LNQ_REQUIRE(grid.y <= 65535, "lnq_mxfp4_rows: in too large");
-  const int R = static_cast<int>(rows), P = (R + 3) / 4 * 4, K = static_cast<int>(in_features);
+  const int R = static_cast<int>(rows), P = mx4::padded_rows(R), K = static_cast<int>(in_features);
 #define LNQ_MXW(DT)                                                                                                     \
   hipLaunchKernelGGL((mxfp4_rows_kernel<DT>), grid, dim3(mxr::THREADS), 0, static_cast<hipStream_t>(stream),            \
                      static_cast<const typename Elem<DT>::storage*>(x), x_stride, reinterpret_cast<uint32_t*>(q),       \
@@ -278,8 +276,8 @@ LNQ_API LnqStatus lnq_mxfp4_scale_tiles(const uint8_t* scales, uint8_t* tiles, i
   }
   LNQ_REQUIRE(scales && tiles, "lnq_mxfp4_scale_tiles: null pointer");
   LNQ_REQUIRE(aligned(tiles, 16), "lnq_mxfp4_scale_tiles: tiles must be 16-byte aligned");
-  LNQ_REQUIRE(count <= 65535 && in_features <= 128 * 65535 && out_features <= INT32_MAX - 4, "lnq_mxfp4_scale_tiles: too large");
-  const int N = static_cast<int>(out_features), padded = (N + 3) / 4 * 4, groups = static_cast<int>(in_features / 32);
+  LNQ_REQUIRE(count <= 65535 && in_features <= 128 * 65535 && out_features <= INT32_MAX - 128, "lnq_mxfp4_scale_tiles: too large");
+  const int N = static_cast<int>(out_features), padded = mx4::padded_rows(N), groups = static_cast<int>(in_features / 32);
   const int units = (groups + 3) / 4;
   const dim3 grid(static_cast<unsigned>((padded + mxr::THREADS - 1) / mxr::THREADS), static_cast<unsigned>(units),
                   static_cast<unsigned>(count));

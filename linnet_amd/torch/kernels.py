@@ -589,7 +589,7 @@ def _mxfp4_operands(what: str, blocks: torch.Tensor, scales: torch.Tensor) -> in
 
 
 def _mxfp4_tiles(what: str, tiles: torch.Tensor, lead: tuple[int, ...], rows: int, in_features: int) -> None:
-    shape = (*lead, -(-in_features // 128), -(-rows // 4) * 4, 4)
+    shape = (*lead, -(-in_features // 128), -(-rows // 128) * 128, 4)
     if tiles.dtype != torch.uint8 or tuple(tiles.shape) != shape:
         raise LinnetError(f"{what}: scale tiles are {list(shape)} uint8, got {list(tiles.shape)} {tiles.dtype}")
 
@@ -637,8 +637,9 @@ def mxfp4_dequantize(blocks: torch.Tensor, scales: torch.Tensor, dtype: torch.dt
 
 def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Each row of `x` [rows, In] (bf16, f16 or f32) rounded to MXFP4 as `mxfp4_quantize` does, laid
-    out for `mxfp4_mm`: `(q [rows, In/2] u8, scales [ceil(In/128), rows rounded up to 4, 4] u8)`,
-    a row's four scales of 128 inputs together ("scale tiles")."""
+    out for `mxfp4_mm`: `(q [rows, In/2] u8, scales [ceil(In/128), rows rounded up to 128, 4] u8)`, a
+    row's four scales of 128 inputs together, the rows of each 128 in the order 0, 32, 64, 96, 1,
+    33, ... ("scale tiles")."""
     device = _on_gpu("mxfp4_rows", x)
     if x.dim() != 2 or x.shape[1] % 32:
         raise LinnetError(f"mxfp4_rows: x is [rows, In] with In % 32 == 0, got {tuple(x.shape)}")
@@ -647,7 +648,7 @@ def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
         x = _aligned(x)
     q = torch.empty(rows, depth // 2, dtype=torch.uint8, device=device)
-    scales = torch.empty(-(-depth // 128), -(-rows // 4) * 4, 4, dtype=torch.uint8, device=device)
+    scales = torch.empty(-(-depth // 128), -(-rows // 128) * 128, 4, dtype=torch.uint8, device=device)
     with _on(device):
         _lib.call("lnq_mxfp4_rows", _ptr(x), x.stride(0), _ptr(q), _ptr(scales), rows, depth, code, _stream(device))
     return q, scales
@@ -655,7 +656,7 @@ def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def mxfp4_scale_tiles(scales: torch.Tensor, in_features: int) -> torch.Tensor:
     """A weight's scales as stored ([Out, In/32], or [E, Out, In/32] for experts) as the scale tiles
-    that `mxfp4_mm` / `mxfp4_experts_mm` read ([(E,) ceil(In/128), Out rounded up to 4, 4]);
+    that `mxfp4_mm` / `mxfp4_experts_mm` read ([(E,) ceil(In/128), Out rounded up to 128, 4]);
     made once, when the weight is loaded."""
     device = _on_gpu("mxfp4_scale_tiles", scales)
     if scales.dtype != torch.uint8 or scales.dim() not in (2, 3) or in_features != 32 * scales.shape[-1]:
@@ -663,7 +664,7 @@ def mxfp4_scale_tiles(scales: torch.Tensor, in_features: int) -> torch.Tensor:
                           f"{tuple(scales.shape)} {scales.dtype}")
     out_features = scales.shape[-2]
     scales = scales.contiguous()
-    tiles = torch.empty(*scales.shape[:-2], -(-in_features // 128), -(-out_features // 4) * 4, 4, dtype=torch.uint8,
+    tiles = torch.empty(*scales.shape[:-2], -(-in_features // 128), -(-out_features // 128) * 128, 4, dtype=torch.uint8,
                         device=device)
     with _on(device):
         _lib.call("lnq_mxfp4_scale_tiles", _ptr(scales), _ptr(tiles), scales.shape[0] if scales.dim() == 3 else 1,

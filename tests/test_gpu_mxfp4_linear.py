@@ -139,11 +139,13 @@ def test_rows_are_quantize_in_tiles(rows: int, depth: int, dtype: torch.dtype) -
         q, tiles = kernels.mxfp4_rows(x)
         blocks, scales = kernels.mxfp4_quantize(x)
         assert torch.equal(q, blocks.view(rows, depth // 2))
-        padded, units = -(-rows // 4) * 4, -(-depth // 128)
+        padded, units = -(-rows // 128) * 128, -(-depth // 128)
         assert tiles.shape == (units, padded, 4)
         want = torch.zeros(padded, units * 4, dtype=torch.uint8, device=DEV)
         want[:rows, : depth // 32] = scales
-        assert torch.equal(tiles, want.view(padded, units, 4).permute(1, 0, 2))
+        # Row 32 f + l of each 128 at place 4 l + f.
+        want = want.view(padded // 128, 4, 32, units, 4).permute(3, 0, 2, 1, 4).reshape(units, padded, 4)
+        assert torch.equal(tiles, want)
         # A weight's scales, laid out once, hold the same.
         assert torch.equal(kernels.mxfp4_scale_tiles(scales, depth), tiles)
 
@@ -151,7 +153,7 @@ def test_rows_are_quantize_in_tiles(rows: int, depth: int, dtype: torch.dtype) -
 def test_scale_tiles_of_experts() -> None:
     scales = torch.randint(0, 256, (5, 70, 9), dtype=torch.uint8, device=DEV)
     tiles = kernels.mxfp4_scale_tiles(scales, 288)
-    assert tiles.shape == (5, 3, 72, 4)
+    assert tiles.shape == (5, 3, 128, 4)
     for e in range(5):
         assert torch.equal(tiles[e], kernels.mxfp4_scale_tiles(scales[e], 288))
 
@@ -244,10 +246,14 @@ def test_nothing_behind_the_last_row_is_read_into_the_sums_or_written() -> None:
             room[: t.numel()] = t.reshape(-1)
             return room
 
-        row_scales = row_scales.clone()
-        row_scales[:, rows:] = 255
-        tiles = tiles.clone()
-        tiles[:, out:] = 255
+        def spoiled(t: torch.Tensor, live: int) -> torch.Tensor:
+            row = torch.arange(t.shape[1], device=DEV)
+            row = row - row % 128 + row % 4 * 32 + row % 128 // 4  # the row of each place
+            t = t.clone()
+            t[:, row >= live] = 255
+            return t
+
+        row_scales, tiles = spoiled(row_scales, rows), spoiled(tiles, out)
         held = [behind(t) for t in (q, row_scales, blocks, tiles)]
         y = torch.full((rows * out + 4096,), 3.0, dtype=torch.bfloat16, device=DEV)
         _lib.call("lnq_mxfp4_mm", *(t.data_ptr() for t in held), None, y.data_ptr(), rows, out, depth, _lib.BF16,
@@ -358,13 +364,13 @@ def test_refusals() -> None:
         (lambda: kernels.mxfp4_w4a16(x, u8(8, 3, 16), u8(8, 3)), "against"),
         (lambda: kernels.mxfp4_w4a16(x.float(), u8(8, 2, 16), u8(8, 2)), "dtype"),
         (lambda: kernels.mxfp4_w4a16(x, u8(8, 2, 16), u8(8, 2), torch.zeros(8, device=DEV)), "bias"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 3, 16), u8(1, 8, 4), torch.bfloat16), "against"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 8, 4), u8(8, 2, 16), u8(1, 8, 4), torch.bfloat16), "scale tiles"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(2, 8, 4), torch.bfloat16), "scale tiles"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(1, 8, 4), torch.float32), "dtype"),
-        (lambda: kernels.mxfp4_experts_mm(u8(5, 32), u8(1, 8, 4), u8(2, 8, 2, 16), u8(2, 1, 8, 4),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 128, 4), u8(8, 3, 16), u8(1, 128, 4), torch.bfloat16), "against"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 256, 4), u8(8, 2, 16), u8(1, 128, 4), torch.bfloat16), "scale tiles"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 128, 4), u8(8, 2, 16), u8(2, 128, 4), torch.bfloat16), "scale tiles"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 128, 4), u8(8, 2, 16), u8(1, 128, 4), torch.float32), "dtype"),
+        (lambda: kernels.mxfp4_experts_mm(u8(5, 32), u8(1, 128, 4), u8(2, 8, 2, 16), u8(2, 1, 128, 4),
                                           torch.zeros(4, 2, dtype=torch.int64, device=DEV), torch.bfloat16), "against"),
-        (lambda: kernels.mxfp4_experts_mm(u8(4, 32), u8(1, 4, 4), u8(2, 8, 2, 16), u8(2, 1, 8, 4),
+        (lambda: kernels.mxfp4_experts_mm(u8(4, 32), u8(1, 128, 4), u8(2, 8, 2, 16), u8(2, 1, 128, 4),
                                           torch.zeros(4, 2, device=DEV), torch.bfloat16), "integers"),
         (lambda: quantized.mxfp4_operands(u8(2, 8, 2, 16), u8(2, 8, 2), 1), "blocks"),
         (lambda: quantized.mxfp4_experts_operands(u8(8, 2, 16), u8(8, 2), 1), "blocks"),
