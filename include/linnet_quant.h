@@ -485,15 +485,16 @@ LNQ_API LnqStatus lnq_mxfp4_dequantize(const uint8_t* blocks, const uint8_t* sca
 
 /* Rows of activations as lnq_mxfp4_mm reads them: lnq_mxfp4_quantize's rounding of x [rows,
  * in] (rows x_stride elements apart, a multiple of 8), the codes in q [rows, in/2], the scales
- * as scale tiles: [units][padded][4] bytes, unit u holding blocks 4u .. 4u + 3 (128 inputs) of
- * every row, units = ceil(in / 128), padded = rows rounded up to a multiple of 128; row r lies at
- * place (r - r % 128) + 4 (r % 32) + r / 32 % 4 (places of no row and blocks past `in` hold 0).
- * x, q and scales 16-byte aligned. No counterpart in the reference. */
+ * in `scales` [units][rows][4], unit u holding blocks 4u .. 4u + 3 (128 inputs) of every row,
+ * units = ceil(in / 128) (blocks past `in` hold 0). x, q and scales 16-byte aligned. No
+ * counterpart in the reference. */
 LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, uint8_t* scales,
                                  int64_t rows, int64_t in_features, int32_t dtype, void* stream);
 
-/* A weight's scales as stored, [count, out, in/32], as scale tiles (of `out` rows), one after
- * another. Made once, as the weight is loaded. tiles 16-byte aligned. */
+/* A weight's scales as stored, [count, out, in/32], as lnq_mxfp4_mm reads them ("scale tiles"):
+ * [count][ceil(in / 256)][ceil(out / 128)][64][16] bytes, of each 128 outputs by 256 inputs byte
+ * 8 h + 4 u + f of place 16 j + r the scale of output 64 h + 16 f + r at block 4 u + j (0 past
+ * the last output or block). Made once, as the weight is loaded. tiles 16-byte aligned. */
 LNQ_API LnqStatus lnq_mxfp4_scale_tiles(const uint8_t* scales, uint8_t* tiles, int64_t count,
                                         int64_t out_features, int64_t in_features, void* stream);
 

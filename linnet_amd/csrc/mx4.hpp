@@ -1,5 +1,5 @@
-// What the MXFP4 x MXFP4 product's kernels share (mxfp4_mm.hip: small tiles; mxfp4_large.hip:
-// the persistent 256 x 256 form): arguments, the experts' tiles and the loads into LDS.
+// The MXFP4 x MXFP4 product's operands (mxfp4_mm.hip), which mxfp4_round.hip lays out, its
+// arguments and loads.
 #pragma once
 
 #include "eight_bit.hpp"
@@ -12,20 +12,25 @@ constexpr int BK = 2 * BKB;                // inputs a step
 constexpr uint32_t NOWHERE = 0x80000000u;  // an offset past every buffer (each below 2 GiB): reads zeros
 constexpr int MAX_EXPERTS = 2048;          // of the pair lists' LDS
 
-// Scale tiles: a dword holds a row's four scale bytes of a unit (128 inputs); [units][rows
-// rounded up to 128], the rows of each 128 dealt so that the 4 rows 32 apart that a lane of the
-// large tiles meets (l, l + 32, l + 64, l + 96) are 16 bytes together.
-__host__ __device__ inline int padded_rows(int rows) { return (rows + 127) / 128 * 128; }
-__host__ __device__ inline int scale_place(int row) { return (row & ~127) + (row & 31) * 4 + ((row >> 5) & 3); }
+// The MFMA (v_mfma_scale_f32_16x16x128_f8f6f4): lane l holds row l % 16, inputs 32 (l / 16) .. +
+// 31 of 128 (a unit) in 16 bytes, and their scale in a byte, which the instruction selects, of a
+// register. Scales lie so that the registers come as they are:
+// x's, a dword a row and unit (its four blocks), [units][rows]: shifted by 8 (l / 16), byte 0;
+// a weight's ("scale tiles"), [pairs of units][blocks of 128 rows][64 lanes][16 bytes]: lane l's
+// dword 2 h + u of a block holds, for unit u of the pair and half h of the block, the
+// bytes of rows 64 h + 16 f + l % 16 (f = 0 .. 3) at block l / 16 of the unit: four MFMAs' scales.
+__host__ __device__ inline int units_of(int K) { return (K + 127) / 128; }
+__host__ __device__ inline int blocks_of(int N) { return (N + 127) / 128; }
+constexpr int TILE_BYTES = 1024;  // of a scale tile: 128 rows by 256 inputs
 
 struct Args {
   const uint8_t* q;      // x's codes [rows, K / 2]
-  const uint32_t* xs;    // and scale tiles [units][xp]
+  const uint32_t* xs;    // and scales [units][M]
   const uint8_t* w;      // codes [N, K / 2], of each expert
-  const uint32_t* ws;    // scale tiles [units][wp], of each expert
+  const uint8_t* ws;     // scale tiles, of each expert
   const uint16_t* bias;
   uint16_t* y;
-  int M, N, K, xp, wp;
+  int M, N, K;
   // Experts: the pairs by expert, and tiles of them: (expert, first place in `order`, pairs + 512 *
   // tiles of the expert, the expert's first tile); used[0]: the tiles there are.
   const int* order;
@@ -46,13 +51,20 @@ __device__ inline void load4(__amdgpu_buffer_rsrc_t r, uint8_t* to, uint32_t at)
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)to, 4, at, 0, 0, 0);
 }
 
-// The MFMA of two operands of 32 codes a lane; `odd`: their scales are byte 2 of sa and sb, byte 0
-// otherwise.
-__device__ inline f32x16 mma(bool odd, i32x4 a, i32x4 b, f32x16 c, int sa, int sb) {
+// The MFMA of 32 codes a lane of a weight (a, scale byte `f` of sa) and of x (b, byte 0 of sb); f is
+// a constant once inlined, which the instruction holds.
+__device__ inline f32x4 mma(i32x4 a, i32x4 b, f32x4 c, int f, uint32_t sa, uint32_t sb) {
   const i32x8 x = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
   const i32x8 y = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
-  return odd ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 4, 2, sa, 2, sb)
-             : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 4, 0, sa, 0, sb);
+#define LNQ_MX4_MMA(F) \
+  __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, F, static_cast<int>(sa), 0, static_cast<int>(sb))
+  switch (f) {
+    case 0: return LNQ_MX4_MMA(0);
+    case 1: return LNQ_MX4_MMA(1);
+    case 2: return LNQ_MX4_MMA(2);
+    default: return LNQ_MX4_MMA(3);
+  }
+#undef LNQ_MX4_MMA
 }
 
 // The b-th of `total` tiles as the XCDs take them (workgroups go to the 8 in turn): each a run
@@ -63,9 +75,6 @@ __device__ inline int xcd_tile(int b, int total) {
   if (at >= each + (xcd < more ? 1 : 0)) return -1;
   return xcd * each + min(xcd, more) + at;
 }
-
-// mxfp4_large.hip. `experts`: the launch's tiles are of 256 pairs.
-LnqStatus launch_large(const Args& a, bool experts, int dtype, hipStream_t s);
 
 }  // namespace mx4
 }  // namespace lnq

@@ -1,18 +1,26 @@
 // The MXFP4 x MXFP4 product on gfx950's block-scaled MFMA, y = x W^T (+ bias), and the same
 // for the experts of a mixture: the (row, choice) pairs of each expert against its weight.
 //
-// Operands: codes [rows, K / 2] bytes, two E2M1 values each, a row's 32-value blocks in a
-// row; scales as scale tiles (mx4.hpp; mxfp4_round.hip writes both so). The MFMA
-// (v_mfma_scale_f32_32x32x64_f8f6f4, 131072 operations in 32 cycles) takes a lane's 32 codes and
-// their scale byte and adds the exact products of 64 inputs in f32; the sum is rounded once,
-// after the bias.
+// Operands: codes [rows, K / 2] bytes, two E2M1 values each, a row's 32-value blocks in a row;
+// scales laid out for the MFMA (mx4.hpp; mxfp4_round.hip writes both so), which adds the exact
+// products of 128 inputs in f32 (65536 operations in 16 cycles). The sum is rounded once, after
+// the bias. (The 32x32x64 form does as much a cycle, but at the clock that the power allows
+// random codes run at 7.6 PFLOP/s on this one and 5.6 on that, registers alone: it reads and
+// writes half the accumulators.)
 //
-// A workgroup owns BM rows by BN columns, its waves WM x WN of them in 32 x 32 MFMA tiles.
-// 256 inputs (128 bytes a row) a step: codes and scales move to LDS by buffer_load ... lds,
-// S - 1 steps ahead, one barrier a step. The codes' 16-byte columns are XOR-swizzled by bits
-// 1..3 of the row. A lane's scale dword of a row holds the unit's 4 bytes; shifted by 8 (lane
-// / 32) once, bytes 0 and 2 are those of its halves of the unit's two MFMAs, named by the
-// instruction's operand selects.
+// A workgroup owns BM rows by BN columns of y, its waves WM x WN of them, FA x FB MFMA tiles
+// each, and walks its tiles of the launch; the k-steps of all of them form one stream: the loads
+// of step g + 2, the next tile's near a tile's end, are issued while step g multiplies. 256
+// inputs (128 bytes a row) a step: codes and scales move to LDS by buffer_load ... lds, the codes'
+// 16-byte columns XOR-swizzled by bits 1..3 of the row, into two stages. Per step, a region a
+// unit (128 inputs): FA x FB MFMAs on the unit's operands while the next ones are read. One
+// barrier, inside the second: past it every wave's loads of step g + 1 have landed and no wave
+// reads step g's stage again, so the rest reads step g + 1's first operands and issues step g +
+// 2's loads into step g's stage. A tile has an even number of steps (one past K loads nothing and
+// adds zeros), so a step's stage is known at compile time.
+//
+// Experts: tiles of BM pairs of one expert, expert by expert with its tiles of rows together for
+// each run of columns; where the next tiles lie is looked up a tile ahead a lookup.
 #include <algorithm>
 #include <cstdlib>
 
@@ -22,236 +30,340 @@ namespace lnq {
 
 namespace mx4 {
 constexpr int LIST_THREADS = 1024;
-}
 
-template <int DT, int BM, int BN, int WM, int WN, int S, bool EXPERTS>
-__global__ __launch_bounds__(64 * WM * WN, 1) void mx4_kernel(mx4::Args a) {
+template <int WM, int WN, int FA_, int FB_>
+struct Form {
+  static constexpr int FA = FA_, FB = FB_;
+  static constexpr int NW = WM * WN, THREADS = 64 * NW;
+  static constexpr int BM = 16 * FA * WM, BN = 16 * FB * WN;
+  static constexpr int CODES = (BM + BN) * BKB;
+  static constexpr int STAGE = CODES + (BM + BN) * 8;     // then x's scales, 2 units, and the weight's
+  static constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;  // loads of a wave a step: 8 rows of codes each
+  static constexpr int XC = BM / 32, ALL = XC + BN / 32;  // loads of 64 scale dwords: x's, all
+  static constexpr int LS = (ALL + NW - 1) / NW;          // of a wave
+  static constexpr int LOADS = LA + LB + LS;
+  static constexpr int GROUPS = 160 * 1024 / (2 * STAGE);  // workgroups that a CU's LDS holds
+  static constexpr int PER_CU = GROUPS < 4 ? GROUPS : 4;
+  static constexpr int WAVES_A_SIMD = NW * PER_CU / 4 > 0 ? NW * PER_CU / 4 : 1;
+  static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN && NW % 2 == 0, "whole loads, one key a wave");
+  static_assert((FB == 2 || FB == 4) && BN % 64 == 0 && (FA == 2 || FA == 4 || FA == 8), "scales a lane");
+};
+}  // namespace mx4
+
+template <int DT, class FORM, bool EXPERTS>
+__global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(mx4::Args a) {
   using namespace mx4;
   using E = Elem<DT>;
-  constexpr int NW = WM * WN, FA = BM / 32 / WM, FB = BN / 32 / WN;
-  constexpr int CODES = (BM + BN) * BKB, STAGE = CODES + (BM + BN) * 8;
-  constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;      // loads of a wave a step: 8 rows of codes each
-  constexpr int LS = ((BM + BN) / 32 + NW - 1) / NW;     // and of 64 scale dwords each
-  constexpr int LOADS = LA + LB + LS;
-  static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN && BM % 32 == 0 && BN % 32 == 0, "whole loads");
-  static_assert(S >= 2 && S <= 4, "stages");
-  // A stage array each (the compiler tracks loads into LDS by variable).
-  __shared__ __attribute__((aligned(16))) uint8_t S0[STAGE];
-  __shared__ __attribute__((aligned(16))) uint8_t S1[STAGE];
-  __shared__ __attribute__((aligned(16))) uint8_t S2[S > 2 ? STAGE : 16];
-  __shared__ __attribute__((aligned(16))) uint8_t S3[S > 3 ? STAGE : 16];
+  constexpr int FA = FORM::FA, FB = FORM::FB, NW = FORM::NW, BM = FORM::BM, BN = FORM::BN, CODES = FORM::CODES;
+  constexpr int LA = FORM::LA, LB = FORM::LB, LS = FORM::LS, LOADS = FORM::LOADS, XC = FORM::XC;
+  constexpr int WN = BN / 16 / FB;
+  // One array per stage: the compiler then waits, before reading a stage, for that stage's
+  // loads only.
+  __shared__ __attribute__((aligned(16))) uint8_t L0[FORM::STAGE];
+  __shared__ __attribute__((aligned(16))) uint8_t L1[FORM::STAGE];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  const int tiles_n = (a.N + BN - 1) / BN;
-  int m0 = 0, tn, live, first = 0;
-  const uint8_t* w = a.w;
-  const uint32_t* ws = a.ws;
+  const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN;
+  const int total = EXPERTS ? a.used[0] * tiles_n : tiles_m * tiles_n;
+  const int G = gridDim.x, b0 = blockIdx.x;
+  // Tiles b0, b0 + G, .. of the XCDs' order.
+  int mine = 0;
   if constexpr (EXPERTS) {
-    // Expert by expert, its tiles of rows together for each run of columns.
-    const int at = xcd_tile(blockIdx.x, a.used[0] * tiles_n);
-    if (at < 0) return;
-    const i32x4 any = a.table[at / tiles_n];
-    const int many = __builtin_amdgcn_readfirstlane(any.z) >> 9, tile0 = __builtin_amdgcn_readfirstlane(any.w);
-    tn = (at - tile0 * tiles_n) / many;
-    const i32x4 entry = a.table[tile0 + (at - tile0 * tiles_n) % many];
-    const int e = __builtin_amdgcn_readfirstlane(entry.x);
-    first = __builtin_amdgcn_readfirstlane(entry.y);
-    live = __builtin_amdgcn_readfirstlane(entry.z) & 511;
-    const int n0 = tn * BN;
-    if (e >= a.count) {  // pairs whose choice is no expert: zeros
-      const int width = min(BN, a.N - n0);
-      for (int i = threadIdx.x; i < live * width; i += 64 * NW)
-        a.y[static_cast<int64_t>(a.order[first + i / width]) * a.N + n0 + i % width] = 0;
-      return;
-    }
-    w += e * a.w_step;
-    ws += e * a.ws_step;
+    // G is a multiple of the XCDs: a run of an XCD in turn.
+    const int xcd = b0 % mm8::XCDS, run = total / mm8::XCDS + (xcd < total % mm8::XCDS ? 1 : 0);
+    const int at = b0 / mm8::XCDS, every = G / mm8::XCDS;
+    mine = at < run ? (run - 1 - at) / every + 1 : 0;
   } else {
-    const int tiles_m = (a.M + BM - 1) / BM;
-    int tm;
-    mm8_tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
-    if (tm >= tiles_m || tn >= tiles_n) return;
-    m0 = tm * BM;
-    live = min(BM, a.M - m0);
+    mine = b0 < total ? (total - 1 - b0) / G + 1 : 0;
   }
-  const int n0 = tn * BN;
-  const int steps = (a.K + BK - 1) / BK;
+  if (mine == 0) return;
+  const int steps = (a.K + 2 * BK - 1) / (2 * BK) * 2;
+  const int nsteps = mine * steps;
   const uint32_t row_bytes = static_cast<uint32_t>(a.K) >> 1;
-  const int units = (a.K + 127) / 128;
+  const int units = units_of(a.K);
+  const uint32_t pair_bytes = static_cast<uint32_t>(blocks_of(a.N)) * TILE_BYTES;
 
-  // Rows of x by place in the tile: the row, or -1 past the last.
-  auto x_row = [&](int r) -> int {
-    if (r >= live) return -1;
-    if constexpr (EXPERTS) return a.order[first + r] / a.chosen;
-    else return m0 + r;
-  };
-  // Load i of this wave: rows 8 (wave + NW i) .. + 7 of the tile, lane l row l / 8, stored
-  // column l % 8 holding source column (l % 8) ^ key(row), key = bits 1..3 of the row (the
-  // same for every i: NW is even).
-  static_assert(NW % 2 == 0, "one key a wave");
-  const int lrow8 = 8 * wave + (lane >> 3);
-  const uint32_t lcol = static_cast<uint32_t>((lane & 7) ^ ((lrow8 >> 1) & 7)) * 16u;
-  uint32_t aoff_g[LA], boff_g[LB], soff_g[LS];
-#pragma unroll
-  for (int i = 0; i < LA; ++i) {
-    const int r = x_row(lrow8 + 8 * NW * i);
-    aoff_g[i] = r < 0 ? NOWHERE : static_cast<uint32_t>(r - m0) * row_bytes + lcol;
-  }
-#pragma unroll
-  for (int i = 0; i < LB; ++i) {
-    const int n = lrow8 + 8 * NW * i;
-    boff_g[i] = n0 + n < a.N ? static_cast<uint32_t>(n) * row_bytes + lcol : NOWHERE;
-  }
-  // Scale dword d of a stage: rows of x at the step's first unit, its second, columns of W
-  // at the first, the second. Loads past the last repeat it.
-  constexpr int XC = BM / 32, SC = (BM + BN) / 32;  // loads of x's scales, of all
+  // Load i of wave w fills stage rows 8 (NW i + w) .. + 7 (i < LA: rows of x; then columns): lane l
+  // row l / 8 at byte 16 l of the 1 KB, stored column l % 8 holding source column (l % 8) ^
+  // key(row), key = (row >> 1) & 7, the same for every i. Rows past the last lie past the buffer,
+  // or nowhere.
+  const int lr = 8 * wave + (lane >> 3);
+  const uint32_t lcol = 16u * ((lane & 7) ^ ((lr >> 1) & 7));
+  const uint32_t voff = static_cast<uint32_t>(lr) * row_bytes + lcol;  // of load i: 8 NW i rows on
+  uint32_t xoff[EXPERTS ? LA : 1];
+  // Scale dwords, 64 a load: x's rows at the step's first unit, at its second; then each 64
+  // columns' of a scale tile, first unit, second. Loads past the last repeat it.
+  auto scale_load = [&](int i) -> int { return min(wave + NW * i, FORM::ALL - 1); };
+  uint32_t soff[LS];
 #pragma unroll
   for (int i = 0; i < LS; ++i) {
-    const int c = min(wave + NW * i, SC - 1);
-    const bool is_x = c < XC;
-    const int d = is_x ? c * 64 + lane : (c - XC) * 64 + lane;
-    const int rows = is_x ? BM : BN, p = is_x ? a.xp : a.wp;
-    const int unit = d / rows, r = d % rows;
-    const int row = is_x ? x_row(r) : (n0 + r < a.N ? n0 + r : -1);
-    soff_g[i] = row < 0 ? NOWHERE : (static_cast<uint32_t>(unit) * p + scale_place(row)) * 4u;
+    const int c = scale_load(i), d = c * 64 + lane;
+    const int half = (c - XC) / 2, u = (c - XC) & 1;
+    soff[i] = c < XC ? (static_cast<uint32_t>(d / BM) * a.M + d % BM) * 4u
+                     : static_cast<uint32_t>(half >> 1) * TILE_BYTES + lane * 16u + (half & 1) * 8u + u * 4u;
   }
-  const uint8_t* const qb = EXPERTS ? a.q : a.q + static_cast<int64_t>(m0) * row_bytes;
-  const uint32_t q_bytes = EXPERTS ? static_cast<uint32_t>(a.M) * row_bytes : static_cast<uint32_t>(live) * row_bytes;
-  const uint8_t* const wb = w + static_cast<int64_t>(n0) * row_bytes;
-  const uint32_t w_bytes = static_cast<uint32_t>(min(BN, a.N - n0)) * row_bytes;
 
-  // Everything of step ks into stage st; a step past the end through descriptors of no
-  // bytes. Columns past K in the last step, and its second unit where there is none, lie
-  // nowhere.
-  auto load = [&](int ks, uint8_t* st) {
-    const bool in = ks < steps, last = ks == steps - 1;
-    const uint32_t k0 = in ? static_cast<uint32_t>(ks) * BKB : 0u;
-    const __amdgpu_buffer_rsrc_t ra = buffer_rsrc(qb + k0, in ? q_bytes - k0 : 0u);
-    const __amdgpu_buffer_rsrc_t rb = buffer_rsrc(wb + k0, in ? w_bytes - k0 : 0u);
-    const uint32_t past = last && k0 + lcol >= row_bytes ? NOWHERE : 0u;
-#pragma unroll
-    for (int i = 0; i < LA; ++i)
-      load16(ra, st + (wave + NW * i) * 1024, aoff_g[i] | past);
-#pragma unroll
-    for (int i = 0; i < LB; ++i)
-      load16(rb, st + BM * BKB + (wave + NW * i) * 1024, boff_g[i] | past);
-    const uint32_t u0 = in ? static_cast<uint32_t>(ks) * 2u : 0u, left = in ? static_cast<uint32_t>(units) - u0 : 0u;
-#pragma unroll
-    for (int i = 0; i < LS; ++i) {
-      const int c = min(wave + NW * i, SC - 1);
-      const bool is_x = c < XC;
-      const uint32_t p = static_cast<uint32_t>(is_x ? a.xp : a.wp);
-      const uint32_t* const from = (is_x ? a.xs : ws) + static_cast<int64_t>(u0) * p;
-      load4(buffer_rsrc(from, min(left, 2u) * p * 4u), st + CODES + c * 256, soff_g[i]);
-    }
+  // A tile of this launch: columns from n0; rows from m0, or an expert's pairs from `first`.
+  struct Tile {
+    int n0, m0, live, first, e;
   };
-
-  f32x16 acc[FA][FB];
-#pragma unroll
-  for (int i = 0; i < FA; ++i)
-#pragma unroll
-    for (int j = 0; j < FB; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
-
-  const int lrow = lane & 31, lk = lane >> 5;
-  uint32_t aoff[4], boff[4];
-#pragma unroll
-  for (int kk = 0; kk < 4; ++kk) {
-    const uint32_t col = static_cast<uint32_t>(((2 * kk + lk) ^ ((lrow >> 1) & 7)) << 4);
-    aoff[kk] = static_cast<uint32_t>((wm * FA * 32 + lrow) * BKB) + col;
-    boff[kk] = static_cast<uint32_t>(BM * BKB + (wn * FB * 32 + lrow) * BKB) + col;
-  }
-  const uint32_t sa_at = static_cast<uint32_t>(CODES + (wm * FA * 32 + lrow) * 4);
-  const uint32_t sb_at = static_cast<uint32_t>(CODES + BM * 8 + (wn * FB * 32 + lrow) * 4);
-
-  auto step = [&](int ks, const uint8_t* st, uint8_t* next) {
-    // This wave's loads of step ks have landed (those of the S - 2 steps after it may be in
-    // flight); past the barrier every wave's have, and every wave is done with step
-    // ks - 1's stage, which step ks + S - 1 fills.
-    wait_vm<(S - 2) * LOADS>();
-    __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    load(ks + S - 1, next);
-    __builtin_amdgcn_sched_barrier(0);
-    int sa[FA][2], sb[FB][2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int i = 0; i < FA; ++i)
-        sa[i][u] = static_cast<int>(*reinterpret_cast<const uint32_t*>(st + sa_at + u * BM * 4 + i * 128) >> (8 * lk));
-#pragma unroll
-      for (int j = 0; j < FB; ++j)
-        sb[j][u] = static_cast<int>(*reinterpret_cast<const uint32_t*>(st + sb_at + u * BN * 4 + j * 128) >> (8 * lk));
-    }
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      i32x4 af[FA], bf[FB];
-      auto fetch = [&](i32x4& o, uint32_t at) { o = *reinterpret_cast<const i32x4*>(st + at); };
-#pragma unroll
-      for (int i = 0; i < FA; ++i) fetch(af[i], aoff[kk] + i * 32 * BKB);
-#pragma unroll
-      for (int j = 0; j < FB; ++j) fetch(bf[j], boff[kk] + j * 32 * BKB);
-#pragma unroll
-      for (int i = 0; i < FA; ++i)
-#pragma unroll
-        for (int j = 0; j < FB; ++j)
-          // The weight is the MFMA's A operand: a lane then holds 4 outputs of a row together.
-          acc[i][j] = mma(kk & 1, bf[j], af[i], acc[i][j], sb[j][kk >> 1], sa[i][kk >> 1]);
-    }
+  auto plain_tile = [&](int r) -> Tile {
+    int tm, tn;
+    mm8_tile_of(b0 + r * G, tiles_m, tiles_n, tm, tn);
+    return Tile{tn * BN, tm * BM, min(BM, a.M - tm * BM), 0, 0};
   };
-
-  uint8_t* const st[4] = {S0, S1, S2, S3};
+  // The experts' tile r in two lookups: the entry of some tile of its expert, then its own.
+  auto place_of = [&](int r) -> int { return max(xcd_tile(b0 + min(r, mine - 1) * G, total), 0); };
+  auto expert_of = [&](int r) -> i32x4 { return a.table[place_of(r) / tiles_n]; };
+  auto entry_of = [&](int r, i32x4 any, int& n0) -> i32x4 {
+    const int many = __builtin_amdgcn_readfirstlane(any.z) >> 9, tile0 = __builtin_amdgcn_readfirstlane(any.w);
+    const int j = place_of(r) - tile0 * tiles_n;
+    n0 = j / many * BN;
+    return a.table[tile0 + j % many];
+  };
+  auto expert_tile = [&](i32x4 entry, int n0) -> Tile {
+    return Tile{n0, 0, __builtin_amdgcn_readfirstlane(entry.z) & 511, __builtin_amdgcn_readfirstlane(entry.y),
+                __builtin_amdgcn_readfirstlane(entry.x)};
+  };
+  // The pairs whose rows of x this thread loads of an experts' tile: codes, then scales.
+  int pairs[EXPERTS ? LA + LS : 1];
+  auto take_pairs = [&](const Tile& t) {
+    if constexpr (EXPERTS) {
 #pragma unroll
-  for (int j = 0; j < S - 1; ++j) {
-    load(j, st[j]);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  for (int ks = 0; ks < steps; ks += S) {
-#pragma unroll
-    for (int j = 0; j < S; ++j) {
-      if (ks + j >= steps) break;
-      step(ks + j, st[j], st[(j + S - 1) % S]);
-    }
-  }
-  __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-
-  // Lane l, register r of a tile: row m = l % 32, output feature 8 (r / 4) + 4 (l / 32) +
-  // r % 4.
-  const bool vec_out = (a.N & 3) == 0;
-#pragma unroll
-  for (int i = 0; i < FA; ++i) {
-    const int m = (wm * FA + i) * 32 + lrow;
-    if (m >= live) continue;
-    int64_t row;
-    if constexpr (EXPERTS) row = a.order[first + m];
-    else row = m0 + m;
-    uint16_t* const yrow = a.y + row * a.N;
-#pragma unroll
-    for (int j = 0; j < FB; ++j) {
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int n = n0 + (wn * FB + j) * 32 + 8 * q4 + 4 * lk;
-        uint16_t out[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float v = acc[i][j][4 * q4 + r];
-          if (!EXPERTS && a.bias != nullptr) v += n + r < a.N ? E::to_f32(a.bias[n + r]) : 0.f;
-          out[r] = E::from_f32(v);
-        }
-        if (vec_out && n + 3 < a.N) {
-          *reinterpret_cast<u32x2*>(yrow + n) =
-              u32x2{static_cast<uint32_t>(out[0]) | (static_cast<uint32_t>(out[1]) << 16),
-                    static_cast<uint32_t>(out[2]) | (static_cast<uint32_t>(out[3]) << 16)};
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n + r < a.N) yrow[n + r] = out[r];
-        }
+      for (int i = 0; i < LA + LS; ++i) {
+        const int r = i < LA ? lr + 8 * NW * i : (min(scale_load(i - LA), XC - 1) * 64 + lane) % BM;
+        pairs[i] = a.order[t.first + min(r, t.live - 1)];
       }
     }
+  };
+
+  // The tile whose steps are being loaded. Of each scale load its base, what a step adds to it, and
+  // the bytes of a step, of a step of one unit. (Chosen here: a choice in the steps would be a branch,
+  // and the compiler then moves the MFMAs across the blocks it splits the step into.)
+  const uint8_t *qb, *wb, *sb[LS];
+  uint32_t q_bytes, w_bytes, s_step[LS], s_two[LS], s_one[LS];
+  auto load_tile = [&](const Tile& t) {
+    const int e = EXPERTS ? min(t.e, a.count - 1) : 0;  // a tile of no expert multiplies the last one's weight, for nothing
+    qb = a.q + static_cast<int64_t>(t.m0) * row_bytes;
+    q_bytes = static_cast<uint32_t>(EXPERTS ? a.M : t.live) * row_bytes;
+    wb = a.w + e * a.w_step + static_cast<int64_t>(t.n0) * row_bytes;
+    w_bytes = static_cast<uint32_t>(min(BN, a.N - t.n0)) * row_bytes;
+    const uint32_t s_rows = static_cast<uint32_t>(EXPERTS ? a.M : t.live);
+    const uint32_t column = static_cast<uint32_t>(t.n0 / 128) * TILE_BYTES + (t.n0 & 64) / 8;
+#pragma unroll
+    for (int i = 0; i < LS; ++i) {
+      const bool x = scale_load(i) < XC;
+      sb[i] = x ? reinterpret_cast<const uint8_t*>(a.xs + t.m0) : a.ws + e * a.ws_step + column;
+      s_step[i] = x ? static_cast<uint32_t>(a.M) * 8u : pair_bytes;
+      s_two[i] = x ? (static_cast<uint32_t>(a.M) + s_rows) * 4u : pair_bytes - column;
+      s_one[i] = x ? s_rows * 4u : pair_bytes - column;
+    }
+    if constexpr (EXPERTS) {
+#pragma unroll
+      for (int i = 0; i < LA; ++i)
+        xoff[i] = lr + 8 * NW * i < t.live ? static_cast<uint32_t>(pairs[i] / a.chosen) * row_bytes + lcol : NOWHERE;
+#pragma unroll
+      for (int i = 0; i < LS; ++i) {
+        const int c = scale_load(i), d = c * 64 + lane;
+        if (c < XC)
+          soff[i] = d % BM < t.live
+                        ? (static_cast<uint32_t>(d / BM) * a.M + static_cast<uint32_t>(pairs[LA + i] / a.chosen)) * 4u
+                        : NOWHERE;
+      }
+    }
+  };
+  // Load i of k-step ks into stage st. Steps past the stream, and columns and units past K, read
+  // through 0-byte descriptors or past the buffer.
+  auto load_one = [&](uint8_t* st, bool in, int ks, int i) __attribute__((always_inline)) {
+    const uint32_t k0 = static_cast<uint32_t>(ks) * BKB;
+    const bool live = in && k0 < row_bytes;
+    if (i < LA + LB) {
+      const bool x = i < LA;
+      const uint32_t past = k0 + lcol >= row_bytes ? NOWHERE : 0u;
+      const uint32_t at = EXPERTS && x ? xoff[EXPERTS && x ? i : 0] : voff + static_cast<uint32_t>(8 * NW * (x ? i : i - LA)) * row_bytes;
+      load16(buffer_rsrc((x ? qb : wb) + k0, live ? (x ? q_bytes : w_bytes) - k0 : 0u), st + (NW * i + wave) * 1024, at | past);
+    } else {
+      const int l = i - LA - LB;
+      const uint32_t bytes = units - 2 * ks >= 2 ? s_two[l] : s_one[l];
+      load4(buffer_rsrc(sb[l] + static_cast<uint64_t>(static_cast<uint32_t>(ks)) * s_step[l], live ? bytes : 0u),
+            st + CODES + scale_load(l) * 256, soff[l]);
+    }
+  };
+
+  f32x4 acc[FA][FB];
+
+  const int lrow = lane & 15, lk = lane >> 4;
+  uint32_t aoff[2], boff[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    aoff[u] = static_cast<uint32_t>(swz8(wm * FA * 16 + lrow, 4 * u + lk));
+    boff[u] = static_cast<uint32_t>(swz8(BM + wn * FB * 16 + lrow, 4 * u + lk));
   }
+  const uint32_t sa_at = static_cast<uint32_t>(CODES + (wm * FA * 16 + lrow) * 4);
+  const uint32_t sw_at = static_cast<uint32_t>(CODES + BM * 8 + wn * FB * 16 / 64 * 512 + lane * 4);
+  const int first_byte = wn * FB % 4;  // of this wave's columns in their dword
+
+  // Operands: the columns' of a unit, a set a unit; the rows' and their scale dwords in a ring of
+  // 4, read three rows of MFMAs ahead (a wave of two rows: a set a unit too).
+  constexpr bool RING = FA >= 4;
+  i32x4 af[4], bf[2][FB];
+  uint32_t sa[4], sw[2];
+  auto read_a = [&](int u, const uint8_t* st, int f) __attribute__((always_inline)) {
+    af[(RING ? 0 : 2 * u) + (f & 3)] = *reinterpret_cast<const i32x4*>(st + aoff[u] + f * 16 * BKB);
+    sa[(RING ? 0 : 2 * u) + (f & 3)] = *reinterpret_cast<const uint32_t*>(st + sa_at + u * BM * 4 + f * 64);
+  };
+  auto read_b = [&](int u, const uint8_t* st, int f) __attribute__((always_inline)) {
+    bf[u][f] = *reinterpret_cast<const i32x4*>(st + boff[u] + f * 16 * BKB);
+  };
+
+  // Unit u of a step on stage `cur`, a slot an MFMA: a row's first slot reads the rows ahead, others
+  // the next unit's columns. In the second unit, from row TURN on, those are the next step's, from
+  // `nxt`, and the slots issue step g + 2's loads (k-step ks2, `in` whether inside the stream) into
+  // `cur`: ahead of that row this wave's loads of step g + 1 have landed and its reads of `cur`,
+  // all of whose operands it has read, are done; past the barrier every wave's.
+  constexpr int SLOTS = FA * FB, TURN = RING ? FA - 3 : 0;
+  auto region = [&](auto unit_tag, auto first_tag, const uint8_t* cur, const uint8_t* nxt, bool in,
+                    int ks2) __attribute__((always_inline)) {
+    constexpr int U = decltype(unit_tag)::value;
+    constexpr bool FIRST = decltype(first_tag)::value;  // a tile's first step
+    constexpr int AT = RING ? 0 : 2 * U, FROM = U == 1 ? TURN * FB : 0;
+    if constexpr (FB == 2) sw[U] >>= 8 * first_byte;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const int i = s / FB, j = s % FB;
+      if (U == 1 && s == FROM) {
+        wait_vm<0>();
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const f32x4 c = FIRST && U == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][j];
+      if (j == 0) sa[AT + (i & 3)] >>= 8 * lk;  // this lane's block of the unit
+      // The weight is the MFMA's A operand: a lane then holds 4 outputs of a row together.
+      acc[i][j] = mma(bf[U][j], af[AT + (i & 3)], c, j, sw[U], sa[AT + (i & 3)]);
+      if (j == 0) {
+        if (!RING) read_a(U ^ 1, nxt, i);
+        else if (i + 3 < FA) read_a(U, cur, i + 3);
+        else read_a(U ^ 1, nxt, i + 3 - FA);
+      }
+#pragma unroll
+      for (int f = 0; f < FB; ++f)
+        if (s == FROM + 1 + 2 * f) read_b(U ^ 1, nxt, f);
+      if (s == FROM + 2) sw[U ^ 1] = *reinterpret_cast<const uint32_t*>(nxt + sw_at + (U ^ 1) * 256);
+      if (U == 1 && s >= FROM) {
+#pragma unroll
+        for (int q = 0; q < LOADS; ++q)
+          if (FROM + q * (SLOTS - FROM) / LOADS == s) load_one(const_cast<uint8_t*>(cur), in, ks2, q);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  using Zero = std::integral_constant<int, 0>;
+  using One = std::integral_constant<int, 1>;
+  using T = std::integral_constant<bool, true>;
+  using No = std::integral_constant<bool, false>;
+  auto step = [&](auto first_tag, const uint8_t* cur, const uint8_t* nxt, bool in, int ks2) __attribute__((always_inline)) {
+    region(Zero{}, first_tag, cur, cur, false, 0);
+    region(One{}, first_tag, cur, nxt, in, ks2);
+  };
+
+  // Lane l, register r of fragment (i, j): row 16 i + l % 16 of the wave's, column 16 j + 4 (l / 16)
+  // + r.
+  const bool vec_out = (a.N & 3) == 0;
+  auto epilogue = [&](const Tile& t) {
+    const bool none = EXPERTS && t.e >= a.count;  // pairs whose choice is no expert: zeros
+#pragma unroll
+    for (int j = 0; j < FB; ++j) {
+      const int n = t.n0 + (wn * FB + j) * 16 + 4 * lk;
+      float b[4] = {0.f, 0.f, 0.f, 0.f};
+      if (!EXPERTS && a.bias != nullptr) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) b[r] = n + r < a.N ? E::to_f32(a.bias[n + r]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < FA; ++i) {
+        const int m = (wm * FA + i) * 16 + lrow;
+        int64_t row;
+        if constexpr (EXPERTS) row = a.order[t.first + min(m, t.live - 1)];
+        else row = t.m0 + m;
+        uint32_t o[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = none ? 0u : E::from_f32(acc[i][j][r] + b[r]);
+        if (m < t.live) {
+          uint16_t* const to = a.y + row * a.N + n;
+          if (vec_out) {
+            if (n < a.N) *reinterpret_cast<u32x2*>(to) = u32x2{o[0] | (o[1] << 16), o[2] | (o[3] << 16)};
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (n + r < a.N) to[r] = static_cast<uint16_t>(o[r]);
+          }
+        }
+        // One fragment at a time: the next tile's operands are live here.
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+
+  // Prologue: tiles 0 .. 2 looked up; steps 0 and 1 requested; step 0 landed (this wave's, then
+  // every wave's); its first operands and scales read.
+  Tile now, next;
+  i32x4 ahead = {0, 0, 0, 0}, ahead2 = {0, 0, 0, 0};
+  int ahead_n0 = 0;
+  if constexpr (EXPERTS) {
+    int n0;
+    const i32x4 entry = entry_of(0, expert_of(0), n0);
+    now = expert_tile(entry, n0);
+    ahead = entry_of(1, expert_of(1), ahead_n0);
+    ahead2 = expert_of(2);
+  } else {
+    now = plain_tile(0);
+  }
+  take_pairs(now);
+  load_tile(now);
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) load_one(L0, true, 0, i);
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) load_one(L1, true, 1, i);
+  wait_vm<0>();
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int i = 0; i < FB; ++i) read_b(0, L0, i);
+#pragma unroll
+  for (int i = 0; i < (RING ? 3 : 2); ++i) read_a(0, L0, i);
+  sw[0] = *reinterpret_cast<const uint32_t*>(L0 + sw_at);
+
+  // Pairs of steps g, g + 1 of a tile at k-step ks on stages L0, L1: they issue steps g + 2, g +
+  // 3, the next pair's (this tile's, or the next one's after its last), with no branch inside.
+  auto pair = [&](int g, int ks, auto first_tag) __attribute__((always_inline)) {
+    const bool ends = ks + 2 == steps;
+    const int ks_n = ends ? 0 : ks + 2;
+    if (ends) load_tile(next);
+    step(first_tag, L0, L1, g + 2 < nsteps, ks_n);
+    step(No{}, L1, L0, g + 3 < nsteps, ks_n + 1);
+  };
+  int g = 0;
+  for (int r = 0; r < mine; ++r) {
+    // Tile r + 1 from what the last tile looked up; its pairs, the entry of r + 2 and the expert of
+    // r + 3 asked for: none is used before this tile's last steps.
+    if constexpr (EXPERTS) {
+      next = expert_tile(ahead, ahead_n0);
+      ahead = entry_of(r + 2, ahead2, ahead_n0);
+      ahead2 = expert_of(r + 3);
+    } else {
+      next = plain_tile(min(r + 1, mine - 1));
+    }
+    take_pairs(next);
+    pair(g, 0, T{});
+    g += 2;
+    for (int ks = 2; ks < steps; ks += 2, g += 2) pair(g, ks, No{});
+    epilogue(now);
+    now = next;
+  }
+  // Loads of the steps past the stream (0-byte reads) may be in flight.
+  wait_vm<0>();
 }
 
 // The pairs of each expert, in order: workgroup e counts every expert's pairs, which tells it
@@ -317,21 +429,32 @@ __global__ __launch_bounds__(mx4::LIST_THREADS) void expert_lists_kernel(const i
 
 namespace mx4 {
 
-template <int DT, int BM, int BN, int WM, int WN, int S, bool EXPERTS>
-static void launch_one(const Args& a, hipStream_t s) {
-  const int64_t tiles_n = (a.N + BN - 1) / BN;
-  const int64_t grid = tiles_n * (EXPERTS ? a.tiles : (a.M + BM - 1) / BM);
-  hipLaunchKernelGGL((mx4_kernel<DT, BM, BN, WM, WN, S, EXPERTS>), dim3(static_cast<unsigned>(grid)), dim3(64 * WM * WN), 0, s, a);
+template <int DT, class FORM, bool EXPERTS>
+static void launch_form(const Args& a, hipStream_t s) {
+  const int64_t tiles_n = (a.N + FORM::BN - 1) / FORM::BN;
+  const int64_t tiles = EXPERTS ? (a.tiles * tiles_n + mm8::XCDS - 1) / mm8::XCDS * mm8::XCDS
+                                : (a.M + FORM::BM - 1) / FORM::BM * tiles_n;
+  const int64_t most = compute_units() / mm8::XCDS * mm8::XCDS * FORM::PER_CU;
+  hipLaunchKernelGGL((mx4_kernel<DT, FORM, EXPERTS>), dim3(static_cast<unsigned>(tiles < most ? tiles : most)),
+                     dim3(FORM::THREADS), 0, s, a);
 }
 
+using Form256 = Form<2, 4, 8, 4>;
+using Form128 = Form<2, 2, 4, 4>;
+using Form64 = Form<2, 2, 2, 2>;
+using Form32 = Form<1, 2, 2, 2>;
+
 // Rows of a tile.
-static int tile_rows(double rows) { return rows > 64 ? 128 : rows > 32 ? 64 : 32; }
+static int tile_rows(double rows) { 
+  if (const char* t = getenv("MXT")) return atoi(t);
+  return rows > 64 ? 128 : rows > 32 ? 64 : 32; }
 
 template <int DT, bool EXPERTS>
 static void launch(const Args& a, int bm, hipStream_t s) {
-  if (bm == 32) launch_one<DT, 32, 64, 1, 2, 4, EXPERTS>(a, s);
-  else if (bm == 64) launch_one<DT, 64, 64, 2, 2, 4, EXPERTS>(a, s);
-  else launch_one<DT, 128, 128, 2, 2, 2, EXPERTS>(a, s);
+  if (bm == 32) launch_form<DT, Form32, EXPERTS>(a, s);
+  else if (bm == 64) launch_form<DT, Form64, EXPERTS>(a, s);
+  else if (bm == 128) launch_form<DT, Form128, EXPERTS>(a, s);
+  else launch_form<DT, Form256, EXPERTS>(a, s);
 }
 
 struct Plan {
@@ -377,17 +500,14 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
   a.q = q;
   a.xs = reinterpret_cast<const uint32_t*>(x_scale);
   a.w = blocks;
-  a.ws = reinterpret_cast<const uint32_t*>(tiles);
+  a.ws = tiles;
   a.bias = static_cast<const uint16_t*>(bias);
   a.y = static_cast<uint16_t*>(y);
   a.M = static_cast<int>(rows);
   a.N = static_cast<int>(out_features);
   a.K = static_cast<int>(in_features);
-  a.xp = mx4::padded_rows(a.M);
-  a.wp = mx4::padded_rows(a.N);
   LNQ_REQUIRE((rows + 31) / 32 * ((out_features + 63) / 64) <= INT32_MAX, "lnq_mxfp4_mm: too large");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (getenv("MXL")) return mx4::launch_large(a, false, dtype, s);
   const int bm = mx4::tile_rows(static_cast<double>(rows));
   if (dtype == LNQ_BF16) mx4::launch<LNQ_BF16, false>(a, bm, s);
   else mx4::launch<LNQ_F16, false>(a, bm, s);
@@ -434,13 +554,11 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   a.q = q;
   a.xs = reinterpret_cast<const uint32_t*>(x_scale);
   a.w = blocks;
-  a.ws = reinterpret_cast<const uint32_t*>(tiles);
+  a.ws = tiles;
   a.y = static_cast<uint16_t*>(y);
   a.M = static_cast<int>(x_rows);
   a.N = static_cast<int>(out_features);
   a.K = static_cast<int>(in_features);
-  a.xp = mx4::padded_rows(a.M);
-  a.wp = mx4::padded_rows(a.N);
   LNQ_REQUIRE(static_cast<int64_t>(plan.tiles) * ((out_features + 63) / 64) <= INT32_MAX,
               "lnq_mxfp4_experts_mm: too large");
   a.order = static_cast<const int*>(workspace);
@@ -450,7 +568,7 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   a.count = static_cast<int>(num_experts);
   a.chosen = shared ? static_cast<int>(chosen) : 1;
   a.w_step = out_features * (in_features / 2);
-  a.ws_step = (in_features + 127) / 128 * a.wp;
+  a.ws_step = static_cast<int64_t>(mx4::units_of(a.K) + 1) / 2 * mx4::blocks_of(a.N) * mx4::TILE_BYTES;
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(expert_lists_kernel, dim3(a.count + 1), dim3(mx4::LIST_THREADS), 0, s, experts, static_cast<int>(pairs),
                      a.count, plan.bm, const_cast<int*>(a.order), const_cast<i32x4*>(a.table), const_cast<int*>(a.used));

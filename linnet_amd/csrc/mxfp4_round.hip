@@ -17,7 +17,7 @@ namespace lnq {
 
 namespace mxr {
 constexpr int THREADS = 256;
-constexpr int ROWS = 128;  // rows of a workgroup of the row-rounding kernel: a whole scale tile
+constexpr int ROWS = 128;  // rows of a workgroup of the row-rounding kernel
 constexpr int UNIT = 128;  // by the inputs of a unit
 
 // 8 values as loaded.
@@ -103,14 +103,13 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_quantize_kernel(const type
   if ((threadIdx.x & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(byte);
 }
 
-// Rows for the product: codes [rows, K / 2] as above, scales as scale tiles (mx4.hpp). A
-// workgroup takes 128 rows by 128 inputs, 16 lanes a row, so that its scales, whose places
-// lie strewn, leave as 512 bytes in a run.
+// Rows for the product: codes [rows, K / 2] as above, scales [units][rows] dwords of four
+// blocks (128 inputs). A workgroup takes 128 rows by 128 inputs, 16 lanes a row, so that its
+// scales leave as 512 bytes in a run.
 template <int DT>
 __global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename Elem<DT>::storage* __restrict__ x,
                                                                   int64_t x_stride, uint32_t* __restrict__ codes,
-                                                                  uint32_t* __restrict__ scales, int rows, int padded,
-                                                                  int K) {
+                                                                  uint32_t* __restrict__ scales, int rows, int K) {
   using namespace mxr;
   constexpr int A_PASS = THREADS / 16;  // rows
   __shared__ uint32_t unit[ROWS];
@@ -130,10 +129,11 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename
     uint32_t word = byte << (8 * ((lane >> 2) & 3));
     word |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(word), 4, 64));
     word |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(word), 8, 64));
-    if ((lane & 15) == 0) unit[mx4::scale_place(r)] = word;
+    if ((lane & 15) == 0) unit[r] = word;
   }
   __syncthreads();
-  if (threadIdx.x < ROWS) scales[static_cast<int64_t>(blockIdx.y) * padded + r0 + threadIdx.x] = unit[threadIdx.x];
+  if (threadIdx.x < ROWS && r0 + static_cast<int>(threadIdx.x) < rows)
+    scales[static_cast<int64_t>(blockIdx.y) * rows + r0 + threadIdx.x] = unit[threadIdx.x];
 }
 
 template <int DT>
@@ -161,21 +161,20 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_dequantize_kernel(const ui
   }
 }
 
-// Scales as stored, [count, N, groups], as scale tiles.
+// Scales as stored, [count, N, groups], as scale tiles (mx4.hpp), a workgroup a tile.
 __global__ __launch_bounds__(mxr::THREADS) void mxfp4_scale_tiles_kernel(const uint8_t* __restrict__ scales,
-                                                                         uint32_t* __restrict__ tiles, int N, int padded,
-                                                                         int groups, int units) {
-  const int n = blockIdx.x * mxr::THREADS + threadIdx.x;
-  if (n >= padded) return;
-  const int u = blockIdx.y, e = blockIdx.z;
+                                                                         uint32_t* __restrict__ tiles, int N, int groups) {
+  const int lane = threadIdx.x >> 2, h = (threadIdx.x >> 1) & 1, u = threadIdx.x & 1;
+  const int g = (2 * blockIdx.y + u) * 4 + (lane >> 4);
   uint32_t word = 0;
-  if (n < N) {
-    const uint8_t* from = scales + (static_cast<int64_t>(e) * N + n) * groups + 4 * u;
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
-      if (4 * u + b < groups) word |= static_cast<uint32_t>(from[b]) << (8 * b);
+  for (int f = 0; f < 4; ++f) {
+    const int n = blockIdx.x * 128 + 64 * h + 16 * f + (lane & 15);
+    if (n < N && g < groups)
+      word |= static_cast<uint32_t>(scales[(static_cast<int64_t>(blockIdx.z) * N + n) * groups + g]) << (8 * f);
   }
-  tiles[(static_cast<int64_t>(e) * units + u) * padded + mx4::scale_place(n)] = word;
+  const int64_t tile = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+  tiles[tile * (mx4::TILE_BYTES / 4) + threadIdx.x] = word;
 }
 
 }  // namespace lnq
@@ -253,11 +252,11 @@ LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, ui
   const dim3 grid(static_cast<unsigned>((rows + mxr::ROWS - 1) / mxr::ROWS),
                   static_cast<unsigned>((in_features + mxr::UNIT - 1) / mxr::UNIT));
   LNQ_REQUIRE(grid.y <= 65535, "lnq_mxfp4_rows: in too large");
-  const int R = static_cast<int>(rows), P = mx4::padded_rows(R), K = static_cast<int>(in_features);
+  const int R = static_cast<int>(rows), K = static_cast<int>(in_features);
 #define LNQ_MXW(DT)                                                                                                     \
   hipLaunchKernelGGL((mxfp4_rows_kernel<DT>), grid, dim3(mxr::THREADS), 0, static_cast<hipStream_t>(stream),            \
                      static_cast<const typename Elem<DT>::storage*>(x), x_stride, reinterpret_cast<uint32_t*>(q),       \
-                     reinterpret_cast<uint32_t*>(scales), R, P, K)
+                     reinterpret_cast<uint32_t*>(scales), R, K)
   if (dtype == LNQ_BF16) LNQ_MXW(LNQ_BF16);
   else if (dtype == LNQ_F16) LNQ_MXW(LNQ_F16);
   else LNQ_MXW(LNQ_F32);
@@ -276,13 +275,12 @@ LNQ_API LnqStatus lnq_mxfp4_scale_tiles(const uint8_t* scales, uint8_t* tiles, i
   }
   LNQ_REQUIRE(scales && tiles, "lnq_mxfp4_scale_tiles: null pointer");
   LNQ_REQUIRE(aligned(tiles, 16), "lnq_mxfp4_scale_tiles: tiles must be 16-byte aligned");
-  LNQ_REQUIRE(count <= 65535 && in_features <= 128 * 65535 && out_features <= INT32_MAX - 128, "lnq_mxfp4_scale_tiles: too large");
-  const int N = static_cast<int>(out_features), padded = mx4::padded_rows(N), groups = static_cast<int>(in_features / 32);
-  const int units = (groups + 3) / 4;
-  const dim3 grid(static_cast<unsigned>((padded + mxr::THREADS - 1) / mxr::THREADS), static_cast<unsigned>(units),
+  LNQ_REQUIRE(count <= 65535 && in_features <= 256 * 65535 && out_features <= INT32_MAX - 128, "lnq_mxfp4_scale_tiles: too large");
+  const int N = static_cast<int>(out_features), K = static_cast<int>(in_features);
+  const dim3 grid(static_cast<unsigned>(mx4::blocks_of(N)), static_cast<unsigned>((mx4::units_of(K) + 1) / 2),
                   static_cast<unsigned>(count));
   hipLaunchKernelGGL(mxfp4_scale_tiles_kernel, grid, dim3(mxr::THREADS), 0, static_cast<hipStream_t>(stream), scales,
-                     reinterpret_cast<uint32_t*>(tiles), N, padded, groups, units);
+                     reinterpret_cast<uint32_t*>(tiles), N, K / 32);
   return launched("mxfp4_scale_tiles");
 }
 

@@ -588,8 +588,18 @@ def _mxfp4_operands(what: str, blocks: torch.Tensor, scales: torch.Tensor) -> in
     return blocks.shape[-2] * 32
 
 
-def _mxfp4_tiles(what: str, tiles: torch.Tensor, lead: tuple[int, ...], rows: int, in_features: int) -> None:
-    shape = (*lead, -(-in_features // 128), -(-rows // 128) * 128, 4)
+def _mxfp4_row_scales(what: str, scales: torch.Tensor, rows: int, in_features: int) -> None:
+    shape = (-(-in_features // 128), rows, 4)
+    if scales.dtype != torch.uint8 or tuple(scales.shape) != shape:
+        raise LinnetError(f"{what}: the rows' scales are {list(shape)} uint8, got {list(scales.shape)} {scales.dtype}")
+
+
+def _mxfp4_tile_shape(lead: tuple[int, ...], out_features: int, in_features: int) -> tuple[int, ...]:
+    return (*lead, -(-in_features // 256), -(-out_features // 128), 64, 16)
+
+
+def _mxfp4_tiles(what: str, tiles: torch.Tensor, lead: tuple[int, ...], out_features: int, in_features: int) -> None:
+    shape = _mxfp4_tile_shape(lead, out_features, in_features)
     if tiles.dtype != torch.uint8 or tuple(tiles.shape) != shape:
         raise LinnetError(f"{what}: scale tiles are {list(shape)} uint8, got {list(tiles.shape)} {tiles.dtype}")
 
@@ -637,9 +647,8 @@ def mxfp4_dequantize(blocks: torch.Tensor, scales: torch.Tensor, dtype: torch.dt
 
 def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Each row of `x` [rows, In] (bf16, f16 or f32) rounded to MXFP4 as `mxfp4_quantize` does, laid
-    out for `mxfp4_mm`: `(q [rows, In/2] u8, scales [ceil(In/128), rows rounded up to 128, 4] u8)`, a
-    row's four scales of 128 inputs together, the rows of each 128 in the order 0, 32, 64, 96, 1,
-    33, ... ("scale tiles")."""
+    out for `mxfp4_mm`: `(q [rows, In/2] u8, scales [ceil(In/128), rows, 4] u8)`, a row's four scales
+    of 128 inputs together."""
     device = _on_gpu("mxfp4_rows", x)
     if x.dim() != 2 or x.shape[1] % 32:
         raise LinnetError(f"mxfp4_rows: x is [rows, In] with In % 32 == 0, got {tuple(x.shape)}")
@@ -648,7 +657,7 @@ def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
         x = _aligned(x)
     q = torch.empty(rows, depth // 2, dtype=torch.uint8, device=device)
-    scales = torch.empty(-(-depth // 128), -(-rows // 128) * 128, 4, dtype=torch.uint8, device=device)
+    scales = torch.empty(-(-depth // 128), rows, 4, dtype=torch.uint8, device=device)
     with _on(device):
         _lib.call("lnq_mxfp4_rows", _ptr(x), x.stride(0), _ptr(q), _ptr(scales), rows, depth, code, _stream(device))
     return q, scales
@@ -656,7 +665,7 @@ def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def mxfp4_scale_tiles(scales: torch.Tensor, in_features: int) -> torch.Tensor:
     """A weight's scales as stored ([Out, In/32], or [E, Out, In/32] for experts) as the scale tiles
-    that `mxfp4_mm` / `mxfp4_experts_mm` read ([(E,) ceil(In/128), Out rounded up to 128, 4]);
+    that `mxfp4_mm` / `mxfp4_experts_mm` read ([(E,) ceil(In/256), ceil(Out/128), 64, 16]);
     made once, when the weight is loaded."""
     device = _on_gpu("mxfp4_scale_tiles", scales)
     if scales.dtype != torch.uint8 or scales.dim() not in (2, 3) or in_features != 32 * scales.shape[-1]:
@@ -664,8 +673,7 @@ def mxfp4_scale_tiles(scales: torch.Tensor, in_features: int) -> torch.Tensor:
                           f"{tuple(scales.shape)} {scales.dtype}")
     out_features = scales.shape[-2]
     scales = scales.contiguous()
-    tiles = torch.empty(*scales.shape[:-2], -(-in_features // 128), -(-out_features // 128) * 128, 4, dtype=torch.uint8,
-                        device=device)
+    tiles = torch.empty(_mxfp4_tile_shape(tuple(scales.shape[:-2]), out_features, in_features), dtype=torch.uint8, device=device)
     with _on(device):
         _lib.call("lnq_mxfp4_scale_tiles", _ptr(scales), _ptr(tiles), scales.shape[0] if scales.dim() == 3 else 1,
                   out_features, in_features, _stream(device))
@@ -713,7 +721,7 @@ def mxfp4_mm(q: torch.Tensor, x_scale: torch.Tensor, blocks: torch.Tensor, tiles
     rows = q.shape[0]
     if q.shape[1] * 2 != depth:
         raise LinnetError(f"mxfp4_mm: q {tuple(q.shape)} against blocks {tuple(blocks.shape)}")
-    _mxfp4_tiles("mxfp4_mm", x_scale, (), rows, depth)
+    _mxfp4_row_scales("mxfp4_mm", x_scale, rows, depth)
     _mxfp4_tiles("mxfp4_mm", tiles, (), out_features, depth)
     code = _code(dtype, "mxfp4_mm")
     bias = _mxfp4_bias("mxfp4_mm", bias, dtype, out_features)
@@ -745,7 +753,7 @@ def mxfp4_experts_mm(q: torch.Tensor, x_scale: torch.Tensor, blocks: torch.Tenso
     if q.shape[0] not in (rows, rows * chosen) or q.shape[1] != groups * 16:
         raise LinnetError(f"mxfp4_experts_mm: q {tuple(q.shape)} against experts {tuple(experts.shape)} and blocks "
                           f"{tuple(blocks.shape)}")
-    _mxfp4_tiles("mxfp4_experts_mm", x_scale, (), q.shape[0], groups * 32)
+    _mxfp4_row_scales("mxfp4_experts_mm", x_scale, q.shape[0], groups * 32)
     _mxfp4_tiles("mxfp4_experts_mm", tiles, (count,), out_features, groups * 32)
     code = _code(dtype, "mxfp4_experts_mm")
     q, x_scale, blocks, tiles = _aligned(q), _aligned(x_scale), _aligned(blocks), _aligned(tiles)

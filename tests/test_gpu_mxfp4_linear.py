@@ -132,30 +132,30 @@ def test_dequantize_every_code_and_scale(dtype: torch.dtype) -> None:
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize(("rows", "depth"), [(1, 32), (2, 96), (4, 128), (33, 2880), (64, 544), (131, 512), (3, 4128), (0, 64)])
-def test_rows_are_quantize_in_tiles(rows: int, depth: int, dtype: torch.dtype) -> None:
+def test_rows_are_quantize_laid_out(rows: int, depth: int, dtype: torch.dtype) -> None:
     print(f"rows {rows} x {depth} {dtype}", flush=True)
     wide = torch.from_numpy(_values(np.random.default_rng(rows + depth), rows, depth + 32)).to(dtype).to(DEV)
     for x in (wide[:, 32:], wide[:, :depth].contiguous()):  # strided rows, packed ones
-        q, tiles = kernels.mxfp4_rows(x)
+        q, row_scales = kernels.mxfp4_rows(x)
         blocks, scales = kernels.mxfp4_quantize(x)
         assert torch.equal(q, blocks.view(rows, depth // 2))
-        padded, units = -(-rows // 128) * 128, -(-depth // 128)
-        assert tiles.shape == (units, padded, 4)
-        want = torch.zeros(padded, units * 4, dtype=torch.uint8, device=DEV)
-        want[:rows, : depth // 32] = scales
-        # Row 32 f + l of each 128 at place 4 l + f.
-        want = want.view(padded // 128, 4, 32, units, 4).permute(3, 0, 2, 1, 4).reshape(units, padded, 4)
-        assert torch.equal(tiles, want)
-        # A weight's scales, laid out once, hold the same.
-        assert torch.equal(kernels.mxfp4_scale_tiles(scales, depth), tiles)
+        units = -(-depth // 128)
+        want = torch.zeros(rows, units * 4, dtype=torch.uint8, device=DEV)
+        want[:, : depth // 32] = scales
+        assert torch.equal(row_scales, want.view(rows, units, 4).permute(1, 0, 2))
 
 
-def test_scale_tiles_of_experts() -> None:
-    scales = torch.randint(0, 256, (5, 70, 9), dtype=torch.uint8, device=DEV)
-    tiles = kernels.mxfp4_scale_tiles(scales, 288)
-    assert tiles.shape == (5, 3, 128, 4)
-    for e in range(5):
-        assert torch.equal(tiles[e], kernels.mxfp4_scale_tiles(scales[e], 288))
+@pytest.mark.parametrize(("lead", "out", "depth"), [((), 1, 32), ((), 128, 256), ((5,), 70, 288), ((2,), 300, 2880)])
+def test_scale_tiles(lead: tuple[int, ...], out: int, depth: int) -> None:
+    scales = torch.randint(0, 256, (*lead, out, depth // 32), dtype=torch.uint8, device=DEV)
+    tiles = kernels.mxfp4_scale_tiles(scales, depth)
+    pairs, blocks = -(-depth // 256), -(-out // 128)
+    assert tiles.shape == (*lead, pairs, blocks, 64, 16)
+    full = torch.zeros(*lead, blocks * 128, pairs * 8, dtype=torch.uint8, device=DEV)
+    full[..., :out, : depth // 32] = scales
+    # [block, h, f, r] x [pair, u, j] -> [pair, block, (j, r), (h, u, f)]
+    full = full.view(-1, blocks, 2, 4, 16, pairs, 2, 4).permute(0, 5, 1, 7, 4, 2, 6, 3)
+    assert torch.equal(tiles.view(-1), full.reshape(-1))
 
 
 # ------------------------------------------------------------------ products
@@ -246,14 +246,10 @@ def test_nothing_behind_the_last_row_is_read_into_the_sums_or_written() -> None:
             room[: t.numel()] = t.reshape(-1)
             return room
 
-        def spoiled(t: torch.Tensor, live: int) -> torch.Tensor:
-            row = torch.arange(t.shape[1], device=DEV)
-            row = row - row % 128 + row % 4 * 32 + row % 128 // 4  # the row of each place
-            t = t.clone()
-            t[:, row >= live] = 255
-            return t
-
-        row_scales, tiles = spoiled(row_scales, rows), spoiled(tiles, out)
+        # Scales of outputs past the last are NaN too.
+        pad = torch.full((-(-out // 128) * 128, depth // 32), 255, dtype=torch.uint8, device=DEV)
+        pad[:out] = scales
+        tiles = kernels.mxfp4_scale_tiles(pad, depth)
         held = [behind(t) for t in (q, row_scales, blocks, tiles)]
         y = torch.full((rows * out + 4096,), 3.0, dtype=torch.bfloat16, device=DEV)
         _lib.call("lnq_mxfp4_mm", *(t.data_ptr() for t in held), None, y.data_ptr(), rows, out, depth, _lib.BF16,
@@ -364,13 +360,13 @@ def test_refusals() -> None:
         (lambda: kernels.mxfp4_w4a16(x, u8(8, 3, 16), u8(8, 3)), "against"),
         (lambda: kernels.mxfp4_w4a16(x.float(), u8(8, 2, 16), u8(8, 2)), "dtype"),
         (lambda: kernels.mxfp4_w4a16(x, u8(8, 2, 16), u8(8, 2), torch.zeros(8, device=DEV)), "bias"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 128, 4), u8(8, 3, 16), u8(1, 128, 4), torch.bfloat16), "against"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 256, 4), u8(8, 2, 16), u8(1, 128, 4), torch.bfloat16), "scale tiles"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 128, 4), u8(8, 2, 16), u8(2, 128, 4), torch.bfloat16), "scale tiles"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 128, 4), u8(8, 2, 16), u8(1, 128, 4), torch.float32), "dtype"),
-        (lambda: kernels.mxfp4_experts_mm(u8(5, 32), u8(1, 128, 4), u8(2, 8, 2, 16), u8(2, 1, 128, 4),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 3, 16), u8(1, 1, 64, 16), torch.bfloat16), "against"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 8, 4), u8(8, 2, 16), u8(1, 1, 64, 16), torch.bfloat16), "rows' scales"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(2, 1, 64, 16), torch.bfloat16), "scale tiles"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(1, 1, 64, 16), torch.float32), "dtype"),
+        (lambda: kernels.mxfp4_experts_mm(u8(5, 32), u8(1, 5, 4), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 16),
                                           torch.zeros(4, 2, dtype=torch.int64, device=DEV), torch.bfloat16), "against"),
-        (lambda: kernels.mxfp4_experts_mm(u8(4, 32), u8(1, 128, 4), u8(2, 8, 2, 16), u8(2, 1, 128, 4),
+        (lambda: kernels.mxfp4_experts_mm(u8(4, 32), u8(1, 4, 4), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 16),
                                           torch.zeros(4, 2, device=DEV), torch.bfloat16), "integers"),
         (lambda: quantized.mxfp4_operands(u8(2, 8, 2, 16), u8(2, 8, 2), 1), "blocks"),
         (lambda: quantized.mxfp4_experts_operands(u8(8, 2, 16), u8(8, 2), 1), "blocks"),

@@ -89,8 +89,8 @@ def test_the_wrappers_refuse_cpu_tensors() -> None:
                  lambda: kernels.mxfp4_dequantize(u8(2, 1, 16), u8(2, 1), torch.float32),
                  lambda: kernels.mxfp4_scale_tiles(u8(2, 1), 32),
                  lambda: kernels.mxfp4_w4a16(torch.zeros(2, 32).bfloat16(), u8(2, 1, 16), u8(2, 1)),
-                 lambda: kernels.mxfp4_mm(u8(2, 16), u8(1, 128, 4), u8(2, 1, 16), u8(1, 128, 4), torch.bfloat16),
-                 lambda: kernels.mxfp4_experts_mm(u8(2, 16), u8(1, 128, 4), u8(3, 2, 1, 16), u8(3, 1, 128, 4),
+                 lambda: kernels.mxfp4_mm(u8(2, 16), u8(1, 2, 4), u8(2, 1, 16), u8(1, 1, 64, 16), torch.bfloat16),
+                 lambda: kernels.mxfp4_experts_mm(u8(2, 16), u8(1, 2, 4), u8(3, 2, 1, 16), u8(3, 1, 1, 64, 16),
                                                   torch.zeros(2, 1, dtype=torch.int64), torch.bfloat16),
                  lambda: kernels.expert_route(torch.zeros(2, 8), 2), lambda: quantized.mxfp4_operands(u8(2, 1, 16), u8(2, 1), 1),
                  lambda: quantized.mxfp4_experts_operands(u8(3, 2, 1, 16), u8(3, 2, 1), 1)):
