@@ -274,6 +274,12 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   const bool vec_out = (a.N & 3) == 0;
   auto epilogue = [&](const Tile& t) {
     const bool none = EXPERTS && t.e >= a.count;  // pairs whose choice is no expert: zeros
+    int to_row[EXPERTS ? FA : 1];
+    if constexpr (EXPERTS) {
+#pragma unroll
+      for (int i = 0; i < FA; ++i) to_row[i] = a.order[t.first + min((wm * FA + i) * 16 + lrow, t.live - 1)];
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int j = 0; j < FB; ++j) {
       const int n = t.n0 + (wn * FB + j) * 16 + 4 * lk;
@@ -286,7 +292,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
       for (int i = 0; i < FA; ++i) {
         const int m = (wm * FA + i) * 16 + lrow;
         int64_t row;
-        if constexpr (EXPERTS) row = a.order[t.first + min(m, t.live - 1)];
+        if constexpr (EXPERTS) row = to_row[i];
         else row = t.m0 + m;
         uint32_t o[4];
 #pragma unroll
@@ -367,25 +373,40 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
 }
 
 // The pairs of each expert, in order: workgroup e counts every expert's pairs, which tells it
-// where its own begin in `order` and in the tile table, then lists them. Workgroup `count`
-// lists the pairs whose choice is no expert and writes how many tiles there are.
+// where its own begin in `order` and in the tile table, then lists them, each wave those of its
+// own run of the pairs. Workgroup `count` lists the pairs whose choice is no expert and writes how
+// many tiles there are.
 __global__ __launch_bounds__(mx4::LIST_THREADS) void expert_lists_kernel(const int64_t* __restrict__ experts, int pairs,
-                                                                         int count, int bm,
-                                                                         int* __restrict__ order, i32x4* __restrict__ table,
-                                                                         int* __restrict__ used) {
+                                                                         int count, int bm, int* __restrict__ order,
+                                                                         i32x4* __restrict__ table, int* __restrict__ used) {
   using namespace mx4;
-  constexpr int WAVES = LIST_THREADS / 64;
+  constexpr int WAVES = LIST_THREADS / 64, DEEP = 8;  // loads in flight
   __shared__ int number[MAX_EXPERTS + 1];
-  __shared__ int part[3][WAVES];
-  __shared__ int found[WAVES];
+  __shared__ int part[3][WAVES], found[WAVES];
   const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  auto bucket = [&](int p) -> int {
-    const int64_t id = experts[p];
-    return id >= 0 && id < count ? static_cast<int>(id) : count;
+  const int run = (pairs + 64 * WAVES - 1) / (64 * WAVES) * 64;  // pairs of a wave
+  const int from = wave * run, to = min(pairs, from + run);
+  // Calls f(pair, its bucket) for this wave's pairs, a lane each; past the last, a bucket of -1.
+  auto each = [&](auto f) {
+    for (int p0 = from; p0 < to; p0 += 64 * DEEP) {
+      int64_t id[DEEP];
+#pragma unroll
+      for (int d = 0; d < DEEP; ++d) id[d] = experts[min(p0 + 64 * d + lane, pairs - 1)];
+#pragma unroll
+      for (int d = 0; d < DEEP; ++d) {
+        const int p = p0 + 64 * d + lane;
+        f(p, p >= to ? -1 : id[d] >= 0 && id[d] < count ? static_cast<int>(id[d]) : count);
+      }
+    }
   };
   for (int i = tid; i <= count; i += LIST_THREADS) number[i] = 0;
   __syncthreads();
-  for (int p = tid; p < pairs; p += LIST_THREADS) atomicAdd(&number[bucket(p)], 1);
+  int here = 0;
+  each([&](int, int bucket) {
+    if (bucket >= 0) atomicAdd(&number[bucket], 1);
+    here += __popcll(__ballot(bucket == e));
+  });
+  if (lane == 0) found[wave] = here;
   __syncthreads();
   // Pairs and tiles of the experts before this one, and tiles of all.
   int sums[3] = {0, 0, 0};
@@ -401,30 +422,23 @@ __global__ __launch_bounds__(mx4::LIST_THREADS) void expert_lists_kernel(const i
     if (lane == 0) part[s][wave] = sums[s];
   }
   __syncthreads();
-  int first = 0, tile = 0, all = 0;
+  int first = 0, tile = 0, all = 0, at = 0;
 #pragma unroll
-  for (int v = 0; v < WAVES; ++v) first += part[0][v], tile += part[1][v], all += part[2][v];
+  for (int v = 0; v < WAVES; ++v) {
+    first += part[0][v], tile += part[1][v], all += part[2][v];
+    if (v < wave) at += found[v];
+  }
   const int mine = number[e];
-  for (int i = tid; i * bm < mine; i += LIST_THREADS) 
+  for (int i = tid; i * bm < mine; i += LIST_THREADS)
     table[tile + i] = i32x4{e, first + i * bm, min(bm, mine - i * bm) + 512 * ((mine + bm - 1) / bm), tile};
   if (e == count && tid == 0) used[0] = all;
   if (mine == 0) return;
-  int at = first;
-  for (int p0 = 0; p0 < pairs; p0 += LIST_THREADS) {
-    const int p = p0 + tid;
-    const bool here = p < pairs && bucket(p) == e;
-    const uint64_t mask = __ballot(here);
-    if (lane == 0) found[wave] = __popcll(mask);
-    __syncthreads();
-    int to = at;
-#pragma unroll
-    for (int v = 0; v < WAVES; ++v) {
-      if (v < wave) to += found[v];
-      at += found[v];
-    }
-    if (here) order[to + __popcll(mask & ((uint64_t{1} << lane) - 1))] = p;
-    __syncthreads();
-  }
+  at += first;
+  each([&](int p, int bucket) {
+    const uint64_t mask = __ballot(bucket == e);
+    if (bucket == e) order[at + __popcll(mask & ((uint64_t{1} << lane) - 1))] = p;
+    at += __popcll(mask);
+  });
 }
 
 namespace mx4 {

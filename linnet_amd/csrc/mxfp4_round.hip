@@ -17,8 +17,7 @@ namespace lnq {
 
 namespace mxr {
 constexpr int THREADS = 256;
-constexpr int ROWS = 128;  // rows of a workgroup of the row-rounding kernel
-constexpr int UNIT = 128;  // by the inputs of a unit
+constexpr int UNIT = 128;  // inputs of a workgroup of the row-rounding kernel
 
 // 8 values as loaded.
 template <int DT>
@@ -104,32 +103,37 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_quantize_kernel(const type
 }
 
 // Rows for the product: codes [rows, K / 2] as above, scales [units][rows] dwords of four
-// blocks (128 inputs). A workgroup takes 128 rows by 128 inputs, 16 lanes a row, so that its
-// scales leave as 512 bytes in a run.
-template <int DT>
+// blocks (128 inputs). A workgroup takes 16 PASSES rows by 128 inputs, 16 lanes a row, all of its
+// loads before its first conversion; its scales leave in a run.
+template <int DT, int PASSES>
 __global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename Elem<DT>::storage* __restrict__ x,
                                                                   int64_t x_stride, uint32_t* __restrict__ codes,
                                                                   uint32_t* __restrict__ scales, int rows, int K) {
   using namespace mxr;
-  constexpr int A_PASS = THREADS / 16;  // rows
+  constexpr int A_PASS = THREADS / 16, ROWS = A_PASS * PASSES;
   __shared__ uint32_t unit[ROWS];
   const int lane = threadIdx.x & 63;
   const int r0 = blockIdx.x * ROWS, k = blockIdx.y * UNIT + (threadIdx.x & 15) * 8;
   const bool in = k < K;
+  Raw<DT> raw[PASSES];
 #pragma unroll
-  for (int i = 0; i < ROWS / A_PASS; ++i) {
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = min(r0 + i * A_PASS + static_cast<int>(threadIdx.x >> 4), rows - 1);
+    raw[i] = load8<DT>(x + r * x_stride + (in ? k : 0));
+  }
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
     const int r = i * A_PASS + (threadIdx.x >> 4);
-    uint32_t byte = 0;
-    if (r0 + r < rows && in) {
-      float v[8];
-      widen8<DT>(load8<DT>(x + (r0 + r) * x_stride + k), v);
-      codes[(static_cast<int64_t>(r0 + r) * K + k) >> 3] = round8(v, byte);
-    }
+    float v[8];
+    widen8<DT>(raw[i], v);
+    uint32_t byte;
+    const uint32_t word = round8(v, byte);
+    if (r0 + r < rows && in) codes[(static_cast<int64_t>(r0 + r) * K + k) >> 3] = word;
     // The four blocks of the unit, 16 lanes: block b's byte at bits 8 b.
-    uint32_t word = byte << (8 * ((lane >> 2) & 3));
-    word |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(word), 4, 64));
-    word |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(word), 8, 64));
-    if ((lane & 15) == 0) unit[r] = word;
+    uint32_t four = in ? byte << (8 * ((lane >> 2) & 3)) : 0u;
+    four |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(four), 4, 64));
+    four |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(four), 8, 64));
+    if ((lane & 15) == 0) unit[r] = four;
   }
   __syncthreads();
   if (threadIdx.x < ROWS && r0 + static_cast<int>(threadIdx.x) < rows)
@@ -249,17 +253,25 @@ LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, ui
   LNQ_REQUIRE(x && q && scales, "lnq_mxfp4_rows: null pointer");
   LNQ_REQUIRE(x_stride >= 0 && x_stride % 8 == 0 && aligned(x, 16) && aligned(q, 16) && aligned(scales, 16),
               "lnq_mxfp4_rows: x (with its row stride), q and scales must be 16-byte aligned");
-  const dim3 grid(static_cast<unsigned>((rows + mxr::ROWS - 1) / mxr::ROWS),
-                  static_cast<unsigned>((in_features + mxr::UNIT - 1) / mxr::UNIT));
+  // 128 rows a workgroup where that still is four workgroups a CU, else 16.
+  const int64_t spans = (in_features + mxr::UNIT - 1) / mxr::UNIT;
+  const int per = (rows + 127) / 128 * spans >= 4 * compute_units() ? 128 : 16;
+  const dim3 grid(static_cast<unsigned>((rows + per - 1) / per), static_cast<unsigned>(spans));
   LNQ_REQUIRE(grid.y <= 65535, "lnq_mxfp4_rows: in too large");
   const int R = static_cast<int>(rows), K = static_cast<int>(in_features);
-#define LNQ_MXW(DT)                                                                                                     \
-  hipLaunchKernelGGL((mxfp4_rows_kernel<DT>), grid, dim3(mxr::THREADS), 0, static_cast<hipStream_t>(stream),            \
-                     static_cast<const typename Elem<DT>::storage*>(x), x_stride, reinterpret_cast<uint32_t*>(q),       \
+#define LNQ_MXW(DT, P)                                                                                                \
+  hipLaunchKernelGGL((mxfp4_rows_kernel<DT, P>), grid, dim3(mxr::THREADS), 0, static_cast<hipStream_t>(stream),       \
+                     static_cast<const typename Elem<DT>::storage*>(x), x_stride, reinterpret_cast<uint32_t*>(q),     \
                      reinterpret_cast<uint32_t*>(scales), R, K)
-  if (dtype == LNQ_BF16) LNQ_MXW(LNQ_BF16);
-  else if (dtype == LNQ_F16) LNQ_MXW(LNQ_F16);
-  else LNQ_MXW(LNQ_F32);
+#define LNQ_MXW_P(DT)                \
+  do {                               \
+    if (per == 128) LNQ_MXW(DT, 8);  \
+    else LNQ_MXW(DT, 1);             \
+  } while (0)
+  if (dtype == LNQ_BF16) LNQ_MXW_P(LNQ_BF16);
+  else if (dtype == LNQ_F16) LNQ_MXW_P(LNQ_F16);
+  else LNQ_MXW_P(LNQ_F32);
+#undef LNQ_MXW_P
 #undef LNQ_MXW
   return launched("mxfp4_rows");
 }
