@@ -485,16 +485,16 @@ LNQ_API LnqStatus lnq_mxfp4_dequantize(const uint8_t* blocks, const uint8_t* sca
 
 /* Rows of activations as lnq_mxfp4_mm reads them: lnq_mxfp4_quantize's rounding of x [rows,
  * in] (rows x_stride elements apart, a multiple of 8), the codes in q [rows, in/2], the scales
- * in `scales` [units][rows][4], unit u holding blocks 4u .. 4u + 3 (128 inputs) of every row,
- * units = ceil(in / 128) (blocks past `in` hold 0). x, q and scales 16-byte aligned. No
- * counterpart in the reference. */
+ * in `scales` [units][padded][4], unit u holding blocks 4u .. 4u + 3 (128 inputs) of every row,
+ * units = ceil(in / 128), padded = rows rounded up to a multiple of 4 (rows past the last and
+ * blocks past `in` hold 0). x, q and scales 16-byte aligned. No counterpart in the reference. */
 LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, uint8_t* scales,
                                  int64_t rows, int64_t in_features, int32_t dtype, void* stream);
 
 /* A weight's scales as stored, [count, out, in/32], as lnq_mxfp4_mm reads them ("scale tiles"):
- * [count][ceil(in / 256)][ceil(out / 128)][64][16] bytes, of each 128 outputs by 256 inputs byte
- * 8 h + 4 u + f of place 16 j + r the scale of output 64 h + 16 f + r at block 4 u + j (0 past
- * the last output or block). Made once, as the weight is loaded. tiles 16-byte aligned. */
+ * [count][ceil(in / 256)][ceil(out / 64)][64][8] bytes, of each 64 outputs by 256 inputs byte 4 u + f
+ * of place 16 j + r the scale of output 16 f + r at block 4 u + j (0 past the last output or
+ * block). Made once, as the weight is loaded. tiles 16-byte aligned. */
 LNQ_API LnqStatus lnq_mxfp4_scale_tiles(const uint8_t* scales, uint8_t* tiles, int64_t count,
                                         int64_t out_features, int64_t in_features, void* stream);
 
@@ -511,7 +511,7 @@ LNQ_API LnqStatus lnq_mxfp4_linear(const void* x, int64_t x_stride, const uint8_
  * as stored and its scales as tiles (lnq_mxfp4_scale_tiles), multiplied on the block-scaled
  * MFMA (exact products, f32 sums), bias added in f32, rounded once to `dtype` (bf16 or f16).
  * NaN where a row's or an output's block has the scale 255. rows, out <= 2^27, in <= 2^22, in %
- * 32 == 0; operands 16-byte aligned, y 8-byte. */
+ * 32 == 0; operands 16-byte aligned. */
 LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const uint8_t* blocks,
                                const uint8_t* tiles, const void* bias, void* y, int64_t rows,
                                int64_t out_features, int64_t in_features, int32_t dtype, void* stream);
@@ -521,9 +521,10 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
  * chosen expert of a row reads it) or rows * chosen; blocks [E, out, in/32, 16] as stored,
  * tiles [E] scale tiles each. An expert index outside 0 .. num_experts - 1 gives zeros.
  * workspace (16-byte aligned, at least lnq_mxfp4_experts_workspace bytes) holds the lists of
- * the pairs, written by the call: calls that overlap on one workspace race. num_experts <=
+ * the pairs and their scales, written by the call: calls that overlap on one workspace race. num_experts <=
  * 2048, rows * chosen <= 2^26, out <= 2^27, x's codes below 2 GiB. */
-LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t num_experts, int64_t* bytes);
+LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t num_experts, int64_t in_features,
+                                              int64_t* bytes);
 LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale, const uint8_t* blocks,
                                        const uint8_t* tiles, const int64_t* experts, void* y,
                                        int64_t rows, int64_t chosen, int64_t num_experts,

@@ -15,22 +15,24 @@ constexpr int MAX_EXPERTS = 2048;          // of the pair lists' LDS
 // The MFMA (v_mfma_scale_f32_16x16x128_f8f6f4): lane l holds row l % 16, inputs 32 (l / 16) .. +
 // 31 of 128 (a unit) in 16 bytes, and their scale in a byte, which the instruction selects, of a
 // register. Scales lie so that the registers come as they are:
-// x's, a dword a row and unit (its four blocks), [units][rows]: shifted by 8 (l / 16), byte 0;
-// a weight's ("scale tiles"), [pairs of units][blocks of 128 rows][64 lanes][16 bytes]: lane l's
-// dword 2 h + u of a block holds, for unit u of the pair and half h of the block, the
-// bytes of rows 64 h + 16 f + l % 16 (f = 0 .. 3) at block l / 16 of the unit: four MFMAs' scales.
+// x's, a dword a row and unit (its four blocks), [units][rows up to a multiple of 4]: shifted by 8
+// (l / 16), byte 0;
+// a weight's ("scale tiles"), [pairs of units][blocks of 64 rows][64 lanes][2 units] dwords: lane l's
+// for a unit holds the bytes of rows 16 f + l % 16 (f = 0 .. 3) of the block at block l / 16 of the
+// unit: four MFMAs' scales.
 __host__ __device__ inline int units_of(int K) { return (K + 127) / 128; }
-__host__ __device__ inline int blocks_of(int N) { return (N + 127) / 128; }
-constexpr int TILE_BYTES = 1024;  // of a scale tile: 128 rows by 256 inputs
+__host__ __device__ inline int blocks_of(int N) { return (N + 63) / 64; }
+__host__ __device__ inline int fours(int rows) { return (rows + 3) / 4 * 4; }
+constexpr int TILE_BYTES = 512;  // of a scale tile: 64 rows by 256 inputs
 
 struct Args {
   const uint8_t* q;      // x's codes [rows, K / 2]
-  const uint32_t* xs;    // and scales [units][M]
+  const uint32_t* xs;    // and scales [units][S], of the rows or of the experts' tiles' rows
   const uint8_t* w;      // codes [N, K / 2], of each expert
   const uint8_t* ws;     // scale tiles, of each expert
   const uint16_t* bias;
   uint16_t* y;
-  int M, N, K;
+  int M, N, K, S;
   // Experts: the pairs by expert, and tiles of them: (expert, first place in `order`, pairs + 512 *
   // tiles of the expert, the expert's first tile); used[0]: the tiles there are.
   const int* order;
@@ -40,15 +42,11 @@ struct Args {
   int64_t w_step, ws_step;   // from an expert's weight / scales to the next one's
 };
 
-// 16 or 4 bytes a lane from `at` of a buffer to LDS, lane l's at to + 16 l (4 l). (Called in a
+// 16 bytes a lane from `at` of a buffer to LDS, lane l's at to + 16 l. (Called in a
 // kernel template with arguments of known types the builtin makes the host's pass drop the
 // kernel's stub without a word.)
 __device__ inline void load16(__amdgpu_buffer_rsrc_t r, uint8_t* to, uint32_t at) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)to, 16, at, 0, 0, 0);
-}
-
-__device__ inline void load4(__amdgpu_buffer_rsrc_t r, uint8_t* to, uint32_t at) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)to, 4, at, 0, 0, 0);
 }
 
 // The MFMA of 32 codes a lane of a weight (a, scale byte `f` of sa) and of x (b, byte 0 of sb); f is

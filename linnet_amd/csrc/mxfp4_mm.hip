@@ -37,16 +37,15 @@ struct Form {
   static constexpr int NW = WM * WN, THREADS = 64 * NW;
   static constexpr int BM = 16 * FA * WM, BN = 16 * FB * WN;
   static constexpr int CODES = (BM + BN) * BKB;
-  static constexpr int STAGE = CODES + (BM + BN) * 8;     // then x's scales, 2 units, and the weight's
+  static constexpr int XC = (BM + 127) / 128, ALL = XC + (BN + 127) / 128;  // loads of a step's scales: x's, all
+  static constexpr int STAGE = CODES + ALL * 1024;         // the codes, x's scales of the 2 units, the weight's
   static constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;  // loads of a wave a step: 8 rows of codes each
-  static constexpr int XC = BM / 32, ALL = XC + BN / 32;  // loads of 64 scale dwords: x's, all
-  static constexpr int LS = (ALL + NW - 1) / NW;          // of a wave
-  static constexpr int LOADS = LA + LB + LS;
+  static constexpr int LOADS = LA + LB + 1;                // and of scales
   static constexpr int GROUPS = 160 * 1024 / (2 * STAGE);  // workgroups that a CU's LDS holds
   static constexpr int PER_CU = GROUPS < 4 ? GROUPS : 4;
   static constexpr int WAVES_A_SIMD = NW * PER_CU / 4 > 0 ? NW * PER_CU / 4 : 1;
   static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN && NW % 2 == 0, "whole loads, one key a wave");
-  static_assert((FB == 2 || FB == 4) && BN % 64 == 0 && (FA == 2 || FA == 4 || FA == 8), "scales a lane");
+  static_assert((FB == 2 || FB == 4) && BN % 64 == 0 && (FA == 2 || FA == 4 || FA == 8) && ALL <= NW, "scales a lane");
 };
 }  // namespace mx4
 
@@ -55,7 +54,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   using namespace mx4;
   using E = Elem<DT>;
   constexpr int FA = FORM::FA, FB = FORM::FB, NW = FORM::NW, BM = FORM::BM, BN = FORM::BN, CODES = FORM::CODES;
-  constexpr int LA = FORM::LA, LB = FORM::LB, LS = FORM::LS, LOADS = FORM::LOADS, XC = FORM::XC;
+  constexpr int LA = FORM::LA, LB = FORM::LB, LOADS = FORM::LOADS, XC = FORM::XC;
   constexpr int WN = BN / 16 / FB;
   // One array per stage: the compiler then waits, before reading a stage, for that stage's
   // loads only.
@@ -93,19 +92,19 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   const uint32_t lcol = 16u * ((lane & 7) ^ ((lr >> 1) & 7));
   const uint32_t voff = static_cast<uint32_t>(lr) * row_bytes + lcol;  // of load i: 8 NW i rows on
   uint32_t xoff[EXPERTS ? LA : 1];
-  // Scale dwords, 64 a load: x's rows at the step's first unit, at its second; then each 64
-  // columns' of a scale tile, first unit, second. Loads past the last repeat it.
-  auto scale_load = [&](int i) -> int { return min(wave + NW * i, FORM::ALL - 1); };
-  uint32_t soff[LS];
-#pragma unroll
-  for (int i = 0; i < LS; ++i) {
-    const int c = scale_load(i), d = c * 64 + lane;
-    const int half = (c - XC) / 2, u = (c - XC) & 1;
-    soff[i] = c < XC ? (static_cast<uint32_t>(d / BM) * a.M + d % BM) * 4u
-                     : static_cast<uint32_t>(half >> 1) * TILE_BYTES + lane * 16u + (half & 1) * 8u + u * 4u;
+  // This wave's load of scales, a kilobyte: x's rows at the step's two units, or the scale tiles of
+  // 128 columns (waves past the last load what others do). soff: nowhere past what a step has.
+  const int chunk = wave % FORM::ALL;
+  const bool x_chunk = chunk < XC;
+  uint32_t soff;
+  {
+    const int d = (x_chunk ? chunk : chunk - XC) * 256 + lane * 4;  // dword
+    if (x_chunk) soff = d < 2 * BM ? (static_cast<uint32_t>(d / BM) * a.S + d % BM) * 4u : NOWHERE;
+    else soff = d < 2 * BN ? static_cast<uint32_t>(d) * 4u : NOWHERE;
   }
 
-  // A tile of this launch: columns from n0; rows from m0, or an expert's pairs from `first`.
+  // A tile of this launch: columns from n0; rows from m0, or an expert's pairs from `first` (their
+  // scales from m0).
   struct Tile {
     int n0, m0, live, first, e;
   };
@@ -117,61 +116,46 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   // The experts' tile r in two lookups: the entry of some tile of its expert, then its own.
   auto place_of = [&](int r) -> int { return max(xcd_tile(b0 + min(r, mine - 1) * G, total), 0); };
   auto expert_of = [&](int r) -> i32x4 { return a.table[place_of(r) / tiles_n]; };
-  auto entry_of = [&](int r, i32x4 any, int& n0) -> i32x4 {
+  auto entry_of = [&](int r, i32x4 any, int& n0, int& m0) -> i32x4 {
     const int many = __builtin_amdgcn_readfirstlane(any.z) >> 9, tile0 = __builtin_amdgcn_readfirstlane(any.w);
     const int j = place_of(r) - tile0 * tiles_n;
     n0 = j / many * BN;
+    m0 = (tile0 + j % many) * BM;
     return a.table[tile0 + j % many];
   };
-  auto expert_tile = [&](i32x4 entry, int n0) -> Tile {
-    return Tile{n0, 0, __builtin_amdgcn_readfirstlane(entry.z) & 511, __builtin_amdgcn_readfirstlane(entry.y),
+  auto expert_tile = [&](i32x4 entry, int n0, int m0) -> Tile {
+    return Tile{n0, m0, __builtin_amdgcn_readfirstlane(entry.z) & 511, __builtin_amdgcn_readfirstlane(entry.y),
                 __builtin_amdgcn_readfirstlane(entry.x)};
   };
-  // The pairs whose rows of x this thread loads of an experts' tile: codes, then scales.
-  int pairs[EXPERTS ? LA + LS : 1];
+  // The pairs whose rows of x this thread loads of an experts' tile.
+  int pairs[EXPERTS ? LA : 1];
   auto take_pairs = [&](const Tile& t) {
     if constexpr (EXPERTS) {
 #pragma unroll
-      for (int i = 0; i < LA + LS; ++i) {
-        const int r = i < LA ? lr + 8 * NW * i : (min(scale_load(i - LA), XC - 1) * 64 + lane) % BM;
-        pairs[i] = a.order[t.first + min(r, t.live - 1)];
-      }
+      for (int i = 0; i < LA; ++i) pairs[i] = a.order[t.first + min(lr + 8 * NW * i, t.live - 1)];
     }
   };
 
-  // The tile whose steps are being loaded. Of each scale load its base, what a step adds to it, and
-  // the bytes of a step, of a step of one unit. (Chosen here: a choice in the steps would be a branch,
-  // and the compiler then moves the MFMAs across the blocks it splits the step into.)
-  const uint8_t *qb, *wb, *sb[LS];
-  uint32_t q_bytes, w_bytes, s_step[LS], s_two[LS], s_one[LS];
+  // The tile whose steps are being loaded; of the scales their base, what a step adds to it, and the
+  // bytes of a step, of a step of one unit. (Chosen here: a choice in the steps would be a branch, and
+  // the compiler then moves the MFMAs across the blocks it splits the step into.)
+  const uint8_t *qb, *wb, *sb;
+  uint32_t q_bytes, w_bytes, s_two, s_one;
+  const uint32_t s_step = x_chunk ? static_cast<uint32_t>(a.S) * 8u : pair_bytes;
   auto load_tile = [&](const Tile& t) {
     const int e = EXPERTS ? min(t.e, a.count - 1) : 0;  // a tile of no expert multiplies the last one's weight, for nothing
-    qb = a.q + static_cast<int64_t>(t.m0) * row_bytes;
+    qb = a.q + (EXPERTS ? 0 : static_cast<int64_t>(t.m0) * row_bytes);
     q_bytes = static_cast<uint32_t>(EXPERTS ? a.M : t.live) * row_bytes;
     wb = a.w + e * a.w_step + static_cast<int64_t>(t.n0) * row_bytes;
     w_bytes = static_cast<uint32_t>(min(BN, a.N - t.n0)) * row_bytes;
-    const uint32_t s_rows = static_cast<uint32_t>(EXPERTS ? a.M : t.live);
-    const uint32_t column = static_cast<uint32_t>(t.n0 / 128) * TILE_BYTES + (t.n0 & 64) / 8;
-#pragma unroll
-    for (int i = 0; i < LS; ++i) {
-      const bool x = scale_load(i) < XC;
-      sb[i] = x ? reinterpret_cast<const uint8_t*>(a.xs + t.m0) : a.ws + e * a.ws_step + column;
-      s_step[i] = x ? static_cast<uint32_t>(a.M) * 8u : pair_bytes;
-      s_two[i] = x ? (static_cast<uint32_t>(a.M) + s_rows) * 4u : pair_bytes - column;
-      s_one[i] = x ? s_rows * 4u : pair_bytes - column;
-    }
+    const uint32_t column = static_cast<uint32_t>(t.n0 / 64) * TILE_BYTES, rows = static_cast<uint32_t>(fours(t.live));
+    sb = x_chunk ? reinterpret_cast<const uint8_t*>(a.xs + t.m0) : a.ws + e * a.ws_step + column;
+    s_two = x_chunk ? (static_cast<uint32_t>(a.S) + rows) * 4u : pair_bytes - column;
+    s_one = x_chunk ? rows * 4u : pair_bytes - column;
     if constexpr (EXPERTS) {
 #pragma unroll
       for (int i = 0; i < LA; ++i)
         xoff[i] = lr + 8 * NW * i < t.live ? static_cast<uint32_t>(pairs[i] / a.chosen) * row_bytes + lcol : NOWHERE;
-#pragma unroll
-      for (int i = 0; i < LS; ++i) {
-        const int c = scale_load(i), d = c * 64 + lane;
-        if (c < XC)
-          soff[i] = d % BM < t.live
-                        ? (static_cast<uint32_t>(d / BM) * a.M + static_cast<uint32_t>(pairs[LA + i] / a.chosen)) * 4u
-                        : NOWHERE;
-      }
     }
   };
   // Load i of k-step ks into stage st. Steps past the stream, and columns and units past K, read
@@ -185,10 +169,9 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
       const uint32_t at = EXPERTS && x ? xoff[EXPERTS && x ? i : 0] : voff + static_cast<uint32_t>(8 * NW * (x ? i : i - LA)) * row_bytes;
       load16(buffer_rsrc((x ? qb : wb) + k0, live ? (x ? q_bytes : w_bytes) - k0 : 0u), st + (NW * i + wave) * 1024, at | past);
     } else {
-      const int l = i - LA - LB;
-      const uint32_t bytes = units - 2 * ks >= 2 ? s_two[l] : s_one[l];
-      load4(buffer_rsrc(sb[l] + static_cast<uint64_t>(static_cast<uint32_t>(ks)) * s_step[l], live ? bytes : 0u),
-            st + CODES + scale_load(l) * 256, soff[l]);
+      const uint32_t bytes = units - 2 * ks >= 2 ? s_two : s_one;
+      load16(buffer_rsrc(sb + static_cast<uint64_t>(static_cast<uint32_t>(ks)) * s_step, live ? bytes : 0u),
+             st + CODES + chunk * 1024, soff);
     }
   };
 
@@ -202,7 +185,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
     boff[u] = static_cast<uint32_t>(swz8(BM + wn * FB * 16 + lrow, 4 * u + lk));
   }
   const uint32_t sa_at = static_cast<uint32_t>(CODES + (wm * FA * 16 + lrow) * 4);
-  const uint32_t sw_at = static_cast<uint32_t>(CODES + BM * 8 + wn * FB * 16 / 64 * 512 + lane * 4);
+  const uint32_t sw_at = static_cast<uint32_t>(CODES + XC * 1024 + wn * FB * 16 / 64 * TILE_BYTES + lane * 8);
   const int first_byte = wn * FB % 4;  // of this wave's columns in their dword
 
   // Operands: the columns' of a unit, a set a unit; the rows' and their scale dwords in a ring of
@@ -251,7 +234,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
 #pragma unroll
       for (int f = 0; f < FB; ++f)
         if (s == FROM + 1 + 2 * f) read_b(U ^ 1, nxt, f);
-      if (s == FROM + 2) sw[U ^ 1] = *reinterpret_cast<const uint32_t*>(nxt + sw_at + (U ^ 1) * 256);
+      if (s == FROM + 2) sw[U ^ 1] = *reinterpret_cast<const uint32_t*>(nxt + sw_at + (U ^ 1) * 4);
       if (U == 1 && s >= FROM) {
 #pragma unroll
         for (int q = 0; q < LOADS; ++q)
@@ -270,46 +253,83 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   };
 
   // Lane l, register r of fragment (i, j): row 16 i + l % 16 of the wave's, column 16 j + 4 (l / 16)
-  // + r.
-  const bool vec_out = (a.N & 3) == 0;
+  // + r. Two fragments' trade between the lanes of a row (v_permlane16_swap) gives each lane 8
+  // columns together, and with four fragments the lanes of rows r and r + 8 trade (row_ror:8), so
+  // that a store writes 8 rows of 128 bytes: whole lines (8 bytes a lane as they come, 32 together,
+  // took a quarter of a 4096 x 8192 -> 28672 call's time, as the next step's wait for its loads waits
+  // for the stores too).
+  typedef u32x4 __attribute__((aligned(2))) loose_u32x4;  // rows of an odd width begin anywhere
   auto epilogue = [&](const Tile& t) {
     const bool none = EXPERTS && t.e >= a.count;  // pairs whose choice is no expert: zeros
-    int to_row[EXPERTS ? FA : 1];
+    const int n0 = t.n0 + wn * FB * 16;
+    float bias[FB][4];
+#pragma unroll
+    for (int j = 0; j < FB; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = n0 + 16 * j + 4 * lk + r;
+        bias[j][r] = !EXPERTS && a.bias != nullptr && n < a.N ? E::to_f32(a.bias[n]) : 0.f;
+      }
+    int to_row[EXPERTS ? 2 * FA : 1];
+    auto row_at = [&](int i, int h) -> int {  // of store h of row i of fragments
+      return (wm * FA + i) * 16 + (FB == 4 ? (lrow & 7) + 8 * h : lrow);
+    };
     if constexpr (EXPERTS) {
 #pragma unroll
-      for (int i = 0; i < FA; ++i) to_row[i] = a.order[t.first + min((wm * FA + i) * 16 + lrow, t.live - 1)];
-      __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < 2 * FA; ++i) to_row[i] = a.order[t.first + min(row_at(i >> 1, i & 1), t.live - 1)];
     }
+    __builtin_amdgcn_sched_barrier(0);
+    auto store = [&](int i, int h, int n, u32x4 v) {
+      const int m = row_at(i, h);
+      int64_t row;
+      if constexpr (EXPERTS) row = to_row[2 * i + h];
+      else row = t.m0 + m;
+      if (m >= t.live) return;
+      uint16_t* const to = a.y + row * a.N + n;
+      if (n + 8 <= a.N) {
+        *reinterpret_cast<loose_u32x4*>(to) = v;
+      } else {
 #pragma unroll
-    for (int j = 0; j < FB; ++j) {
-      const int n = t.n0 + (wn * FB + j) * 16 + 4 * lk;
-      float b[4] = {0.f, 0.f, 0.f, 0.f};
-      if (!EXPERTS && a.bias != nullptr) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) b[r] = n + r < a.N ? E::to_f32(a.bias[n + r]) : 0.f;
+        for (int r = 0; r < 8; ++r)
+          if (n + r < a.N) to[r] = static_cast<uint16_t>(v[r >> 1] >> (16 * (r & 1)));
       }
+    };
 #pragma unroll
-      for (int i = 0; i < FA; ++i) {
-        const int m = (wm * FA + i) * 16 + lrow;
-        int64_t row;
-        if constexpr (EXPERTS) row = to_row[i];
-        else row = t.m0 + m;
-        uint32_t o[4];
+    for (int i = 0; i < FA; ++i) {
+      uint32_t o[FB][2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = none ? 0u : E::from_f32(acc[i][j][r] + b[r]);
-        if (m < t.live) {
-          uint16_t* const to = a.y + row * a.N + n;
-          if (vec_out) {
-            if (n < a.N) *reinterpret_cast<u32x2*>(to) = u32x2{o[0] | (o[1] << 16), o[2] | (o[3] << 16)};
-          } else {
+      for (int j = 0; j < FB; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (n + r < a.N) to[r] = static_cast<uint16_t>(o[r]);
-          }
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t lo = E::from_f32(acc[i][j][2 * h] + bias[j][2 * h]), hi = E::from_f32(acc[i][j][2 * h + 1] + bias[j][2 * h + 1]);
+          o[j][h] = none ? 0u : lo | (hi << 16);
         }
-        // One fragment at a time: the next tile's operands are live here.
-        __builtin_amdgcn_sched_barrier(0);
+      // Lane quarter k of fragments 2 p, 2 p + 1 then holds columns 8 (k / 2) .. + 7 of fragment 2 p + k % 2.
+#pragma unroll
+      for (int j = 0; j < FB; j += 2)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const auto r = __builtin_amdgcn_permlane16_swap(o[j][h], o[j + 1][h], false, false);
+          o[j][h] = r[0], o[j + 1][h] = r[1];
+        }
+      const int n = n0 + 16 * (lk & 1) + 8 * (lk >> 1);
+      if constexpr (FB == 4) {
+        u32x4 p, q;
+        const uint32_t pv[4] = {o[0][0], o[0][1], o[1][0], o[1][1]}, qv[4] = {o[2][0], o[2][1], o[3][0], o[3][1]};
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          // Rows 0 .. 7: the first half of the columns from their own lanes, the second in the lanes of
+          // rows 8 .. 15; then the same of those rows.
+          p[d] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(pv[d]), static_cast<int>(qv[d]), 0x128, 0xf, 0xc, false));
+          q[d] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(qv[d]), static_cast<int>(pv[d]), 0x128, 0xf, 0x3, false));
+        }
+        store(i, 0, n + 32 * (lrow >> 3), p);
+        store(i, 1, n + 32 * (lrow >> 3), q);
+      } else {
+        store(i, 0, n, u32x4{o[0][0], o[0][1], o[1][0], o[1][1]});
       }
+      // One row of fragments at a time: the next tile's operands are live here.
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -317,12 +337,12 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   // every wave's); its first operands and scales read.
   Tile now, next;
   i32x4 ahead = {0, 0, 0, 0}, ahead2 = {0, 0, 0, 0};
-  int ahead_n0 = 0;
+  int ahead_n0 = 0, ahead_m0 = 0;
   if constexpr (EXPERTS) {
-    int n0;
-    const i32x4 entry = entry_of(0, expert_of(0), n0);
-    now = expert_tile(entry, n0);
-    ahead = entry_of(1, expert_of(1), ahead_n0);
+    int n0, m0;
+    const i32x4 entry = entry_of(0, expert_of(0), n0, m0);
+    now = expert_tile(entry, n0, m0);
+    ahead = entry_of(1, expert_of(1), ahead_n0, ahead_m0);
     ahead2 = expert_of(2);
   } else {
     now = plain_tile(0);
@@ -355,8 +375,8 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
     // Tile r + 1 from what the last tile looked up; its pairs, the entry of r + 2 and the expert of
     // r + 3 asked for: none is used before this tile's last steps.
     if constexpr (EXPERTS) {
-      next = expert_tile(ahead, ahead_n0);
-      ahead = entry_of(r + 2, ahead2, ahead_n0);
+      next = expert_tile(ahead, ahead_n0, ahead_m0);
+      ahead = entry_of(r + 2, ahead2, ahead_n0, ahead_m0);
       ahead2 = expert_of(r + 3);
     } else {
       next = plain_tile(min(r + 1, mine - 1));
@@ -441,6 +461,20 @@ __global__ __launch_bounds__(mx4::LIST_THREADS) void expert_lists_kernel(const i
   });
 }
 
+// x's scales by the tiles' rows, [units][tiles][bm]: a tile's then lie together (read row by row, a
+// dword each, they were as many lines as the codes).
+__global__ __launch_bounds__(256) void expert_scales_kernel(const uint32_t* __restrict__ from, uint32_t* __restrict__ to,
+                                                            const int* __restrict__ order, const i32x4* __restrict__ table,
+                                                            const int* __restrict__ used, int rows, int places, int bm,
+                                                            int chosen) {
+  const int i = blockIdx.x * 256 + threadIdx.x, t = i / bm, r = i - t * bm;
+  if (t >= used[0]) return;
+  const i32x4 entry = table[t];
+  if (r >= mx4::fours(entry.z & 511)) return;
+  const int row = order[entry.y + min(r, (entry.z & 511) - 1)] / chosen;
+  to[static_cast<int64_t>(blockIdx.y) * places + i] = from[static_cast<int64_t>(blockIdx.y) * rows + row];
+}
+
 namespace mx4 {
 
 template <int DT, class FORM, bool EXPERTS>
@@ -473,16 +507,19 @@ static void launch(const Args& a, int bm, hipStream_t s) {
 
 struct Plan {
   int bm, tiles;
-  int64_t order_bytes, bytes;
+  int64_t places, order_bytes, table_bytes, bytes;
 };
 
-// Tiles of the pairs at most: a partial one for each expert that is named.
-static Plan experts_plan(int64_t pairs, int64_t count) {
+// Tiles of the pairs at most: a partial one for each expert that is named. The workspace: order,
+// table, how many tiles, scales.
+static Plan experts_plan(int64_t pairs, int64_t count, int64_t in_features) {
   Plan p{};
   p.bm = tile_rows(static_cast<double>(pairs) / static_cast<double>(count));
   p.tiles = static_cast<int>(pairs / p.bm + std::min(pairs, count + 1));
   p.order_bytes = (pairs * 4 + 15) / 16 * 16;
-  p.bytes = p.order_bytes + static_cast<int64_t>(p.tiles) * 16 + 16;
+  p.table_bytes = static_cast<int64_t>(p.tiles) * 16 + 16;
+  p.places = static_cast<int64_t>(p.tiles) * p.bm;
+  p.bytes = p.order_bytes + p.table_bytes + (in_features + 127) / 128 * p.places * 4;
   return p;
 }
 
@@ -508,8 +545,8 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
     return LNQ_OK;
   }
   LNQ_REQUIRE(q && x_scale && blocks && tiles && y, "lnq_mxfp4_mm: null pointer");
-  LNQ_REQUIRE(aligned(q, 16) && aligned(x_scale, 16) && aligned(blocks, 16) && aligned(tiles, 16) && aligned(y, 8),
-              "lnq_mxfp4_mm: operands must be 16-byte aligned, y 8-byte");
+  LNQ_REQUIRE(aligned(q, 16) && aligned(x_scale, 16) && aligned(blocks, 16) && aligned(tiles, 16) && aligned(y, 2),
+              "lnq_mxfp4_mm: operands must be 16-byte aligned");
   mx4::Args a{};
   a.q = q;
   a.xs = reinterpret_cast<const uint32_t*>(x_scale);
@@ -518,6 +555,7 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
   a.bias = static_cast<const uint16_t*>(bias);
   a.y = static_cast<uint16_t*>(y);
   a.M = static_cast<int>(rows);
+  a.S = mx4::fours(a.M);
   a.N = static_cast<int>(out_features);
   a.K = static_cast<int>(in_features);
   LNQ_REQUIRE((rows + 31) / 32 * ((out_features + 63) / 64) <= INT32_MAX, "lnq_mxfp4_mm: too large");
@@ -528,12 +566,13 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
   return launched("mxfp4_mm");
 }
 
-LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t num_experts, int64_t* bytes) {
+LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t num_experts, int64_t in_features, int64_t* bytes) {
   LNQ_REQUIRE(bytes != nullptr, "lnq_mxfp4_experts_workspace: null pointer");
-  LNQ_REQUIRE(pairs >= 0 && pairs <= (1 << 26) && num_experts > 0 && num_experts <= mx4::MAX_EXPERTS,
-              "lnq_mxfp4_experts_workspace: %lld pairs of %lld experts (1 to %d)", static_cast<long long>(pairs),
-              static_cast<long long>(num_experts), mx4::MAX_EXPERTS);
-  *bytes = pairs == 0 ? 0 : mx4::experts_plan(pairs, num_experts).bytes;
+  LNQ_REQUIRE(pairs >= 0 && pairs <= (1 << 26) && num_experts > 0 && num_experts <= mx4::MAX_EXPERTS && in_features > 0 &&
+                  in_features <= (1 << 22),
+              "lnq_mxfp4_experts_workspace: %lld pairs of %lld experts (1 to %d) of %lld inputs", static_cast<long long>(pairs),
+              static_cast<long long>(num_experts), mx4::MAX_EXPERTS, static_cast<long long>(in_features));
+  *bytes = pairs == 0 ? 0 : mx4::experts_plan(pairs, num_experts, in_features).bytes;
   clear_error();
   return LNQ_OK;
 }
@@ -556,12 +595,13 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
     return LNQ_OK;
   }
   LNQ_REQUIRE(q && x_scale && blocks && tiles && experts && y, "lnq_mxfp4_experts_mm: null pointer");
-  LNQ_REQUIRE(aligned(q, 16) && aligned(x_scale, 16) && aligned(blocks, 16) && aligned(tiles, 16) && aligned(y, 8) &&
+  LNQ_REQUIRE(aligned(q, 16) && aligned(x_scale, 16) && aligned(blocks, 16) && aligned(tiles, 16) && aligned(y, 2) &&
                   aligned(workspace, 16),
-              "lnq_mxfp4_experts_mm: operands and workspace must be 16-byte aligned, y 8-byte");
+              "lnq_mxfp4_experts_mm: operands and workspace must be 16-byte aligned");
   const int64_t pairs = rows * chosen, x_rows = shared ? rows : pairs;
   LNQ_REQUIRE(x_rows * (in_features / 2) < (int64_t{1} << 31), "lnq_mxfp4_experts_mm: x's codes past 2 GiB");
-  const mx4::Plan plan = mx4::experts_plan(pairs, num_experts);
+  const mx4::Plan plan = mx4::experts_plan(pairs, num_experts, in_features);
+  LNQ_REQUIRE(plan.places <= (1 << 27), "lnq_mxfp4_experts_mm: too large");
   LNQ_REQUIRE(workspace && workspace_bytes >= plan.bytes, "lnq_mxfp4_experts_mm: workspace of %lld bytes, %lld needed",
               static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));
   mx4::Args a{};
@@ -571,12 +611,16 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   a.ws = tiles;
   a.y = static_cast<uint16_t*>(y);
   a.M = static_cast<int>(x_rows);
+  a.S = static_cast<int>(plan.places);
   a.N = static_cast<int>(out_features);
   a.K = static_cast<int>(in_features);
   LNQ_REQUIRE(static_cast<int64_t>(plan.tiles) * ((out_features + 63) / 64) <= INT32_MAX,
               "lnq_mxfp4_experts_mm: too large");
-  a.order = static_cast<const int*>(workspace);
-  a.table = reinterpret_cast<const i32x4*>(static_cast<const uint8_t*>(workspace) + plan.order_bytes);
+  auto* const space = static_cast<uint8_t*>(workspace);
+  auto* const order = reinterpret_cast<int*>(space);
+  auto* const sorted = reinterpret_cast<uint32_t*>(space + plan.order_bytes + plan.table_bytes);
+  a.order = order;
+  a.table = reinterpret_cast<const i32x4*>(space + plan.order_bytes);
   a.used = reinterpret_cast<const int*>(a.table + plan.tiles);
   a.tiles = plan.tiles;
   a.count = static_cast<int>(num_experts);
@@ -585,8 +629,13 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   a.ws_step = static_cast<int64_t>(mx4::units_of(a.K) + 1) / 2 * mx4::blocks_of(a.N) * mx4::TILE_BYTES;
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(expert_lists_kernel, dim3(a.count + 1), dim3(mx4::LIST_THREADS), 0, s, experts, static_cast<int>(pairs),
-                     a.count, plan.bm, const_cast<int*>(a.order), const_cast<i32x4*>(a.table), const_cast<int*>(a.used));
+                     a.count, plan.bm, order, const_cast<i32x4*>(a.table), const_cast<int*>(a.used));
   if (const LnqStatus st = launched("expert_lists")) return st;
+  hipLaunchKernelGGL(expert_scales_kernel,
+                     dim3(static_cast<unsigned>((plan.places + 255) / 256), static_cast<unsigned>(mx4::units_of(a.K))), dim3(256),
+                     0, s, a.xs, sorted, order, a.table, a.used, mx4::fours(a.M), a.S, plan.bm, a.chosen);
+  if (const LnqStatus st = launched("expert_scales")) return st;
+  a.xs = sorted;
   if (dtype == LNQ_BF16) mx4::launch<LNQ_BF16, true>(a, plan.bm, s);
   else mx4::launch<LNQ_F16, true>(a, plan.bm, s);
   return launched("mxfp4_experts_mm");

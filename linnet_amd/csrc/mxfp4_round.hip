@@ -102,8 +102,7 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_quantize_kernel(const type
   if ((threadIdx.x & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(byte);
 }
 
-// Rows for the product: codes [rows, K / 2] as above, scales [units][rows] dwords of four
-// blocks (128 inputs). A workgroup takes 16 PASSES rows by 128 inputs, 16 lanes a row, all of its
+// Rows for the product: codes [rows, K / 2] as above, scales as mx4.hpp has x's. A workgroup takes 16 PASSES rows by 128 inputs, 16 lanes a row, all of its
 // loads before its first conversion; its scales leave in a run.
 template <int DT, int PASSES>
 __global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename Elem<DT>::storage* __restrict__ x,
@@ -136,8 +135,8 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename
     if ((lane & 15) == 0) unit[r] = four;
   }
   __syncthreads();
-  if (threadIdx.x < ROWS && r0 + static_cast<int>(threadIdx.x) < rows)
-    scales[static_cast<int64_t>(blockIdx.y) * rows + r0 + threadIdx.x] = unit[threadIdx.x];
+  const int padded = mx4::fours(rows), r = r0 + threadIdx.x;
+  if (threadIdx.x < ROWS && r < padded) scales[static_cast<int64_t>(blockIdx.y) * padded + r] = r < rows ? unit[threadIdx.x] : 0u;
 }
 
 template <int DT>
@@ -165,20 +164,22 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_dequantize_kernel(const ui
   }
 }
 
-// Scales as stored, [count, N, groups], as scale tiles (mx4.hpp), a workgroup a tile.
+// Scales as stored, [count, N, groups], as scale tiles (mx4.hpp), a workgroup two tiles.
 __global__ __launch_bounds__(mxr::THREADS) void mxfp4_scale_tiles_kernel(const uint8_t* __restrict__ scales,
                                                                          uint32_t* __restrict__ tiles, int N, int groups) {
-  const int lane = threadIdx.x >> 2, h = (threadIdx.x >> 1) & 1, u = threadIdx.x & 1;
+  const int block = blockIdx.x * 2 + (threadIdx.x >> 7), blocks = mx4::blocks_of(N);
+  if (block >= blocks) return;
+  const int lane = (threadIdx.x >> 1) & 63, u = threadIdx.x & 1;
   const int g = (2 * blockIdx.y + u) * 4 + (lane >> 4);
   uint32_t word = 0;
 #pragma unroll
   for (int f = 0; f < 4; ++f) {
-    const int n = blockIdx.x * 128 + 64 * h + 16 * f + (lane & 15);
+    const int n = block * 64 + 16 * f + (lane & 15);
     if (n < N && g < groups)
       word |= static_cast<uint32_t>(scales[(static_cast<int64_t>(blockIdx.z) * N + n) * groups + g]) << (8 * f);
   }
-  const int64_t tile = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
-  tiles[tile * (mx4::TILE_BYTES / 4) + threadIdx.x] = word;
+  const int64_t tile = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * blocks + block;
+  tiles[tile * (mx4::TILE_BYTES / 4) + (threadIdx.x & 127)] = word;
 }
 
 }  // namespace lnq
@@ -289,7 +290,7 @@ LNQ_API LnqStatus lnq_mxfp4_scale_tiles(const uint8_t* scales, uint8_t* tiles, i
   LNQ_REQUIRE(aligned(tiles, 16), "lnq_mxfp4_scale_tiles: tiles must be 16-byte aligned");
   LNQ_REQUIRE(count <= 65535 && in_features <= 256 * 65535 && out_features <= INT32_MAX - 128, "lnq_mxfp4_scale_tiles: too large");
   const int N = static_cast<int>(out_features), K = static_cast<int>(in_features);
-  const dim3 grid(static_cast<unsigned>(mx4::blocks_of(N)), static_cast<unsigned>((mx4::units_of(K) + 1) / 2),
+  const dim3 grid(static_cast<unsigned>((mx4::blocks_of(N) + 1) / 2), static_cast<unsigned>((mx4::units_of(K) + 1) / 2),
                   static_cast<unsigned>(count));
   hipLaunchKernelGGL(mxfp4_scale_tiles_kernel, grid, dim3(mxr::THREADS), 0, static_cast<hipStream_t>(stream), scales,
                      reinterpret_cast<uint32_t*>(tiles), N, K / 32);

@@ -589,13 +589,13 @@ def _mxfp4_operands(what: str, blocks: torch.Tensor, scales: torch.Tensor) -> in
 
 
 def _mxfp4_row_scales(what: str, scales: torch.Tensor, rows: int, in_features: int) -> None:
-    shape = (-(-in_features // 128), rows, 4)
+    shape = (-(-in_features // 128), -(-rows // 4) * 4, 4)
     if scales.dtype != torch.uint8 or tuple(scales.shape) != shape:
         raise LinnetError(f"{what}: the rows' scales are {list(shape)} uint8, got {list(scales.shape)} {scales.dtype}")
 
 
 def _mxfp4_tile_shape(lead: tuple[int, ...], out_features: int, in_features: int) -> tuple[int, ...]:
-    return (*lead, -(-in_features // 256), -(-out_features // 128), 64, 16)
+    return (*lead, -(-in_features // 256), -(-out_features // 64), 64, 8)
 
 
 def _mxfp4_tiles(what: str, tiles: torch.Tensor, lead: tuple[int, ...], out_features: int, in_features: int) -> None:
@@ -647,8 +647,8 @@ def mxfp4_dequantize(blocks: torch.Tensor, scales: torch.Tensor, dtype: torch.dt
 
 def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Each row of `x` [rows, In] (bf16, f16 or f32) rounded to MXFP4 as `mxfp4_quantize` does, laid
-    out for `mxfp4_mm`: `(q [rows, In/2] u8, scales [ceil(In/128), rows, 4] u8)`, a row's four scales
-    of 128 inputs together."""
+    out for `mxfp4_mm`: `(q [rows, In/2] u8, scales [ceil(In/128), rows rounded up to 4, 4] u8)`, a
+    row's four scales of 128 inputs together."""
     device = _on_gpu("mxfp4_rows", x)
     if x.dim() != 2 or x.shape[1] % 32:
         raise LinnetError(f"mxfp4_rows: x is [rows, In] with In % 32 == 0, got {tuple(x.shape)}")
@@ -657,7 +657,7 @@ def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
         x = _aligned(x)
     q = torch.empty(rows, depth // 2, dtype=torch.uint8, device=device)
-    scales = torch.empty(-(-depth // 128), rows, 4, dtype=torch.uint8, device=device)
+    scales = torch.empty(-(-depth // 128), -(-rows // 4) * 4, 4, dtype=torch.uint8, device=device)
     with _on(device):
         _lib.call("lnq_mxfp4_rows", _ptr(x), x.stride(0), _ptr(q), _ptr(scales), rows, depth, code, _stream(device))
     return q, scales
@@ -665,7 +665,7 @@ def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def mxfp4_scale_tiles(scales: torch.Tensor, in_features: int) -> torch.Tensor:
     """A weight's scales as stored ([Out, In/32], or [E, Out, In/32] for experts) as the scale tiles
-    that `mxfp4_mm` / `mxfp4_experts_mm` read ([(E,) ceil(In/256), ceil(Out/128), 64, 16]);
+    that `mxfp4_mm` / `mxfp4_experts_mm` read ([(E,) ceil(In/256), ceil(Out/64), 64, 8]);
     made once, when the weight is loaded."""
     device = _on_gpu("mxfp4_scale_tiles", scales)
     if scales.dtype != torch.uint8 or scales.dim() not in (2, 3) or in_features != 32 * scales.shape[-1]:
@@ -761,7 +761,7 @@ def mxfp4_experts_mm(q: torch.Tensor, x_scale: torch.Tensor, blocks: torch.Tenso
     y = torch.empty(rows, chosen, out_features, dtype=dtype, device=device)
     need = ctypes.c_int64(0)
     with _on(device):
-        _lib.call("lnq_mxfp4_experts_workspace", rows * chosen, count, ctypes.byref(need))
+        _lib.call("lnq_mxfp4_experts_workspace", rows * chosen, count, groups * 32, ctypes.byref(need))
         space = torch.empty(need.value, dtype=torch.uint8, device=device)
         _lib.call("lnq_mxfp4_experts_mm", _ptr(q), _ptr(x_scale), _ptr(blocks), _ptr(tiles), _ptr(ids), _ptr(y), rows, chosen,
                   count, out_features, groups * 32, int(q.shape[0] == rows), code, _ptr(space), need.value, _stream(device))

@@ -140,21 +140,22 @@ def test_rows_are_quantize_laid_out(rows: int, depth: int, dtype: torch.dtype) -
         blocks, scales = kernels.mxfp4_quantize(x)
         assert torch.equal(q, blocks.view(rows, depth // 2))
         units = -(-depth // 128)
-        want = torch.zeros(rows, units * 4, dtype=torch.uint8, device=DEV)
-        want[:, : depth // 32] = scales
-        assert torch.equal(row_scales, want.view(rows, units, 4).permute(1, 0, 2))
+        padded = -(-rows // 4) * 4
+        want = torch.zeros(padded, units * 4, dtype=torch.uint8, device=DEV)
+        want[:rows, : depth // 32] = scales
+        assert torch.equal(row_scales, want.view(padded, units, 4).permute(1, 0, 2))
 
 
 @pytest.mark.parametrize(("lead", "out", "depth"), [((), 1, 32), ((), 128, 256), ((5,), 70, 288), ((2,), 300, 2880)])
 def test_scale_tiles(lead: tuple[int, ...], out: int, depth: int) -> None:
     scales = torch.randint(0, 256, (*lead, out, depth // 32), dtype=torch.uint8, device=DEV)
     tiles = kernels.mxfp4_scale_tiles(scales, depth)
-    pairs, blocks = -(-depth // 256), -(-out // 128)
-    assert tiles.shape == (*lead, pairs, blocks, 64, 16)
-    full = torch.zeros(*lead, blocks * 128, pairs * 8, dtype=torch.uint8, device=DEV)
+    pairs, blocks = -(-depth // 256), -(-out // 64)
+    assert tiles.shape == (*lead, pairs, blocks, 64, 8)
+    full = torch.zeros(*lead, blocks * 64, pairs * 8, dtype=torch.uint8, device=DEV)
     full[..., :out, : depth // 32] = scales
-    # [block, h, f, r] x [pair, u, j] -> [pair, block, (j, r), (h, u, f)]
-    full = full.view(-1, blocks, 2, 4, 16, pairs, 2, 4).permute(0, 5, 1, 7, 4, 2, 6, 3)
+    # [block, f, r] x [pair, u, j] -> [pair, block, (j, r), (u, f)]
+    full = full.view(-1, blocks, 4, 16, pairs, 2, 4).permute(0, 4, 1, 6, 3, 5, 2)
     assert torch.equal(tiles.view(-1), full.reshape(-1))
 
 
@@ -247,9 +248,11 @@ def test_nothing_behind_the_last_row_is_read_into_the_sums_or_written() -> None:
             return room
 
         # Scales of outputs past the last are NaN too.
-        pad = torch.full((-(-out // 128) * 128, depth // 32), 255, dtype=torch.uint8, device=DEV)
+        pad = torch.full((-(-out // 64) * 64, depth // 32), 255, dtype=torch.uint8, device=DEV)
         pad[:out] = scales
         tiles = kernels.mxfp4_scale_tiles(pad, depth)
+        row_scales = row_scales.clone()
+        row_scales[:, rows:] = 255
         held = [behind(t) for t in (q, row_scales, blocks, tiles)]
         y = torch.full((rows * out + 4096,), 3.0, dtype=torch.bfloat16, device=DEV)
         _lib.call("lnq_mxfp4_mm", *(t.data_ptr() for t in held), None, y.data_ptr(), rows, out, depth, _lib.BF16,
@@ -360,13 +363,13 @@ def test_refusals() -> None:
         (lambda: kernels.mxfp4_w4a16(x, u8(8, 3, 16), u8(8, 3)), "against"),
         (lambda: kernels.mxfp4_w4a16(x.float(), u8(8, 2, 16), u8(8, 2)), "dtype"),
         (lambda: kernels.mxfp4_w4a16(x, u8(8, 2, 16), u8(8, 2), torch.zeros(8, device=DEV)), "bias"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 3, 16), u8(1, 1, 64, 16), torch.bfloat16), "against"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 8, 4), u8(8, 2, 16), u8(1, 1, 64, 16), torch.bfloat16), "rows' scales"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(2, 1, 64, 16), torch.bfloat16), "scale tiles"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(1, 1, 64, 16), torch.float32), "dtype"),
-        (lambda: kernels.mxfp4_experts_mm(u8(5, 32), u8(1, 5, 4), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 16),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 3, 16), u8(1, 1, 64, 8), torch.bfloat16), "against"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 8, 4), u8(8, 2, 16), u8(1, 1, 64, 8), torch.bfloat16), "rows' scales"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(2, 1, 64, 8), torch.bfloat16), "scale tiles"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(1, 1, 64, 8), torch.float32), "dtype"),
+        (lambda: kernels.mxfp4_experts_mm(u8(5, 32), u8(1, 8, 4), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8),
                                           torch.zeros(4, 2, dtype=torch.int64, device=DEV), torch.bfloat16), "against"),
-        (lambda: kernels.mxfp4_experts_mm(u8(4, 32), u8(1, 4, 4), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 16),
+        (lambda: kernels.mxfp4_experts_mm(u8(4, 32), u8(1, 4, 4), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8),
                                           torch.zeros(4, 2, device=DEV), torch.bfloat16), "integers"),
         (lambda: quantized.mxfp4_operands(u8(2, 8, 2, 16), u8(2, 8, 2), 1), "blocks"),
         (lambda: quantized.mxfp4_experts_operands(u8(8, 2, 16), u8(8, 2), 1), "blocks"),
@@ -379,7 +382,7 @@ def test_refusals() -> None:
 
 def test_workspace_is_checked() -> None:
     need = ctypes.c_int64(0)
-    _lib.call("lnq_mxfp4_experts_workspace", 64, 8, ctypes.byref(need))
+    _lib.call("lnq_mxfp4_experts_workspace", 64, 8, 64, ctypes.byref(need))
     with pytest.raises(LinnetError, match="workspace"):
         _lib.call("lnq_mxfp4_experts_mm", *[4096] * 6, 16, 4, 8, 64, 64, 1, _lib.BF16, 4096, need.value - 1, None)
 

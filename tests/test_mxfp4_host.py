@@ -51,8 +51,8 @@ def _status(name: str, *args: object) -> tuple[int, str]:
     ("lnq_mxfp4_mm", (FAKE, ODD, FAKE, FAKE, NULL, FAKE, 4, 8, 64, 0, NULL), "aligned"),
     ("lnq_mxfp4_mm", (FAKE, FAKE, FAKE, FAKE, NULL, FAKE, 1 << 28, 8, 64, 0, NULL), "2^27"),
     ("lnq_mxfp4_mm", (FAKE, FAKE, FAKE, FAKE, NULL, FAKE, 1 << 27, 1 << 27, 64, 0, NULL), "too large"),
-    ("lnq_mxfp4_experts_workspace", (-1, 4, ctypes.byref(ctypes.c_int64())), "pairs"),
-    ("lnq_mxfp4_experts_workspace", (4, 4096, ctypes.byref(ctypes.c_int64())), "experts"),
+    ("lnq_mxfp4_experts_workspace", (-1, 4, 64, ctypes.byref(ctypes.c_int64())), "pairs"),
+    ("lnq_mxfp4_experts_workspace", (4, 4096, 64, ctypes.byref(ctypes.c_int64())), "experts"),
     ("lnq_mxfp4_experts_mm", (*[FAKE] * 6, 4, 2, 4096, 8, 64, 1, 0, FAKE, 1 << 30, NULL), "experts=4096"),
     ("lnq_mxfp4_experts_mm", (*[FAKE] * 6, 4, 2, 4, 8, 64, 1, 2, FAKE, 1 << 30, NULL), "bf16 or f16"),
     ("lnq_mxfp4_experts_mm", (*[FAKE] * 6, 4, 2, 4, 8, 64, 1, 0, FAKE, 16, NULL), "workspace of 16 bytes"),
@@ -89,8 +89,8 @@ def test_the_wrappers_refuse_cpu_tensors() -> None:
                  lambda: kernels.mxfp4_dequantize(u8(2, 1, 16), u8(2, 1), torch.float32),
                  lambda: kernels.mxfp4_scale_tiles(u8(2, 1), 32),
                  lambda: kernels.mxfp4_w4a16(torch.zeros(2, 32).bfloat16(), u8(2, 1, 16), u8(2, 1)),
-                 lambda: kernels.mxfp4_mm(u8(2, 16), u8(1, 2, 4), u8(2, 1, 16), u8(1, 1, 64, 16), torch.bfloat16),
-                 lambda: kernels.mxfp4_experts_mm(u8(2, 16), u8(1, 2, 4), u8(3, 2, 1, 16), u8(3, 1, 1, 64, 16),
+                 lambda: kernels.mxfp4_mm(u8(2, 16), u8(1, 4, 4), u8(2, 1, 16), u8(1, 1, 64, 8), torch.bfloat16),
+                 lambda: kernels.mxfp4_experts_mm(u8(2, 16), u8(1, 4, 4), u8(3, 2, 1, 16), u8(3, 1, 1, 64, 8),
                                                   torch.zeros(2, 1, dtype=torch.int64), torch.bfloat16),
                  lambda: kernels.expert_route(torch.zeros(2, 8), 2), lambda: quantized.mxfp4_operands(u8(2, 1, 16), u8(2, 1), 1),
                  lambda: quantized.mxfp4_experts_operands(u8(3, 2, 1, 16), u8(3, 2, 1), 1)):
