@@ -9,20 +9,17 @@
 // writes half the accumulators.)
 //
 // A workgroup owns BM rows by BN columns of y, its waves WM x WN of them, FA x FB MFMA tiles
-// each, and walks its tiles of the launch; the k-steps of all of them form one stream: the loads
-// of step g + 2, the next tile's near a tile's end, are issued while step g multiplies. 256
-// inputs (128 bytes a row) a step: codes and scales move to LDS by buffer_load ... lds, the codes'
-// 16-byte columns XOR-swizzled by bits 1..3 of the row, into two stages. Per step, a region a
-// unit (128 inputs): FA x FB MFMAs on the unit's operands while the next ones are read. One
-// barrier, inside the second: past it every wave's loads of step g + 1 have landed and no wave
-// reads step g's stage again, so the rest reads step g + 1's first operands and issues step g +
-// 2's loads into step g's stage. A tile has an even number of steps (one past K loads nothing and
-// adds zeros), so a step's stage is known at compile time.
+// each, and walks its tiles of the launch; the k-steps of all of them form one stream. 256 inputs
+// (128 bytes a row) a step: codes and scales move to LDS by buffer_load ... lds, the codes' 16-byte
+// columns XOR-swizzled by bits 1..3 of the row, into two stages. Per step, a region a unit (128
+// inputs): FA x FB MFMAs on the unit's operands while the next ones are read. One barrier, inside
+// the second: past it every wave's loads of step g + 1 have landed and no wave reads step g's stage
+// again, so the rest reads step g + 1's first operands and issues step g + 2's loads, the next
+// tile's near a tile's end, into step g's stage.
 //
 // Experts: tiles of BM pairs of one expert, expert by expert with its tiles of rows together for
 // each run of columns; where the next tiles lie is looked up a tile ahead a lookup.
 #include <algorithm>
-#include <cstdlib>
 
 #include "mx4.hpp"
 
@@ -33,11 +30,11 @@ constexpr int LIST_THREADS = 1024;
 
 template <int WM, int WN, int FA_, int FB_>
 struct Form {
-  static constexpr int FA = FA_, FB = FB_;
+  static constexpr int FA = FA_, FB = FB_, BLOCKS = FA_ * WM / 4 > 0 ? FA_ * WM / 4 : 1;  // blocks of 64 rows
   static constexpr int NW = WM * WN, THREADS = 64 * NW;
   static constexpr int BM = 16 * FA * WM, BN = 16 * FB * WN;
   static constexpr int CODES = (BM + BN) * BKB;
-  static constexpr int XC = (BM + 127) / 128, ALL = XC + (BN + 127) / 128;  // loads of a step's scales: x's, all
+  static constexpr int XC = (BLOCKS + 1) / 2, ALL = XC + (BN + 127) / 128;  // loads of a step's scales: x's, all
   static constexpr int STAGE = CODES + ALL * 1024;         // the codes, x's scales of the 2 units, the weight's
   static constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;  // loads of a wave a step: 8 rows of codes each
   static constexpr int LOADS = LA + LB + 1;                // and of scales
@@ -45,7 +42,7 @@ struct Form {
   static constexpr int PER_CU = GROUPS < 4 ? GROUPS : 4;
   static constexpr int WAVES_A_SIMD = NW * PER_CU / 4 > 0 ? NW * PER_CU / 4 : 1;
   static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN && NW % 2 == 0, "whole loads, one key a wave");
-  static_assert((FB == 2 || FB == 4) && BN % 64 == 0 && (FA == 2 || FA == 4 || FA == 8) && ALL <= NW, "scales a lane");
+  static_assert((FB == 2 || FB == 4 || FB == 8) && BN % 64 == 0 && (FA == 2 || FA == 4 || FA == 8) && ALL <= NW, "scales a lane");
 };
 }  // namespace mx4
 
@@ -54,7 +51,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   using namespace mx4;
   using E = Elem<DT>;
   constexpr int FA = FORM::FA, FB = FORM::FB, NW = FORM::NW, BM = FORM::BM, BN = FORM::BN, CODES = FORM::CODES;
-  constexpr int LA = FORM::LA, LB = FORM::LB, LOADS = FORM::LOADS, XC = FORM::XC;
+  constexpr int LA = FORM::LA, LB = FORM::LB, LOADS = FORM::LOADS, XC = FORM::XC, BLOCKS = FORM::BLOCKS;
   constexpr int WN = BN / 16 / FB;
   // One array per stage: the compiler then waits, before reading a stage, for that stage's
   // loads only.
@@ -78,33 +75,25 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
     mine = b0 < total ? (total - 1 - b0) / G + 1 : 0;
   }
   if (mine == 0) return;
-  const int steps = (a.K + 2 * BK - 1) / (2 * BK) * 2;
+  const int steps = (a.K + 2 * BK - 1) / (2 * BK) * 2;  // a step past K adds zeros
   const int nsteps = mine * steps;
   const uint32_t row_bytes = static_cast<uint32_t>(a.K) >> 1;
-  const int units = units_of(a.K);
-  const uint32_t pair_bytes = static_cast<uint32_t>(blocks_of(a.N)) * TILE_BYTES;
 
   // Load i of wave w fills stage rows 8 (NW i + w) .. + 7 (i < LA: rows of x; then columns): lane l
   // row l / 8 at byte 16 l of the 1 KB, stored column l % 8 holding source column (l % 8) ^
-  // key(row), key = (row >> 1) & 7, the same for every i. Rows past the last lie past the buffer,
-  // or nowhere.
+  // key(row), key = (row >> 1) & 7, the same for every i. Rows past the last lie nowhere.
   const int lr = 8 * wave + (lane >> 3);
   const uint32_t lcol = 16u * ((lane & 7) ^ ((lr >> 1) & 7));
-  const uint32_t voff = static_cast<uint32_t>(lr) * row_bytes + lcol;  // of load i: 8 NW i rows on
-  uint32_t xoff[EXPERTS ? LA : 1];
-  // This wave's load of scales, a kilobyte: x's rows at the step's two units, or the scale tiles of
-  // 128 columns (waves past the last load what others do). soff: nowhere past what a step has.
+  // This wave's load of scales, a kilobyte: two tiles of x's rows or of columns (waves past the last
+  // load what others do). soff: nowhere past what a step has.
   const int chunk = wave % FORM::ALL;
   const bool x_chunk = chunk < XC;
-  uint32_t soff;
-  {
-    const int d = (x_chunk ? chunk : chunk - XC) * 256 + lane * 4;  // dword
-    if (x_chunk) soff = d < 2 * BM ? (static_cast<uint32_t>(d / BM) * a.S + d % BM) * 4u : NOWHERE;
-    else soff = d < 2 * BN ? static_cast<uint32_t>(d) * 4u : NOWHERE;
-  }
+  const uint32_t scale_at = static_cast<uint32_t>(x_chunk ? chunk : chunk - XC) * 1024 + lane * 16;
+  const uint32_t soff = scale_at < static_cast<uint32_t>((x_chunk ? BLOCKS : BN / 64) * TILE_BYTES) ? scale_at : NOWHERE;
+  const uint32_t s_step = static_cast<uint32_t>(x_chunk ? a.x_blocks : blocks_of(a.N)) * TILE_BYTES;
 
   // A tile of this launch: columns from n0; rows from m0, or an expert's pairs from `first` (their
-  // scales from m0).
+  // scales as rows from m0).
   struct Tile {
     int n0, m0, live, first, e;
   };
@@ -120,7 +109,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
     const int many = __builtin_amdgcn_readfirstlane(any.z) >> 9, tile0 = __builtin_amdgcn_readfirstlane(any.w);
     const int j = place_of(r) - tile0 * tiles_n;
     n0 = j / many * BN;
-    m0 = (tile0 + j % many) * BM;
+    m0 = (tile0 + j % many) * (BLOCKS * 64);
     return a.table[tile0 + j % many];
   };
   auto expert_tile = [&](i32x4 entry, int n0, int m0) -> Tile {
@@ -136,43 +125,50 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
     }
   };
 
-  // The tile whose steps are being loaded; of the scales their base, what a step adds to it, and the
-  // bytes of a step, of a step of one unit. (Chosen here: a choice in the steps would be a branch, and
-  // the compiler then moves the MFMAs across the blocks it splits the step into.)
+  // The tile whose steps are being loaded: where this wave's rows lie from the bases, and the bytes
+  // from there. (Chosen here: a choice in the steps would be a branch, and the compiler then moves the
+  // MFMAs across the blocks it splits the step into.)
   const uint8_t *qb, *wb, *sb;
-  uint32_t q_bytes, w_bytes, s_two, s_one;
-  const uint32_t s_step = x_chunk ? static_cast<uint32_t>(a.S) * 8u : pair_bytes;
+  uint32_t q_bytes, w_bytes, s_bytes, xoff[LA], woff[LB];
   auto load_tile = [&](const Tile& t) {
     const int e = EXPERTS ? min(t.e, a.count - 1) : 0;  // a tile of no expert multiplies the last one's weight, for nothing
     qb = a.q + (EXPERTS ? 0 : static_cast<int64_t>(t.m0) * row_bytes);
     q_bytes = static_cast<uint32_t>(EXPERTS ? a.M : t.live) * row_bytes;
     wb = a.w + e * a.w_step + static_cast<int64_t>(t.n0) * row_bytes;
-    w_bytes = static_cast<uint32_t>(min(BN, a.N - t.n0)) * row_bytes;
-    const uint32_t column = static_cast<uint32_t>(t.n0 / 64) * TILE_BYTES, rows = static_cast<uint32_t>(fours(t.live));
-    sb = x_chunk ? reinterpret_cast<const uint8_t*>(a.xs + t.m0) : a.ws + e * a.ws_step + column;
-    s_two = x_chunk ? (static_cast<uint32_t>(a.S) + rows) * 4u : pair_bytes - column;
-    s_one = x_chunk ? rows * 4u : pair_bytes - column;
-    if constexpr (EXPERTS) {
+    const int outs = min(BN, a.N - t.n0);
+    w_bytes = static_cast<uint32_t>(outs) * row_bytes;
+    const uint32_t from = static_cast<uint32_t>(x_chunk ? t.m0 : t.n0) / 64 * TILE_BYTES;
+    sb = (x_chunk ? a.xs : a.ws + e * a.ws_step) + from;
+    s_bytes = s_step - from;
 #pragma unroll
-      for (int i = 0; i < LA; ++i)
-        xoff[i] = lr + 8 * NW * i < t.live ? static_cast<uint32_t>(pairs[i] / a.chosen) * row_bytes + lcol : NOWHERE;
+    for (int i = 0; i < LA; ++i) {
+      const int r = lr + 8 * NW * i;
+      xoff[i] = r < t.live ? static_cast<uint32_t>(EXPERTS ? pairs[EXPERTS ? i : 0] / a.chosen : r) * row_bytes + lcol : NOWHERE;
+    }
+#pragma unroll
+    for (int i = 0; i < LB; ++i) {
+      const int r = lr + 8 * NW * i;
+      woff[i] = r < outs ? static_cast<uint32_t>(r) * row_bytes + lcol : NOWHERE;
     }
   };
-  // Load i of k-step ks into stage st. Steps past the stream, and columns and units past K, read
-  // through 0-byte descriptors or past the buffer.
-  auto load_one = [&](uint8_t* st, bool in, int ks, int i) __attribute__((always_inline)) {
+  // The sources of a k-step's loads; steps past the stream or past K read through 0-byte ones. The
+  // last step of a row may end inside a line: x's bytes past it are left out, the weight's then
+  // multiply zeros (every code is finite, and scales past K are 0).
+  struct Source {
+    __amdgpu_buffer_rsrc_t q, w, s;
+    uint32_t past;
+  };
+  auto source_of = [&](bool in, int ks) __attribute__((always_inline)) -> Source {
     const uint32_t k0 = static_cast<uint32_t>(ks) * BKB;
     const bool live = in && k0 < row_bytes;
-    if (i < LA + LB) {
-      const bool x = i < LA;
-      const uint32_t past = k0 + lcol >= row_bytes ? NOWHERE : 0u;
-      const uint32_t at = EXPERTS && x ? xoff[EXPERTS && x ? i : 0] : voff + static_cast<uint32_t>(8 * NW * (x ? i : i - LA)) * row_bytes;
-      load16(buffer_rsrc((x ? qb : wb) + k0, live ? (x ? q_bytes : w_bytes) - k0 : 0u), st + (NW * i + wave) * 1024, at | past);
-    } else {
-      const uint32_t bytes = units - 2 * ks >= 2 ? s_two : s_one;
-      load16(buffer_rsrc(sb + static_cast<uint64_t>(static_cast<uint32_t>(ks)) * s_step, live ? bytes : 0u),
-             st + CODES + chunk * 1024, soff);
-    }
+    return Source{buffer_rsrc(qb + k0, live ? q_bytes - k0 : 0u), buffer_rsrc(wb + k0, live ? w_bytes - k0 : 0u),
+                  buffer_rsrc(sb + static_cast<uint64_t>(static_cast<uint32_t>(ks)) * s_step, live ? s_bytes : 0u),
+                  k0 + lcol >= row_bytes ? NOWHERE : 0u};
+  };
+  auto load_one = [&](uint8_t* st, const Source& from, int i) __attribute__((always_inline)) {
+    if (i < LA) load16(from.q, st + (NW * i + wave) * 1024, xoff[i < LA ? i : 0] | from.past);
+    else if (i < LA + LB) load16(from.w, st + (NW * i + wave) * 1024, woff[i >= LA && i < LA + LB ? i - LA : 0]);
+    else load16(from.s, st + CODES + chunk * 1024, soff);
   };
 
   f32x4 acc[FA][FB];
@@ -184,74 +180,67 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
     aoff[u] = static_cast<uint32_t>(swz8(wm * FA * 16 + lrow, 4 * u + lk));
     boff[u] = static_cast<uint32_t>(swz8(BM + wn * FB * 16 + lrow, 4 * u + lk));
   }
-  const uint32_t sa_at = static_cast<uint32_t>(CODES + (wm * FA * 16 + lrow) * 4);
-  const uint32_t sw_at = static_cast<uint32_t>(CODES + XC * 1024 + wn * FB * 16 / 64 * TILE_BYTES + lane * 8);
-  const int first_byte = wn * FB % 4;  // of this wave's columns in their dword
+  // Scales of this wave's rows and columns, a dword a unit for 4 fragments (for 2: the half of a
+  // dword from these bits on).
+  constexpr int SA = FA == 8 ? 2 : 1, SB = FB == 8 ? 2 : 1;
+  const uint32_t sa_at = static_cast<uint32_t>(CODES + wm * FA / 4 * TILE_BYTES + lane * 8);
+  const uint32_t sw_at = static_cast<uint32_t>(CODES + XC * 1024 + wn * FB / 4 * TILE_BYTES + lane * 8);
+  const int a_bits = 8 * (wm * FA % 4), w_bits = 8 * (wn * FB % 4);
 
-  // Operands: the columns' of a unit, a set a unit; the rows' and their scale dwords in a ring of
-  // 4, read three rows of MFMAs ahead (a wave of two rows: a set a unit too).
+  // Operands: the columns' of a unit, a set a unit; the rows' in a ring of 4, read three rows of
+  // MFMAs ahead (a wave of two rows: a set a unit too); both's scales, a set a unit.
   constexpr bool RING = FA >= 4;
   i32x4 af[4], bf[2][FB];
-  uint32_t sa[4], sw[2];
+  uint32_t sa[2][SA], sw[2][SB];
   auto read_a = [&](int u, const uint8_t* st, int f) __attribute__((always_inline)) {
     af[(RING ? 0 : 2 * u) + (f & 3)] = *reinterpret_cast<const i32x4*>(st + aoff[u] + f * 16 * BKB);
-    sa[(RING ? 0 : 2 * u) + (f & 3)] = *reinterpret_cast<const uint32_t*>(st + sa_at + u * BM * 4 + f * 64);
   };
   auto read_b = [&](int u, const uint8_t* st, int f) __attribute__((always_inline)) {
     bf[u][f] = *reinterpret_cast<const i32x4*>(st + boff[u] + f * 16 * BKB);
   };
+  auto read_scales = [&](int u, const uint8_t* st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < SA; ++h) sa[u][h] = *reinterpret_cast<const uint32_t*>(st + sa_at + h * TILE_BYTES + u * 4);
+#pragma unroll
+    for (int h = 0; h < SB; ++h) sw[u][h] = *reinterpret_cast<const uint32_t*>(st + sw_at + h * TILE_BYTES + u * 4);
+  };
 
   // Unit u of a step on stage `cur`, a slot an MFMA: a row's first slot reads the rows ahead, others
-  // the next unit's columns. In the second unit, from row TURN on, those are the next step's, from
-  // `nxt`, and the slots issue step g + 2's loads (k-step ks2, `in` whether inside the stream) into
-  // `cur`: ahead of that row this wave's loads of step g + 1 have landed and its reads of `cur`,
-  // all of whose operands it has read, are done; past the barrier every wave's.
+  // the next unit's columns and scales. In the second unit, from row TURN on, those are the next
+  // step's, from `nxt`, and the slots issue step g + 2's loads into `cur`: ahead of that row this
+  // wave's loads of step g + 1 have landed and its reads of `cur`, all of whose operands it has read,
+  // are done; past the barrier every wave's.
   constexpr int SLOTS = FA * FB, TURN = RING ? FA - 3 : 0;
-  auto region = [&](auto unit_tag, auto first_tag, const uint8_t* cur, const uint8_t* nxt, bool in,
-                    int ks2) __attribute__((always_inline)) {
+  auto region = [&](auto unit_tag, const uint8_t* cur, const uint8_t* nxt, const Source& from) __attribute__((always_inline)) {
     constexpr int U = decltype(unit_tag)::value;
-    constexpr bool FIRST = decltype(first_tag)::value;  // a tile's first step
     constexpr int AT = RING ? 0 : 2 * U, FROM = U == 1 ? TURN * FB : 0;
-    if constexpr (FB == 2) sw[U] >>= 8 * first_byte;
-#pragma unroll
-    for (int s = 0; s < SLOTS; ++s) {
-      const int i = s / FB, j = s % FB;
-      if (U == 1 && s == FROM) {
+    if constexpr (FA == 2) sa[U][0] >>= a_bits;
+    if constexpr (FB == 2) sw[U][0] >>= w_bits;
+    each_of([&](auto slot) __attribute__((always_inline)) {
+      constexpr int s = decltype(slot)::value, i = s / FB, j = s % FB;
+      if constexpr (U == 1 && s == FROM) {
         wait_vm<0>();
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
       }
-      const f32x4 c = FIRST && U == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][j];
-      if (j == 0) sa[AT + (i & 3)] >>= 8 * lk;  // this lane's block of the unit
       // The weight is the MFMA's A operand: a lane then holds 4 outputs of a row together.
-      acc[i][j] = mma(bf[U][j], af[AT + (i & 3)], c, j, sw[U], sa[AT + (i & 3)]);
-      if (j == 0) {
-        if (!RING) read_a(U ^ 1, nxt, i);
-        else if (i + 3 < FA) read_a(U, cur, i + 3);
+      acc[i][j] = mma<j & 3, i & 3>(bf[U][j], af[AT + (i & 3)], acc[i][j], sw[U][j / 4], sa[U][i / 4]);
+      if constexpr (j == 0) {
+        if constexpr (!RING) read_a(U ^ 1, nxt, i);
+        else if constexpr (i + 3 < FA) read_a(U, cur, i + 3);
         else read_a(U ^ 1, nxt, i + 3 - FA);
       }
-#pragma unroll
-      for (int f = 0; f < FB; ++f)
-        if (s == FROM + 1 + 2 * f) read_b(U ^ 1, nxt, f);
-      if (s == FROM + 2) sw[U ^ 1] = *reinterpret_cast<const uint32_t*>(nxt + sw_at + (U ^ 1) * 4);
-      if (U == 1 && s >= FROM) {
+      if constexpr (s > FROM && (s - FROM - 1) % 2 == 0 && (s - FROM - 1) / 2 < FB) read_b(U ^ 1, nxt, (s - FROM - 1) / 2);
+      if constexpr (s == FROM + 2) read_scales(U ^ 1, nxt);
+      if constexpr (U == 1 && s >= FROM) {
 #pragma unroll
         for (int q = 0; q < LOADS; ++q)
-          if (FROM + q * (SLOTS - FROM) / LOADS == s) load_one(const_cast<uint8_t*>(cur), in, ks2, q);
+          if (FROM + q * (SLOTS - FROM) / LOADS == s) load_one(const_cast<uint8_t*>(cur), from, q);
       }
       __builtin_amdgcn_sched_barrier(0);
-    }
+    }, std::make_integer_sequence<int, SLOTS>{});
   };
-  using Zero = std::integral_constant<int, 0>;
-  using One = std::integral_constant<int, 1>;
-  using T = std::integral_constant<bool, true>;
-  using No = std::integral_constant<bool, false>;
-  auto step = [&](auto first_tag, const uint8_t* cur, const uint8_t* nxt, bool in, int ks2) __attribute__((always_inline)) {
-    region(Zero{}, first_tag, cur, cur, false, 0);
-    region(One{}, first_tag, cur, nxt, in, ks2);
-  };
-
   // Lane l, register r of fragment (i, j): row 16 i + l % 16 of the wave's, column 16 j + 4 (l / 16)
   // + r. Two fragments' trade between the lanes of a row (v_permlane16_swap) gives each lane 8
   // columns together, and with four fragments the lanes of rows r and r + 8 trade (row_ror:8), so
@@ -259,39 +248,38 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   // took a quarter of a 4096 x 8192 -> 28672 call's time, as the next step's wait for its loads waits
   // for the stores too).
   typedef u32x4 __attribute__((aligned(2))) loose_u32x4;  // rows of an odd width begin anywhere
-  auto epilogue = [&](const Tile& t) {
-    const bool none = EXPERTS && t.e >= a.count;  // pairs whose choice is no expert: zeros
+  constexpr int STORES = FB == 2 ? 1 : 2;                // of a row of (up to four) fragments
+  auto epilogue_of = [&](const Tile& t, auto bias_tag) __attribute__((always_inline)) {
+    constexpr bool BIAS = decltype(bias_tag)::value;
     const int n0 = t.n0 + wn * FB * 16;
-    float bias[FB][4];
+    float bias[BIAS ? FB : 1][4];
+    if constexpr (BIAS) {
 #pragma unroll
-    for (int j = 0; j < FB; ++j)
+      for (int j = 0; j < FB; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = n0 + 16 * j + 4 * lk + r;
-        bias[j][r] = !EXPERTS && a.bias != nullptr && n < a.N ? E::to_f32(a.bias[n]) : 0.f;
-      }
-    int to_row[EXPERTS ? 2 * FA : 1];
-    auto row_at = [&](int i, int h) -> int {  // of store h of row i of fragments
-      return (wm * FA + i) * 16 + (FB == 4 ? (lrow & 7) + 8 * h : lrow);
-    };
+        for (int r = 0; r < 4; ++r) bias[j][r] = E::to_f32(a.bias[min(n0 + 16 * j + 4 * lk + r, a.N - 1)]);
+    }
+    // This lane's row of store h of row i of fragments, of the tile: first + 16 i + 8 h; its columns.
+    const int first = wm * FA * 16 + (FB == 2 ? lrow : lrow & 7);
+    const int n = n0 + 16 * (lk & 1) + 8 * (lk >> 1) + (FB == 2 ? 0 : 32 * (lrow >> 3));
+    int to_row[EXPERTS ? STORES * FA : 1];
     if constexpr (EXPERTS) {
 #pragma unroll
-      for (int i = 0; i < 2 * FA; ++i) to_row[i] = a.order[t.first + min(row_at(i >> 1, i & 1), t.live - 1)];
+      for (int i = 0; i < STORES * FA; ++i) to_row[i] = a.order[t.first + min(first + (16 / STORES) * i, t.live - 1)];
     }
     __builtin_amdgcn_sched_barrier(0);
-    auto store = [&](int i, int h, int n, u32x4 v) {
-      const int m = row_at(i, h);
-      int64_t row;
-      if constexpr (EXPERTS) row = to_row[2 * i + h];
-      else row = t.m0 + m;
-      if (m >= t.live) return;
-      uint16_t* const to = a.y + row * a.N + n;
-      if (n + 8 <= a.N) {
-        *reinterpret_cast<loose_u32x4*>(to) = v;
-      } else {
+    uint16_t* to = EXPERTS ? a.y + n : a.y + static_cast<int64_t>(t.m0 + first) * a.N + n;
+    const int64_t step = static_cast<int64_t>(16 / STORES) * a.N;
+    auto store = [&](int i, int c, u32x4 v) {  // at column n + c
+      uint16_t* const at = (EXPERTS ? to + static_cast<int64_t>(to_row[EXPERTS ? i : 0]) * a.N : to) + c;
+      if (first + (16 / STORES) * i < t.live) {
+        if (n + c + 8 <= a.N) {
+          *reinterpret_cast<loose_u32x4*>(at) = v;
+        } else {
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (n + r < a.N) to[r] = static_cast<uint16_t>(v[r >> 1] >> (16 * (r & 1)));
+          for (int r = 0; r < 8; ++r)
+            if (n + c + r < a.N) at[r] = static_cast<uint16_t>(v[r >> 1] >> (16 * (r & 1)));
+        }
       }
     };
 #pragma unroll
@@ -301,8 +289,9 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
       for (int j = 0; j < FB; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t lo = E::from_f32(acc[i][j][2 * h] + bias[j][2 * h]), hi = E::from_f32(acc[i][j][2 * h + 1] + bias[j][2 * h + 1]);
-          o[j][h] = none ? 0u : lo | (hi << 16);
+          float lo = acc[i][j][2 * h], hi = acc[i][j][2 * h + 1];
+          if constexpr (BIAS) lo += bias[j][2 * h], hi += bias[j][2 * h + 1];
+          o[j][h] = DT == LNQ_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
         }
       // Lane quarter k of fragments 2 p, 2 p + 1 then holds columns 8 (k / 2) .. + 7 of fragment 2 p + k % 2.
 #pragma unroll
@@ -312,32 +301,64 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
           const auto r = __builtin_amdgcn_permlane16_swap(o[j][h], o[j + 1][h], false, false);
           o[j][h] = r[0], o[j + 1][h] = r[1];
         }
-      const int n = n0 + 16 * (lk & 1) + 8 * (lk >> 1);
-      if constexpr (FB == 4) {
-        u32x4 p, q;
-        const uint32_t pv[4] = {o[0][0], o[0][1], o[1][0], o[1][1]}, qv[4] = {o[2][0], o[2][1], o[3][0], o[3][1]};
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          // Rows 0 .. 7: the first half of the columns from their own lanes, the second in the lanes of
-          // rows 8 .. 15; then the same of those rows.
-          p[d] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(pv[d]), static_cast<int>(qv[d]), 0x128, 0xf, 0xc, false));
-          q[d] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(qv[d]), static_cast<int>(pv[d]), 0x128, 0xf, 0x3, false));
-        }
-        store(i, 0, n + 32 * (lrow >> 3), p);
-        store(i, 1, n + 32 * (lrow >> 3), q);
+      if constexpr (FB == 2) {
+        store(i, 0, u32x4{o[0][0], o[0][1], o[1][0], o[1][1]});
+        if (!EXPERTS) to += step;
       } else {
-        store(i, 0, n, u32x4{o[0][0], o[0][1], o[1][0], o[1][1]});
+        u32x4 p[FB / 4], q[FB / 4];
+#pragma unroll
+        for (int j = 0; j < FB; j += 4) {
+          const uint32_t pv[4] = {o[j][0], o[j][1], o[j + 1][0], o[j + 1][1]};
+          const uint32_t qv[4] = {o[j + 2][0], o[j + 2][1], o[j + 3][0], o[j + 3][1]};
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            // Rows 0 .. 7: the first half of the columns from their own lanes, the second in the lanes of
+            // rows 8 .. 15; then the same of those rows.
+            p[j / 4][d] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(pv[d]), static_cast<int>(qv[d]), 0x128, 0xf, 0xc, false));
+            q[j / 4][d] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(qv[d]), static_cast<int>(pv[d]), 0x128, 0xf, 0x3, false));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < FB / 4; ++j) store(2 * i, 64 * j, p[j]);
+        if (!EXPERTS) to += step;
+#pragma unroll
+        for (int j = 0; j < FB / 4; ++j) store(2 * i + 1, 64 * j, q[j]);
+        if (!EXPERTS) to += step;
       }
       // One row of fragments at a time: the next tile's operands are live here.
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  auto epilogue = [&](const Tile& t) __attribute__((always_inline)) {
+    if (!EXPERTS && a.bias != nullptr) {
+      epilogue_of(t, std::true_type{});
+    } else {
+      if (EXPERTS && t.e >= a.count) {  // pairs whose choice is no expert: zeros
+#pragma unroll
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+          for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      epilogue_of(t, std::false_type{});
+    }
+  };
 
-  // Prologue: tiles 0 .. 2 looked up; steps 0 and 1 requested; step 0 landed (this wave's, then
-  // every wave's); its first operands and scales read.
-  Tile now, next;
+  // `now` multiplies, `loading` is the tile of the loads (the same, or the next one: a tile has two
+  // steps or more), tile `ready` comes after it. Experts: its rows' pairs are asked for, the entry of
+  // the one after and the expert of the one after that, a tile before they are used.
+  Tile now, loading, next;
   i32x4 ahead = {0, 0, 0, 0}, ahead2 = {0, 0, 0, 0};
-  int ahead_n0 = 0, ahead_m0 = 0;
+  int ahead_n0 = 0, ahead_m0 = 0, ready = 1;
+  auto prepare = [&]() {
+    if constexpr (EXPERTS) {
+      next = expert_tile(ahead, ahead_n0, ahead_m0);
+      ahead = entry_of(ready + 1, ahead2, ahead_n0, ahead_m0);
+      ahead2 = expert_of(ready + 2);
+      take_pairs(next);
+    } else {
+      next = plain_tile(min(ready, mine - 1));
+    }
+  };
   if constexpr (EXPERTS) {
     int n0, m0;
     const i32x4 entry = entry_of(0, expert_of(0), n0, m0);
@@ -348,45 +369,51 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
     now = plain_tile(0);
   }
   take_pairs(now);
-  load_tile(now);
+  loading = now;
+  load_tile(loading);
+  // Steps 0 and 1 requested; step 0 landed (this wave's, then every wave's); its first operands and
+  // scales read.
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) load_one(L0, true, 0, i);
+  for (int j = 0; j < 2; ++j) {
+    const Source from = source_of(true, j);
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) load_one(L1, true, 1, i);
-  wait_vm<0>();
+    for (int i = 0; i < LOADS; ++i) load_one(j ? L1 : L0, from, i);
+  }
+  wait_vm<LOADS>();
   __builtin_amdgcn_s_barrier();
 #pragma unroll
   for (int i = 0; i < FB; ++i) read_b(0, L0, i);
 #pragma unroll
   for (int i = 0; i < (RING ? 3 : 2); ++i) read_a(0, L0, i);
-  sw[0] = *reinterpret_cast<const uint32_t*>(L0 + sw_at);
+  read_scales(0, L0);
+  prepare();
 
-  // Pairs of steps g, g + 1 of a tile at k-step ks on stages L0, L1: they issue steps g + 2, g +
-  // 3, the next pair's (this tile's, or the next one's after its last), with no branch inside.
-  auto pair = [&](int g, int ks, auto first_tag) __attribute__((always_inline)) {
-    const bool ends = ks + 2 == steps;
-    const int ks_n = ends ? 0 : ks + 2;
-    if (ends) load_tile(next);
-    step(first_tag, L0, L1, g + 2 < nsteps, ks_n);
-    step(No{}, L1, L0, g + 3 < nsteps, ks_n + 1);
+  int ks = 2;  // k-step of the next load
+  // Step g on stage `cur`, no branch inside.
+  auto step = [&](uint8_t* cur, uint8_t* nxt, bool in) __attribute__((always_inline)) {
+    const Source from = source_of(in, ks);
+    region(std::integral_constant<int, 0>{}, cur, cur, from);
+    region(std::integral_constant<int, 1>{}, cur, nxt, from);
+    ++ks;
   };
-  int g = 0;
-  for (int r = 0; r < mine; ++r) {
-    // Tile r + 1 from what the last tile looked up; its pairs, the entry of r + 2 and the expert of
-    // r + 3 asked for: none is used before this tile's last steps.
-    if constexpr (EXPERTS) {
-      next = expert_tile(ahead, ahead_n0, ahead_m0);
-      ahead = entry_of(r + 2, ahead2, ahead_n0, ahead_m0);
-      ahead2 = expert_of(r + 3);
-    } else {
-      next = plain_tile(min(r + 1, mine - 1));
+  for (int g = 0; g < nsteps;) {
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (const int end = g + steps; g < end; g += 2) {
+      if (ks == steps) {
+        ks = 0;
+        loading = next;
+        load_tile(loading);
+        ++ready;
+        prepare();
+      }
+      step(L0, L1, g + 2 < nsteps);
+      step(L1, L0, g + 3 < nsteps);
     }
-    take_pairs(next);
-    pair(g, 0, T{});
-    g += 2;
-    for (int ks = 2; ks < steps; ks += 2, g += 2) pair(g, ks, No{});
     epilogue(now);
-    now = next;
+    now = loading;
   }
   // Loads of the steps past the stream (0-byte reads) may be in flight.
   wait_vm<0>();
@@ -461,18 +488,25 @@ __global__ __launch_bounds__(mx4::LIST_THREADS) void expert_lists_kernel(const i
   });
 }
 
-// x's scales by the tiles' rows, [units][tiles][bm]: a tile's then lie together (read row by row, a
-// dword each, they were as many lines as the codes).
-__global__ __launch_bounds__(256) void expert_scales_kernel(const uint32_t* __restrict__ from, uint32_t* __restrict__ to,
+// x's scales by the tiles' rows, as scale tiles: `each` blocks of 64 rows a tile of the product.
+__global__ __launch_bounds__(256) void expert_scales_kernel(const uint8_t* __restrict__ from, uint32_t* __restrict__ to,
                                                             const int* __restrict__ order, const i32x4* __restrict__ table,
-                                                            const int* __restrict__ used, int rows, int places, int bm,
-                                                            int chosen) {
-  const int i = blockIdx.x * 256 + threadIdx.x, t = i / bm, r = i - t * bm;
+                                                            const int* __restrict__ used, int from_blocks, int blocks,
+                                                            int each, int chosen) {
+  const int i = blockIdx.x * 256 + threadIdx.x, block = i >> 7, t = block / each;
   if (t >= used[0]) return;
   const i32x4 entry = table[t];
-  if (r >= mx4::fours(entry.z & 511)) return;
-  const int row = order[entry.y + min(r, (entry.z & 511) - 1)] / chosen;
-  to[static_cast<int64_t>(blockIdx.y) * places + i] = from[static_cast<int64_t>(blockIdx.y) * rows + row];
+  const int live = entry.z & 511, r0 = (block - t * each) * 64 + (i >> 1 & 15);  // of the tile
+  const int64_t pair = blockIdx.y;
+  const uint32_t at = (i >> 5 & 3) * 128 + (i & 1) * 4;  // block of the unit, unit
+  uint32_t word = 0;
+#pragma unroll
+  for (int f = 0; f < 4; ++f) {
+    const int row = order[entry.y + min(r0 + 16 * f, live - 1)] / chosen;
+    const uint8_t byte = from[(pair * from_blocks + (row >> 6)) * mx4::TILE_BYTES + at + (row & 15) * 8 + (row >> 4 & 3)];
+    word |= static_cast<uint32_t>(byte) << (8 * f);
+  }
+  to[pair * blocks * 128 + i] = word;
 }
 
 namespace mx4 {
@@ -493,21 +527,21 @@ using Form64 = Form<2, 2, 2, 2>;
 using Form32 = Form<1, 2, 2, 2>;
 
 // Rows of a tile.
-static int tile_rows(double rows) { 
-  if (const char* t = getenv("MXT")) return atoi(t);
-  return rows > 64 ? 128 : rows > 32 ? 64 : 32; }
+static int tile_rows(double rows) { return rows > 256 ? 256 : rows > 64 ? 128 : rows > 32 ? 64 : 32; }
 
 template <int DT, bool EXPERTS>
 static void launch(const Args& a, int bm, hipStream_t s) {
-  if (bm == 32) launch_form<DT, Form32, EXPERTS>(a, s);
-  else if (bm == 64) launch_form<DT, Form64, EXPERTS>(a, s);
+  if constexpr (EXPERTS) {
+    if (bm == 32) return launch_form<DT, Form32, EXPERTS>(a, s);
+  }
+  if (bm == 64 || bm == 32) launch_form<DT, Form64, EXPERTS>(a, s);
   else if (bm == 128) launch_form<DT, Form128, EXPERTS>(a, s);
   else launch_form<DT, Form256, EXPERTS>(a, s);
 }
 
 struct Plan {
-  int bm, tiles;
-  int64_t places, order_bytes, table_bytes, bytes;
+  int bm, tiles, each;
+  int64_t blocks, order_bytes, table_bytes, bytes;
 };
 
 // Tiles of the pairs at most: a partial one for each expert that is named. The workspace: order,
@@ -518,8 +552,9 @@ static Plan experts_plan(int64_t pairs, int64_t count, int64_t in_features) {
   p.tiles = static_cast<int>(pairs / p.bm + std::min(pairs, count + 1));
   p.order_bytes = (pairs * 4 + 15) / 16 * 16;
   p.table_bytes = static_cast<int64_t>(p.tiles) * 16 + 16;
-  p.places = static_cast<int64_t>(p.tiles) * p.bm;
-  p.bytes = p.order_bytes + p.table_bytes + (in_features + 127) / 128 * p.places * 4;
+  p.each = (p.bm + 63) / 64;
+  p.blocks = static_cast<int64_t>(p.tiles) * p.each;
+  p.bytes = p.order_bytes + p.table_bytes + (in_features + 255) / 256 * p.blocks * TILE_BYTES;
   return p;
 }
 
@@ -549,13 +584,13 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
               "lnq_mxfp4_mm: operands must be 16-byte aligned");
   mx4::Args a{};
   a.q = q;
-  a.xs = reinterpret_cast<const uint32_t*>(x_scale);
+  a.xs = x_scale;
   a.w = blocks;
   a.ws = tiles;
   a.bias = static_cast<const uint16_t*>(bias);
   a.y = static_cast<uint16_t*>(y);
   a.M = static_cast<int>(rows);
-  a.S = mx4::fours(a.M);
+  a.x_blocks = mx4::blocks_of(a.M);
   a.N = static_cast<int>(out_features);
   a.K = static_cast<int>(in_features);
   LNQ_REQUIRE((rows + 31) / 32 * ((out_features + 63) / 64) <= INT32_MAX, "lnq_mxfp4_mm: too large");
@@ -601,24 +636,24 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   const int64_t pairs = rows * chosen, x_rows = shared ? rows : pairs;
   LNQ_REQUIRE(x_rows * (in_features / 2) < (int64_t{1} << 31), "lnq_mxfp4_experts_mm: x's codes past 2 GiB");
   const mx4::Plan plan = mx4::experts_plan(pairs, num_experts, in_features);
-  LNQ_REQUIRE(plan.places <= (1 << 27), "lnq_mxfp4_experts_mm: too large");
+  LNQ_REQUIRE(plan.blocks <= (1 << 21), "lnq_mxfp4_experts_mm: too large");
   LNQ_REQUIRE(workspace && workspace_bytes >= plan.bytes, "lnq_mxfp4_experts_mm: workspace of %lld bytes, %lld needed",
               static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));
   mx4::Args a{};
   a.q = q;
-  a.xs = reinterpret_cast<const uint32_t*>(x_scale);
+  a.xs = x_scale;
   a.w = blocks;
   a.ws = tiles;
   a.y = static_cast<uint16_t*>(y);
   a.M = static_cast<int>(x_rows);
-  a.S = static_cast<int>(plan.places);
+  a.x_blocks = static_cast<int>(plan.blocks);
   a.N = static_cast<int>(out_features);
   a.K = static_cast<int>(in_features);
   LNQ_REQUIRE(static_cast<int64_t>(plan.tiles) * ((out_features + 63) / 64) <= INT32_MAX,
               "lnq_mxfp4_experts_mm: too large");
   auto* const space = static_cast<uint8_t*>(workspace);
   auto* const order = reinterpret_cast<int*>(space);
-  auto* const sorted = reinterpret_cast<uint32_t*>(space + plan.order_bytes + plan.table_bytes);
+  uint8_t* const sorted = space + plan.order_bytes + plan.table_bytes;
   a.order = order;
   a.table = reinterpret_cast<const i32x4*>(space + plan.order_bytes);
   a.used = reinterpret_cast<const int*>(a.table + plan.tiles);
@@ -626,14 +661,14 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   a.count = static_cast<int>(num_experts);
   a.chosen = shared ? static_cast<int>(chosen) : 1;
   a.w_step = out_features * (in_features / 2);
-  a.ws_step = static_cast<int64_t>(mx4::units_of(a.K) + 1) / 2 * mx4::blocks_of(a.N) * mx4::TILE_BYTES;
+  a.ws_step = static_cast<int64_t>(mx4::pairs_of(a.K)) * mx4::blocks_of(a.N) * mx4::TILE_BYTES;
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(expert_lists_kernel, dim3(a.count + 1), dim3(mx4::LIST_THREADS), 0, s, experts, static_cast<int>(pairs),
                      a.count, plan.bm, order, const_cast<i32x4*>(a.table), const_cast<int*>(a.used));
   if (const LnqStatus st = launched("expert_lists")) return st;
-  hipLaunchKernelGGL(expert_scales_kernel,
-                     dim3(static_cast<unsigned>((plan.places + 255) / 256), static_cast<unsigned>(mx4::units_of(a.K))), dim3(256),
-                     0, s, a.xs, sorted, order, a.table, a.used, mx4::fours(a.M), a.S, plan.bm, a.chosen);
+  hipLaunchKernelGGL(expert_scales_kernel, dim3(static_cast<unsigned>((plan.blocks + 1) / 2), static_cast<unsigned>(mx4::pairs_of(a.K))),
+                     dim3(256), 0, s, x_scale, reinterpret_cast<uint32_t*>(sorted), order, a.table, a.used, mx4::blocks_of(a.M),
+                     a.x_blocks, plan.each, a.chosen);
   if (const LnqStatus st = launched("expert_scales")) return st;
   a.xs = sorted;
   if (dtype == LNQ_BF16) mx4::launch<LNQ_BF16, true>(a, plan.bm, s);

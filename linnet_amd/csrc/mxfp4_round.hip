@@ -102,8 +102,9 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_quantize_kernel(const type
   if ((threadIdx.x & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(byte);
 }
 
-// Rows for the product: codes [rows, K / 2] as above, scales as mx4.hpp has x's. A workgroup takes 16 PASSES rows by 128 inputs, 16 lanes a row, all of its
-// loads before its first conversion; its scales leave in a run.
+// Rows for the product: codes [rows, K / 2] as above, scales as scale tiles (mx4.hpp). A workgroup
+// takes 16 PASSES rows by 128 inputs, 16 lanes a row, all of its loads before its first conversion;
+// then its scales: dwords of two blocks of 64 rows, or one byte of each dword of its block.
 template <int DT, int PASSES>
 __global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename Elem<DT>::storage* __restrict__ x,
                                                                   int64_t x_stride, uint32_t* __restrict__ codes,
@@ -132,11 +133,28 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename
     uint32_t four = in ? byte << (8 * ((lane >> 2) & 3)) : 0u;
     four |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(four), 4, 64));
     four |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(four), 8, 64));
-    if ((lane & 15) == 0) unit[r] = four;
+    if ((lane & 15) == 0) unit[r] = r0 + r < rows ? four : 0u;
   }
   __syncthreads();
-  const int padded = mx4::fours(rows), r = r0 + threadIdx.x;
-  if (threadIdx.x < ROWS && r < padded) scales[static_cast<int64_t>(blockIdx.y) * padded + r] = r < rows ? unit[threadIdx.x] : 0u;
+  const int blocks = mx4::blocks_of(rows), block = r0 / 64 + static_cast<int>(threadIdx.x >> 6);
+  if (threadIdx.x >= (ROWS > 64 ? ROWS : 64) || block >= blocks) return;
+  const int u = blockIdx.y & 1, row = lane & 15, shift = 8 * (lane >> 4);
+  const bool alone = u == 0 && blockIdx.y + 1 == gridDim.y;  // the pair's second unit lies past K
+  uint32_t* const at = scales + ((static_cast<int64_t>(blockIdx.y >> 1) * blocks + block) * 64 + lane) * 2;
+  if constexpr (ROWS >= 64) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int f = 0; f < 4; ++f) word |= (unit[(threadIdx.x >> 6) * 64 + 16 * f + row] >> shift & 255u) << (8 * f);
+    at[u] = word;
+    if (alone) at[1] = 0;
+  } else {
+    uint8_t* const bytes = reinterpret_cast<uint8_t*>(at);
+    const int f = r0 % 64 / 16, last = r0 + ROWS >= rows ? 4 : f + 1;  // the last rows' workgroup writes the block's rest
+    for (int i = f; i < last; ++i) {
+      bytes[4 * u + i] = static_cast<uint8_t>(i == f ? unit[row] >> shift : 0u);
+      if (alone) bytes[4 + i] = 0;
+    }
+  }
 }
 
 template <int DT>

@@ -588,12 +588,6 @@ def _mxfp4_operands(what: str, blocks: torch.Tensor, scales: torch.Tensor) -> in
     return blocks.shape[-2] * 32
 
 
-def _mxfp4_row_scales(what: str, scales: torch.Tensor, rows: int, in_features: int) -> None:
-    shape = (-(-in_features // 128), -(-rows // 4) * 4, 4)
-    if scales.dtype != torch.uint8 or tuple(scales.shape) != shape:
-        raise LinnetError(f"{what}: the rows' scales are {list(shape)} uint8, got {list(scales.shape)} {scales.dtype}")
-
-
 def _mxfp4_tile_shape(lead: tuple[int, ...], out_features: int, in_features: int) -> tuple[int, ...]:
     return (*lead, -(-in_features // 256), -(-out_features // 64), 64, 8)
 
@@ -647,8 +641,8 @@ def mxfp4_dequantize(blocks: torch.Tensor, scales: torch.Tensor, dtype: torch.dt
 
 def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Each row of `x` [rows, In] (bf16, f16 or f32) rounded to MXFP4 as `mxfp4_quantize` does, laid
-    out for `mxfp4_mm`: `(q [rows, In/2] u8, scales [ceil(In/128), rows rounded up to 4, 4] u8)`, a
-    row's four scales of 128 inputs together."""
+    out for `mxfp4_mm`: `(q [rows, In/2] u8, scales [ceil(In/256), ceil(rows/64), 64, 8] u8)`, the
+    scales as `mxfp4_scale_tiles` lays out a weight's."""
     device = _on_gpu("mxfp4_rows", x)
     if x.dim() != 2 or x.shape[1] % 32:
         raise LinnetError(f"mxfp4_rows: x is [rows, In] with In % 32 == 0, got {tuple(x.shape)}")
@@ -657,7 +651,7 @@ def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
         x = _aligned(x)
     q = torch.empty(rows, depth // 2, dtype=torch.uint8, device=device)
-    scales = torch.empty(-(-depth // 128), -(-rows // 4) * 4, 4, dtype=torch.uint8, device=device)
+    scales = torch.empty(_mxfp4_tile_shape((), rows, depth), dtype=torch.uint8, device=device)
     with _on(device):
         _lib.call("lnq_mxfp4_rows", _ptr(x), x.stride(0), _ptr(q), _ptr(scales), rows, depth, code, _stream(device))
     return q, scales
@@ -721,7 +715,7 @@ def mxfp4_mm(q: torch.Tensor, x_scale: torch.Tensor, blocks: torch.Tensor, tiles
     rows = q.shape[0]
     if q.shape[1] * 2 != depth:
         raise LinnetError(f"mxfp4_mm: q {tuple(q.shape)} against blocks {tuple(blocks.shape)}")
-    _mxfp4_row_scales("mxfp4_mm", x_scale, rows, depth)
+    _mxfp4_tiles("mxfp4_mm", x_scale, (), rows, depth)
     _mxfp4_tiles("mxfp4_mm", tiles, (), out_features, depth)
     code = _code(dtype, "mxfp4_mm")
     bias = _mxfp4_bias("mxfp4_mm", bias, dtype, out_features)
@@ -753,7 +747,7 @@ def mxfp4_experts_mm(q: torch.Tensor, x_scale: torch.Tensor, blocks: torch.Tenso
     if q.shape[0] not in (rows, rows * chosen) or q.shape[1] != groups * 16:
         raise LinnetError(f"mxfp4_experts_mm: q {tuple(q.shape)} against experts {tuple(experts.shape)} and blocks "
                           f"{tuple(blocks.shape)}")
-    _mxfp4_row_scales("mxfp4_experts_mm", x_scale, q.shape[0], groups * 32)
+    _mxfp4_tiles("mxfp4_experts_mm", x_scale, (), q.shape[0], groups * 32)
     _mxfp4_tiles("mxfp4_experts_mm", tiles, (count,), out_features, groups * 32)
     code = _code(dtype, "mxfp4_experts_mm")
     q, x_scale, blocks, tiles = _aligned(q), _aligned(x_scale), _aligned(blocks), _aligned(tiles)

@@ -139,11 +139,7 @@ def test_rows_are_quantize_laid_out(rows: int, depth: int, dtype: torch.dtype) -
         q, row_scales = kernels.mxfp4_rows(x)
         blocks, scales = kernels.mxfp4_quantize(x)
         assert torch.equal(q, blocks.view(rows, depth // 2))
-        units = -(-depth // 128)
-        padded = -(-rows // 4) * 4
-        want = torch.zeros(padded, units * 4, dtype=torch.uint8, device=DEV)
-        want[:rows, : depth // 32] = scales
-        assert torch.equal(row_scales, want.view(padded, units, 4).permute(1, 0, 2))
+        assert torch.equal(row_scales, kernels.mxfp4_scale_tiles(scales, depth))
 
 
 @pytest.mark.parametrize(("lead", "out", "depth"), [((), 1, 32), ((), 128, 256), ((5,), 70, 288), ((2,), 300, 2880)])
@@ -251,8 +247,9 @@ def test_nothing_behind_the_last_row_is_read_into_the_sums_or_written() -> None:
         pad = torch.full((-(-out // 64) * 64, depth // 32), 255, dtype=torch.uint8, device=DEV)
         pad[:out] = scales
         tiles = kernels.mxfp4_scale_tiles(pad, depth)
-        row_scales = row_scales.clone()
-        row_scales[:, rows:] = 255
+        pad = torch.full((-(-rows // 64) * 64, depth // 32), 255, dtype=torch.uint8, device=DEV)
+        pad[:rows] = kernels.mxfp4_quantize(x)[1]
+        row_scales = kernels.mxfp4_scale_tiles(pad, depth)
         held = [behind(t) for t in (q, row_scales, blocks, tiles)]
         y = torch.full((rows * out + 4096,), 3.0, dtype=torch.bfloat16, device=DEV)
         _lib.call("lnq_mxfp4_mm", *(t.data_ptr() for t in held), None, y.data_ptr(), rows, out, depth, _lib.BF16,
@@ -363,13 +360,13 @@ def test_refusals() -> None:
         (lambda: kernels.mxfp4_w4a16(x, u8(8, 3, 16), u8(8, 3)), "against"),
         (lambda: kernels.mxfp4_w4a16(x.float(), u8(8, 2, 16), u8(8, 2)), "dtype"),
         (lambda: kernels.mxfp4_w4a16(x, u8(8, 2, 16), u8(8, 2), torch.zeros(8, device=DEV)), "bias"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 3, 16), u8(1, 1, 64, 8), torch.bfloat16), "against"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 8, 4), u8(8, 2, 16), u8(1, 1, 64, 8), torch.bfloat16), "rows' scales"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(2, 1, 64, 8), torch.bfloat16), "scale tiles"),
-        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 4, 4), u8(8, 2, 16), u8(1, 1, 64, 8), torch.float32), "dtype"),
-        (lambda: kernels.mxfp4_experts_mm(u8(5, 32), u8(1, 8, 4), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 1, 64, 8), u8(8, 3, 16), u8(1, 1, 64, 8), torch.bfloat16), "against"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 2, 64, 8), u8(8, 2, 16), u8(1, 1, 64, 8), torch.bfloat16), "scale tiles"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 1, 64, 8), u8(8, 2, 16), u8(2, 1, 64, 8), torch.bfloat16), "scale tiles"),
+        (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 1, 64, 8), u8(8, 2, 16), u8(1, 1, 64, 8), torch.float32), "dtype"),
+        (lambda: kernels.mxfp4_experts_mm(u8(5, 32), u8(1, 1, 64, 8), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8),
                                           torch.zeros(4, 2, dtype=torch.int64, device=DEV), torch.bfloat16), "against"),
-        (lambda: kernels.mxfp4_experts_mm(u8(4, 32), u8(1, 4, 4), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8),
+        (lambda: kernels.mxfp4_experts_mm(u8(4, 32), u8(1, 1, 64, 8), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8),
                                           torch.zeros(4, 2, device=DEV), torch.bfloat16), "integers"),
         (lambda: quantized.mxfp4_operands(u8(2, 8, 2, 16), u8(2, 8, 2), 1), "blocks"),
         (lambda: quantized.mxfp4_experts_operands(u8(8, 2, 16), u8(8, 2), 1), "blocks"),
