@@ -20,6 +20,7 @@
 // Experts: tiles of BM pairs of one expert, expert by expert with its tiles of rows together for
 // each run of columns; where the next tiles lie is looked up a tile ahead a lookup.
 #include <algorithm>
+#include <cmath>
 
 #include "mx4.hpp"
 
@@ -274,7 +275,8 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
       uint16_t* const at = (EXPERTS ? to + static_cast<int64_t>(to_row[EXPERTS ? i : 0]) * a.N : to) + c;
       if (first + (16 / STORES) * i < t.live) {
         if (n + c + 8 <= a.N) {
-          *reinterpret_cast<loose_u32x4*>(at) = v;
+          // Past the L2's usual order: what y would push out there, the operands, is read again.
+          __builtin_nontemporal_store(v, reinterpret_cast<loose_u32x4*>(at));
         } else {
 #pragma unroll
           for (int r = 0; r < 8; ++r)
@@ -526,36 +528,58 @@ using Form128 = Form<2, 2, 4, 4>;
 using Form64 = Form<2, 2, 2, 2>;
 using Form32 = Form<1, 2, 2, 2>;
 
-// Rows of a tile.
-static int tile_rows(double rows) { return rows > 256 ? 256 : rows > 64 ? 128 : rows > 32 ? 64 : 32; }
+// Rows of a tile, for `count` matrices of N outputs that multiply `rows` rows each (experts: on
+// average). A larger tile reads each operand less often (a wave of 128 x 64 outputs, 24 KB of LDS for
+// 64 MFMAs; of 64 x 64, 32 KB; of 32 x 32, 64 KB), a smaller one leaves fewer CUs idle and fewer rows
+// empty. Measured on both sides of each bound (256 CUs; us of the smaller | the larger tile):
+// 256 rows from 3/4 of a tile a CU: 2048 x 2880 -> 5760, 184 tiles: 28.7 | 29.9; 1024 x 4096 -> 14336,
+// 224: 37.2 | 34.3; 4096 x 8192 -> 8192, 512: 135 | 117. 128 rows from 5/8: 128 x 4096 -> 14336, 112
+// tiles: 11.4 | 13.6; 512 x 2880 -> 5760, 180: 13.7 | 11.5; 1024 x 4096 -> 4096, 256: 18.9 | 14.2.
+// Of an expert's rows: 256 past 128 (32 experts, 2880 -> 5760: at 75 rows 84 | 95, 188: 142 | 110; 128
+// experts, 2048 -> 1536: at 125 69 | 72, 188: 102 | 89); 128 past 48 (8 experts, 4096 -> 14336: at 25
+// 47 | 51, 100: 74 | 60); 64 past 20 (32 experts, 2880 -> 5760: at 12 61 | 67, 25: 74 | 73).
+static int tile_rows(double rows, int64_t count, int64_t N, bool experts) {
+  const auto tiles = [&](int bm, int bn) {
+    return static_cast<double>(count) * std::ceil(rows / bm) * static_cast<double>((N + bn - 1) / bn);
+  };
+  if (rows > 128 && tiles(256, 256) >= 0.75 * compute_units()) return 256;
+  if (rows > 48 && tiles(128, 128) >= 0.625 * compute_units()) return 128;
+  return rows > 20 || !experts ? 64 : 32;
+}
 
 template <int DT, bool EXPERTS>
 static void launch(const Args& a, int bm, hipStream_t s) {
   if constexpr (EXPERTS) {
     if (bm == 32) return launch_form<DT, Form32, EXPERTS>(a, s);
   }
-  if (bm == 64 || bm == 32) launch_form<DT, Form64, EXPERTS>(a, s);
+  if (bm == 64) launch_form<DT, Form64, EXPERTS>(a, s);
   else if (bm == 128) launch_form<DT, Form128, EXPERTS>(a, s);
   else launch_form<DT, Form256, EXPERTS>(a, s);
 }
 
 struct Plan {
-  int bm, tiles, each;
+  int tiles, each;  // blocks of 64 rows a tile
   int64_t blocks, order_bytes, table_bytes, bytes;
 };
 
-// Tiles of the pairs at most: a partial one for each expert that is named. The workspace: order,
+// Tiles of `bm` pairs at most: a partial one for each expert that is named. The workspace: order,
 // table, how many tiles, scales.
-static Plan experts_plan(int64_t pairs, int64_t count, int64_t in_features) {
+static Plan experts_plan(int bm, int64_t pairs, int64_t count, int64_t in_features) {
   Plan p{};
-  p.bm = tile_rows(static_cast<double>(pairs) / static_cast<double>(count));
-  p.tiles = static_cast<int>(pairs / p.bm + std::min(pairs, count + 1));
+  p.tiles = static_cast<int>(pairs / bm + std::min(pairs, count + 1));
   p.order_bytes = (pairs * 4 + 15) / 16 * 16;
   p.table_bytes = static_cast<int64_t>(p.tiles) * 16 + 16;
-  p.each = (p.bm + 63) / 64;
+  p.each = (bm + 63) / 64;
   p.blocks = static_cast<int64_t>(p.tiles) * p.each;
   p.bytes = p.order_bytes + p.table_bytes + (in_features + 255) / 256 * p.blocks * TILE_BYTES;
   return p;
+}
+
+// Of any outputs: whichever tiles they take.
+static int64_t workspace_of(int64_t pairs, int64_t count, int64_t in_features) {
+  int64_t bytes = 0;
+  for (const int bm : {32, 64, 128, 256}) bytes = std::max(bytes, experts_plan(bm, pairs, count, in_features).bytes);
+  return bytes;
 }
 
 }  // namespace mx4
@@ -595,7 +619,7 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
   a.K = static_cast<int>(in_features);
   LNQ_REQUIRE((rows + 31) / 32 * ((out_features + 63) / 64) <= INT32_MAX, "lnq_mxfp4_mm: too large");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int bm = mx4::tile_rows(static_cast<double>(rows));
+  const int bm = mx4::tile_rows(static_cast<double>(rows), 1, out_features, false);
   if (dtype == LNQ_BF16) mx4::launch<LNQ_BF16, false>(a, bm, s);
   else mx4::launch<LNQ_F16, false>(a, bm, s);
   return launched("mxfp4_mm");
@@ -607,7 +631,7 @@ LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t num_experts
                   in_features <= (1 << 22),
               "lnq_mxfp4_experts_workspace: %lld pairs of %lld experts (1 to %d) of %lld inputs", static_cast<long long>(pairs),
               static_cast<long long>(num_experts), mx4::MAX_EXPERTS, static_cast<long long>(in_features));
-  *bytes = pairs == 0 ? 0 : mx4::experts_plan(pairs, num_experts, in_features).bytes;
+  *bytes = pairs == 0 ? 0 : mx4::workspace_of(pairs, num_experts, in_features);
   clear_error();
   return LNQ_OK;
 }
@@ -635,10 +659,12 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
               "lnq_mxfp4_experts_mm: operands and workspace must be 16-byte aligned");
   const int64_t pairs = rows * chosen, x_rows = shared ? rows : pairs;
   LNQ_REQUIRE(x_rows * (in_features / 2) < (int64_t{1} << 31), "lnq_mxfp4_experts_mm: x's codes past 2 GiB");
-  const mx4::Plan plan = mx4::experts_plan(pairs, num_experts, in_features);
+  const int bm = mx4::tile_rows(static_cast<double>(pairs) / static_cast<double>(num_experts), num_experts, out_features, true);
+  const mx4::Plan plan = mx4::experts_plan(bm, pairs, num_experts, in_features);
   LNQ_REQUIRE(plan.blocks <= (1 << 21), "lnq_mxfp4_experts_mm: too large");
-  LNQ_REQUIRE(workspace && workspace_bytes >= plan.bytes, "lnq_mxfp4_experts_mm: workspace of %lld bytes, %lld needed",
-              static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));
+  const int64_t need = mx4::workspace_of(pairs, num_experts, in_features);
+  LNQ_REQUIRE(workspace && workspace_bytes >= need, "lnq_mxfp4_experts_mm: workspace of %lld bytes, %lld needed",
+              static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   mx4::Args a{};
   a.q = q;
   a.xs = x_scale;
@@ -664,15 +690,15 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   a.ws_step = static_cast<int64_t>(mx4::pairs_of(a.K)) * mx4::blocks_of(a.N) * mx4::TILE_BYTES;
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(expert_lists_kernel, dim3(a.count + 1), dim3(mx4::LIST_THREADS), 0, s, experts, static_cast<int>(pairs),
-                     a.count, plan.bm, order, const_cast<i32x4*>(a.table), const_cast<int*>(a.used));
+                     a.count, bm, order, const_cast<i32x4*>(a.table), const_cast<int*>(a.used));
   if (const LnqStatus st = launched("expert_lists")) return st;
   hipLaunchKernelGGL(expert_scales_kernel, dim3(static_cast<unsigned>((plan.blocks + 1) / 2), static_cast<unsigned>(mx4::pairs_of(a.K))),
                      dim3(256), 0, s, x_scale, reinterpret_cast<uint32_t*>(sorted), order, a.table, a.used, mx4::blocks_of(a.M),
                      a.x_blocks, plan.each, a.chosen);
   if (const LnqStatus st = launched("expert_scales")) return st;
   a.xs = sorted;
-  if (dtype == LNQ_BF16) mx4::launch<LNQ_BF16, true>(a, plan.bm, s);
-  else mx4::launch<LNQ_F16, true>(a, plan.bm, s);
+  if (dtype == LNQ_BF16) mx4::launch<LNQ_BF16, true>(a, bm, s);
+  else mx4::launch<LNQ_F16, true>(a, bm, s);
   return launched("mxfp4_experts_mm");
 }
 

@@ -159,11 +159,13 @@ def test_scale_tiles(lead: tuple[int, ...], out: int, depth: int) -> None:
 
 SIZES = [(1, 1, 32), (3, 7, 96), (33, 64, 128), (64, 100, 160), (65, 257, 256), (129, 130, 288), (300, 513, 544),
          (40, 96, 2880), (257, 300, 1056)]
+# Of 64, 128 and 256 rows a tile, with fewer tiles than workgroups at a time and with more.
+WIDE = [(40, 66000, 64), (70, 20600, 96), (400, 17000, 544), (300, 24701, 288), (1030, 14000, 160), (260, 49500, 32)]
 
 
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("dtype", list(HALF))
-@pytest.mark.parametrize(("rows", "out", "depth"), SIZES)
+@pytest.mark.parametrize(("rows", "out", "depth"), SIZES + WIDE)
 def test_mm(rows: int, out: int, depth: int, dtype: torch.dtype, bias: bool) -> None:
     print(f"mm {rows} x {depth} -> {out} {dtype} bias={bias}", flush=True)
     rng = np.random.default_rng(rows * 7 + out + depth)
@@ -302,7 +304,7 @@ def _experts(rng: np.random.Generator, kind: str, rows: int, chosen: int, count:
 @pytest.mark.parametrize("dtype", list(HALF))
 @pytest.mark.parametrize(("rows", "chosen", "count", "out", "depth"), [
     (1, 1, 1, 1, 32), (33, 4, 8, 70, 96), (40, 2, 5, 128, 288), (70, 1, 3, 33, 160), (257, 4, 4, 64, 128),
-    (300, 3, 40, 36, 64), (64, 8, 2, 200, 544)])
+    (300, 3, 40, 36, 64), (64, 8, 2, 200, 544), (700, 4, 40, 520, 160), (1400, 4, 40, 1100, 96)])
 def test_experts_mm(rows: int, chosen: int, count: int, out: int, depth: int, dtype: torch.dtype, kind: str) -> None:
     print(f"experts {kind} rows={rows} chosen={chosen} E={count} {depth} -> {out} {dtype}", flush=True)
     rng = np.random.default_rng(rows + chosen + count + out)

@@ -141,3 +141,14 @@ def test_route_against_a_search(score: str, groups: int) -> None:
         assert tuple(experts[r]) == best
         chosen = s[list(best)]
         assert np.allclose(weights[r], 2.0 * chosen / chosen.sum(), rtol=1e-14)
+
+
+@pytest.mark.parametrize(("rows", "chosen", "count", "out", "depth"), [(16, 4, 8, 64, 64), (1, 1, 1, 64, 32), (4000, 4, 32, 5760, 2880),
+                                                                       (9, 3, 2048, 100, 288), (300, 8, 4, 30000, 96)])
+def test_experts_workspace_of_one_byte_less_is_refused(rows: int, chosen: int, count: int, out: int, depth: int) -> None:
+    need = ctypes.c_int64(0)
+    _lib.call("lnq_mxfp4_experts_workspace", rows * chosen, count, depth, ctypes.byref(need))
+    assert need.value >= rows * chosen * 4
+    for space, size in ((FAKE, need.value - 1), (FAKE, 0), (NULL, need.value)):
+        with pytest.raises(LinnetError, match="workspace"):
+            _lib.call("lnq_mxfp4_experts_mm", *[FAKE] * 6, rows, chosen, count, out, depth, 1, _lib.BF16, space, size, NULL)
