@@ -17,10 +17,12 @@
 // A wave takes a row: with G groups rounded up to a power of two, 64 / G lanes hold a group, S
 // experts a lane, so that experts rise with the lane and its slot. Bound by VALU issue, not by
 // the row's bytes: so
+// * an exponential is 2^n times a polynomial and a quotient a reciprocal with two Newton steps, a
+//   third of the instructions that the library's functions take for every case;
 // * a group's two best are a butterfly over its lanes, and its rank among the groups a count;
-// * a choice is the wave's largest f32 key, the choice rounded once (order survives rounding):
-//   six DPP maxima. Only where several lanes hold that key, which differ in 64 bits, are
-//   those compared.
+// * a choice is the wave's largest key, the choice rounded once to f32 (order survives rounding)
+//   with its bits in integer order: six DPP maxima. Only where several experts hold that key,
+//   which differ in 64 bits, are those compared.
 #include "common.hpp"
 
 namespace lnq {
@@ -72,16 +74,61 @@ __device__ inline double lane_of(double v, int lane) {
 
 // The wave's largest value: within rows of 16 lanes (row_shr 1, 2, 4, 8), then over the rows
 // (row_bcast 15, 31); lane 63 ends with it.
-template <class T>
-__device__ inline T wave_top(T v) {
-  auto larger = [](T a, T b) { return a > b ? a : b; };
-  v = larger(v, dpp<0x111>(v, v));
-  v = larger(v, dpp<0x112>(v, v));
-  v = larger(v, dpp<0x114>(v, v));
-  v = larger(v, dpp<0x118>(v, v));
-  v = larger(v, dpp<0x142>(v, v));
-  v = larger(v, dpp<0x143>(v, v));
+__device__ inline double wave_top(double v) {
+  v = fmax(v, dpp<0x111>(v, v));
+  v = fmax(v, dpp<0x112>(v, v));
+  v = fmax(v, dpp<0x114>(v, v));
+  v = fmax(v, dpp<0x118>(v, v));
+  v = fmax(v, dpp<0x142>(v, v));
+  v = fmax(v, dpp<0x143>(v, v));
   return lane_of(v, 63);
+}
+
+template <int CTRL>
+__device__ inline uint32_t larger(uint32_t v) {  // 0: what lanes without a partner compare with
+  return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, false)));
+}
+
+__device__ inline uint32_t wave_top(uint32_t v) {
+  v = larger<0x111>(v);
+  v = larger<0x112>(v);
+  v = larger<0x114>(v);
+  v = larger<0x118>(v);
+  v = larger<0x142>(v);
+  v = larger<0x143>(v);
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+}
+
+// A float's bits in the order of integers, above 0 (the place of no choice); both zeros alike.
+__device__ inline uint32_t key_of(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+}
+
+__device__ inline float value_of(uint32_t key) {
+  return __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+// e^x for |x| <= 800 (past a double's range: infinity, 0): x = n ln 2 + r, |r| <= ln 2 / 2, and e^r's
+// series up to r^13 / 13! (the next term is below 2^-57 of it).
+__device__ inline double exp_of(double x) {
+  const double n = rint(x * 0x1.71547652b82fep+0);
+  const double r = fma(n, -0x1.abc9e3b39803fp-56, fma(n, -0x1.62e42fefa39efp-1, x));
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, r, 1.0 / 479001600.0);
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __builtin_amdgcn_ldexp(p, static_cast<int>(n));
 }
 
 // The wave's sum: that of each row of 16 lanes in its last lane, the four added.
@@ -136,11 +183,12 @@ __global__ __launch_bounds__(route::THREADS) void expert_route_kernel(const type
 
   double s[S];
   if (a.softmax) {
-    const double top = wave_top(most);
+    const float high = value_of(wave_top(key_of(most)));
+    const double top = high == nothing ? 0 : high;
     double sum = 0;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      s[i] = l[i] == nothing ? 0 : exp(l[i] - top);
+      s[i] = l[i] == nothing ? 0 : exp_of(fmax(l[i] - top, -800.0));
       sum += s[i];
     }
     sum = wave_total(sum);
@@ -148,21 +196,36 @@ __global__ __launch_bounds__(route::THREADS) void expert_route_kernel(const type
 #pragma unroll
     for (int i = 0; i < S; ++i) s[i] *= part;
   } else {
+    bool far = false;
+    double d[S];
 #pragma unroll
-    for (int i = 0; i < S; ++i) s[i] = l[i] == nothing ? 0 : 1 / (1 + exp(-static_cast<double>(l[i])));
+    for (int i = 0; i < S; ++i) {
+      d[i] = 1 + exp_of(-static_cast<double>(fminf(fmaxf(l[i], -800.0f), 800.0f)));
+      far = far || d[i] > 0x1p1000;
+      double y = __builtin_amdgcn_rcp(d[i]);
+      y = fma(fma(-d[i], y, 1.0), y, y);
+      s[i] = fma(fma(-d[i], y, 1.0), y, y);
+    }
+    if (__ballot(far)) {  // where the steps' products leave a double's range
+#pragma unroll
+      for (int i = 0; i < S; ++i) s[i] = d[i] > 0x1p1000 ? 1 / d[i] : s[i];
+    }
+#pragma unroll
+    for (int i = 0; i < S; ++i) s[i] = l[i] == nothing ? 0 : s[i];
   }
   // The choices and their keys.
   const bool biased = a.bias != nullptr;
   double c[S];
-  float key[S];
+  uint32_t key[S];
 #pragma unroll
   for (int i = 0; i < S; ++i) {
     c[i] = l[i];
+    key[i] = l[i] == nothing ? 0 : key_of(l[i]);
     if (biased && i < held && l[i] != nothing) {
       c[i] = s[i] + static_cast<double>(a.bias[e0 + i]);
-      if (c[i] != c[i]) c[i] = none;
+      if (!(c[i] > none)) c[i] = none;
+      key[i] = c[i] == none ? 0 : key_of(static_cast<float>(c[i]));
     }
-    key[i] = static_cast<float>(c[i]);
   }
 
   if (a.groups > 1) {
@@ -187,47 +250,55 @@ __global__ __launch_bounds__(route::THREADS) void expert_route_kernel(const type
     }
     if (rank >= a.group_top) {
 #pragma unroll
-      for (int i = 0; i < S; ++i) key[i] = nothing;
+      for (int i = 0; i < S; ++i) key[i] = 0;
     }
   }
 
-  // This lane's best: its key, choice, score and expert (the first slot of the largest choice).
-  float best;
-  double best_c, best_s;
-  int best_e;
-  auto look = [&]() {
-    best = nothing, best_c = none, best_s = 0, best_e = -1;
-#pragma unroll
-    for (int i = 0; i < S; ++i) {
-      const bool better = key[i] > best || (key[i] == best && key[i] != nothing && c[i] > best_c);
-      best = better ? key[i] : best;
-      best_c = better ? c[i] : best_c;
-      best_s = better ? s[i] : best_s;
-      best_e = better ? i : best_e;
-    }
-  };
-  look();
   int mine = -1;
   double weight = 0, total = 0;
   for (int i = 0; i < a.top; ++i) {
-    const float top = wave_top(best);
-    if (top == nothing) break;
-    uint64_t mask = __ballot(best == top);
-    if (biased && (mask & (mask - 1))) {
-      const double first = wave_top(best == top ? best_c : none);
-      mask = __ballot(best == top && best_c == first);
+    uint32_t best = key[0];
+#pragma unroll
+    for (int j = 1; j < S; ++j) best = max(best, key[j]);
+    const uint32_t top = wave_top(best);
+    if (top == 0) break;
+    // The lanes that hold it in each slot; of several the first expert, by the choices themselves
+    // where those are more than the key shows.
+    uint64_t with[S], any = 0, twice = 0;
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      with[j] = __ballot(key[j] == top);
+      twice |= any & with[j];
+      any |= with[j];
     }
-    const int owner = __builtin_ctzll(mask);
-    const double v = lane_of(best_s, owner);
-    const int at = __builtin_amdgcn_readlane(e0 + best_e, owner);
+    if (biased && (twice | (any & (any - 1)))) {
+      double most_c = none;
+#pragma unroll
+      for (int j = 0; j < S; ++j) most_c = fmax(most_c, key[j] == top ? c[j] : none);
+      most_c = wave_top(most_c);
+      any = 0;
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        with[j] = __ballot(key[j] == top && c[j] == most_c);
+        any |= with[j];
+      }
+    }
+    const int owner = __builtin_ctzll(any);
+    const uint64_t bit = uint64_t{1} << owner;
+    int slot = 0;
+    double v = 0;
+    bool open = true;
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      if (open && (with[j] & bit)) {
+        open = false, slot = j;
+        v = lane_of(s[j], owner);
+        key[j] = lane == owner ? 0 : key[j];
+      }
+    }
+    const int at = __builtin_amdgcn_readlane(e0, owner) + slot;
     total += v;
     if (lane == i) mine = at, weight = v;
-    if (lane == owner) {
-#pragma unroll
-      for (int j = 0; j < S; ++j)
-        if (j == best_e) key[j] = nothing;
-      look();
-    }
   }
   if (a.renormalize) weight = total > 0 ? weight / total : 0;
   if (lane < a.top) experts[lane] = mine, weights[lane] = static_cast<float>(weight * a.scale);

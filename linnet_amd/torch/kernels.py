@@ -690,15 +690,26 @@ def mxfp4_w4a16(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bia
     depth = _mxfp4_operands("mxfp4_w4a16", blocks, scales)
     if x.dim() != 2 or blocks.dim() != 3 or x.shape[1] != depth:
         raise LinnetError(f"mxfp4_w4a16: x {tuple(x.shape)} against blocks {tuple(blocks.shape)}")
-    code = _code(x.dtype, "mxfp4_w4a16")
-    rows, out_features = x.shape[0], blocks.shape[0]
-    bias = _mxfp4_bias("mxfp4_w4a16", bias, x.dtype, out_features)
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16 or x.stride(0) < depth or x.stride(0) >= 1 << 23:
+    return _mxfp4_few_rows(x, _aligned(blocks), scales.contiguous(), bias, device)
+
+
+def _mxfp4_few_rows(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None,
+                    device: torch.device) -> torch.Tensor:
+    """`mxfp4_w4a16` of operands that were looked over before (`x` [rows, In] on their device)."""
+    rows, depth = x.shape
+    out_features = blocks.shape[0]
+    dtype = x.dtype
+    code = _code(dtype, "mxfp4_w4a16")
+    if bias is not None:
+        bias = _mxfp4_bias("mxfp4_w4a16", bias, dtype, out_features)
+    stride, step = x.stride()
+    at = x.data_ptr()
+    if step != 1 or stride % 8 or at % 16 or stride < depth or stride >= 1 << 23:
         x = _aligned(x)
-    blocks, scales = _aligned(blocks), scales.contiguous()
-    y = torch.empty(rows, out_features, dtype=x.dtype, device=device)
+        stride, at = depth, x.data_ptr()
+    y = torch.empty(rows, out_features, dtype=dtype, device=device)
     with _on(device):
-        _lib.call("lnq_mxfp4_linear", _ptr(x), max(x.stride(0), depth), _ptr(blocks), _ptr(scales), _ptr(bias), _ptr(y), rows,
+        _lib.call("lnq_mxfp4_linear", at, stride, blocks.data_ptr(), scales.data_ptr(), _ptr(bias), y.data_ptr(), rows,
                   out_features, depth, code, _stream(device))
     return y
 

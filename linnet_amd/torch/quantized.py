@@ -185,10 +185,11 @@ def mxfp4_operands(blocks: torch.Tensor, scales: torch.Tensor, rounded: int) -> 
     (`kernels.mxfp4_quantize`; gpt-oss's expert layout for one weight), with, where `rounded`, the
     scales laid out for the 4-bit product too."""
     _gpu(blocks)
-    if blocks.dim() != 3 or tuple(scales.shape) != tuple(blocks.shape[:2]):
-        raise LinnetError(f"mxfp4_operands: blocks [Out, In/32, 16] and scales [Out, In/32], got {tuple(blocks.shape)} and "
-                          f"{tuple(scales.shape)}")
-    blocks, scales = blocks.contiguous(), scales.contiguous()
+    kernels._on_gpu("mxfp4_operands", blocks, scales)
+    if blocks.dim() != 3:
+        raise LinnetError(f"mxfp4_operands: blocks are [Out, In/32, 16], got {tuple(blocks.shape)}")
+    kernels._mxfp4_operands("mxfp4_operands", blocks, scales)
+    blocks, scales = kernels._aligned(blocks), scales.contiguous()
     tiles = kernels.mxfp4_scale_tiles(scales, blocks.shape[1] * 32) if rounded else None
     return blocks, scales, tiles, rounded
 
@@ -199,17 +200,21 @@ def mxfp4_linear(x: torch.Tensor, operands: Mxfp4Operands, bias: torch.Tensor | 
     `TILED_ROWS` rows the weight widened in registers, and past those dequantized for the call.
     bf16 and f16; the bias is added in f32, before the one rounding."""
     blocks, scales, tiles, rounded = operands
-    out_features, in_features = blocks.shape[0], blocks.shape[1] * 32
+    out_features, groups, _ = blocks.shape
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    rows = flat.shape[0]
-    if flat.dtype in _HALF and 0 < in_features <= _MXFP4_IN and out_features <= _MXFP4_OUT:
+    rows, depth = flat.shape
+    dtype = flat.dtype
+    if depth != groups * 32:
+        raise LinnetError(f"mxfp4_linear: x {tuple(x.shape)} against a weight [{out_features}, {groups * 32}]")
+    if dtype in _HALF and 0 < depth <= _MXFP4_IN and out_features <= _MXFP4_OUT:
         if rounded and tiles is not None and rows > FEW_ROWS:
             q, row_scales = kernels.mxfp4_rows(flat)
-            y = kernels.mxfp4_mm(q, row_scales, blocks, tiles, flat.dtype, bias)
-            return _finish(x, y, None)
+            y = kernels.mxfp4_mm(q, row_scales, blocks, tiles, dtype, bias)
+            return y if flat is x else _finish(x, y, None)
         if rows <= TILED_ROWS:
-            return _finish(x, kernels.mxfp4_w4a16(flat, blocks, scales, bias), None)
-    return _finish(x, functional.linear(flat, kernels.mxfp4_dequantize(blocks, scales, flat.dtype), bias), None)
+            y = kernels._mxfp4_few_rows(flat, blocks, scales, bias, kernels._on_gpu("mxfp4_linear", flat, blocks, bias))
+            return y if flat is x else _finish(x, y, None)
+    return _finish(x, functional.linear(flat, kernels.mxfp4_dequantize(blocks, scales, dtype), bias), None)
 
 
 def mxfp4_experts_operands(blocks: torch.Tensor, scales: torch.Tensor, rounded: int) -> Mxfp4Operands:
