@@ -166,11 +166,20 @@ __global__ __launch_bounds__(route::THREADS) void expert_route_kernel(const type
   const int group = lane / a.lanes, place = (lane - group * a.lanes) * S;
   const int e0 = group * a.size + place;  // this lane's first expert
   const int held = group < a.groups ? min(S, a.size - place) : 0;
-  float l[S], most = nothing;
+  const bool biased = a.bias != nullptr;
+  float l[S], b[S], most = nothing;
   bool bad = false;
+  // All loads before the first use; slots past the held ones read the last expert, for nothing.
+  typename E::storage raw[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) raw[i] = from[min(e0 + i, a.count - 1)];
+  if (biased) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) b[i] = a.bias[min(e0 + i, a.count - 1)];
+  }
 #pragma unroll
   for (int i = 0; i < S; ++i) {
-    l[i] = i < held ? E::to_f32(from[e0 + i]) : nothing;
+    l[i] = i < held ? E::to_f32(raw[i]) : nothing;
     bad = bad || l[i] != l[i] || (a.softmax && l[i] == __builtin_huge_valf());
     most = fmaxf(most, l[i]);
   }
@@ -214,18 +223,17 @@ __global__ __launch_bounds__(route::THREADS) void expert_route_kernel(const type
     for (int i = 0; i < S; ++i) s[i] = l[i] == nothing ? 0 : s[i];
   }
   // The choices and their keys.
-  const bool biased = a.bias != nullptr;
   double c[S];
   uint32_t key[S];
 #pragma unroll
   for (int i = 0; i < S; ++i) {
-    c[i] = l[i];
-    key[i] = l[i] == nothing ? 0 : key_of(l[i]);
-    if (biased && i < held && l[i] != nothing) {
-      c[i] = s[i] + static_cast<double>(a.bias[e0 + i]);
-      if (!(c[i] > none)) c[i] = none;
-      key[i] = c[i] == none ? 0 : key_of(static_cast<float>(c[i]));
+    if (biased) {
+      c[i] = s[i] + static_cast<double>(b[i]);
+      c[i] = l[i] != nothing && c[i] > none ? c[i] : none;
+    } else {
+      c[i] = l[i];
     }
+    key[i] = c[i] == none ? 0 : key_of(static_cast<float>(c[i]));
   }
 
   if (a.groups > 1) {
