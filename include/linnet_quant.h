@@ -515,16 +515,17 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
                                const uint8_t* tiles, const void* bias, void* y, int64_t rows,
                                int64_t out_features, int64_t in_features, int32_t dtype, void* stream);
 
-/* lnq_mxfp4_experts with x rounded to MXFP4: y[r, k, :] = x[r (, k)] @ W[experts[r, k]]^T, the
- * pairs of each expert multiplied together. q and x_scale hold `rows` rows (shared: every
- * chosen expert of a row reads it) or rows * chosen; blocks [E, out, in/32, 16] as stored,
- * tiles [E] scale tiles each. An expert index outside 0 .. num_experts - 1 gives zeros.
- * workspace (16-byte aligned, at least lnq_mxfp4_experts_workspace bytes) holds the lists of
- * the pairs and their scales, written by the call: calls that overlap on one workspace race. num_experts <=
- * 2048, rows * chosen <= 2^26, out <= 2^27, x's codes below 2 GiB. */
-LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t num_experts, int64_t in_features,
-                                              int64_t* bytes);
-LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale, const uint8_t* blocks,
+/* lnq_mxfp4_experts with x rounded to MXFP4 (as lnq_mxfp4_rows does): y[r, k, :] = x[r (, k)] @
+ * W[experts[r, k]]^T, the pairs of each expert multiplied together. x (of y's dtype, bf16 or f16;
+ * rows x_stride elements apart, a multiple of 8) holds `rows` rows (shared: every chosen expert of a
+ * row reads it) or rows * chosen; blocks [E, out, in/32, 16] as stored, tiles [E] scale tiles each.
+ * An expert index outside 0 .. num_experts - 1 gives zeros. workspace (16-byte aligned, at least
+ * lnq_mxfp4_experts_workspace bytes for rows * chosen pairs and x's rows) holds the rounded x and
+ * the lists of the pairs, written by the call: calls that overlap on one workspace race.
+ * num_experts <= 2048, rows * chosen <= 2^26, out <= 2^27, x's codes below 2 GiB. */
+LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t x_rows, int64_t num_experts,
+                                              int64_t in_features, int64_t* bytes);
+LNQ_API LnqStatus lnq_mxfp4_experts_mm(const void* x, int64_t x_stride, const uint8_t* blocks,
                                        const uint8_t* tiles, const int64_t* experts, void* y,
                                        int64_t rows, int64_t chosen, int64_t num_experts,
                                        int64_t out_features, int64_t in_features, int32_t shared,

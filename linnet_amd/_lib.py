@@ -72,8 +72,8 @@ SIGNATURES: dict[str, list[object]] = {
     "lnq_mxfp4_scale_tiles": [_p, _p, _i64, _i64, _i64, _p],
     "lnq_mxfp4_linear": [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p],
     "lnq_mxfp4_mm": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p],
-    "lnq_mxfp4_experts_workspace": [_i64, _i64, _i64, ctypes.POINTER(_i64)],
-    "lnq_mxfp4_experts_mm": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _p, _i64, _p],
+    "lnq_mxfp4_experts_workspace": [_i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "lnq_mxfp4_experts_mm": [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _p, _i64, _p],
     "lnq_expert_route": [_p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, ctypes.c_double,
                          _i32, _p],
     "lnq_nf4_dequant": [_p, _p, _p, _i64, _i64, _i64, _i32, _p],

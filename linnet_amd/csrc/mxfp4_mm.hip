@@ -22,7 +22,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "mx4.hpp"
+#include "mx4_round.hpp"
 
 namespace lnq {
 
@@ -425,14 +425,12 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
 // where its own begin in `order` and in the tile table, then lists them, each wave those of its
 // own run of the pairs. Workgroup `count` lists the pairs whose choice is no expert and writes how
 // many tiles there are.
-__global__ __launch_bounds__(mx4::LIST_THREADS) void expert_lists_kernel(const int64_t* __restrict__ experts, int pairs,
-                                                                         int count, int bm, int* __restrict__ order,
-                                                                         i32x4* __restrict__ table, int* __restrict__ used) {
+__device__ __attribute__((always_inline)) inline void list_pairs(int e, const int64_t* experts, int pairs, int count, int bm, int* order, i32x4* table, int* used) {
   using namespace mx4;
   constexpr int WAVES = LIST_THREADS / 64, DEEP = 8;  // loads in flight
   __shared__ int number[MAX_EXPERTS + 1];
   __shared__ int part[3][WAVES], found[WAVES];
-  const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int run = (pairs + 64 * WAVES - 1) / (64 * WAVES) * 64;  // pairs of a wave
   const int from = wave * run, to = min(pairs, from + run);
   // Calls f(pair, its bucket) for this wave's pairs, a lane each; past the last, a bucket of -1.
@@ -472,7 +470,7 @@ __global__ __launch_bounds__(mx4::LIST_THREADS) void expert_lists_kernel(const i
   }
   __syncthreads();
   int first = 0, tile = 0, all = 0, at = 0;
-#pragma unroll
+#pragma unroll 4
   for (int v = 0; v < WAVES; ++v) {
     first += part[0][v], tile += part[1][v], all += part[2][v];
     if (v < wave) at += found[v];
@@ -488,6 +486,29 @@ __global__ __launch_bounds__(mx4::LIST_THREADS) void expert_lists_kernel(const i
     if (bucket == e) order[at + __popcll(mask & ((uint64_t{1} << lane) - 1))] = p;
     at += __popcll(mask);
   });
+}
+
+// What the product of the experts needs: workgroups 0 .. count list the pairs, and the others round
+// x's rows, four blocks of mxr::THREADS threads each (`spans` of them to a run of rows, `blocks` in
+// all). Neither waits for the other: in one launch the shorter costs nothing (4 to 10 us).
+template <int DT, int PASSES>
+__global__ __launch_bounds__(mx4::LIST_THREADS, 8) void expert_prepare_kernel(const int64_t* __restrict__ experts, int pairs,
+                                                                           int count, int bm, int* __restrict__ order,
+                                                                           i32x4* __restrict__ table, int* __restrict__ used,
+                                                                           const uint16_t* __restrict__ x, int64_t x_stride,
+                                                                           uint32_t* __restrict__ codes,
+                                                                           uint32_t* __restrict__ scales, int rows, int K,
+                                                                           int spans, int blocks) {
+  if (static_cast<int>(blockIdx.x) <= count) {
+    list_pairs(blockIdx.x, experts, pairs, count, bm, order, table, used);
+  } else {
+    constexpr int EACH = mx4::LIST_THREADS / mxr::THREADS;
+    __shared__ uint32_t unit[EACH][16 * PASSES];
+    const int part = __builtin_amdgcn_readfirstlane(threadIdx.x / mxr::THREADS);
+    const int b = (blockIdx.x - count - 1) * EACH + part, block = min(b, blocks - 1);
+    mxr::round_rows<DT, PASSES>(x, x_stride, codes, scales, rows, K, unit[part], threadIdx.x % mxr::THREADS, block / spans,
+                                block % spans, b < blocks);
+  }
 }
 
 // x's scales by the tiles' rows, as scale tiles: `each` blocks of 64 rows a tile of the product.
@@ -557,29 +578,50 @@ static void launch(const Args& a, int bm, hipStream_t s) {
   else launch_form<DT, Form256, EXPERTS>(a, s);
 }
 
+// The workspace of a call with tiles of `bm` pairs (tiles at most: a partial one for each expert that
+// is named): x's codes and scale tiles, the pairs in order, the tile table with how many there are, x's
+// scales by the tiles' rows.
 struct Plan {
   int tiles, each;  // blocks of 64 rows a tile
-  int64_t blocks, order_bytes, table_bytes, bytes;
+  int64_t blocks, scales, order, table, sorted, bytes;  // of 64 rows in all; where each begins
 };
 
-// Tiles of `bm` pairs at most: a partial one for each expert that is named. The workspace: order,
-// table, how many tiles, scales.
-static Plan experts_plan(int bm, int64_t pairs, int64_t count, int64_t in_features) {
+static Plan experts_plan(int bm, int64_t pairs, int64_t x_rows, int64_t count, int64_t in_features) {
+  const auto whole = [](int64_t bytes) { return (bytes + 127) / 128 * 128; };
+  const int64_t spans = (in_features + 255) / 256;
   Plan p{};
   p.tiles = static_cast<int>(pairs / bm + std::min(pairs, count + 1));
-  p.order_bytes = (pairs * 4 + 15) / 16 * 16;
-  p.table_bytes = static_cast<int64_t>(p.tiles) * 16 + 16;
   p.each = (bm + 63) / 64;
   p.blocks = static_cast<int64_t>(p.tiles) * p.each;
-  p.bytes = p.order_bytes + p.table_bytes + (in_features + 255) / 256 * p.blocks * TILE_BYTES;
+  p.scales = whole(x_rows * (in_features / 2));
+  p.order = p.scales + spans * ((x_rows + 63) / 64) * TILE_BYTES;
+  p.table = p.order + whole(pairs * 4);
+  p.sorted = p.table + whole(static_cast<int64_t>(p.tiles) * 16 + 16);
+  p.bytes = p.sorted + spans * p.blocks * TILE_BYTES;
   return p;
 }
 
 // Of any outputs: whichever tiles they take.
-static int64_t workspace_of(int64_t pairs, int64_t count, int64_t in_features) {
+static int64_t workspace_of(int64_t pairs, int64_t x_rows, int64_t count, int64_t in_features) {
   int64_t bytes = 0;
-  for (const int bm : {32, 64, 128, 256}) bytes = std::max(bytes, experts_plan(bm, pairs, count, in_features).bytes);
+  for (const int bm : {32, 64, 128, 256}) bytes = std::max(bytes, experts_plan(bm, pairs, x_rows, count, in_features).bytes);
   return bytes;
+}
+
+template <int DT>
+static void prepare(const Args& a, const int64_t* experts, int pairs, int bm, const void* x, int64_t x_stride, uint8_t* scales,
+                    hipStream_t s) {
+  const int per = mxr::rows_a_block(a.M, a.K), spans = units_of(a.K);
+  const int blocks = (a.M + per - 1) / per * spans, each = LIST_THREADS / mxr::THREADS;
+  const dim3 grid(static_cast<unsigned>(a.count + 1 + (blocks + each - 1) / each));
+#define LNQ_MXP(P)                                                                                                             \
+  hipLaunchKernelGGL((expert_prepare_kernel<DT, P>), grid, dim3(LIST_THREADS), 0, s, experts, pairs, a.count, bm,              \
+                     const_cast<int*>(a.order), const_cast<i32x4*>(a.table), const_cast<int*>(a.used),                         \
+                     static_cast<const uint16_t*>(x), x_stride, reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(a.q)),        \
+                     reinterpret_cast<uint32_t*>(scales), a.M, a.K, spans, blocks)
+  if (per == 128) LNQ_MXP(8);
+  else LNQ_MXP(1);
+#undef LNQ_MXP
 }
 
 }  // namespace mx4
@@ -625,22 +667,24 @@ LNQ_API LnqStatus lnq_mxfp4_mm(const uint8_t* q, const uint8_t* x_scale, const u
   return launched("mxfp4_mm");
 }
 
-LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t num_experts, int64_t in_features, int64_t* bytes) {
+LNQ_API LnqStatus lnq_mxfp4_experts_workspace(int64_t pairs, int64_t x_rows, int64_t num_experts, int64_t in_features,
+                                              int64_t* bytes) {
   LNQ_REQUIRE(bytes != nullptr, "lnq_mxfp4_experts_workspace: null pointer");
-  LNQ_REQUIRE(pairs >= 0 && pairs <= (1 << 26) && num_experts > 0 && num_experts <= mx4::MAX_EXPERTS && in_features > 0 &&
-                  in_features <= (1 << 22),
-              "lnq_mxfp4_experts_workspace: %lld pairs of %lld experts (1 to %d) of %lld inputs", static_cast<long long>(pairs),
-              static_cast<long long>(num_experts), mx4::MAX_EXPERTS, static_cast<long long>(in_features));
-  *bytes = pairs == 0 ? 0 : mx4::workspace_of(pairs, num_experts, in_features);
+  LNQ_REQUIRE(pairs >= 0 && pairs <= (1 << 26) && x_rows >= 0 && x_rows <= (1 << 27) && num_experts > 0 &&
+                  num_experts <= mx4::MAX_EXPERTS && in_features > 0 && in_features <= (1 << 22),
+              "lnq_mxfp4_experts_workspace: %lld pairs and %lld rows of %lld experts (1 to %d) of %lld inputs",
+              static_cast<long long>(pairs), static_cast<long long>(x_rows), static_cast<long long>(num_experts),
+              mx4::MAX_EXPERTS, static_cast<long long>(in_features));
+  *bytes = pairs == 0 ? 0 : mx4::workspace_of(pairs, x_rows, num_experts, in_features);
   clear_error();
   return LNQ_OK;
 }
 
-LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale, const uint8_t* blocks, const uint8_t* tiles,
+LNQ_API LnqStatus lnq_mxfp4_experts_mm(const void* x, int64_t x_stride, const uint8_t* blocks, const uint8_t* tiles,
                                        const int64_t* experts, void* y, int64_t rows, int64_t chosen, int64_t num_experts,
                                        int64_t out_features, int64_t in_features, int32_t shared, int32_t dtype,
                                        void* workspace, int64_t workspace_bytes, void* stream) {
-  LNQ_REQUIRE(dtype == LNQ_BF16 || dtype == LNQ_F16, "lnq_mxfp4_experts_mm: output is bf16 or f16, not dtype %d", dtype);
+  LNQ_REQUIRE(dtype == LNQ_BF16 || dtype == LNQ_F16, "lnq_mxfp4_experts_mm: x and y are bf16 or f16, not dtype %d", dtype);
   LNQ_REQUIRE(rows >= 0 && chosen >= 0 && num_experts > 0 && num_experts <= mx4::MAX_EXPERTS && out_features >= 0 &&
                   in_features > 0 && in_features % 32 == 0,
               "lnq_mxfp4_experts_mm: bad shape rows=%lld chosen=%lld experts=%lld (1 to %d) out=%lld in=%lld (in %% 32 == 0)",
@@ -653,21 +697,24 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
     clear_error();
     return LNQ_OK;
   }
-  LNQ_REQUIRE(q && x_scale && blocks && tiles && experts && y, "lnq_mxfp4_experts_mm: null pointer");
-  LNQ_REQUIRE(aligned(q, 16) && aligned(x_scale, 16) && aligned(blocks, 16) && aligned(tiles, 16) && aligned(y, 2) &&
-                  aligned(workspace, 16),
-              "lnq_mxfp4_experts_mm: operands and workspace must be 16-byte aligned");
+  LNQ_REQUIRE(x && blocks && tiles && experts && y, "lnq_mxfp4_experts_mm: null pointer");
+  LNQ_REQUIRE(x_stride >= 0 && x_stride % 8 == 0 && aligned(x, 16) && aligned(blocks, 16) && aligned(tiles, 16) &&
+                  aligned(y, 2) && aligned(workspace, 16),
+              "lnq_mxfp4_experts_mm: x (with its row stride), the weight and the workspace must be 16-byte aligned");
   const int64_t pairs = rows * chosen, x_rows = shared ? rows : pairs;
   LNQ_REQUIRE(x_rows * (in_features / 2) < (int64_t{1} << 31), "lnq_mxfp4_experts_mm: x's codes past 2 GiB");
   const int bm = mx4::tile_rows(static_cast<double>(pairs) / static_cast<double>(num_experts), num_experts, out_features, true);
-  const mx4::Plan plan = mx4::experts_plan(bm, pairs, num_experts, in_features);
-  LNQ_REQUIRE(plan.blocks <= (1 << 21), "lnq_mxfp4_experts_mm: too large");
-  const int64_t need = mx4::workspace_of(pairs, num_experts, in_features);
+  const mx4::Plan plan = mx4::experts_plan(bm, pairs, x_rows, num_experts, in_features);
+  LNQ_REQUIRE(plan.blocks <= (1 << 21) && static_cast<int64_t>(plan.tiles) * ((out_features + 63) / 64) <= INT32_MAX,
+              "lnq_mxfp4_experts_mm: too large");
+  const int64_t need = mx4::workspace_of(pairs, x_rows, num_experts, in_features);
   LNQ_REQUIRE(workspace && workspace_bytes >= need, "lnq_mxfp4_experts_mm: workspace of %lld bytes, %lld needed",
               static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  auto* const space = static_cast<uint8_t*>(workspace);
+  uint8_t *const scales = space + plan.scales, *const sorted = space + plan.sorted;
   mx4::Args a{};
-  a.q = q;
-  a.xs = x_scale;
+  a.q = space;
+  a.xs = sorted;
   a.w = blocks;
   a.ws = tiles;
   a.y = static_cast<uint16_t*>(y);
@@ -675,13 +722,8 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   a.x_blocks = static_cast<int>(plan.blocks);
   a.N = static_cast<int>(out_features);
   a.K = static_cast<int>(in_features);
-  LNQ_REQUIRE(static_cast<int64_t>(plan.tiles) * ((out_features + 63) / 64) <= INT32_MAX,
-              "lnq_mxfp4_experts_mm: too large");
-  auto* const space = static_cast<uint8_t*>(workspace);
-  auto* const order = reinterpret_cast<int*>(space);
-  uint8_t* const sorted = space + plan.order_bytes + plan.table_bytes;
-  a.order = order;
-  a.table = reinterpret_cast<const i32x4*>(space + plan.order_bytes);
+  a.order = reinterpret_cast<const int*>(space + plan.order);
+  a.table = reinterpret_cast<const i32x4*>(space + plan.table);
   a.used = reinterpret_cast<const int*>(a.table + plan.tiles);
   a.tiles = plan.tiles;
   a.count = static_cast<int>(num_experts);
@@ -689,14 +731,13 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const uint8_t* q, const uint8_t* x_scale,
   a.w_step = out_features * (in_features / 2);
   a.ws_step = static_cast<int64_t>(mx4::pairs_of(a.K)) * mx4::blocks_of(a.N) * mx4::TILE_BYTES;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(expert_lists_kernel, dim3(a.count + 1), dim3(mx4::LIST_THREADS), 0, s, experts, static_cast<int>(pairs),
-                     a.count, bm, order, const_cast<i32x4*>(a.table), const_cast<int*>(a.used));
-  if (const LnqStatus st = launched("expert_lists")) return st;
+  if (dtype == LNQ_BF16) mx4::prepare<LNQ_BF16>(a, experts, static_cast<int>(pairs), bm, x, x_stride, scales, s);
+  else mx4::prepare<LNQ_F16>(a, experts, static_cast<int>(pairs), bm, x, x_stride, scales, s);
+  if (const LnqStatus st = launched("expert_prepare")) return st;
   hipLaunchKernelGGL(expert_scales_kernel, dim3(static_cast<unsigned>((plan.blocks + 1) / 2), static_cast<unsigned>(mx4::pairs_of(a.K))),
-                     dim3(256), 0, s, x_scale, reinterpret_cast<uint32_t*>(sorted), order, a.table, a.used, mx4::blocks_of(a.M),
+                     dim3(256), 0, s, scales, reinterpret_cast<uint32_t*>(sorted), a.order, a.table, a.used, mx4::blocks_of(a.M),
                      a.x_blocks, plan.each, a.chosen);
   if (const LnqStatus st = launched("expert_scales")) return st;
-  a.xs = sorted;
   if (dtype == LNQ_BF16) mx4::launch<LNQ_BF16, true>(a, bm, s);
   else mx4::launch<LNQ_F16, true>(a, bm, s);
   return launched("mxfp4_experts_mm");

@@ -11,80 +11,10 @@
 //
 // Bound by HBM: 2 or 4 bytes a value read, 17/32 written (back: the reverse). Four lanes
 // take a block, 8 values each: a wave's loads are whole kilobytes.
-#include "mx4.hpp"
+#include "mx4_round.hpp"
 
 namespace lnq {
 
-namespace mxr {
-constexpr int THREADS = 256;
-constexpr int UNIT = 128;  // inputs of a workgroup of the row-rounding kernel
-
-// 8 values as loaded.
-template <int DT>
-struct Raw {
-  u32x4 v;
-};
-template <>
-struct Raw<LNQ_F32> {
-  f32x4 a, b;
-};
-
-template <int DT>
-__device__ inline Raw<DT> load8(const typename Elem<DT>::storage* p) {
-  Raw<DT> r;
-  if constexpr (DT == LNQ_F32) {
-    r.a = *reinterpret_cast<const f32x4*>(p);
-    r.b = *reinterpret_cast<const f32x4*>(p + 4);
-  } else {
-    r.v = *reinterpret_cast<const u32x4*>(p);
-  }
-  return r;
-}
-
-template <int DT>
-__device__ inline void widen8(const Raw<DT>& r, float (&v)[8]) {
-  if constexpr (DT == LNQ_F32) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = r.a[e], v[4 + e] = r.b[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t d = r.v[e];
-      v[2 * e] = Elem<DT>::to_f32(static_cast<uint16_t>(d & 0xffffu));
-      v[2 * e + 1] = Elem<DT>::to_f32(static_cast<uint16_t>(d >> 16));
-    }
-  }
-}
-
-// This lane's 8 values of a block whose other values the lanes of its quad (l & ~3 .. l | 3)
-// hold: the scale byte (the same in all four) and the 8 codes, element 0 lowest.
-__device__ inline uint32_t round8(const float (&v)[8], uint32_t& byte) {
-  uint32_t top = 0;  // magnitudes order as their bits
-#pragma unroll
-  for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
-  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1, 64)));
-  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2, 64)));
-  const uint32_t exponent = top >> 23;
-  if (exponent == 255) {
-    byte = 255;
-    return 0;
-  }
-  byte = max(exponent, 2u) - 2u;
-  const float inverse = __builtin_bit_cast(float, (254u - byte) << 23);  // 2^(127 - byte), byte <= 252
-  uint32_t word = 0;
-  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0] * inverse, v[1] * inverse, 1.0f, 0);
-  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2] * inverse, v[3] * inverse, 1.0f, 1);
-  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4] * inverse, v[5] * inverse, 1.0f, 2);
-  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6] * inverse, v[7] * inverse, 1.0f, 3);
-  return word;
-}
-
-// 2^(byte - 127); 255 is NaN.
-__device__ inline float scale_of(uint32_t byte) {
-  const uint32_t bits = byte == 255 ? 0x7fc00000u : byte == 0 ? 0x00400000u : byte << 23;
-  return __builtin_bit_cast(float, bits);
-}
-}  // namespace mxr
 
 // Blocks one after another, as a checkpoint stores them: thread i of the grid takes values
 // 8 i .. 8 i + 7 of all, UNROLL of them a grid apart.
@@ -102,59 +32,13 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_quantize_kernel(const type
   if ((threadIdx.x & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(byte);
 }
 
-// Rows for the product: codes [rows, K / 2] as above, scales as scale tiles (mx4.hpp). A workgroup
-// takes 16 PASSES rows by 128 inputs, 16 lanes a row, all of its loads before its first conversion;
-// then its scales: dwords of two blocks of 64 rows, or one byte of each dword of its block.
+// Rows for the product, 16 PASSES by 128 inputs a workgroup.
 template <int DT, int PASSES>
 __global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename Elem<DT>::storage* __restrict__ x,
                                                                   int64_t x_stride, uint32_t* __restrict__ codes,
                                                                   uint32_t* __restrict__ scales, int rows, int K) {
-  using namespace mxr;
-  constexpr int A_PASS = THREADS / 16, ROWS = A_PASS * PASSES;
-  __shared__ uint32_t unit[ROWS];
-  const int lane = threadIdx.x & 63;
-  const int r0 = blockIdx.x * ROWS, k = blockIdx.y * UNIT + (threadIdx.x & 15) * 8;
-  const bool in = k < K;
-  Raw<DT> raw[PASSES];
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = min(r0 + i * A_PASS + static_cast<int>(threadIdx.x >> 4), rows - 1);
-    raw[i] = load8<DT>(x + r * x_stride + (in ? k : 0));
-  }
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = i * A_PASS + (threadIdx.x >> 4);
-    float v[8];
-    widen8<DT>(raw[i], v);
-    uint32_t byte;
-    const uint32_t word = round8(v, byte);
-    if (r0 + r < rows && in) codes[(static_cast<int64_t>(r0 + r) * K + k) >> 3] = word;
-    // The four blocks of the unit, 16 lanes: block b's byte at bits 8 b.
-    uint32_t four = in ? byte << (8 * ((lane >> 2) & 3)) : 0u;
-    four |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(four), 4, 64));
-    four |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(four), 8, 64));
-    if ((lane & 15) == 0) unit[r] = r0 + r < rows ? four : 0u;
-  }
-  __syncthreads();
-  const int blocks = mx4::blocks_of(rows), block = r0 / 64 + static_cast<int>(threadIdx.x >> 6);
-  if (threadIdx.x >= (ROWS > 64 ? ROWS : 64) || block >= blocks) return;
-  const int u = blockIdx.y & 1, row = lane & 15, shift = 8 * (lane >> 4);
-  const bool alone = u == 0 && blockIdx.y + 1 == gridDim.y;  // the pair's second unit lies past K
-  uint32_t* const at = scales + ((static_cast<int64_t>(blockIdx.y >> 1) * blocks + block) * 64 + lane) * 2;
-  if constexpr (ROWS >= 64) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int f = 0; f < 4; ++f) word |= (unit[(threadIdx.x >> 6) * 64 + 16 * f + row] >> shift & 255u) << (8 * f);
-    at[u] = word;
-    if (alone) at[1] = 0;
-  } else {
-    uint8_t* const bytes = reinterpret_cast<uint8_t*>(at);
-    const int f = r0 % 64 / 16, last = r0 + ROWS >= rows ? 4 : f + 1;  // the last rows' workgroup writes the block's rest
-    for (int i = f; i < last; ++i) {
-      bytes[4 * u + i] = static_cast<uint8_t>(i == f ? unit[row] >> shift : 0u);
-      if (alone) bytes[4 + i] = 0;
-    }
-  }
+  __shared__ uint32_t unit[16 * PASSES];
+  mxr::round_rows<DT, PASSES>(x, x_stride, codes, scales, rows, K, unit, threadIdx.x, blockIdx.x, blockIdx.y, true);
 }
 
 template <int DT>
@@ -272,9 +156,8 @@ LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, ui
   LNQ_REQUIRE(x && q && scales, "lnq_mxfp4_rows: null pointer");
   LNQ_REQUIRE(x_stride >= 0 && x_stride % 8 == 0 && aligned(x, 16) && aligned(q, 16) && aligned(scales, 16),
               "lnq_mxfp4_rows: x (with its row stride), q and scales must be 16-byte aligned");
-  // 128 rows a workgroup where that still is four workgroups a CU, else 16.
   const int64_t spans = (in_features + mxr::UNIT - 1) / mxr::UNIT;
-  const int per = (rows + 127) / 128 * spans >= 4 * compute_units() ? 128 : 16;
+  const int per = mxr::rows_a_block(rows, in_features);
   const dim3 grid(static_cast<unsigned>((rows + per - 1) / per), static_cast<unsigned>(spans));
   LNQ_REQUIRE(grid.y <= 65535, "lnq_mxfp4_rows: in too large");
   const int R = static_cast<int>(rows), K = static_cast<int>(in_features);

@@ -741,35 +741,35 @@ def mxfp4_mm(q: torch.Tensor, x_scale: torch.Tensor, blocks: torch.Tensor, tiles
 MXFP4_MM_EXPERTS = 2048  # experts that `mxfp4_experts_mm` takes at most
 
 
-def mxfp4_experts_mm(q: torch.Tensor, x_scale: torch.Tensor, blocks: torch.Tensor, tiles: torch.Tensor,
-                     experts: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """`mxfp4_experts` of rows rounded to MXFP4: `y[r, k] = x[r (, k)] @ W[experts[r, k]].T` in
-    `dtype`, each expert's pairs multiplied together on the block-scaled MFMA. `q` and `x_scale`
-    (`mxfp4_rows`) hold R rows (every chosen expert of a row reads it) or R * K, one a pair; with
-    K = 1 the two are the same. `blocks` [E, Out, In/32, 16] as stored, `tiles` of
+def mxfp4_experts_mm(x: torch.Tensor, blocks: torch.Tensor, tiles: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
+    """`mxfp4_experts` with x rounded to MXFP4 (as `mxfp4_rows` does): `y[r, k] = x[r (, k)] @
+    W[experts[r, k]].T` [R, K, Out], each expert's pairs multiplied together on the block-scaled MFMA.
+    `x` (bf16 or f16) holds R rows [R, In] (every chosen expert of a row reads it) or R * K, one a pair;
+    with K = 1 the two are the same. `blocks` [E, Out, In/32, 16] as stored, `tiles` of
     `mxfp4_scale_tiles`. An expert outside 0 .. E - 1 gives zeros."""
-    device = _on_gpu("mxfp4_experts_mm", q, x_scale, blocks, tiles, experts)
-    if blocks.dim() != 4 or blocks.shape[3] != 16 or blocks.dtype != torch.uint8 or q.dim() != 2 or q.dtype != torch.uint8:
-        raise LinnetError("mxfp4_experts_mm: q is [rows, In/2] and blocks [E, Out, In/32, 16], both uint8")
+    device = _on_gpu("mxfp4_experts_mm", x, blocks, tiles, experts)
+    if blocks.dim() != 4 or blocks.shape[3] != 16 or blocks.dtype != torch.uint8:
+        raise LinnetError("mxfp4_experts_mm: blocks are [E, Out, In/32, 16] uint8")
     count, out_features, groups, _ = blocks.shape
     if experts.dim() != 2 or experts.is_floating_point():
         raise LinnetError(f"mxfp4_experts_mm: experts are integers [R, K], got {tuple(experts.shape)} {experts.dtype}")
     rows, chosen = experts.shape
-    if q.shape[0] not in (rows, rows * chosen) or q.shape[1] != groups * 16:
-        raise LinnetError(f"mxfp4_experts_mm: q {tuple(q.shape)} against experts {tuple(experts.shape)} and blocks "
+    if x.dim() != 2 or x.shape[0] not in (rows, rows * chosen) or x.shape[1] != groups * 32:
+        raise LinnetError(f"mxfp4_experts_mm: x {tuple(x.shape)} against experts {tuple(experts.shape)} and blocks "
                           f"{tuple(blocks.shape)}")
-    _mxfp4_tiles("mxfp4_experts_mm", x_scale, (), q.shape[0], groups * 32)
     _mxfp4_tiles("mxfp4_experts_mm", tiles, (count,), out_features, groups * 32)
-    code = _code(dtype, "mxfp4_experts_mm")
-    q, x_scale, blocks, tiles = _aligned(q), _aligned(x_scale), _aligned(blocks), _aligned(tiles)
+    code = _code(x.dtype, "mxfp4_experts_mm")
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = _aligned(x)
+    blocks, tiles = _aligned(blocks), _aligned(tiles)
     ids = experts.to(torch.int64).contiguous()
-    y = torch.empty(rows, chosen, out_features, dtype=dtype, device=device)
+    y = torch.empty(rows, chosen, out_features, dtype=x.dtype, device=device)
     need = ctypes.c_int64(0)
     with _on(device):
-        _lib.call("lnq_mxfp4_experts_workspace", rows * chosen, count, groups * 32, ctypes.byref(need))
+        _lib.call("lnq_mxfp4_experts_workspace", rows * chosen, x.shape[0], count, groups * 32, ctypes.byref(need))
         space = torch.empty(need.value, dtype=torch.uint8, device=device)
-        _lib.call("lnq_mxfp4_experts_mm", _ptr(q), _ptr(x_scale), _ptr(blocks), _ptr(tiles), _ptr(ids), _ptr(y), rows, chosen,
-                  count, out_features, groups * 32, int(q.shape[0] == rows), code, _ptr(space), need.value, _stream(device))
+        _lib.call("lnq_mxfp4_experts_mm", _ptr(x), x.stride(0), _ptr(blocks), _ptr(tiles), _ptr(ids), _ptr(y), rows, chosen,
+                  count, out_features, groups * 32, int(x.shape[0] == rows), code, _ptr(space), need.value, _stream(device))
     return y
 
 

@@ -242,7 +242,6 @@ def mxfp4_experts_linear(x: torch.Tensor, operands: Mxfp4Operands, experts: torc
     x_rows = rows if x.dim() == 2 else rows * chosen
     if (rounded and tiles is not None and rows > FEW_ROWS and x.dtype in _HALF and blocks.shape[0] <= kernels.MXFP4_MM_EXPERTS
             and x_rows * x.shape[-1] < 1 << 32):
-        q, row_scales = kernels.mxfp4_rows(x.reshape(x_rows, x.shape[-1]))
-        return kernels.mxfp4_experts_mm(q, row_scales, blocks, tiles, experts, x.dtype)
+        return kernels.mxfp4_experts_mm(x.reshape(x_rows, x.shape[-1]), blocks, tiles, experts)
     shared = x[:, None, :].expand(rows, chosen, x.shape[1]) if x.dim() == 2 else x
     return kernels.mxfp4_experts(shared, blocks, scales, experts)

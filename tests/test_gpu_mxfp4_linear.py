@@ -314,8 +314,7 @@ def test_experts_mm(rows: int, chosen: int, count: int, out: int, depth: int, dt
     ids = torch.from_numpy(experts).to(DEV)
     for shared in (True, False):
         x = torch.from_numpy(_values(rng, rows if shared else rows * chosen, depth)).to(dtype).to(DEV)
-        q, row_scales = kernels.mxfp4_rows(x)
-        y = kernels.mxfp4_experts_mm(q, row_scales, blocks, tiles, ids, dtype)
+        y = kernels.mxfp4_experts_mm(x, blocks, tiles, ids)
         assert y.shape == (rows, chosen, out)
         values = _rounded(x)
         for e in range(count):
@@ -366,10 +365,11 @@ def test_refusals() -> None:
         (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 2, 64, 8), u8(8, 2, 16), u8(1, 1, 64, 8), torch.bfloat16), "scale tiles"),
         (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 1, 64, 8), u8(8, 2, 16), u8(2, 1, 64, 8), torch.bfloat16), "scale tiles"),
         (lambda: kernels.mxfp4_mm(u8(4, 32), u8(1, 1, 64, 8), u8(8, 2, 16), u8(1, 1, 64, 8), torch.float32), "dtype"),
-        (lambda: kernels.mxfp4_experts_mm(u8(5, 32), u8(1, 1, 64, 8), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8),
-                                          torch.zeros(4, 2, dtype=torch.int64, device=DEV), torch.bfloat16), "against"),
-        (lambda: kernels.mxfp4_experts_mm(u8(4, 32), u8(1, 1, 64, 8), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8),
-                                          torch.zeros(4, 2, device=DEV), torch.bfloat16), "integers"),
+        (lambda: kernels.mxfp4_experts_mm(x[:3], u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8),
+                                          torch.zeros(4, 2, dtype=torch.int64, device=DEV)), "against"),
+        (lambda: kernels.mxfp4_experts_mm(x, u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8), torch.zeros(4, 2, device=DEV)), "integers"),
+        (lambda: kernels.mxfp4_experts_mm(x.float(), u8(2, 8, 2, 16), u8(2, 1, 1, 64, 8),
+                                          torch.zeros(4, 2, dtype=torch.int64, device=DEV)), "dtype"),
         (lambda: quantized.mxfp4_operands(u8(2, 8, 2, 16), u8(2, 8, 2), 1), "blocks"),
         (lambda: quantized.mxfp4_experts_operands(u8(8, 2, 16), u8(8, 2), 1), "blocks"),
         (lambda: quantized.mxfp4_experts_linear(x, quantized.mxfp4_experts_operands(u8(2, 8, 2, 16), u8(2, 8, 2), 1),
@@ -381,9 +381,9 @@ def test_refusals() -> None:
 
 def test_workspace_is_checked() -> None:
     need = ctypes.c_int64(0)
-    _lib.call("lnq_mxfp4_experts_workspace", 64, 8, 64, ctypes.byref(need))
+    _lib.call("lnq_mxfp4_experts_workspace", 64, 16, 8, 64, ctypes.byref(need))
     with pytest.raises(LinnetError, match="workspace"):
-        _lib.call("lnq_mxfp4_experts_mm", *[4096] * 6, 16, 4, 8, 64, 64, 1, _lib.BF16, 4096, need.value - 1, None)
+        _lib.call("lnq_mxfp4_experts_mm", 4096, 64, *[4096] * 4, 16, 4, 8, 64, 64, 1, _lib.BF16, 4096, need.value - 1, None)
 
 
 def _mixture(x: torch.Tensor, router: torch.Tensor, gate_up: tuple, down: tuple) -> torch.Tensor:

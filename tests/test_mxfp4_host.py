@@ -51,13 +51,14 @@ def _status(name: str, *args: object) -> tuple[int, str]:
     ("lnq_mxfp4_mm", (FAKE, ODD, FAKE, FAKE, NULL, FAKE, 4, 8, 64, 0, NULL), "aligned"),
     ("lnq_mxfp4_mm", (FAKE, FAKE, FAKE, FAKE, NULL, FAKE, 1 << 28, 8, 64, 0, NULL), "2^27"),
     ("lnq_mxfp4_mm", (FAKE, FAKE, FAKE, FAKE, NULL, FAKE, 1 << 27, 1 << 27, 64, 0, NULL), "too large"),
-    ("lnq_mxfp4_experts_workspace", (-1, 4, 64, ctypes.byref(ctypes.c_int64())), "pairs"),
-    ("lnq_mxfp4_experts_workspace", (4, 4096, 64, ctypes.byref(ctypes.c_int64())), "experts"),
-    ("lnq_mxfp4_experts_mm", (*[FAKE] * 6, 4, 2, 4096, 8, 64, 1, 0, FAKE, 1 << 30, NULL), "experts=4096"),
-    ("lnq_mxfp4_experts_mm", (*[FAKE] * 6, 4, 2, 4, 8, 64, 1, 2, FAKE, 1 << 30, NULL), "bf16 or f16"),
-    ("lnq_mxfp4_experts_mm", (*[FAKE] * 6, 4, 2, 4, 8, 64, 1, 0, FAKE, 16, NULL), "workspace of 16 bytes"),
-    ("lnq_mxfp4_experts_mm", (*[FAKE] * 6, 4, 2, 4, 8, 64, 1, 0, NULL, 1 << 30, NULL), "workspace"),
-    ("lnq_mxfp4_experts_mm", (*[FAKE] * 6, 1 << 20, 2, 4, 8, 8192, 1, 0, FAKE, 1 << 40, NULL), "2 GiB"),
+    ("lnq_mxfp4_experts_workspace", (-1, 4, 4, 64, ctypes.byref(ctypes.c_int64())), "pairs"),
+    ("lnq_mxfp4_experts_workspace", (4, 4, 4096, 64, ctypes.byref(ctypes.c_int64())), "experts"),
+    ("lnq_mxfp4_experts_mm", (FAKE, 64, *[FAKE] * 4, 4, 2, 4096, 8, 64, 1, 0, FAKE, 1 << 30, NULL), "experts=4096"),
+    ("lnq_mxfp4_experts_mm", (FAKE, 64, *[FAKE] * 4, 4, 2, 4, 8, 64, 1, 2, FAKE, 1 << 30, NULL), "bf16 or f16"),
+    ("lnq_mxfp4_experts_mm", (FAKE, 64, *[FAKE] * 4, 4, 2, 4, 8, 64, 1, 0, FAKE, 16, NULL), "workspace of 16 bytes"),
+    ("lnq_mxfp4_experts_mm", (FAKE, 64, *[FAKE] * 4, 4, 2, 4, 8, 64, 1, 0, NULL, 1 << 30, NULL), "workspace"),
+    ("lnq_mxfp4_experts_mm", (FAKE, 60, *[FAKE] * 4, 4, 2, 4, 8, 64, 1, 0, FAKE, 1 << 30, NULL), "aligned"),
+    ("lnq_mxfp4_experts_mm", (FAKE, 8192, *[FAKE] * 4, 1 << 20, 2, 4, 8, 8192, 1, 0, FAKE, 1 << 40, NULL), "2 GiB"),
     ("lnq_expert_route", (FAKE, 8, NULL, FAKE, FAKE, 4, 8, 9, 1, 1, 1, 1, 1, 1.0, 0, NULL), "choices a row"),
     ("lnq_expert_route", (FAKE, 8, NULL, FAKE, FAKE, 4, 8, 2, 3, 1, 1, 1, 1, 1.0, 0, NULL), "3 groups"),
     ("lnq_expert_route", (FAKE, 8, NULL, FAKE, FAKE, 4, 2048, 2, 1, 1, 1, 1, 1, 1.0, 0, NULL), "2048 experts"),
@@ -77,7 +78,7 @@ def test_empty_calls_succeed_without_a_device() -> None:
         ("lnq_mxfp4_scale_tiles", (NULL, NULL, 0, 4, 64, NULL)),
         ("lnq_mxfp4_linear", (NULL, 64, NULL, NULL, NULL, NULL, 0, 8, 64, 0, NULL)),
         ("lnq_mxfp4_mm", (NULL, NULL, NULL, NULL, NULL, NULL, 0, 8, 64, 0, NULL)),
-        ("lnq_mxfp4_experts_mm", (*[NULL] * 6, 0, 2, 4, 8, 64, 1, 0, NULL, 0, NULL)),
+        ("lnq_mxfp4_experts_mm", (NULL, 64, *[NULL] * 4, 0, 2, 4, 8, 64, 1, 0, NULL, 0, NULL)),
         ("lnq_expert_route", (NULL, 8, NULL, NULL, NULL, 0, 8, 2, 1, 1, 1, 1, 1, 1.0, 0, NULL)),
     ]:
         assert _status(name, *args)[0] == _lib.LNQ_OK, name
@@ -89,9 +90,9 @@ def test_the_wrappers_refuse_cpu_tensors() -> None:
                  lambda: kernels.mxfp4_dequantize(u8(2, 1, 16), u8(2, 1), torch.float32),
                  lambda: kernels.mxfp4_scale_tiles(u8(2, 1), 32),
                  lambda: kernels.mxfp4_w4a16(torch.zeros(2, 32).bfloat16(), u8(2, 1, 16), u8(2, 1)),
-                 lambda: kernels.mxfp4_mm(u8(2, 16), u8(1, 4, 4), u8(2, 1, 16), u8(1, 1, 64, 8), torch.bfloat16),
-                 lambda: kernels.mxfp4_experts_mm(u8(2, 16), u8(1, 4, 4), u8(3, 2, 1, 16), u8(3, 1, 1, 64, 8),
-                                                  torch.zeros(2, 1, dtype=torch.int64), torch.bfloat16),
+                 lambda: kernels.mxfp4_mm(u8(2, 16), u8(1, 1, 64, 8), u8(2, 1, 16), u8(1, 1, 64, 8), torch.bfloat16),
+                 lambda: kernels.mxfp4_experts_mm(torch.zeros(2, 32).bfloat16(), u8(3, 2, 1, 16), u8(3, 1, 1, 64, 8),
+                                                  torch.zeros(2, 1, dtype=torch.int64)),
                  lambda: kernels.expert_route(torch.zeros(2, 8), 2), lambda: quantized.mxfp4_operands(u8(2, 1, 16), u8(2, 1), 1),
                  lambda: quantized.mxfp4_experts_operands(u8(3, 2, 1, 16), u8(3, 2, 1), 1)):
         with pytest.raises(LinnetError, match="GPU"):
@@ -147,8 +148,8 @@ def test_route_against_a_search(score: str, groups: int) -> None:
                                                                        (9, 3, 2048, 100, 288), (300, 8, 4, 30000, 96)])
 def test_experts_workspace_of_one_byte_less_is_refused(rows: int, chosen: int, count: int, out: int, depth: int) -> None:
     need = ctypes.c_int64(0)
-    _lib.call("lnq_mxfp4_experts_workspace", rows * chosen, count, depth, ctypes.byref(need))
+    _lib.call("lnq_mxfp4_experts_workspace", rows * chosen, rows, count, depth, ctypes.byref(need))
     assert need.value >= rows * chosen * 4
     for space, size in ((FAKE, need.value - 1), (FAKE, 0), (NULL, need.value)):
         with pytest.raises(LinnetError, match="workspace"):
-            _lib.call("lnq_mxfp4_experts_mm", *[FAKE] * 6, rows, chosen, count, out, depth, 1, _lib.BF16, space, size, NULL)
+            _lib.call("lnq_mxfp4_experts_mm", FAKE, depth, *[FAKE] * 4, rows, chosen, count, out, depth, 1, _lib.BF16, space, size, NULL)
