@@ -270,41 +270,47 @@ __global__ __launch_bounds__(route::THREADS) void expert_route_kernel(const type
     for (int j = 1; j < S; ++j) best = max(best, key[j]);
     const uint32_t top = wave_top(best);
     if (top == 0) break;
-    // The lanes that hold it in each slot; of several the first expert, by the choices themselves
-    // where those are more than the key shows.
-    uint64_t with[S], any = 0, twice = 0;
+    // The lanes that hold it in each slot. One place, mostly: taken by selects, without a branch.
+    uint64_t with[S], any = 0;
+    int places = 0;
 #pragma unroll
     for (int j = 0; j < S; ++j) {
       with[j] = __ballot(key[j] == top);
-      twice |= any & with[j];
+      places += __popcll(with[j]);
       any |= with[j];
     }
-    if (biased && (twice | (any & (any - 1)))) {
-      double most_c = none;
+    // Of several the first expert, by the choices themselves where those are more than the key shows.
+    if (places > 1) {
+      if (biased) {
+        double most_c = none;
 #pragma unroll
-      for (int j = 0; j < S; ++j) most_c = fmax(most_c, key[j] == top ? c[j] : none);
-      most_c = wave_top(most_c);
-      any = 0;
+        for (int j = 0; j < S; ++j) most_c = fmax(most_c, key[j] == top ? c[j] : none);
+        most_c = wave_top(most_c);
+        any = 0;
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+          with[j] = __ballot(key[j] == top && c[j] == most_c);
+          any |= with[j];
+        }
+      }
+      uint64_t bit = any & (~any + 1);
 #pragma unroll
       for (int j = 0; j < S; ++j) {
-        with[j] = __ballot(key[j] == top && c[j] == most_c);
-        any |= with[j];
+        with[j] &= bit;
+        bit &= ~with[j];
       }
     }
     const int owner = __builtin_ctzll(any);
-    const uint64_t bit = uint64_t{1} << owner;
-    int slot = 0;
-    double v = 0;
-    bool open = true;
+    int e = e0;
+    double v = s[0];
 #pragma unroll
     for (int j = 0; j < S; ++j) {
-      if (open && (with[j] & bit)) {
-        open = false, slot = j;
-        v = lane_of(s[j], owner);
-        key[j] = lane == owner ? 0 : key[j];
-      }
+      const bool here = __builtin_amdgcn_inverse_ballot_w64(with[j]);
+      if (j > 0) e = here ? e0 + j : e, v = here ? s[j] : v;
+      key[j] = here ? 0 : key[j];
     }
-    const int at = __builtin_amdgcn_readlane(e0, owner) + slot;
+    const int at = __builtin_amdgcn_readlane(e, owner);
+    v = lane_of(v, owner);
     total += v;
     if (lane == i) mine = at, weight = v;
   }
