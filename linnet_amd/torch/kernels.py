@@ -738,7 +738,41 @@ def mxfp4_mm(q: torch.Tensor, x_scale: torch.Tensor, blocks: torch.Tensor, tiles
     return y
 
 
+def _mxfp4_rounded(x: torch.Tensor, blocks: torch.Tensor, tiles: torch.Tensor, bias: torch.Tensor | None,
+                   device: torch.device) -> torch.Tensor:
+    """`mxfp4_mm` of `mxfp4_rows(x)` for operands that were looked over before (`x` [rows, In] on their
+    device), the rounded rows in one allocation."""
+    rows, depth = x.shape
+    out_features = blocks.shape[0]
+    dtype = x.dtype
+    code = _code(dtype, "mxfp4_mm")
+    if bias is not None:
+        bias = _mxfp4_bias("mxfp4_mm", bias, dtype, out_features)
+    stride, step = x.stride()
+    at = x.data_ptr()
+    if step != 1 or stride % 8 or at % 16:
+        x = _aligned(x)
+        stride, at = depth, x.data_ptr()
+    codes = rows * depth // 2  # a multiple of 16
+    space = torch.empty(codes + -(-depth // 256) * -(-rows // 64) * 512, dtype=torch.uint8, device=device)
+    y = torch.empty(rows, out_features, dtype=dtype, device=device)
+    q = space.data_ptr()
+    with _on(device):
+        stream = _stream(device)
+        _lib.call("lnq_mxfp4_rows", at, stride, q, q + codes, rows, depth, code, stream)
+        _lib.call("lnq_mxfp4_mm", q, q + codes, blocks.data_ptr(), tiles.data_ptr(), _ptr(bias), y.data_ptr(), rows,
+                  out_features, depth, code, stream)
+    return y
+
+
 MXFP4_MM_EXPERTS = 2048  # experts that `mxfp4_experts_mm` takes at most
+
+
+@functools.lru_cache(maxsize=256)
+def _mxfp4_workspace(pairs: int, x_rows: int, count: int, in_features: int) -> int:
+    need = ctypes.c_int64(0)
+    _lib.call("lnq_mxfp4_experts_workspace", pairs, x_rows, count, in_features, ctypes.byref(need))
+    return need.value
 
 
 def mxfp4_experts_mm(x: torch.Tensor, blocks: torch.Tensor, tiles: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
@@ -764,12 +798,11 @@ def mxfp4_experts_mm(x: torch.Tensor, blocks: torch.Tensor, tiles: torch.Tensor,
     blocks, tiles = _aligned(blocks), _aligned(tiles)
     ids = experts.to(torch.int64).contiguous()
     y = torch.empty(rows, chosen, out_features, dtype=x.dtype, device=device)
-    need = ctypes.c_int64(0)
+    need = _mxfp4_workspace(rows * chosen, x.shape[0], count, groups * 32)
+    space = torch.empty(need, dtype=torch.uint8, device=device)
     with _on(device):
-        _lib.call("lnq_mxfp4_experts_workspace", rows * chosen, x.shape[0], count, groups * 32, ctypes.byref(need))
-        space = torch.empty(need.value, dtype=torch.uint8, device=device)
         _lib.call("lnq_mxfp4_experts_mm", _ptr(x), x.stride(0), _ptr(blocks), _ptr(tiles), _ptr(ids), _ptr(y), rows, chosen,
-                  count, out_features, groups * 32, int(x.shape[0] == rows), code, _ptr(space), need.value, _stream(device))
+                  count, out_features, groups * 32, int(x.shape[0] == rows), code, _ptr(space), need, _stream(device))
     return y
 
 

@@ -207,12 +207,13 @@ def mxfp4_linear(x: torch.Tensor, operands: Mxfp4Operands, bias: torch.Tensor | 
     if depth != groups * 32:
         raise LinnetError(f"mxfp4_linear: x {tuple(x.shape)} against a weight [{out_features}, {groups * 32}]")
     if dtype in _HALF and 0 < depth <= _MXFP4_IN and out_features <= _MXFP4_OUT:
+        product = None
         if rounded and tiles is not None and rows > FEW_ROWS:
-            q, row_scales = kernels.mxfp4_rows(flat)
-            y = kernels.mxfp4_mm(q, row_scales, blocks, tiles, dtype, bias)
-            return y if flat is x else _finish(x, y, None)
-        if rows <= TILED_ROWS:
-            y = kernels._mxfp4_few_rows(flat, blocks, scales, bias, kernels._on_gpu("mxfp4_linear", flat, blocks, bias))
+            product, scaled = kernels._mxfp4_rounded, tiles
+        elif rows <= TILED_ROWS:
+            product, scaled = kernels._mxfp4_few_rows, scales
+        if product is not None:
+            y = product(flat, blocks, scaled, bias, kernels._on_gpu("mxfp4_linear", flat, blocks, bias))
             return y if flat is x else _finish(x, y, None)
     return _finish(x, functional.linear(flat, kernels.mxfp4_dequantize(blocks, scales, dtype), bias), None)
 
