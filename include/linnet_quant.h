@@ -485,8 +485,8 @@ LNQ_API LnqStatus lnq_mxfp4_dequantize(const uint8_t* blocks, const uint8_t* sca
 
 /* Rows of activations as lnq_mxfp4_mm reads them: lnq_mxfp4_quantize's rounding of x [rows,
  * in] (rows x_stride elements apart, a multiple of 8), the codes in q [rows, in/2], the scales
- * in `scales` as scale tiles (lnq_mxfp4_scale_tiles, with `rows` for `out`). x, q and scales
- * 16-byte aligned. No counterpart in the reference. */
+ * in `scales` as scale tiles (lnq_mxfp4_scale_tiles, with `rows` for `out`). in <= 2^22; x, q and
+ * scales 16-byte aligned. No counterpart in the reference. */
 LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, uint8_t* scales,
                                  int64_t rows, int64_t in_features, int32_t dtype, void* stream);
 

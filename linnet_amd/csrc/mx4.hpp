@@ -20,7 +20,6 @@ constexpr int MAX_EXPERTS = 2048;          // of the pair lists' LDS
 // weight's by its outputs: [pairs of units][blocks of 64 rows][64 lanes][2 units] dwords, lane l's for
 // a unit holding the bytes of rows 16 f + l % 16 (f = 0 .. 3) of the block at block l / 16 of the
 // unit: four MFMAs' scales. Rows and inputs past the last have 0.
-__host__ __device__ inline int units_of(int K) { return (K + 127) / 128; }
 __host__ __device__ inline int pairs_of(int K) { return (K + 255) / 256; }
 __host__ __device__ inline int blocks_of(int N) { return (N + 63) / 64; }
 constexpr int TILE_BYTES = 512;  // of a scale tile: 64 rows by 256 inputs

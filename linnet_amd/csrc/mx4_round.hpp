@@ -8,7 +8,7 @@ namespace lnq {
 
 namespace mxr {
 constexpr int THREADS = 256;
-constexpr int UNIT = 128;  // inputs of a workgroup of the row-rounding kernel
+constexpr int SPAN = 256;  // inputs of a block of threads that rounds rows: a line of codes
 
 // 8 values as loaded.
 template <int DT>
@@ -77,63 +77,58 @@ __device__ inline float scale_of(uint32_t byte) {
 }
 
 // Rows for the product: codes [rows, K / 2], blocks in a row, and scale tiles. 256 threads (tid)
-// take 16 PASSES rows (from `bx` times that) by the 128 inputs of unit `by`, 16 lanes a row, all of
-// their loads before the first conversion; then their scales: dwords of two blocks of 64 rows, or
-// one byte of each dword of their block. `unit`: 16 PASSES dwords of LDS. Every thread of the
-// workgroup calls it (one barrier), without `live` for nothing.
+// take 8 PASSES rows (from `bx` times that) by SPAN inputs (from `by` times that), 32 lanes a row, all
+// of their loads before the first conversion; then their scales: dwords of 64 rows, or one byte of each
+// dword of 16. `unit`: 16 PASSES dwords of LDS. Every thread of the workgroup calls it (one barrier),
+// without `live` for nothing.
 template <int DT, int PASSES>
 __device__ __attribute__((always_inline)) inline void round_rows(const typename Elem<DT>::storage* x, int64_t x_stride, uint32_t* codes, uint32_t* scales,
-                                  int rows, int K, uint32_t* unit, int tid, int bx, int by, bool live) {
-  constexpr int A_PASS = THREADS / 16, ROWS = A_PASS * PASSES;
+                                                                 int rows, int K, uint32_t* unit, int tid, int bx, int by, bool live) {
+  constexpr int A_PASS = THREADS / 32, ROWS = A_PASS * PASSES;
+  static_assert(ROWS == 64 || ROWS == 16, "a block of scales or a byte of its dwords");
   const int lane = tid & 63;
-  const int r0 = bx * ROWS, k = by * UNIT + (tid & 15) * 8;
+  const int r0 = bx * ROWS, k = by * SPAN + (tid & 31) * 8;
   const bool in = live && k < K;
   Raw<DT> raw[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    const int r = min(r0 + i * A_PASS + (tid >> 4), rows - 1);
+    const int r = min(r0 + i * A_PASS + (tid >> 5), rows - 1);
     raw[i] = load8<DT>(x + r * x_stride + (in ? k : 0));
   }
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    const int r = i * A_PASS + (tid >> 4);
+    const int r = i * A_PASS + (tid >> 5);
     float v[8];
     widen8<DT>(raw[i], v);
     uint32_t byte;
     const uint32_t word = round8(v, byte);
     if (r0 + r < rows && in) codes[(static_cast<int64_t>(r0 + r) * K + k) >> 3] = word;
-    // The four blocks of the unit, 16 lanes: block b's byte at bits 8 b.
+    // The four blocks of a unit, 16 lanes: block b's byte at bits 8 b.
     uint32_t four = in ? byte << (8 * ((lane >> 2) & 3)) : 0u;
     four |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(four), 4, 64));
     four |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(four), 8, 64));
-    if ((lane & 15) == 0) unit[r] = r0 + r < rows ? four : 0u;
+    if ((lane & 15) == 0) unit[2 * r + (lane >> 4 & 1)] = r0 + r < rows ? four : 0u;
   }
   __syncthreads();
-  const int blocks = mx4::blocks_of(rows), block = r0 / 64 + (tid >> 6);
-  if (!live || tid >= (ROWS > 64 ? ROWS : 64) || block >= blocks) return;
-  const int u = by & 1, row = lane & 15, shift = 8 * (lane >> 4);
-  const bool alone = u == 0 && by + 1 == mx4::units_of(K);  // the pair's second unit lies past K
-  uint32_t* const at = scales + ((static_cast<int64_t>(by >> 1) * blocks + block) * 64 + lane) * 2;
-  if constexpr (ROWS >= 64) {
+  if (!live || tid >= 128) return;
+  // Dword `tid` of the scale tile: place tid / 2 (row % 16, block of the unit), unit tid % 2.
+  const int row = tid >> 1 & 15, u = tid & 1, shift = 8 * (tid >> 5);
+  uint32_t* const at = scales + (static_cast<int64_t>(by) * mx4::blocks_of(rows) + r0 / 64) * (mx4::TILE_BYTES / 4) + tid;
+  if constexpr (ROWS == 64) {
     uint32_t word = 0;
 #pragma unroll
-    for (int f = 0; f < 4; ++f) word |= (unit[(tid >> 6) * 64 + 16 * f + row] >> shift & 255u) << (8 * f);
-    at[u] = word;
-    if (alone) at[1] = 0;
+    for (int f = 0; f < 4; ++f) word |= (unit[2 * (16 * f + row) + u] >> shift & 255u) << (8 * f);
+    *at = word;
   } else {
-    uint8_t* const bytes = reinterpret_cast<uint8_t*>(at);
-    const int f = r0 % 64 / 16, last = r0 + ROWS >= rows ? 4 : f + 1;  // the last rows' threads write the block's rest
-    for (int i = f; i < last; ++i) {
-      bytes[4 * u + i] = static_cast<uint8_t>(i == f ? unit[row] >> shift : 0u);
-      if (alone) bytes[4 + i] = 0;
-    }
+    const int f = r0 % 64 / 16, last = r0 + ROWS >= rows ? 4 : f + 1;  // the last rows' threads write the tile's rest
+    for (int i = f; i < last; ++i) reinterpret_cast<uint8_t*>(at)[i] = static_cast<uint8_t>(i == f ? unit[2 * row + u] >> shift : 0u);
   }
 }
 
-// Rows that 256 threads take: 128 where that still is four workgroups a CU, else 16.
-inline int rows_a_block(int64_t rows, int64_t K) {
-  return (rows + 127) / 128 * ((K + UNIT - 1) / UNIT) >= 4 * compute_units() ? 128 : 16;
-}
+inline int spans_of(int64_t K) { return static_cast<int>((K + SPAN - 1) / SPAN); }
+
+// Rows that 256 threads take: 64 where that still is four workgroups a CU, else 16.
+inline int rows_a_block(int64_t rows, int64_t K) { return (rows + 63) / 64 * spans_of(K) >= 4 * compute_units() ? 64 : 16; }
 }  // namespace mxr
 
 }  // namespace lnq

@@ -17,6 +17,11 @@
 // again, so the rest reads step g + 1's first operands and issues step g + 2's loads, the next
 // tile's near a tile's end, into step g's stage.
 //
+// Bound by the power that MFMAs, LDS and loads share (a 4096 x 8192 -> 28672 call: 410 to 490 us by
+// the card's warmth, 3.9 to 4.7 PFLOP/s at 1.75 GHz; its MFMAs alone 213, its loads alone 218, all but
+// the stores 390), with few tiles by a step's latency (0.4 us of 64-row tiles, 0.6 of 128), with few
+// rows by HBM (32 experts of 2880 -> 5760: 61 us, 4.4 TB/s).
+//
 // Experts: tiles of BM pairs of one expert, expert by expert with its tiles of rows together for
 // each run of columns; where the next tiles lie is looked up a tile ahead a lookup.
 #include <algorithm>
@@ -611,7 +616,7 @@ static int64_t workspace_of(int64_t pairs, int64_t x_rows, int64_t count, int64_
 template <int DT>
 static void prepare(const Args& a, const int64_t* experts, int pairs, int bm, const void* x, int64_t x_stride, uint8_t* scales,
                     hipStream_t s) {
-  const int per = mxr::rows_a_block(a.M, a.K), spans = units_of(a.K);
+  const int per = mxr::rows_a_block(a.M, a.K), spans = mxr::spans_of(a.K);
   const int blocks = (a.M + per - 1) / per * spans, each = LIST_THREADS / mxr::THREADS;
   const dim3 grid(static_cast<unsigned>(a.count + 1 + (blocks + each - 1) / each));
 #define LNQ_MXP(P)                                                                                                             \
@@ -619,8 +624,8 @@ static void prepare(const Args& a, const int64_t* experts, int pairs, int bm, co
                      const_cast<int*>(a.order), const_cast<i32x4*>(a.table), const_cast<int*>(a.used),                         \
                      static_cast<const uint16_t*>(x), x_stride, reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(a.q)),        \
                      reinterpret_cast<uint32_t*>(scales), a.M, a.K, spans, blocks)
-  if (per == 128) LNQ_MXP(8);
-  else LNQ_MXP(1);
+  if (per == 64) LNQ_MXP(8);
+  else LNQ_MXP(2);
 #undef LNQ_MXP
 }
 

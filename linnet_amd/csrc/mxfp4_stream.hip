@@ -1,5 +1,6 @@
 // The MXFP4 linear layer at few rows, y = x W^T (+ bias) with x in 16 bits: the streaming
-// product (stream.hpp) over codes and E8M0 scales as a checkpoint stores them.
+// product (stream.hpp) over codes and E8M0 scales as a checkpoint stores them. 16 rows, 4096 ->
+// 14336: 13.0 us, 2.4 TB/s.
 #include "stream.hpp"
 
 using namespace lnq;

@@ -23,6 +23,8 @@
 // * a choice is the wave's largest key, the choice rounded once to f32 (order survives rounding)
 //   with its bits in integer order: six DPP maxima. Only where several experts hold that key,
 //   which differ in 64 bits, are those compared.
+// 8192 rows of 256 experts in 8 groups, top 8: 13.9 us, 730 vector instructions a row (54 us with a
+// lane a group in turn, 18.7 with the library's exponential and choices by floats).
 #include "common.hpp"
 
 namespace lnq {
