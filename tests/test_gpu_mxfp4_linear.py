@@ -348,6 +348,57 @@ def test_experts_linear_takes_the_documented_product() -> None:
 # ------------------------------------------------------------------ refusals, streams, graphs
 
 
+@pytest.mark.parametrize(("rows", "out", "depth"), [(70001, 40000, 32), (140000, 64, 32768), (40, 140000, 65536)])
+def test_offsets_past_32_bits(rows: int, out: int, depth: int) -> None:
+    """More than 2^31 outputs, codes of x and of the weight: rows and outputs of both ends and between."""
+    print(f"mm {rows} x {depth} -> {out}", flush=True)
+    gen = torch.Generator(DEV).manual_seed(rows)
+    code = [torch.randint(0, 256, (n, depth // 32, 16), dtype=torch.uint8, device=DEV, generator=gen) for n in (rows, out)]
+    scale = [torch.randint(120, 127, (n, depth // 32), dtype=torch.uint8, device=DEV, generator=gen) for n in (rows, out)]
+    y = kernels.mxfp4_mm(code[0].view(rows, -1), kernels.mxfp4_scale_tiles(scale[0], depth), code[1],
+                         kernels.mxfp4_scale_tiles(scale[1], depth), torch.bfloat16)
+    at = [torch.tensor(sorted({0, 1, n // 3, n // 2, n - 2, n - 1}), device=DEV) for n in (rows, out)]
+    values = [quant.dequantize_mxfp4(c[i].cpu().numpy(), s[i].cpu().numpy()) for c, s, i in zip(code, scale, at)]
+    _check(y[at[0]][:, at[1]], *values)
+
+
+def test_experts_past_32_bits() -> None:
+    """Expert weights of more than 2^32 bytes, the last expert's among those read."""
+    rows, chosen, count, out, depth = 40, 2, 65, 8192, 16384
+    gen = torch.Generator(DEV).manual_seed(1)
+    blocks = torch.randint(0, 256, (count, out, depth // 32, 16), dtype=torch.uint8, device=DEV, generator=gen)
+    scales = torch.randint(120, 127, (count, out, depth // 32), dtype=torch.uint8, device=DEV, generator=gen)
+    x = torch.randn(rows, depth, device=DEV, generator=gen).to(torch.bfloat16)
+    experts = torch.randint(0, count, (rows, chosen), device=DEV, generator=gen)
+    experts[0], experts[-1] = count - 1, torch.tensor([0, count - 1], device=DEV)
+    y = kernels.mxfp4_experts_mm(x, blocks, kernels.mxfp4_scale_tiles(scales, depth), experts)
+    at = torch.tensor([0, 1, out // 2, out - 1], device=DEV)
+    values = _rounded(x)
+    for r, k in ((0, 0), (0, 1), (7, 1), (rows - 1, 0), (rows - 1, 1)):
+        e = int(experts[r, k])
+        w = quant.dequantize_mxfp4(blocks[e, at].cpu().numpy(), scales[e, at].cpu().numpy())
+        _check(y[r, k, at][None], values[r : r + 1], w)
+
+
+@pytest.mark.parametrize("rows", [20, 45])
+def test_experts_of_views(rows: int) -> None:
+    """x with gaps between its rows, transposed and expanded, experts in 32 bits and of a view: as packed ones."""
+    rng = np.random.default_rng(rows)
+    blocks, scales, _ = _weight(rng, 5, 72, 96)
+    operands = quantized.mxfp4_experts_operands(blocks, scales, 1)
+    wide = torch.from_numpy(_values(rng, rows, 160)).to(torch.bfloat16).to(DEV)
+    ids = torch.from_numpy(rng.integers(0, 5, (rows, 6))).to(DEV)
+    for x in (wide[:, 32:128], wide[:, 4:100], wide[:, :96].t().contiguous().t(), wide[:1, :96].expand(rows, 96)):
+        want = quantized.mxfp4_experts_linear(x.contiguous(), operands, ids[:, ::2].contiguous())
+        assert torch.equal(quantized.mxfp4_experts_linear(x, operands, ids[:, ::2]), want)
+        assert torch.equal(quantized.mxfp4_experts_linear(x, operands, ids[:, ::2].to(torch.int32)), want)
+        each = x[:, None, :].expand(rows, 3, 96)
+        assert torch.equal(quantized.mxfp4_experts_linear(each, operands, ids[:, ::2]), want)
+    plain = quantized.mxfp4_operands(blocks[0], scales[0], 1)
+    for x in (wide[:, 32:128], wide[:, 4:100], wide[:, :96].t().contiguous().t(), wide[:1, :96].expand(rows, 96)):
+        assert torch.equal(quantized.mxfp4_linear(x, plain, None), quantized.mxfp4_linear(x.contiguous(), plain, None))
+
+
 def test_refusals() -> None:
     u8 = lambda *shape: torch.zeros(*shape, dtype=torch.uint8, device=DEV)  # noqa: E731
     x = torch.zeros(4, 64, dtype=torch.bfloat16, device=DEV)
