@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import dataclasses
 import functools
+import math
 
 import torch
 from torch.autograd import forward_ad
@@ -64,6 +65,16 @@ _HERE = _Here()
 
 def _on(device: torch.device) -> _Here | torch.cuda.device:
     return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _launch(device: torch.device, name: str, *args: object) -> None:
+    """Calls entry point `name` on the current stream of `device`, its last argument."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _stream(device))
 
 
 def _on_gpu(what: str, *tensors: torch.Tensor | None) -> torch.device:
@@ -611,16 +622,15 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     ties to the even code, past 6 to 6 (the OCP microscaling format's conversion). A block with
     an infinity or a NaN gets s = 255, which every reader but `mxfp4_experts` takes as NaN."""
     device = _on_gpu("mxfp4_quantize", x)
-    if x.dim() == 0 or x.shape[-1] % 32:
-        raise LinnetError(f"mxfp4_quantize: x is [..., In] with In % 32 == 0, got {tuple(x.shape)}")
+    shape = x.shape
+    if not shape or shape[-1] % 32:
+        raise LinnetError(f"mxfp4_quantize: x is [..., In] with In % 32 == 0, got {tuple(shape)}")
     code = _code(x.dtype, "mxfp4_quantize", _ANY)
-    depth = x.shape[-1]
     x = _aligned(x)
-    blocks = torch.empty(*x.shape[:-1], depth // 32, 16, dtype=torch.uint8, device=device)
-    scales = torch.empty(*x.shape[:-1], depth // 32, dtype=torch.uint8, device=device)
-    with _on(device):
-        _lib.call("lnq_mxfp4_quantize", _ptr(x), _ptr(blocks), _ptr(scales), x.numel() // max(depth, 1), depth, code,
-                  _stream(device))
+    *lead, depth = shape
+    blocks = torch.empty(*lead, depth // 32, 16, dtype=torch.uint8, device=device)
+    scales = torch.empty(*lead, depth // 32, dtype=torch.uint8, device=device)
+    _launch(device, "lnq_mxfp4_quantize", x.data_ptr(), blocks.data_ptr(), scales.data_ptr(), math.prod(lead), depth, code)
     return blocks, scales
 
 
@@ -632,10 +642,9 @@ def mxfp4_dequantize(blocks: torch.Tensor, scales: torch.Tensor, dtype: torch.dt
     depth = _mxfp4_operands("mxfp4_dequantize", blocks, scales)
     code = _code(dtype, "mxfp4_dequantize", _ANY)
     blocks, scales = _aligned(blocks), scales.contiguous()
-    out = torch.empty(*blocks.shape[:-2], depth, dtype=dtype, device=device)
-    with _on(device):
-        _lib.call("lnq_mxfp4_dequantize", _ptr(blocks), _ptr(scales), _ptr(out), out.numel() // max(depth, 1), depth, code,
-                  _stream(device))
+    lead = blocks.shape[:-2]
+    out = torch.empty(*lead, depth, dtype=dtype, device=device)
+    _launch(device, "lnq_mxfp4_dequantize", blocks.data_ptr(), scales.data_ptr(), out.data_ptr(), math.prod(lead), depth, code)
     return out
 
 
@@ -708,9 +717,8 @@ def _mxfp4_few_rows(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor,
         x = _aligned(x)
         stride, at = depth, x.data_ptr()
     y = torch.empty(rows, out_features, dtype=dtype, device=device)
-    with _on(device):
-        _lib.call("lnq_mxfp4_linear", at, stride, blocks.data_ptr(), scales.data_ptr(), _ptr(bias), y.data_ptr(), rows,
-                  out_features, depth, code, _stream(device))
+    _launch(device, "lnq_mxfp4_linear", at, stride, blocks.data_ptr(), scales.data_ptr(),
+            None if bias is None else bias.data_ptr(), y.data_ptr(), rows, out_features, depth, code)
     return y
 
 
@@ -819,27 +827,29 @@ def expert_route(logits: torch.Tensor, top: int, bias: torch.Tensor | None = Non
     a place left over holds -1 with weight 0, which the experts' products take as zeros. A row with
     a NaN logit (or +inf under softmax) gets -1 and NaN. E <= 1024, top <= 64, groups <= 64."""
     device = _on_gpu("expert_route", logits, bias)
-    if logits.dim() == 0:
+    shape = logits.shape
+    if not shape:
         raise LinnetError("expert_route: logits are [..., E]")
     if top < 1:
         raise LinnetError(f"expert_route: {top} choices a row")
     if score not in ("softmax", "sigmoid"):
         raise LinnetError(f"expert_route: score is softmax or sigmoid, not {score}")
-    count = logits.shape[-1]
+    *lead, count = shape
     code = _code(logits.dtype, "expert_route", _ANY)
     if bias is not None:
         if bias.dtype != torch.float32 or bias.shape != (count,):
             raise LinnetError(f"expert_route: bias is [{count}] float32, got {tuple(bias.shape)} {bias.dtype}")
         bias = bias.contiguous()
-    lead = logits.shape[:-1]
-    flat = logits if logits.dim() == 2 else logits.reshape(-1, count)
-    if flat.stride(1) != 1 and count > 1:
+    flat = logits if len(shape) == 2 else logits.reshape(-1, count)
+    stride, step = flat.stride()
+    if step != 1 and count > 1:
         flat = flat.contiguous()
+        stride = count
     experts = torch.empty(*lead, top, dtype=torch.int64, device=device)
     weights = torch.empty(*lead, top, dtype=torch.float32, device=device)
-    with _on(device):
-        _lib.call("lnq_expert_route", _ptr(flat), flat.stride(0), _ptr(bias), _ptr(experts), _ptr(weights), flat.shape[0], count,
-                  top, groups, group_top, group_best, int(score == "softmax"), int(renormalize), scale, code, _stream(device))
+    _launch(device, "lnq_expert_route", flat.data_ptr(), stride, None if bias is None else bias.data_ptr(), experts.data_ptr(),
+            weights.data_ptr(), math.prod(lead), count, top, groups, group_top, group_best, 1 if score == "softmax" else 0,
+            1 if renormalize else 0, scale, code)
     return experts, weights
 
 
