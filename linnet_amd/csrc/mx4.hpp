@@ -33,7 +33,7 @@ struct Args {
   uint16_t* y;
   int M, N, K;
   int x_blocks;          // of 64 rows, of x's scale tiles
-  // Experts: the pairs by expert, and tiles of them: (expert, first place in `order`, pairs + 512 *
+  // Experts: the pairs by the places of their tiles, and the tiles: (expert, first place, pairs + 512 *
   // tiles of the expert, the expert's first tile); used[0]: the tiles there are.
   const int* order;
   const i32x4* table;

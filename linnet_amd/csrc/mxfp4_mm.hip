@@ -426,15 +426,15 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   wait_vm<0>();
 }
 
-// The pairs of each expert, in order: workgroup e counts every expert's pairs, which tells it
-// where its own begin in `order` and in the tile table, then lists them, each wave those of its
-// own run of the pairs. Workgroup `count` lists the pairs whose choice is no expert and writes how
-// many tiles there are.
+// The pairs of each expert, in order, by the places of its tiles: workgroup e counts every expert's
+// pairs, which tells it where its own tiles begin, then lists them, each wave those of its own run
+// of the pairs; places past them name pair 0. Workgroup `count` lists the pairs whose choice is no
+// expert and writes how many tiles there are.
 __device__ __attribute__((always_inline)) inline void list_pairs(int e, const int64_t* experts, int pairs, int count, int bm, int* order, i32x4* table, int* used) {
   using namespace mx4;
   constexpr int WAVES = LIST_THREADS / 64, DEEP = 8;  // loads in flight
   __shared__ int number[MAX_EXPERTS + 1];
-  __shared__ int part[3][WAVES], found[WAVES];
+  __shared__ int part[2][WAVES], found[WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int run = (pairs + 64 * WAVES - 1) / (64 * WAVES) * 64;  // pairs of a wave
   const int from = wave * run, to = min(pairs, from + run);
@@ -460,32 +460,32 @@ __device__ __attribute__((always_inline)) inline void list_pairs(int e, const in
   });
   if (lane == 0) found[wave] = here;
   __syncthreads();
-  // Pairs and tiles of the experts before this one, and tiles of all.
-  int sums[3] = {0, 0, 0};
+  // Tiles of the experts before this one, and of all.
+  int sums[2] = {0, 0};
   for (int i = tid; i <= count; i += LIST_THREADS) {
-    const int n = number[i], t = (n + bm - 1) / bm;
-    if (i < e) sums[0] += n, sums[1] += t;
-    sums[2] += t;
+    const int t = (number[i] + bm - 1) / bm;
+    if (i < e) sums[0] += t;
+    sums[1] += t;
   }
 #pragma unroll
-  for (int s = 0; s < 3; ++s) {
+  for (int s = 0; s < 2; ++s) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) sums[s] += __shfl_xor(sums[s], off, 64);
     if (lane == 0) part[s][wave] = sums[s];
   }
   __syncthreads();
-  int first = 0, tile = 0, all = 0, at = 0;
+  int tile = 0, all = 0, at = 0;
 #pragma unroll 4
   for (int v = 0; v < WAVES; ++v) {
-    first += part[0][v], tile += part[1][v], all += part[2][v];
+    tile += part[0][v], all += part[1][v];
     if (v < wave) at += found[v];
   }
-  const int mine = number[e];
-  for (int i = tid; i * bm < mine; i += LIST_THREADS)
-    table[tile + i] = i32x4{e, first + i * bm, min(bm, mine - i * bm) + 512 * ((mine + bm - 1) / bm), tile};
+  const int mine = number[e], tiles = (mine + bm - 1) / bm;
+  for (int i = tid; i < tiles; i += LIST_THREADS) table[tile + i] = i32x4{e, (tile + i) * bm, min(bm, mine - i * bm) + 512 * tiles, tile};
   if (e == count && tid == 0) used[0] = all;
   if (mine == 0) return;
-  at += first;
+  at += tile * bm;
+  if (mine + tid < tiles * bm) order[tile * bm + mine + tid] = 0;
   each([&](int p, int bucket) {
     const uint64_t mask = __ballot(bucket == e);
     if (bucket == e) order[at + __popcll(mask & ((uint64_t{1} << lane) - 1))] = p;
@@ -516,21 +516,24 @@ __global__ __launch_bounds__(mx4::LIST_THREADS, 8) void expert_prepare_kernel(co
   }
 }
 
-// x's scales by the tiles' rows, as scale tiles: `each` blocks of 64 rows a tile of the product.
+// x's scales by the tiles' rows, as scale tiles: `each` blocks of 64 rows a tile of bm.
 __global__ __launch_bounds__(256) void expert_scales_kernel(const uint8_t* __restrict__ from, uint32_t* __restrict__ to,
-                                                            const int* __restrict__ order, const i32x4* __restrict__ table,
-                                                            const int* __restrict__ used, int from_blocks, int blocks,
-                                                            int each, int chosen) {
-  const int i = blockIdx.x * 256 + threadIdx.x, block = i >> 7, t = block / each;
-  if (t >= used[0]) return;
-  const i32x4 entry = table[t];
-  const int live = entry.z & 511, r0 = (block - t * each) * 64 + (i >> 1 & 15);  // of the tile
+                                                            const int* __restrict__ order, const int* __restrict__ used,
+                                                            int from_blocks, int blocks, int each, int bm, int chosen) {
+  const int i = blockIdx.x * 256 + threadIdx.x, block = i >> 7;
+  if (block >= blocks) return;
+  const int t = block / each, r0 = (block - t * each) * 64 + (i >> 1 & 15);  // of the tile
   const int64_t pair = blockIdx.y;
   const uint32_t at = (i >> 5 & 3) * 128 + (i & 1) * 4;  // block of the unit, unit
+  const int tiles = used[0];
+  int place[4];  // beside the load above, and used only if the tile is there
+#pragma unroll
+  for (int f = 0; f < 4; ++f) place[f] = order[t * bm + min(r0 + 16 * f, bm - 1)];
+  if (t >= tiles) return;
   uint32_t word = 0;
 #pragma unroll
   for (int f = 0; f < 4; ++f) {
-    const int row = order[entry.y + min(r0 + 16 * f, live - 1)] / chosen;
+    const int row = place[f] / chosen;
     const uint8_t byte = from[(pair * from_blocks + (row >> 6)) * mx4::TILE_BYTES + at + (row & 15) * 8 + (row >> 4 & 3)];
     word |= static_cast<uint32_t>(byte) << (8 * f);
   }
@@ -584,7 +587,7 @@ static void launch(const Args& a, int bm, hipStream_t s) {
 }
 
 // The workspace of a call with tiles of `bm` pairs (tiles at most: a partial one for each expert that
-// is named): x's codes and scale tiles, the pairs in order, the tile table with how many there are, x's
+// is named): x's codes and scale tiles, the pairs by the tiles' places, the tile table with how many there are, x's
 // scales by the tiles' rows.
 struct Plan {
   int tiles, each;  // blocks of 64 rows a tile
@@ -600,7 +603,7 @@ static Plan experts_plan(int bm, int64_t pairs, int64_t x_rows, int64_t count, i
   p.blocks = static_cast<int64_t>(p.tiles) * p.each;
   p.scales = whole(x_rows * (in_features / 2));
   p.order = p.scales + spans * ((x_rows + 63) / 64) * TILE_BYTES;
-  p.table = p.order + whole(pairs * 4);
+  p.table = p.order + whole(static_cast<int64_t>(p.tiles) * bm * 4);
   p.sorted = p.table + whole(static_cast<int64_t>(p.tiles) * 16 + 16);
   p.bytes = p.sorted + spans * p.blocks * TILE_BYTES;
   return p;
@@ -740,8 +743,8 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const void* x, int64_t x_stride, const ui
   else mx4::prepare<LNQ_F16>(a, experts, static_cast<int>(pairs), bm, x, x_stride, scales, s);
   if (const LnqStatus st = launched("expert_prepare")) return st;
   hipLaunchKernelGGL(expert_scales_kernel, dim3(static_cast<unsigned>((plan.blocks + 1) / 2), static_cast<unsigned>(mx4::pairs_of(a.K))),
-                     dim3(256), 0, s, scales, reinterpret_cast<uint32_t*>(sorted), a.order, a.table, a.used, mx4::blocks_of(a.M),
-                     a.x_blocks, plan.each, a.chosen);
+                     dim3(256), 0, s, scales, reinterpret_cast<uint32_t*>(sorted), a.order, a.used, mx4::blocks_of(a.M), a.x_blocks,
+                     plan.each, bm, a.chosen);
   if (const LnqStatus st = launched("expert_scales")) return st;
   if (dtype == LNQ_BF16) mx4::launch<LNQ_BF16, true>(a, bm, s);
   else mx4::launch<LNQ_F16, true>(a, bm, s);

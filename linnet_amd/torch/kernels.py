@@ -800,17 +800,29 @@ def mxfp4_experts_mm(x: torch.Tensor, blocks: torch.Tensor, tiles: torch.Tensor,
         raise LinnetError(f"mxfp4_experts_mm: x {tuple(x.shape)} against experts {tuple(experts.shape)} and blocks "
                           f"{tuple(blocks.shape)}")
     _mxfp4_tiles("mxfp4_experts_mm", tiles, (count,), out_features, groups * 32)
-    code = _code(x.dtype, "mxfp4_experts_mm")
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+    return _mxfp4_experts_product(x, _aligned(blocks), _aligned(tiles), experts, device)
+
+
+def _mxfp4_experts_product(x: torch.Tensor, blocks: torch.Tensor, tiles: torch.Tensor, experts: torch.Tensor,
+                           device: torch.device) -> torch.Tensor:
+    """`mxfp4_experts_mm` of operands that were looked over before."""
+    count, out_features, groups, _ = blocks.shape
+    rows, chosen = experts.shape
+    x_rows, depth = x.shape
+    dtype = x.dtype
+    code = _code(dtype, "mxfp4_experts_mm")
+    stride, step = x.stride()
+    at = x.data_ptr()
+    if step != 1 or stride % 8 or at % 16:
         x = _aligned(x)
-    blocks, tiles = _aligned(blocks), _aligned(tiles)
-    ids = experts.to(torch.int64).contiguous()
-    y = torch.empty(rows, chosen, out_features, dtype=x.dtype, device=device)
-    need = _mxfp4_workspace(rows * chosen, x.shape[0], count, groups * 32)
+        stride, at = depth, x.data_ptr()
+    ids = experts if experts.dtype == torch.int64 else experts.to(torch.int64)
+    ids = ids.contiguous()
+    y = torch.empty(rows, chosen, out_features, dtype=dtype, device=device)
+    need = _mxfp4_workspace(rows * chosen, x_rows, count, depth)
     space = torch.empty(need, dtype=torch.uint8, device=device)
-    with _on(device):
-        _lib.call("lnq_mxfp4_experts_mm", _ptr(x), x.stride(0), _ptr(blocks), _ptr(tiles), _ptr(ids), _ptr(y), rows, chosen,
-                  count, out_features, groups * 32, int(x.shape[0] == rows), code, _ptr(space), need, _stream(device))
+    _launch(device, "lnq_mxfp4_experts_mm", at, stride, blocks.data_ptr(), tiles.data_ptr(), ids.data_ptr(), y.data_ptr(), rows,
+            chosen, count, out_features, depth, 1 if x_rows == rows else 0, code, space.data_ptr(), need)
     return y
 
 

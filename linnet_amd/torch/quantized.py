@@ -222,10 +222,11 @@ def mxfp4_experts_operands(blocks: torch.Tensor, scales: torch.Tensor, rounded: 
     """The experts of an MXFP4 mixture as stored, `blocks` [E, Out, In/32, 16] and `scales` [E, Out,
     In/32] u8, with, where `rounded`, the scales laid out for the 4-bit product too."""
     _gpu(blocks)
-    if blocks.dim() != 4 or tuple(scales.shape) != tuple(blocks.shape[:3]):
-        raise LinnetError(f"mxfp4_experts_operands: blocks [E, Out, In/32, 16] and scales [E, Out, In/32], got "
-                          f"{tuple(blocks.shape)} and {tuple(scales.shape)}")
-    blocks, scales = blocks.contiguous(), scales.contiguous()
+    kernels._on_gpu("mxfp4_experts_operands", blocks, scales)
+    if blocks.dim() != 4:
+        raise LinnetError(f"mxfp4_experts_operands: blocks are [E, Out, In/32, 16], got {tuple(blocks.shape)}")
+    kernels._mxfp4_operands("mxfp4_experts_operands", blocks, scales)
+    blocks, scales = kernels._aligned(blocks), scales.contiguous()
     tiles = kernels.mxfp4_scale_tiles(scales, blocks.shape[2] * 32) if rounded else None
     return blocks, scales, tiles, rounded
 
@@ -236,13 +237,18 @@ def mxfp4_experts_linear(x: torch.Tensor, operands: Mxfp4Operands, experts: torc
     `FEW_ROWS` rows with `rounded`, x rounded to MXFP4 and each expert's pairs multiplied together
     in 4 bits; else `kernels.mxfp4_experts`. An expert outside 0 .. E - 1 gives zeros."""
     blocks, scales, tiles, rounded = operands
-    if experts.dim() != 2 or x.dim() not in (2, 3) or tuple(x.shape[:-1]) != tuple(experts.shape[: x.dim() - 1]):
-        raise LinnetError(f"mxfp4_experts_linear: x [R, In] or [R, K, In] and experts [R, K], got {tuple(x.shape)} and "
-                          f"{tuple(experts.shape)}")
+    shape = x.shape
+    if experts.dim() != 2 or experts.is_floating_point() or len(shape) not in (2, 3) or shape[:-1] != experts.shape[: len(shape) - 1]:
+        raise LinnetError(f"mxfp4_experts_linear: x [R, In] or [R, K, In] and experts [R, K] of integers, got {tuple(shape)} and "
+                          f"{tuple(experts.shape)} {experts.dtype}")
     rows, chosen = experts.shape
-    x_rows = rows if x.dim() == 2 else rows * chosen
+    depth = shape[-1]
+    if depth != blocks.shape[2] * 32:
+        raise LinnetError(f"mxfp4_experts_linear: x {tuple(shape)} against experts of {blocks.shape[2] * 32} inputs")
+    x_rows = rows if len(shape) == 2 else rows * chosen
     if (rounded and tiles is not None and rows > FEW_ROWS and x.dtype in _HALF and blocks.shape[0] <= kernels.MXFP4_MM_EXPERTS
-            and x_rows * x.shape[-1] < 1 << 32):
-        return kernels.mxfp4_experts_mm(x.reshape(x_rows, x.shape[-1]), blocks, tiles, experts)
+            and x_rows * depth < 1 << 32):
+        flat = x if len(shape) == 2 else x.reshape(x_rows, depth)
+        return kernels._mxfp4_experts_product(flat, blocks, tiles, experts, kernels._on_gpu("mxfp4_experts_linear", x, blocks, experts))
     shared = x[:, None, :].expand(rows, chosen, x.shape[1]) if x.dim() == 2 else x
     return kernels.mxfp4_experts(shared, blocks, scales, experts)
