@@ -255,38 +255,34 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   // for the stores too).
   typedef u32x4 __attribute__((aligned(2))) loose_u32x4;  // rows of an odd width begin anywhere
   constexpr int STORES = FB == 2 ? 1 : 2;                // of a row of (up to four) fragments
-  auto epilogue_of = [&](const Tile& t, auto bias_tag) __attribute__((always_inline)) {
-    constexpr bool BIAS = decltype(bias_tag)::value;
+  auto store_tile = [&](const Tile& t, auto whole_tag) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole_tag)::value;  // all columns are there
     const int n0 = t.n0 + wn * FB * 16;
-    float bias[BIAS ? FB : 1][4];
-    if constexpr (BIAS) {
-#pragma unroll
-      for (int j = 0; j < FB; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) bias[j][r] = E::to_f32(a.bias[min(n0 + 16 * j + 4 * lk + r, a.N - 1)]);
-    }
-    // This lane's row of store h of row i of fragments, of the tile: first + 16 i + 8 h; its columns.
+    // This lane's row of store i, of the tile: first + 16 / STORES i; its columns, from n0.
     const int first = wm * FA * 16 + (FB == 2 ? lrow : lrow & 7);
-    const int n = n0 + 16 * (lk & 1) + 8 * (lk >> 1) + (FB == 2 ? 0 : 32 * (lrow >> 3));
+    const int col = 16 * (lk & 1) + 8 * (lk >> 1) + (FB == 2 ? 0 : 32 * (lrow >> 3));
     int to_row[EXPERTS ? STORES * FA : 1];
     if constexpr (EXPERTS) {
 #pragma unroll
       for (int i = 0; i < STORES * FA; ++i) to_row[i] = a.order[t.first + min(first + (16 / STORES) * i, t.live - 1)];
     }
+    // The rows are here before the first store: a wait for them between stores would wait for the
+    // stores too, each in turn.
+    if constexpr (EXPERTS) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     __builtin_amdgcn_sched_barrier(0);
-    uint16_t* to = EXPERTS ? a.y + n : a.y + static_cast<int64_t>(t.m0 + first) * a.N + n;
+    // The next store's row, or with experts the columns of any.
+    uint16_t* to = EXPERTS ? a.y + n0 + col : a.y + static_cast<int64_t>(t.m0 + first) * a.N + n0 + col;
     const int64_t step = static_cast<int64_t>(16 / STORES) * a.N;
-    auto store = [&](int i, int c, u32x4 v) {  // at column n + c
+    auto store = [&](int i, int c, u32x4 v) __attribute__((always_inline)) {  // at column n0 + col + c
+      if (first + (16 / STORES) * i >= t.live) return;
       uint16_t* const at = (EXPERTS ? to + static_cast<int64_t>(to_row[EXPERTS ? i : 0]) * a.N : to) + c;
-      if (first + (16 / STORES) * i < t.live) {
-        if (n + c + 8 <= a.N) {
-          // Past the L2's usual order: what y would push out there, the operands, is read again.
-          __builtin_nontemporal_store(v, reinterpret_cast<loose_u32x4*>(at));
-        } else {
+      if (WHOLE || n0 + col + c + 8 <= a.N) {
+        // Past the L2's usual order: what y would push out there, the operands, is read again.
+        __builtin_nontemporal_store(v, reinterpret_cast<loose_u32x4*>(at));
+      } else {
 #pragma unroll
-          for (int r = 0; r < 8; ++r)
-            if (n + c + r < a.N) at[r] = static_cast<uint16_t>(v[r >> 1] >> (16 * (r & 1)));
-        }
+        for (int r = 0; r < 8; ++r)
+          if (n0 + col + c + r < a.N) at[r] = static_cast<uint16_t>(v[r >> 1] >> (16 * (r & 1)));
       }
     };
 #pragma unroll
@@ -296,8 +292,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
       for (int j = 0; j < FB; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float lo = acc[i][j][2 * h], hi = acc[i][j][2 * h + 1];
-          if constexpr (BIAS) lo += bias[j][2 * h], hi += bias[j][2 * h + 1];
+          const float lo = acc[i][j][2 * h], hi = acc[i][j][2 * h + 1];
           o[j][h] = DT == LNQ_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
         }
       // Lane quarter k of fragments 2 p, 2 p + 1 then holds columns 8 (k / 2) .. + 7 of fragment 2 p + k % 2.
@@ -337,17 +332,26 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
     }
   };
   auto epilogue = [&](const Tile& t) __attribute__((always_inline)) {
+    if (EXPERTS && t.e >= a.count) {  // pairs whose choice is no expert: zeros
+#pragma unroll
+      for (int i = 0; i < FA; ++i)
+#pragma unroll
+        for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     if (!EXPERTS && a.bias != nullptr) {
-      epilogue_of(t, std::true_type{});
-    } else {
-      if (EXPERTS && t.e >= a.count) {  // pairs whose choice is no expert: zeros
+#pragma unroll
+      for (int j = 0; j < FB; ++j) {
+        f32x4 bias;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bias[r] = E::to_f32(a.bias[min(t.n0 + (wn * FB + j) * 16 + 4 * lk + r, a.N - 1)]);
 #pragma unroll
         for (int i = 0; i < FA; ++i)
 #pragma unroll
-          for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int r = 0; r < 4; ++r) acc[i][j][r] += bias[r];
       }
-      epilogue_of(t, std::false_type{});
     }
+    if (t.n0 + BN <= a.N) store_tile(t, std::true_type{});
+    else store_tile(t, std::false_type{});
   };
 
   // `now` multiplies, `loading` is the tile of the loads (the same, or the next one: a tile has two
