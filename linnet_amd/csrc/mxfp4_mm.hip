@@ -17,8 +17,8 @@
 // again, so the rest reads step g + 1's first operands and issues step g + 2's loads, the next
 // tile's near a tile's end, into step g's stage.
 //
-// Bound by the power that MFMAs, LDS and loads share (a 4096 x 8192 -> 28672 call: 410 to 490 us by
-// the card's warmth, 3.9 to 4.7 PFLOP/s at 1.75 GHz; its MFMAs alone 213, its loads alone 218, all but
+// Bound by the power that MFMAs, LDS and loads share (a 4096 x 8192 -> 28672 call: 400 to 475 us by
+// the card's warmth, 4.1 to 4.8 PFLOP/s at 1.75 GHz; its MFMAs alone 213, its loads alone 218, all but
 // the stores 390), with few tiles by a step's latency (0.4 us of 64-row tiles, 0.6 of 128), with few
 // rows by HBM (32 experts of 2880 -> 5760: 61 us, 4.4 TB/s).
 //
@@ -48,7 +48,7 @@ struct Form {
   static constexpr int PER_CU = GROUPS < 4 ? GROUPS : 4;
   static constexpr int WAVES_A_SIMD = NW * PER_CU / 4 > 0 ? NW * PER_CU / 4 : 1;
   static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN && NW % 2 == 0, "whole loads, one key a wave");
-  static_assert((FB == 2 || FB == 4 || FB == 8) && BN % 64 == 0 && (FA == 2 || FA == 4 || FA == 8) && ALL <= NW, "scales a lane");
+  static_assert((FB == 2 || FB == 4) && BN % 64 == 0 && (FA == 2 || FA == 4 || FA == 8) && ALL <= NW, "scales a lane");
 };
 }  // namespace mx4
 
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   }
   // Scales of this wave's rows and columns, a dword a unit for 4 fragments (for 2: the half of a
   // dword from these bits on).
-  constexpr int SA = FA == 8 ? 2 : 1, SB = FB == 8 ? 2 : 1;
+  constexpr int SA = FA == 8 ? 2 : 1;
   const uint32_t sa_at = static_cast<uint32_t>(CODES + wm * FA / 4 * TILE_BYTES + lane * 8);
   const uint32_t sw_at = static_cast<uint32_t>(CODES + XC * 1024 + wn * FB / 4 * TILE_BYTES + lane * 8);
   const int a_bits = 8 * (wm * FA % 4), w_bits = 8 * (wn * FB % 4);
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   // MFMAs ahead (a wave of two rows: a set a unit too); both's scales, a set a unit.
   constexpr bool RING = FA >= 4;
   i32x4 af[4], bf[2][FB];
-  uint32_t sa[2][SA], sw[2][SB];
+  uint32_t sa[2][SA], sw[2];
   auto read_a = [&](int u, const uint8_t* st, int f) __attribute__((always_inline)) {
     af[(RING ? 0 : 2 * u) + (f & 3)] = *reinterpret_cast<const i32x4*>(st + aoff[u] + f * 16 * BKB);
   };
@@ -207,8 +207,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   auto read_scales = [&](int u, const uint8_t* st) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < SA; ++h) sa[u][h] = *reinterpret_cast<const uint32_t*>(st + sa_at + h * TILE_BYTES + u * 4);
-#pragma unroll
-    for (int h = 0; h < SB; ++h) sw[u][h] = *reinterpret_cast<const uint32_t*>(st + sw_at + h * TILE_BYTES + u * 4);
+    sw[u] = *reinterpret_cast<const uint32_t*>(st + sw_at + u * 4);
   };
 
   // Unit u of a step on stage `cur`, a slot an MFMA: a row's first slot reads the rows ahead, others
@@ -221,7 +220,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
     constexpr int U = decltype(unit_tag)::value;
     constexpr int AT = RING ? 0 : 2 * U, FROM = U == 1 ? TURN * FB : 0;
     if constexpr (FA == 2) sa[U][0] >>= a_bits;
-    if constexpr (FB == 2) sw[U][0] >>= w_bits;
+    if constexpr (FB == 2) sw[U] >>= w_bits;
     each_of([&](auto slot) __attribute__((always_inline)) {
       constexpr int s = decltype(slot)::value, i = s / FB, j = s % FB;
       if constexpr (U == 1 && s == FROM) {
@@ -231,7 +230,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
         __builtin_amdgcn_sched_barrier(0);
       }
       // The weight is the MFMA's A operand: a lane then holds 4 outputs of a row together.
-      acc[i][j] = mma<j & 3, i & 3>(bf[U][j], af[AT + (i & 3)], acc[i][j], sw[U][j / 4], sa[U][i / 4]);
+      acc[i][j] = mma<j & 3, i & 3>(bf[U][j], af[AT + (i & 3)], acc[i][j], sw[U], sa[U][i / 4]);
       if constexpr (j == 0) {
         if constexpr (!RING) read_a(U ^ 1, nxt, i);
         else if constexpr (i + 3 < FA) read_a(U, cur, i + 3);
@@ -254,7 +253,7 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
   // took a quarter of a 4096 x 8192 -> 28672 call's time, as the next step's wait for its loads waits
   // for the stores too).
   typedef u32x4 __attribute__((aligned(2))) loose_u32x4;  // rows of an odd width begin anywhere
-  constexpr int STORES = FB == 2 ? 1 : 2;                // of a row of (up to four) fragments
+  constexpr int STORES = FB == 2 ? 1 : 2;                // of a row of fragments
   auto store_tile = [&](const Tile& t, auto whole_tag) __attribute__((always_inline)) {
     constexpr bool WHOLE = decltype(whole_tag)::value;  // all columns are there
     const int n0 = t.n0 + wn * FB * 16;
@@ -273,16 +272,16 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
     // The next store's row, or with experts the columns of any.
     uint16_t* to = EXPERTS ? a.y + n0 + col : a.y + static_cast<int64_t>(t.m0 + first) * a.N + n0 + col;
     const int64_t step = static_cast<int64_t>(16 / STORES) * a.N;
-    auto store = [&](int i, int c, u32x4 v) __attribute__((always_inline)) {  // at column n0 + col + c
+    auto store = [&](int i, u32x4 v) __attribute__((always_inline)) {
       if (first + (16 / STORES) * i >= t.live) return;
-      uint16_t* const at = (EXPERTS ? to + static_cast<int64_t>(to_row[EXPERTS ? i : 0]) * a.N : to) + c;
-      if (WHOLE || n0 + col + c + 8 <= a.N) {
+      uint16_t* const at = EXPERTS ? to + static_cast<int64_t>(to_row[EXPERTS ? i : 0]) * a.N : to;
+      if (WHOLE || n0 + col + 8 <= a.N) {
         // Past the L2's usual order: what y would push out there, the operands, is read again.
         __builtin_nontemporal_store(v, reinterpret_cast<loose_u32x4*>(at));
       } else {
 #pragma unroll
         for (int r = 0; r < 8; ++r)
-          if (n0 + col + c + r < a.N) at[r] = static_cast<uint16_t>(v[r >> 1] >> (16 * (r & 1)));
+          if (n0 + col + r < a.N) at[r] = static_cast<uint16_t>(v[r >> 1] >> (16 * (r & 1)));
       }
     };
 #pragma unroll
@@ -304,27 +303,21 @@ __global__ __launch_bounds__(FORM::THREADS, FORM::WAVES_A_SIMD) void mx4_kernel(
           o[j][h] = r[0], o[j + 1][h] = r[1];
         }
       if constexpr (FB == 2) {
-        store(i, 0, u32x4{o[0][0], o[0][1], o[1][0], o[1][1]});
+        store(i, u32x4{o[0][0], o[0][1], o[1][0], o[1][1]});
         if (!EXPERTS) to += step;
       } else {
-        u32x4 p[FB / 4], q[FB / 4];
+        u32x4 p, q;
+        const uint32_t pv[4] = {o[0][0], o[0][1], o[1][0], o[1][1]}, qv[4] = {o[2][0], o[2][1], o[3][0], o[3][1]};
 #pragma unroll
-        for (int j = 0; j < FB; j += 4) {
-          const uint32_t pv[4] = {o[j][0], o[j][1], o[j + 1][0], o[j + 1][1]};
-          const uint32_t qv[4] = {o[j + 2][0], o[j + 2][1], o[j + 3][0], o[j + 3][1]};
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            // Rows 0 .. 7: the first half of the columns from their own lanes, the second in the lanes of
-            // rows 8 .. 15; then the same of those rows.
-            p[j / 4][d] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(pv[d]), static_cast<int>(qv[d]), 0x128, 0xf, 0xc, false));
-            q[j / 4][d] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(qv[d]), static_cast<int>(pv[d]), 0x128, 0xf, 0x3, false));
-          }
+        for (int d = 0; d < 4; ++d) {
+          // Rows 0 .. 7: the first half of the columns from their own lanes, the second in the lanes of
+          // rows 8 .. 15; then the same of those rows.
+          p[d] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(pv[d]), static_cast<int>(qv[d]), 0x128, 0xf, 0xc, false));
+          q[d] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(qv[d]), static_cast<int>(pv[d]), 0x128, 0xf, 0x3, false));
         }
-#pragma unroll
-        for (int j = 0; j < FB / 4; ++j) store(2 * i, 64 * j, p[j]);
+        store(2 * i, p);
         if (!EXPERTS) to += step;
-#pragma unroll
-        for (int j = 0; j < FB / 4; ++j) store(2 * i + 1, 64 * j, q[j]);
+        store(2 * i + 1, q);
         if (!EXPERTS) to += step;
       }
       // One row of fragments at a time: the next tile's operands are live here.
