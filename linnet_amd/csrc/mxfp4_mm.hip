@@ -558,19 +558,22 @@ using Form32 = Form<1, 2, 2, 2>;
 // average). A larger tile reads each operand less often (a wave of 128 x 64 outputs, 24 KB of LDS for
 // 64 MFMAs; of 64 x 64, 32 KB; of 32 x 32, 64 KB), a smaller one leaves fewer CUs idle and fewer rows
 // empty. Measured on both sides of each bound (256 CUs; us of the smaller | the larger tile):
-// 256 rows from 3/4 of a tile a CU: 2048 x 2880 -> 5760, 184 tiles: 28.7 | 29.9; 1024 x 4096 -> 14336,
-// 224: 37.2 | 34.3; 4096 x 8192 -> 8192, 512: 135 | 117. 128 rows from 5/8: 128 x 4096 -> 14336, 112
-// tiles: 11.4 | 13.6; 512 x 2880 -> 5760, 180: 13.7 | 11.5; 1024 x 4096 -> 4096, 256: 18.9 | 14.2.
-// Of an expert's rows: 256 past 128 (32 experts, 2880 -> 5760: at 75 rows 84 | 95, 188: 142 | 110; 128
-// experts, 2048 -> 1536: at 125 69 | 72, 188: 102 | 89); 128 past 48 (8 experts, 4096 -> 14336: at 25
-// 47 | 51, 100: 74 | 60); 64 past 20 (32 experts, 2880 -> 5760: at 12 61 | 67, 25: 74 | 73).
+// 256 rows from 0.7 of a tile a CU: 2048 x 4096 -> 4096, 128 tiles: 21.6 | 28.7; 2048 x 2880 -> 5760,
+// 184: 27.4 | 26.7; 1024 x 4096 -> 14336, 224: 37.2 | 32.4; 4096 x 8192 -> 8192, 512: 132 | 116. 128
+// rows from 5/8: 128 x 4096 -> 14336, 112 tiles: 11.2 | 13.5; 512 x 2880 -> 5760, 180: 13.6 | 11.2;
+// 1024 x 4096 -> 4096, 256: 18.5 | 14.1.
+// Of an expert's rows: 256 past 128 (32 experts, 2880 -> 5760: at 75 rows 77 | 89, 188: 129 | 105; 128
+// experts, 2048 -> 1536: at 125 63 | 65, 188: 81 | 72; worst, 8 experts, 4096 -> 14336 at 250, whose
+// tiles then fill a third round: 85 | 109); 128 past 28 (32 experts, 2880 -> 5760, 32 rows a tile | 128:
+// at 25 66 | 69, 50: 99 | 72; 2880 -> 2880: at 25 36 | 39, 50: 45 | 40; 64 rows: 39).
 static int tile_rows(double rows, int64_t count, int64_t N, bool experts) {
   const auto tiles = [&](int bm, int bn) {
     return static_cast<double>(count) * std::ceil(rows / bm) * static_cast<double>((N + bn - 1) / bn);
   };
-  if (rows > 128 && tiles(256, 256) >= 0.75 * compute_units()) return 256;
-  if (rows > 48 && tiles(128, 128) >= 0.625 * compute_units()) return 128;
-  return rows > 20 || !experts ? 64 : 32;
+  const int many = experts ? 28 : 64;
+  if (rows > 128 && tiles(256, 256) >= 0.7 * compute_units()) return 256;
+  if (rows > many && tiles(128, 128) >= 0.625 * compute_units()) return 128;
+  return rows > many || !experts ? 64 : 32;
 }
 
 template <int DT, bool EXPERTS>

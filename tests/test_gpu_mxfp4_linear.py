@@ -304,7 +304,7 @@ def _experts(rng: np.random.Generator, kind: str, rows: int, chosen: int, count:
 @pytest.mark.parametrize("dtype", list(HALF))
 @pytest.mark.parametrize(("rows", "chosen", "count", "out", "depth"), [
     (1, 1, 1, 1, 32), (33, 4, 8, 70, 96), (40, 2, 5, 128, 288), (70, 1, 3, 33, 160), (257, 4, 4, 64, 128),
-    (300, 3, 40, 36, 64), (64, 8, 2, 200, 544), (700, 4, 40, 520, 160), (1400, 4, 40, 1100, 96)])
+    (300, 3, 40, 36, 64), (64, 8, 2, 200, 544), (100, 2, 3, 500, 96), (700, 4, 40, 520, 160), (1400, 4, 40, 1100, 96)])
 def test_experts_mm(rows: int, chosen: int, count: int, out: int, depth: int, dtype: torch.dtype, kind: str) -> None:
     print(f"experts {kind} rows={rows} chosen={chosen} E={count} {depth} -> {out} {dtype}", flush=True)
     rng = np.random.default_rng(rows + chosen + count + out)
