@@ -493,7 +493,7 @@ __device__ __attribute__((always_inline)) inline void list_pairs(int e, const in
 // What the product of the experts needs: workgroups 0 .. count list the pairs, and the others round
 // x's rows, four blocks of mxr::THREADS threads each (`spans` of them to a run of rows, `blocks` in
 // all). Neither waits for the other: in one launch the shorter costs nothing (4 to 10 us).
-template <int DT, int PASSES>
+template <int DT>
 __global__ __launch_bounds__(mx4::LIST_THREADS, 8) void expert_prepare_kernel(const int64_t* __restrict__ experts, int pairs,
                                                                            int count, int bm, int* __restrict__ order,
                                                                            i32x4* __restrict__ table, int* __restrict__ used,
@@ -505,10 +505,10 @@ __global__ __launch_bounds__(mx4::LIST_THREADS, 8) void expert_prepare_kernel(co
     list_pairs(blockIdx.x, experts, pairs, count, bm, order, table, used);
   } else {
     constexpr int EACH = mx4::LIST_THREADS / mxr::THREADS;
-    __shared__ uint32_t unit[EACH][16 * PASSES];
+    __shared__ uint32_t unit[EACH][2 * mxr::ROWS];
     const int part = __builtin_amdgcn_readfirstlane(threadIdx.x / mxr::THREADS);
     const int b = (blockIdx.x - count - 1) * EACH + part, block = min(b, blocks - 1);
-    mxr::round_rows<DT, PASSES>(x, x_stride, codes, scales, rows, K, unit[part], threadIdx.x % mxr::THREADS, block / spans,
+    mxr::round_rows<DT>(x, x_stride, codes, scales, rows, K, unit[part], threadIdx.x % mxr::THREADS, block / spans,
                                 block % spans, b < blocks);
   }
 }
@@ -619,17 +619,12 @@ static int64_t workspace_of(int64_t pairs, int64_t x_rows, int64_t count, int64_
 template <int DT>
 static void prepare(const Args& a, const int64_t* experts, int pairs, int bm, const void* x, int64_t x_stride, uint8_t* scales,
                     hipStream_t s) {
-  const int per = mxr::rows_a_block(a.M, a.K), spans = mxr::spans_of(a.K);
-  const int blocks = (a.M + per - 1) / per * spans, each = LIST_THREADS / mxr::THREADS;
+  const int spans = mxr::spans_of(a.K), blocks = (a.M + mxr::ROWS - 1) / mxr::ROWS * spans, each = LIST_THREADS / mxr::THREADS;
   const dim3 grid(static_cast<unsigned>(a.count + 1 + (blocks + each - 1) / each));
-#define LNQ_MXP(P)                                                                                                             \
-  hipLaunchKernelGGL((expert_prepare_kernel<DT, P>), grid, dim3(LIST_THREADS), 0, s, experts, pairs, a.count, bm,              \
-                     const_cast<int*>(a.order), const_cast<i32x4*>(a.table), const_cast<int*>(a.used),                         \
-                     static_cast<const uint16_t*>(x), x_stride, reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(a.q)),        \
-                     reinterpret_cast<uint32_t*>(scales), a.M, a.K, spans, blocks)
-  if (per == 64) LNQ_MXP(8);
-  else LNQ_MXP(2);
-#undef LNQ_MXP
+  hipLaunchKernelGGL((expert_prepare_kernel<DT>), grid, dim3(LIST_THREADS), 0, s, experts, pairs, a.count, bm,
+                     const_cast<int*>(a.order), const_cast<i32x4*>(a.table), const_cast<int*>(a.used), static_cast<const uint16_t*>(x),
+                     x_stride, reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(a.q)), reinterpret_cast<uint32_t*>(scales), a.M, a.K,
+                     spans, blocks);
 }
 
 }  // namespace mx4

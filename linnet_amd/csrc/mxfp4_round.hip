@@ -11,8 +11,8 @@
 //
 // Bound by HBM: 2 or 4 bytes a value read, 17/32 written (back: the reverse). Four lanes
 // take a block, 8 values each: a wave's loads are whole kilobytes. 8192 x 14336 bf16: 50 us each
-// way, 5.9 TB/s; as rows of the product, 4096 x 8192: 19.0 us, 4.4 TB/s (24.7 with half a line of
-// codes a workgroup and a row, the other half written from another XCD).
+// way, 5.9 TB/s; as rows of the product, 4096 x 8192: 16.6 us, 5.1 TB/s (half
+// a line of codes a workgroup and a row, the other half written from another XCD: 24.7).
 #include "mx4_round.hpp"
 
 namespace lnq {
@@ -33,13 +33,13 @@ __global__ __launch_bounds__(mxr::THREADS) void mxfp4_quantize_kernel(const type
   if ((threadIdx.x & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(byte);
 }
 
-// Rows for the product, 8 PASSES by SPAN inputs a workgroup, those of a row together.
-template <int DT, int PASSES>
+// Rows for the product, ROWS by SPAN inputs a workgroup, those of a row together.
+template <int DT>
 __global__ __launch_bounds__(mxr::THREADS) void mxfp4_rows_kernel(const typename Elem<DT>::storage* __restrict__ x,
                                                                   int64_t x_stride, uint32_t* __restrict__ codes,
                                                                   uint32_t* __restrict__ scales, int rows, int K, int spans) {
-  __shared__ uint32_t unit[16 * PASSES];
-  mxr::round_rows<DT, PASSES>(x, x_stride, codes, scales, rows, K, unit, threadIdx.x, blockIdx.x / spans, blockIdx.x % spans, true);
+  __shared__ uint32_t unit[2 * mxr::ROWS];
+  mxr::round_rows<DT>(x, x_stride, codes, scales, rows, K, unit, threadIdx.x, blockIdx.x / spans, blockIdx.x % spans, true);
 }
 
 template <int DT>
@@ -157,23 +157,17 @@ LNQ_API LnqStatus lnq_mxfp4_rows(const void* x, int64_t x_stride, uint8_t* q, ui
   LNQ_REQUIRE(x && q && scales, "lnq_mxfp4_rows: null pointer");
   LNQ_REQUIRE(x_stride >= 0 && x_stride % 8 == 0 && aligned(x, 16) && aligned(q, 16) && aligned(scales, 16),
               "lnq_mxfp4_rows: x (with its row stride), q and scales must be 16-byte aligned");
-  const int spans = mxr::spans_of(in_features), per = mxr::rows_a_block(rows, in_features);
-  const int64_t grid = (rows + per - 1) / per * spans;
+  const int spans = mxr::spans_of(in_features);
+  const int64_t grid = (rows + mxr::ROWS - 1) / mxr::ROWS * spans;
   LNQ_REQUIRE(in_features <= (1 << 22) && grid <= INT32_MAX, "lnq_mxfp4_rows: too large (in past 2^22)");
   const int R = static_cast<int>(rows), K = static_cast<int>(in_features);
-#define LNQ_MXW(DT, P)                                                                                                \
-  hipLaunchKernelGGL((mxfp4_rows_kernel<DT, P>), dim3(static_cast<unsigned>(grid)), dim3(mxr::THREADS), 0, static_cast<hipStream_t>(stream), \
-                     static_cast<const typename Elem<DT>::storage*>(x), x_stride, reinterpret_cast<uint32_t*>(q),     \
-                     reinterpret_cast<uint32_t*>(scales), R, K, spans)
-#define LNQ_MXW_P(DT)                \
-  do {                               \
-    if (per == 64) LNQ_MXW(DT, 8);   \
-    else LNQ_MXW(DT, 2);             \
-  } while (0)
-  if (dtype == LNQ_BF16) LNQ_MXW_P(LNQ_BF16);
-  else if (dtype == LNQ_F16) LNQ_MXW_P(LNQ_F16);
-  else LNQ_MXW_P(LNQ_F32);
-#undef LNQ_MXW_P
+#define LNQ_MXW(DT)                                                                                                         \
+  hipLaunchKernelGGL((mxfp4_rows_kernel<DT>), dim3(static_cast<unsigned>(grid)), dim3(mxr::THREADS), 0,                    \
+                     static_cast<hipStream_t>(stream), static_cast<const typename Elem<DT>::storage*>(x), x_stride,        \
+                     reinterpret_cast<uint32_t*>(q), reinterpret_cast<uint32_t*>(scales), R, K, spans)
+  if (dtype == LNQ_BF16) LNQ_MXW(LNQ_BF16);
+  else if (dtype == LNQ_F16) LNQ_MXW(LNQ_F16);
+  else LNQ_MXW(LNQ_F32);
 #undef LNQ_MXW
   return launched("mxfp4_rows");
 }
