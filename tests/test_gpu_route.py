@@ -60,6 +60,29 @@ def test_ties_go_to_the_lower_index(score: str, biased: bool) -> None:
         _same(kernels.expert_route(logits, 8, bias, **kw), logits, 8, bias, **kw)
 
 
+@pytest.mark.parametrize("best", [1, 2])
+def test_groups_that_only_64_bits_tell_apart(best: int) -> None:
+    """Groups whose scores differ by less than f32 holds, tie, underflow f32 or pass its largest value."""
+    count, groups = 64, 8
+    bias = torch.zeros(count)
+    logits = torch.full((6, count), -3.0)
+    for g in range(groups):
+        logits[0, 8 * g] = 1.0 + (g * 5 % 8) * 2.0 ** -23  # neighbours in f32; their scores closer still
+        logits[0, 8 * g + 1] = 0.5 + (g * 3 % 8) * 2.0 ** -24
+        logits[1, 8 * g] = 2.0
+        logits[2, 8 * g] = -120.0 - (g * 3 % 8)
+    logits[2, 0::8] -= 30
+    logits[3] = -100.0 - 0.25 * torch.arange(count)
+    logits[4, :8], logits[4, 32:40] = -float("inf"), -float("inf")
+    logits[5] = torch.linspace(-1, 1, count).flip(0)
+    for top in (1, 6):
+        for score in ("softmax", "sigmoid"):
+            kw = dict(score=score, groups=groups, group_top=3, group_best=best)
+            _same(kernels.expert_route(logits.to(DEV), top, **kw), logits, top, **kw)
+            for b in (bias, bias + 3.0e38, bias + 1024.0):
+                _same(kernels.expert_route(logits.to(DEV), top, b.to(DEV), **kw), logits, top, b, **kw)
+
+
 def test_neighbours_in_the_last_bit() -> None:
     """Choices one f32 step apart, as logits and through the bias: 64 bits tell them apart."""
     g = torch.Generator().manual_seed(6)
