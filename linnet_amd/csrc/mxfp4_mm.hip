@@ -20,7 +20,7 @@
 // Bound by the power that MFMAs, LDS and loads share (a 4096 x 8192 -> 28672 call: 400 to 475 us by
 // the card's warmth, 4.1 to 4.8 PFLOP/s at 1.75 GHz; its MFMAs alone 213, its loads alone 218, all but
 // the stores 390), with few tiles by a step's latency (0.4 us of 64-row tiles, 0.6 of 128), with few
-// rows by HBM (32 experts of 2880 -> 5760: 61 us, 4.4 TB/s).
+// rows by HBM (32 experts of 2880 -> 5760: 59 us, 4.7 TB/s).
 //
 // Experts: tiles of BM pairs of one expert, expert by expert with its tiles of rows together for
 // each run of columns; where the next tiles lie is looked up a tile ahead a lookup.
@@ -552,7 +552,7 @@ static void launch_form(const Args& a, hipStream_t s) {
 using Form256 = Form<2, 4, 8, 4>;
 using Form128 = Form<2, 2, 4, 4>;
 using Form64 = Form<2, 2, 2, 2>;
-using Form32 = Form<1, 2, 2, 2>;
+using Form32 = Form<1, 2, 2, 4>;  // (of 64 columns, 100 rows' experts 72.1 us against 68.5)
 
 // Rows of a tile, for `count` matrices of N outputs that multiply `rows` rows each (experts: on
 // average). A larger tile reads each operand less often (a wave of 128 x 64 outputs, 24 KB of LDS for
@@ -564,13 +564,14 @@ using Form32 = Form<1, 2, 2, 2>;
 // 1024 x 4096 -> 4096, 256: 18.5 | 14.1.
 // Of an expert's rows: 256 past 128 (32 experts, 2880 -> 5760: at 75 rows 77 | 89, 188: 129 | 105; 128
 // experts, 2048 -> 1536: at 125 63 | 65, 188: 81 | 72; worst, 8 experts, 4096 -> 14336 at 250, whose
-// tiles then fill a third round: 85 | 109); 128 past 28 (32 experts, 2880 -> 5760, 32 rows a tile | 128:
-// at 25 66 | 69, 50: 99 | 72; 2880 -> 2880: at 25 36 | 39, 50: 45 | 40; 64 rows: 39).
+// tiles then fill a third round: 85 | 109); 128 past 20 (32 experts, 2880 -> 5760, 32 rows a tile | 128:
+// at 12 62 | 66, 25: 65 | 68, 38: 82 | 70; 2880 -> 2880: at 12 35 | 38, 25: 43 | 39; 64 rows are the best
+// by 7 percent at most between them, and taken where 128 leave CUs idle).
 static int tile_rows(double rows, int64_t count, int64_t N, bool experts) {
   const auto tiles = [&](int bm, int bn) {
     return static_cast<double>(count) * std::ceil(rows / bm) * static_cast<double>((N + bn - 1) / bn);
   };
-  const int many = experts ? 28 : 64;
+  const int many = experts ? 20 : 64;
   if (rows > 128 && tiles(256, 256) >= 0.7 * compute_units()) return 256;
   if (rows > many && tiles(128, 128) >= 0.625 * compute_units()) return 128;
   return rows > many || !experts ? 64 : 32;
