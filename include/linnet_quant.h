@@ -443,7 +443,7 @@ LNQ_API LnqStatus lnq_mm8_block(const uint8_t* qx, const uint8_t* weight, const 
 /* ------------------------------------------------------------------- MXFP4
  * gpt-oss's expert weights: blocks [E, out, in/32, 16] bytes (32 FP4 E2M1 values a
  * block, element 2j in the low nibble of byte j), scales [E, out, in/32] E8M0 bytes
- * (a block's weights are its E2M1 values times 2^(scale - 127)).
+ * (a block's weights are its E2M1 values times 2^(scale - 127); 255 is NaN).
  */
 
 /* y[r, k, o] = sum_i x[r, k, i] * W[experts[r, k], o, i] for rows x chosen (r, k)

@@ -156,6 +156,11 @@ __device__ inline u32x4 fp4_widen(uint32_t w) {
   return v;
 }
 
+// An E8M0 scale byte: 2^(byte - 127) (0 is below f32's normal range), 255 is NaN.
+__device__ inline float e8m0(uint32_t byte) {
+  return __builtin_bit_cast(float, byte == 255 ? 0x7fc00000u : max(byte << 23, 0x00400000u));
+}
+
 // Four weight bytes as four 16-bit values (two dwords): exactly, but int8 in bf16 plus
 // 128 (0..255 are exact in bf16).
 template <int DT, int F>
@@ -201,8 +206,8 @@ inline int scale_lds(int f, bool per_row, bool blocks, int rows, int cols, int r
 // rows 0 .. 4 XI - 1), and `put(m, n, v)` for every output (m < 16 MT, n < n_end; m may
 // lie past the rows that exist). XI: instructions that move a step's x (4 rows each).
 // GPS: groups a step (0: one scale a row). NW: the workgroup's waves, which
-// all call it. NANS (FP4): a scale byte of 255 is E8M0's NaN, and not 2^128.
-template <int NW, int DT, int F, int GPS, int MT, int XI, int NT, int KIND, bool NANS = false, class RowOf, class Put>
+// all call it.
+template <int NW, int DT, int F, int GPS, int MT, int XI, int NT, int KIND, class RowOf, class Put>
 __device__ inline void product(const Args& a, int n0, int n_end, const uint16_t* xbase, uint32_t xbytes, uint16_t* X0, uint16_t* X1,
                                uint8_t* SC, RowOf row_of, Put put) {
   using E = Elem<DT>;
@@ -430,16 +435,12 @@ __device__ inline void product(const Args& a, int n0, int n_end, const uint16_t*
             const bool in = eight(F) || c < a.cols;
             const int cc = eight(F) ? c : min(c, a.cols - 1);
             float sf = 0.f, off = 128.0f;
-            int e = 0;
             if constexpr (F == INT4) {
               const uint32_t v = *reinterpret_cast<const uint16_t*>(SC + sat[T] + 2 * cc);
               sf = E::to_f32(static_cast<uint16_t>(in ? v : 0u));
               off = E::MAGIC_VALUE + static_cast<float>(SC[zat[T] + cc]);
-            } else if constexpr (F == FP4 && NANS) {
-              const uint32_t v = SC[sat[T] + cc];
-              sf = __builtin_bit_cast(float, v == 255 ? 0x7fc00000u : max(v << 23, 0x00400000u));
             } else if constexpr (F == FP4) {
-              e = static_cast<int>(SC[sat[T] + cc]) - 127;
+              sf = e8m0(SC[sat[T] + cc]);
             } else {
               const uint32_t v = *reinterpret_cast<const uint32_t*>(SC + sat[T] + 4 * cc);
               sf = __builtin_bit_cast(float, in ? v : 0u);
@@ -451,8 +452,7 @@ __device__ inline void product(const Args& a, int n0, int n_end, const uint16_t*
               for (int t = g * TPG; t < (g + 1) * TPG; ++t) p = mfma16x16x32<DT>(xa[h][mt][t], b[t], p);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                if constexpr (F == FP4 && !NANS) acc[mt][T][r] += ldexpf(p[r], e);
-                else if constexpr (XS) acc[mt][T][r] = fmaf(sf, fmaf(-off, cx[h][mt][g][r], p[r]), acc[mt][T][r]);
+                if constexpr (XS) acc[mt][T][r] = fmaf(sf, fmaf(-off, cx[h][mt][g][r], p[r]), acc[mt][T][r]);
                 else acc[mt][T][r] = fmaf(sf, p[r], acc[mt][T][r]);
               }
             }
@@ -555,7 +555,7 @@ __global__ __launch_bounds__(64 * WAVES) void dense_kernel(Args a) {
   const int live = min(a.M - m0, 16 * MT);
   const uint16_t* x = a.x + static_cast<int64_t>(m0) * a.x_stride;
   const uint32_t xbytes = static_cast<uint32_t>(((live - 1) * a.x_stride + a.K) * 2);
-  product<WAVES, DT, F, GPS, MT, XI, NT, KIND, F == FP4>(
+  product<WAVES, DT, F, GPS, MT, XI, NT, KIND>(
       a, n0, n_end, x, xbytes, X0, X1, SC, [&](int i) -> int { return i < live ? i * a.x_stride : -1; },
       [&](int m, int n, float v) {
         if (m < live) {

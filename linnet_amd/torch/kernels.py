@@ -561,9 +561,9 @@ def int4_repack(
 def mxfp4_experts(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, experts: torch.Tensor) -> torch.Tensor:
     """`y[r, k, o] = sum_i x[r, k, i] * W[experts[r, k], o, i]`, with `W` the MXFP4
     weights `blocks` ([E, Out, G, 16] u8) and `scales` ([E, Out, G] u8, E8M0)
-    read as they are and widened in registers (`torch/kernels.py:94-209`). `x` is
-    [R, K, In] bf16 or f16 (an expanded view with a zero slot stride, for an input
-    the chosen experts share, is read without a copy)."""
+    read as they are and widened in registers (`torch/kernels.py:94-209`); a scale of
+    255 is NaN. `x` is [R, K, In] bf16 or f16 (an expanded view with a zero slot stride,
+    for an input the chosen experts share, is read without a copy)."""
     device = _on_gpu("mxfp4_experts", x, blocks, scales, experts)
     if x.dim() != 3 or blocks.dim() != 4 or scales.dim() != 3 or experts.dim() != 2:
         raise LinnetError("mxfp4_experts: x [R, K, In], blocks [E, Out, G, 16], scales [E, Out, G], experts [R, K]")
@@ -620,7 +620,7 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     [..., In/32] u8)` as checkpoints store it: every 32 values share the scale 2^(s - 127), s -
     127 the exponent of their largest magnitude less 2 (at least -127), and are rounded to E2M1,
     ties to the even code, past 6 to 6 (the OCP microscaling format's conversion). A block with
-    an infinity or a NaN gets s = 255, which every reader but `mxfp4_experts` takes as NaN."""
+    an infinity or a NaN gets s = 255, which every reader takes as NaN."""
     device = _on_gpu("mxfp4_quantize", x)
     shape = x.shape
     if not shape or shape[-1] % 32:

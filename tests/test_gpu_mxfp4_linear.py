@@ -345,6 +345,30 @@ def test_experts_linear_takes_the_documented_product() -> None:
                         _check(y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)], pairs[r, k], w[e])
 
 
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("rounded", [0, 1])
+@pytest.mark.parametrize(("rows", "chosen", "depth"), [(1, 1, 288), (2, 3, 2112), (20, 2, 288), (32, 4, 96), (40, 2, 288), (600, 4, 96)])
+def test_experts_scales_that_are_nan(rows: int, chosen: int, depth: int, rounded: int, dtype: torch.dtype) -> None:
+    """A block with the scale 255 (as `mxfp4_quantize` marks one that is not finite, its codes 0) makes its output of
+    its expert NaN, and no other value, whichever kernel takes the rows."""
+    print(f"experts nan rows={rows} chosen={chosen} {depth} rounded={rounded} {dtype}", flush=True)
+    rng = np.random.default_rng(rows)
+    count, out = 4, 72
+    blocks, scales, _ = _weight(rng, count, out, depth)
+    for e, o, g in ((0, 0, 0), (1, 5, depth // 32 - 1), (3, 71, depth // 64)):
+        scales[e, o, g] = 255
+        blocks[e, o, g] = 0
+    experts = rng.integers(-1, count, (rows, chosen))
+    experts[0, 0] = 1
+    want = torch.zeros(rows, chosen, out, dtype=torch.bool)
+    for e, o in ((0, 0), (1, 5), (3, 71)):
+        want[..., o] |= torch.from_numpy(experts == e)
+    operands = quantized.mxfp4_experts_operands(blocks, scales, rounded)
+    x = torch.from_numpy(_values(rng, rows, depth)).to(dtype).to(DEV)
+    y = quantized.mxfp4_experts_linear(x, operands, torch.from_numpy(experts).to(DEV)).cpu()
+    assert torch.equal(y.isnan(), want) and y[~want].isfinite().all()
+
+
 # ------------------------------------------------------------------ refusals, streams, graphs
 
 
