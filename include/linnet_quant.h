@@ -538,8 +538,9 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const void* x, int64_t x_stride, const ui
  * Scores are a softmax over the experts or a sigmoid of each; the choice goes by score + bias
  * (f32 [num_experts]; NULL: by the logits, which order as the scores do), in 64 bits, equal ones
  * by the lower index. With groups > 1 (equal runs of experts, at most 64) only the group_top
- * groups with the largest sum of their group_best (1 or 2) best choices are chosen from (a group
- * with fewer counts -inf; by the scores' sum without a bias). Weights are the chosen experts'
+ * groups with the largest sum of their group_best (1 or 2; 1 where a group is one expert) best
+ * choices are chosen from (a group with fewer that may be chosen counts -inf; by the scores' sum
+ * without a bias). Weights are the chosen experts'
  * scores, without the bias, over their sum if `renormalize` (0 where that is 0), times `scale`.
  * An expert with a logit of -inf, or a choice of -inf or NaN, is never chosen; places left over
  * hold -1 and weight 0. A row with a NaN logit (or +inf, for softmax): -1 and NaN throughout.

@@ -3,7 +3,8 @@
 //
 //   s_e = exp(l_e) / sum_j exp(l_j)  or  1 / (1 + exp(-l_e))      the scores
 //   c_e = s_e + b_e                                               what the choice goes by
-//   a group's score: the sum of its best one or two c_e; the best groups are kept
+//   a group's score: the sum of its best one or two c_e (of a group of one expert, its c_e);
+//   the best groups are kept
 //   the `top` kept experts of largest c, equal ones by the lower index
 //   w_e = s_e (over the sum of the chosen s), times a factor
 //
@@ -25,6 +26,8 @@
 //   which differ in 64 bits, are those compared.
 // 8192 rows of 256 experts in 8 groups, top 8: 13.9 us, 730 vector instructions a row (54 us with a
 // lane a group in turn, 18.7 with the library's exponential and choices by floats).
+#include <algorithm>
+
 #include "common.hpp"
 
 namespace lnq {
@@ -359,8 +362,8 @@ LNQ_API LnqStatus lnq_expert_route(const void* logits, int64_t stride, const flo
   a.top = static_cast<int>(top);
   a.groups = static_cast<int>(groups);
   a.group_top = static_cast<int>(group_top);
-  a.group_best = static_cast<int>(group_best);
   a.size = a.count / a.groups;
+  a.group_best = static_cast<int>(std::min<int64_t>(group_best, a.size));
   int wide = 1;
   while (wide < a.groups) wide *= 2;
   a.lanes = 64 / wide;

@@ -36,13 +36,14 @@ def expert_route(logits: np.ndarray, top: int, bias: np.ndarray | None = None, s
             c = [-math.inf if math.isnan(v) else v for v in c]
         if groups > 1:
             size = count // groups
+            best = min(group_best, size)
             totals = []
             for g in range(groups):
-                order = sorted(range(g * size, (g + 1) * size), key=lambda e: (-c[e], e))[:group_best]
-                if len(order) < group_best or any(c[e] == -math.inf for e in order):
+                order = sorted(range(g * size, (g + 1) * size), key=lambda e: (-c[e], e))[:best]
+                if any(c[e] == -math.inf for e in order):
                     totals.append(-math.inf)
                 else:
-                    totals.append(c[order[0]] if group_best == 1 else sum((s if bias is None else c)[e] for e in order))
+                    totals.append(c[order[0]] if best == 1 else sum((s if bias is None else c)[e] for e in order))
             kept = sorted(range(groups), key=lambda g: (-totals[g], g))[:group_top]
             c = [c[e] if e // size in kept else -math.inf for e in range(count)]
         chosen = [e for e in sorted(range(count), key=lambda e: (-c[e], e)) if c[e] > -math.inf][:top]

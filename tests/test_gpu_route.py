@@ -83,6 +83,21 @@ def test_groups_that_only_64_bits_tell_apart(best: int) -> None:
                 _same(kernels.expert_route(logits.to(DEV), top, b.to(DEV), **kw), logits, top, b, **kw)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("count", [1, 7, 64])
+def test_groups_of_one(count: int, score: str) -> None:
+    """A group of one expert goes by that expert, also with the default `group_best` of 2."""
+    print(f"groups of one, {count} experts {score}", flush=True)
+    g = torch.Generator().manual_seed(count)
+    logits = torch.randn(9, count, generator=g).to(DEV)
+    bias = (0.3 * torch.randn(count, generator=g)).to(DEV)
+    top = min(2, count)
+    for b in (None, bias):
+        got = kernels.expert_route(logits, top, b, score=score, groups=count, group_top=top)
+        _same(got, logits, top, b, score=score)
+        _same(got, logits, top, b, score=score, groups=count, group_top=top)
+
+
 def test_neighbours_in_the_last_bit() -> None:
     """Choices one f32 step apart, as logits and through the bias: 64 bits tell them apart."""
     g = torch.Generator().manual_seed(6)

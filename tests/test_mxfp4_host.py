@@ -144,6 +144,19 @@ def test_route_against_a_search(score: str, groups: int) -> None:
         assert np.allclose(weights[r], 2.0 * chosen / chosen.sum(), rtol=1e-14)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_of_groups_of_one(score: str, biased: bool) -> None:
+    """A group of one expert goes by that expert, whatever `group_best`: the best groups' experts are the best experts."""
+    rng = np.random.default_rng(4)
+    logits = rng.standard_normal((20, 6))
+    bias = 0.3 * rng.standard_normal(6) if biased else None
+    want = route.expert_route(logits, 2, bias, score=score)
+    for best in (1, 2):
+        got = route.expert_route(logits, 2, bias, score=score, groups=6, group_top=3, group_best=best)
+        assert all(np.array_equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize(("rows", "chosen", "count", "out", "depth"), [(16, 4, 8, 64, 64), (1, 1, 1, 64, 32), (4000, 4, 32, 5760, 2880),
                                                                        (9, 3, 2048, 100, 288), (300, 8, 4, 30000, 96)])
 def test_experts_workspace_of_one_byte_less_is_refused(rows: int, chosen: int, count: int, out: int, depth: int) -> None:
