@@ -453,7 +453,8 @@ LNQ_API LnqStatus lnq_mm8_block(const uint8_t* qx, const uint8_t* weight, const 
  * experts [rows, chosen] int64, y [rows, chosen, out] of `dtype`. Each block's
  * products are summed in f32 and scaled, the blocks added in f32, the sum rounded
  * once. An expert index outside 0 .. num_experts-1 gives zeros. in % 32 == 0,
- * in <= 8192. Replaces: torch/kernels.py:94-209 `mxfp4_experts` (the generated
+ * in <= 65536; past 8192 chosen <= 2048, num_experts <= 65534, out <= 2^24 and a row's
+ * choices within 2^29 elements of x. Replaces: torch/kernels.py:94-209 `mxfp4_experts` (the generated
  * `_mxfp4_experts`, src/backend/torch_source.cpp:1579-1600). */
 LNQ_API LnqStatus lnq_mxfp4_experts(const void* x, int64_t x_row_stride, int64_t x_slot_stride,
                                     const uint8_t* blocks, const uint8_t* scales,

@@ -22,6 +22,7 @@
 // (buffer loads: rows past Out, blocks past G and the rows of an out-of-range
 // expert read zeros through the range check). A row's sum is the lanes' partial
 // sums added across the wave (fixed order).
+#include <algorithm>
 #include <cmath>
 
 #include "stream.hpp"
@@ -30,7 +31,8 @@ namespace lnq {
 
 namespace mx {
 constexpr int WAVES = 4;
-constexpr int MAX_SLOTS = 4;  // blocks of a lane per row: G <= 256 (In <= 8192)
+constexpr int MAX_SLOTS = 4;  // blocks of a lane per row: G <= 256
+constexpr int PAIR_IN = 32 * 64 * MAX_SLOTS;  // inputs of the pair kernel; wider layers take the grouped one at any rows
 // Output rows of a wave (gpt-oss's 2880 -> 5760 at one token: 11.3 us with 4,
 // 11.9 with 2, 12.4 with 8; 32 tokens: 55, 63, 55 us).
 constexpr int ROWS = 4;
@@ -150,6 +152,7 @@ __global__ __launch_bounds__(64 * mx::WAVES) void mxfp4_experts_kernel(
 namespace mx {
 constexpr int MAX_PAIRS = 2048;  // pairs of a launch (the list's LDS)
 constexpr int GROUP_WAVES = 4;
+constexpr int64_t X_SPAN = int64_t{1} << 29;  // elements from a launch's first x to its last: offsets below 1 GiB
 }
 
 struct ExpertArgs {
@@ -216,7 +219,11 @@ __global__ __launch_bounds__(64 * mx::GROUP_WAVES, MT == 1 ? 4 : 2) void mxfp4_g
 }
 
 template <int DT, int MT, int XI>
-static void launch_grouped(const ExpertArgs& g, hipStream_t stream) {
+static void launch_grouped(ExpertArgs g, hipStream_t stream) {
+  // Output rows whose scales fit LDS beside the stages and the list (past 40,000 inputs fewer than MAX_R).
+  constexpr int REST = 2 * mx::GROUP_WAVES * stream::stage_values(XI, MT, 4) * 2 + 2 * mx::MAX_PAIRS + 64;
+  g.a.R = stream::MAX_R;
+  while (g.a.R > 8 && stream::scale_lds(stream::FP4, false, false, g.a.R, g.a.cols, 1) + REST > stream::LDS_BYTES) g.a.R -= 8;
   const int lds = stream::scale_lds(stream::FP4, false, false, g.a.R, g.a.cols, 1);
   hipLaunchKernelGGL((mxfp4_grouped_kernel<DT, MT, XI>),
                      dim3(static_cast<unsigned>((g.a.N + g.a.R - 1) / g.a.R), static_cast<unsigned>(g.num_experts + 1)),
@@ -243,11 +250,14 @@ static void launch_grouped_dt(const ExpertArgs& g, int pass, hipStream_t stream)
 // send every token to the same experts are not what is estimated: over a narrow layer the pair
 // kernel's reads of one expert then come from the caches, and the grouped kernel has few workgroups
 // (4096 -> 1536, 128 experts, top 1, 1024 tokens to one expert 366 / 793; of wide layers the grouped
-// kernel is ahead there too, 2880 -> 5760, 32 tokens of top 1 to one of 32 experts 55 / 44).
+// kernel is ahead there too, 2880 -> 5760, 32 tokens of top 1 to one of 32 experts 55 / 44). Past PAIR_IN
+// inputs there is the grouped kernel only (14336 -> 4096, 8 experts, top 2: one token 35 us, a workgroup
+// on half the CUs; 8 tokens 48, 5.2 TB/s).
 static int mxfp4_pass(int64_t rows, int64_t chosen, int64_t num_experts, int64_t out_features, int64_t in_features) {
   const double pairs = static_cast<double>(rows) * chosen, experts = static_cast<double>(num_experts);
   const int pass = pairs > 12 * experts ? 32 : pairs > 3 * experts ? 16 : 8;
   const double named = experts * (1 - std::pow(1 - std::fmin(1.0, chosen / experts), static_cast<double>(rows)));
+  if (in_features > mx::PAIR_IN) return pass;
   const int64_t groups = in_features / 32, slots = (groups + 63) / 64;
   const double mb = static_cast<double>(out_features) * groups * 17e-6;
   const double pair = 3.5 + mb * (0.05 * pairs + 0.018 * named) +
@@ -272,9 +282,8 @@ LNQ_API LnqStatus lnq_mxfp4_experts(const void* x, int64_t x_row_stride, int64_t
   LNQ_REQUIRE(dtype == LNQ_BF16 || dtype == LNQ_F16, "lnq_mxfp4_experts: x is bf16 or f16, not dtype %d", dtype);
   LNQ_REQUIRE(rows >= 0 && chosen >= 0 && num_experts > 0 && out_features >= 0 && in_features >= 0,
               "lnq_mxfp4_experts: negative size");
-  LNQ_REQUIRE(in_features % 32 == 0 && in_features <= 32 * 64 * mx::MAX_SLOTS,
-              "lnq_mxfp4_experts: in %lld is not a multiple of 32 up to %d", static_cast<long long>(in_features),
-              32 * 64 * mx::MAX_SLOTS);
+  LNQ_REQUIRE(in_features % 32 == 0 && in_features <= stream::MAX_K,
+              "lnq_mxfp4_experts: in %lld is not a multiple of 32 up to %d", static_cast<long long>(in_features), stream::MAX_K);
   LNQ_REQUIRE(rows * chosen <= INT32_MAX && out_features * (in_features / 32) * 16 < (int64_t{1} << 32) - 16,
               "lnq_mxfp4_experts: too large (one expert's blocks past 4 GiB)");
   if (rows == 0 || chosen == 0 || out_features == 0) {
@@ -288,12 +297,18 @@ LNQ_API LnqStatus lnq_mxfp4_experts(const void* x, int64_t x_row_stride, int64_t
   hipStream_t s = static_cast<hipStream_t>(stream);
   const auto* xs = static_cast<const uint16_t*>(x);
   auto* ys = static_cast<uint16_t*>(y);
-  // x as the range-checked buffers need it: below 1 GiB, rows and slots forward.
-  const int64_t x_span = (rows - 1) * x_row_stride + (chosen - 1) * x_slot_stride + in_features;
-  const int pass = in_features >= 32 && x_row_stride >= 0 && x_slot_stride >= 0 && x_span < (int64_t{1} << 29) &&
+  // x as the range-checked buffers need it: below 1 GiB (of wide layers a launch's rows, else all), rows
+  // and slots forward.
+  const bool wide = in_features > mx::PAIR_IN;
+  const int64_t row_span = (chosen - 1) * x_slot_stride + in_features, x_span = (rows - 1) * x_row_stride + row_span;
+  const int pass = in_features >= 32 && x_row_stride >= 0 && x_slot_stride >= 0 && (wide ? row_span : x_span) < mx::X_SPAN &&
                            num_experts < 65535 && out_features <= (1 << 24) && chosen <= mx::MAX_PAIRS
                        ? mxfp4_pass(rows, chosen, num_experts, out_features, in_features)
                        : 0;
+  LNQ_REQUIRE(pass || !wide,
+              "lnq_mxfp4_experts: past %d inputs rows choose up to %d of up to 65534 experts of up to 2^24 outputs, with x's strides "
+              "not negative and a row's choices within 2^29 elements",
+              mx::PAIR_IN, mx::MAX_PAIRS);
   if (pass) {
     ExpertArgs g{};
     g.a.w = blocks;
@@ -301,7 +316,6 @@ LNQ_API LnqStatus lnq_mxfp4_experts(const void* x, int64_t x_row_stride, int64_t
     g.a.row_bytes = groups * 16;
     g.a.N = static_cast<int>(out_features);
     g.a.K = static_cast<int>(in_features);
-    g.a.R = stream::MAX_R;
     g.a.span = 1;
     g.a.cols = groups;
     g.a.row_block = 1;
@@ -309,7 +323,8 @@ LNQ_API LnqStatus lnq_mxfp4_experts(const void* x, int64_t x_row_stride, int64_t
     g.chosen = static_cast<int>(chosen);
     g.x_row_stride = static_cast<int>(x_row_stride);
     g.x_slot_stride = static_cast<int>(x_slot_stride);
-    const int64_t part = mx::MAX_PAIRS / chosen;
+    int64_t part = mx::MAX_PAIRS / chosen;
+    if (x_row_stride > 0) part = std::min(part, 1 + (mx::X_SPAN - 1 - row_span) / x_row_stride);
     for (int64_t r0 = 0; r0 < rows; r0 += part) {
       const int64_t rc = rows - r0 < part ? rows - r0 : part;
       g.a.x = xs + r0 * x_row_stride;

@@ -563,7 +563,7 @@ def mxfp4_experts(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, e
     weights `blocks` ([E, Out, G, 16] u8) and `scales` ([E, Out, G] u8, E8M0)
     read as they are and widened in registers (`torch/kernels.py:94-209`); a scale of
     255 is NaN. `x` is [R, K, In] bf16 or f16 (an expanded view with a zero slot stride,
-    for an input the chosen experts share, is read without a copy)."""
+    for an input the chosen experts share, is read without a copy), In up to 65536."""
     device = _on_gpu("mxfp4_experts", x, blocks, scales, experts)
     if x.dim() != 3 or blocks.dim() != 4 or scales.dim() != 3 or experts.dim() != 2:
         raise LinnetError("mxfp4_experts: x [R, K, In], blocks [E, Out, G, 16], scales [E, Out, G], experts [R, K]")

@@ -235,7 +235,8 @@ def mxfp4_experts_linear(x: torch.Tensor, operands: Mxfp4Operands, experts: torc
     """`y[r, k] = x[r (, k)] W[experts[r, k]]^T` [R, K, Out] for `experts` [R, K] (`kernels.expert_route`'s
     choice) and `x` [R, In], which the chosen experts of a row share, or [R, K, In]: past
     `FEW_ROWS` rows with `rounded`, x rounded to MXFP4 and each expert's pairs multiplied together
-    in 4 bits; else `kernels.mxfp4_experts`. An expert outside 0 .. E - 1 gives zeros."""
+    in 4 bits (up to 2048 experts and 2^32 values of x); else `kernels.mxfp4_experts`, x unrounded.
+    bf16 and f16, In up to 65536 (where x is rounded 4194304). An expert outside 0 .. E - 1 gives zeros."""
     blocks, scales, tiles, rounded = operands
     shape = x.shape
     if experts.dim() != 2 or experts.is_floating_point() or len(shape) not in (2, 3) or shape[:-1] != experts.shape[: len(shape) - 1]:

@@ -345,6 +345,62 @@ def test_experts_linear_takes_the_documented_product() -> None:
                         _check(y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)], pairs[r, k], w[e])
 
 
+@pytest.mark.parametrize("rounded", [0, 1])
+@pytest.mark.parametrize("rows", [1, 32, 33])
+@pytest.mark.parametrize(("depth", "out"), [(8192, 40), (8224, 40), (14336, 65), (65536, 70)])
+def test_experts_linear_of_wide_layers(depth: int, out: int, rows: int, rounded: int) -> None:
+    """A layer's width is taken at one token as over a prompt."""
+    print(f"wide experts {depth} -> {out} rows={rows} rounded={rounded}", flush=True)
+    rng = np.random.default_rng(rows + depth)
+    count, chosen = 3, 2
+    blocks, scales, w = _weight(rng, count, out, depth)
+    operands = quantized.mxfp4_experts_operands(blocks, scales, rounded)
+    experts = _experts(rng, "spread", rows, chosen, count)
+    experts[-1, 1] = -1
+    for shape in ((rows, depth), (rows, chosen, depth)):
+        x = torch.from_numpy(_values(rng, *shape)).to(torch.bfloat16).to(DEV)
+        y = quantized.mxfp4_experts_linear(x, operands, torch.from_numpy(experts).to(DEV))
+        values = _rounded(x) if rounded and rows > 32 else x.double().cpu().numpy()
+        pairs = values if len(shape) == 3 else values[:, None].repeat(chosen, 1)
+        for e in range(count):
+            r, k = np.nonzero(experts == e)
+            if r.size:
+                _check(y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)], pairs[r, k], w[e])
+        assert not y[-1, 1].any()
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize(("rows", "chosen", "count", "out", "depth"), [
+    (1, 1, 2, 8, 8224), (40, 2, 2, 130, 46080), (9, 4, 5, 33, 65536), (300, 2, 3, 72, 16384), (700, 4, 300, 9, 8224)])
+def test_wide_experts_at_decode(rows: int, chosen: int, count: int, out: int, depth: int, dtype: torch.dtype) -> None:
+    """`mxfp4_experts` past the width a pair's workgroup holds: each number of pairs a pass, and the widest rows' scales."""
+    print(f"mxfp4_experts {rows} x {chosen} of {count} {depth} -> {out} {dtype}", flush=True)
+    rng = np.random.default_rng(rows + depth)
+    blocks, scales, w = _weight(rng, count, out, depth)
+    experts = _experts(rng, "ends", rows, chosen, count).astype(np.int64)
+    x = torch.from_numpy(_values(rng, rows, depth)).to(dtype).to(DEV)
+    y = kernels.mxfp4_experts(x[:, None].expand(rows, chosen, depth), blocks, scales, torch.from_numpy(experts).to(DEV))
+    values = x.double().cpu().numpy()
+    for e in range(count):
+        r, k = np.nonzero(experts == e)
+        if r.size:
+            _check(y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)], values[r], w[e])
+    r, k = np.nonzero((experts < 0) | (experts >= count))
+    assert not y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)].any()
+
+
+def test_wide_experts_of_far_rows() -> None:
+    """Rows of x 2^28 elements apart: more than a launch's offsets hold."""
+    rng = np.random.default_rng(3)
+    blocks, scales, w = _weight(rng, 2, 24, 8224)
+    far = torch.empty(2 * 2 ** 28 + 8224, dtype=torch.bfloat16, device=DEV)
+    x = far.as_strided((3, 1, 8224), (2 ** 28, 8224, 1))
+    x.copy_(torch.from_numpy(_values(rng, 3, 1, 8224)))
+    y = kernels.mxfp4_experts(x, blocks, scales, torch.tensor([[1], [0], [1]], device=DEV))
+    for r, e in enumerate((1, 0, 1)):
+        _check(y[r], x[r].double().cpu().numpy(), w[e])
+
+
 @pytest.mark.parametrize("dtype", list(HALF))
 @pytest.mark.parametrize("rounded", [0, 1])
 @pytest.mark.parametrize(("rows", "chosen", "depth"), [(1, 1, 288), (2, 3, 2112), (20, 2, 288), (32, 4, 96), (40, 2, 288), (600, 4, 96)])

@@ -70,6 +70,23 @@ def test_the_abi_refuses(name: str, args: tuple, message: str) -> None:
     assert status == _lib.LNQ_ERROR and message in error, error
 
 
+@pytest.mark.parametrize(("sizes", "strides", "message"), [
+    ((4, 2, 8, 64, 65568), (65568, 0), "multiple of 32 up to 65536"), ((4, 2, 8, 64, 8208), (8208, 0), "multiple of 32"),
+    ((4, 4096, 8, 64, 8224), (8224, 0), "rows choose up to 2048"), ((4, 2, 65535, 64, 8224), (8224, 0), "65534 experts"),
+    ((4, 2, 8, 64, 8224), (8224, 1 << 29), "2.29 elements"), ((4, 2, 8, 64, 8224), (-8224, 0), "not negative")])
+def test_wide_experts_refuse(sizes: tuple, strides: tuple, message: str) -> None:
+    with pytest.raises(LinnetError, match=message):
+        _lib.call("lnq_mxfp4_experts", FAKE, *strides, *[FAKE] * 4, *sizes, _lib.BF16, NULL)
+
+
+@pytest.mark.parametrize(("rows", "pairs"), [(1, 8), (4, 8), (20, 16), (200, 32)])
+def test_wide_experts_take_the_grouped_kernel(rows: int, pairs: int) -> None:
+    got = ctypes.c_int32(-1)
+    for out, width in ((64, 8224), (4096, 14336), (100000, 65536)):
+        _lib.call("lnq_mxfp4_experts_plan", rows, 2, 8, out, width, ctypes.byref(got))
+        assert got.value == pairs
+
+
 def test_empty_calls_succeed_without_a_device() -> None:
     for name, args in [
         ("lnq_mxfp4_quantize", (NULL, NULL, NULL, 0, 64, 0, NULL)),
