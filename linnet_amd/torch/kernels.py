@@ -657,12 +657,13 @@ def mxfp4_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise LinnetError(f"mxfp4_rows: x is [rows, In] with In % 32 == 0, got {tuple(x.shape)}")
     rows, depth = x.shape
     code = _code(x.dtype, "mxfp4_rows", _ANY)
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
-        x = _aligned(x)
+    stride, step = x.stride()
+    if step != 1 or stride % 8 or x.data_ptr() % 16:
+        x, stride = _aligned(x), depth  # one row keeps its own stride when it is copied
     q = torch.empty(rows, depth // 2, dtype=torch.uint8, device=device)
     scales = torch.empty(_mxfp4_tile_shape((), rows, depth), dtype=torch.uint8, device=device)
     with _on(device):
-        _lib.call("lnq_mxfp4_rows", _ptr(x), x.stride(0), _ptr(q), _ptr(scales), rows, depth, code, _stream(device))
+        _lib.call("lnq_mxfp4_rows", _ptr(x), stride, _ptr(q), _ptr(scales), rows, depth, code, _stream(device))
     return q, scales
 
 

@@ -142,6 +142,15 @@ def test_rows_are_quantize_laid_out(rows: int, depth: int, dtype: torch.dtype) -
         assert torch.equal(row_scales, kernels.mxfp4_scale_tiles(scales, depth))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("at", [0, 3, 4])
+def test_rows_of_one_row_of_an_odd_pitch(at: int, dtype: torch.dtype) -> None:
+    x = torch.from_numpy(_values(np.random.default_rng(at), 5, 128)).to(dtype).to(DEV)[:, :101].contiguous()[2:3, at : at + 96]
+    q, row_scales = kernels.mxfp4_rows(x)
+    blocks, scales = kernels.mxfp4_quantize(x.clone(memory_format=torch.contiguous_format))
+    assert torch.equal(q, blocks.view(1, 48)) and torch.equal(row_scales, kernels.mxfp4_scale_tiles(scales, 96))
+
+
 @pytest.mark.parametrize(("lead", "out", "depth"), [((), 1, 32), ((), 128, 256), ((5,), 70, 288), ((2,), 300, 2880)])
 def test_scale_tiles(lead: tuple[int, ...], out: int, depth: int) -> None:
     scales = torch.randint(0, 256, (*lead, out, depth // 32), dtype=torch.uint8, device=DEV)
