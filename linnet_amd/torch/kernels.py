@@ -576,13 +576,16 @@ def mxfp4_experts(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, e
     if experts.shape != (rows, chosen) or experts.is_floating_point():
         raise LinnetError(f"mxfp4_experts: experts are integers [{rows}, {chosen}]")
     code = _code(x.dtype, "mxfp4_experts")
-    if (x.stride(2) != 1 or x.data_ptr() % 16 or x.stride(0) % 8 or x.stride(1) % 8):
-        x = x.contiguous()
-    blocks, scales = blocks.contiguous(), scales.contiguous()
+    # The strides that are used: those of one row, or of one choice, say nothing.
+    row, slot, step = x.stride()
+    row, slot = row if rows > 1 else 0, slot if chosen > 1 else 0
+    if step != 1 or row % 8 or slot % 8 or x.data_ptr() % 16:
+        x, row, slot = _aligned(x), chosen * width, width
+    blocks, scales = _aligned(blocks), scales.contiguous()
     ids = experts.to(torch.int64).contiguous()
     y = torch.empty(rows, chosen, out_features, dtype=x.dtype, device=device)
     with _on(device):
-        _lib.call("lnq_mxfp4_experts", _ptr(x), x.stride(0), x.stride(1), _ptr(blocks), _ptr(scales), _ptr(ids),
+        _lib.call("lnq_mxfp4_experts", _ptr(x), row, slot, _ptr(blocks), _ptr(scales), _ptr(ids),
                   _ptr(y), rows, chosen, count, out_features, width, code, _stream(device))
     return y
 

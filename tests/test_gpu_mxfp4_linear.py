@@ -469,6 +469,25 @@ def test_experts_past_32_bits() -> None:
         _check(y[r, k, at][None], values[r : r + 1], w)
 
 
+@pytest.mark.parametrize(("rows", "chosen"), [(1, 1), (1, 3), (3, 1), (6, 2)])
+@pytest.mark.parametrize(("pitch", "at"), [(101, 0), (101, 3), (96, 0), (96, 4), (104, 0)])
+def test_experts_at_decode_of_views(rows: int, chosen: int, pitch: int, at: int) -> None:
+    """x of an odd pitch, of one row or one choice too, and packed but off 16 bytes; blocks off 16 bytes: as packed ones."""
+    print(f"mxfp4_experts of a view {rows} x {chosen} pitch={pitch} at={at}", flush=True)
+    rng = np.random.default_rng(rows)
+    blocks, scales, _ = _weight(rng, 5, 72, 96)
+    ids = torch.from_numpy(rng.integers(0, 5, (rows, chosen))).to(DEV)
+    room = torch.from_numpy(_values(rng, 1, 4096)[0]).to(torch.bfloat16).to(DEV)
+    x = room[at : at + rows * chosen * pitch].view(rows, chosen, pitch)[..., :96]
+    want = kernels.mxfp4_experts(x.clone(memory_format=torch.contiguous_format), blocks, scales, ids)
+    assert torch.equal(kernels.mxfp4_experts(x, blocks, scales, ids), want)
+    off = torch.empty(blocks.numel() + 8, dtype=torch.uint8, device=DEV)[8:].view(blocks.shape).copy_(blocks)
+    assert torch.equal(kernels.mxfp4_experts(x, off, scales, ids), want)
+    if chosen == 1:
+        operands = quantized.mxfp4_experts_operands(blocks, scales, 1)
+        assert torch.equal(quantized.mxfp4_experts_linear(x[:, 0], operands, ids), want)
+
+
 @pytest.mark.parametrize("rows", [20, 45])
 def test_experts_of_views(rows: int) -> None:
     """x with gaps between its rows, transposed and expanded, experts in 32 bits and of a view: as packed ones."""
