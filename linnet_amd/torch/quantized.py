@@ -176,8 +176,9 @@ def int8_group_linear(x: torch.Tensor, operands: Int8GroupOperands, bias: torch.
     return _finish(x, y, bias)
 
 
-# Widest MXFP4 layer that the few-row kernel and the 4-bit product take.
-_MXFP4_IN, _MXFP4_OUT = 65536, 65535 * 64
+# Widest MXFP4 layer that the few-row kernel takes, and the 4-bit product.
+_MXFP4_FEW_IN, _MXFP4_FEW_OUT = 65536, 65535 * 64
+_MXFP4_MM_IN, _MXFP4_MM_OUT = 1 << 22, 1 << 27
 
 
 def mxfp4_operands(blocks: torch.Tensor, scales: torch.Tensor, rounded: int) -> Mxfp4Operands:
@@ -198,7 +199,8 @@ def mxfp4_linear(x: torch.Tensor, operands: Mxfp4Operands, bias: torch.Tensor | 
     """`x W^T (+ bias)` for an MXFP4 weight, as the 8-bit layers dispatch: past `FEW_ROWS` rows with
     `rounded`, x rounded to MXFP4 (`mxfp4_rows`) and the two multiplied in 4 bits; else up to
     `TILED_ROWS` rows the weight widened in registers, and past those dequantized for the call.
-    bf16 and f16; the bias is added in f32, before the one rounding."""
+    bf16 and f16; the bias is added in f32, before the one rounding. f32 x, and wider layers than the
+    few-row kernel's 65536 inputs or 4194240 outputs at few rows, take the dequantized weight."""
     blocks, scales, tiles, rounded = operands
     out_features, groups, _ = blocks.shape
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
@@ -206,11 +208,11 @@ def mxfp4_linear(x: torch.Tensor, operands: Mxfp4Operands, bias: torch.Tensor | 
     dtype = flat.dtype
     if depth != groups * 32:
         raise LinnetError(f"mxfp4_linear: x {tuple(x.shape)} against a weight [{out_features}, {groups * 32}]")
-    if dtype in _HALF and 0 < depth <= _MXFP4_IN and out_features <= _MXFP4_OUT:
+    if dtype in _HALF and depth > 0:
         product = None
-        if rounded and tiles is not None and rows > FEW_ROWS:
+        if rounded and tiles is not None and rows > FEW_ROWS and depth <= _MXFP4_MM_IN and out_features <= _MXFP4_MM_OUT:
             product, scaled = kernels._mxfp4_rounded, tiles
-        elif rows <= TILED_ROWS:
+        elif rows <= TILED_ROWS and depth <= _MXFP4_FEW_IN and out_features <= _MXFP4_FEW_OUT:
             product, scaled = kernels._mxfp4_few_rows, scales
         if product is not None:
             y = product(flat, blocks, scaled, bias, kernels._on_gpu("mxfp4_linear", flat, blocks, bias))

@@ -294,6 +294,22 @@ def test_linear_takes_the_documented_product(dtype: torch.dtype) -> None:
                                rtol=288 * 2.0 ** -24, atol=288 * 2.0 ** -23 * float(np.abs(w).max() * x.abs().max().item() * 288))
 
 
+@pytest.mark.parametrize(("out", "depth"), [(70, 65536), (70, 65568), (4194304, 32)])
+def test_linear_of_the_widest_layers(out: int, depth: int) -> None:
+    """x is rounded past a few rows at any width, and unrounded up to those."""
+    gen = torch.Generator(DEV).manual_seed(depth)
+    blocks = torch.randint(0, 256, (out, depth // 32, 16), dtype=torch.uint8, device=DEV, generator=gen)
+    scales = torch.randint(120, 127, (out, depth // 32), dtype=torch.uint8, device=DEV, generator=gen)
+    operands = quantized.mxfp4_operands(blocks, scales, 1)
+    at = torch.tensor(sorted({0, 1, out // 2, out - 1}), device=DEV)
+    w = quant.dequantize_mxfp4(blocks[at].cpu().numpy(), scales[at].cpu().numpy())
+    for rows in (1, 32, 33, 65):
+        print(f"linear {depth} -> {out} rows={rows}", flush=True)
+        x = torch.from_numpy(_values(np.random.default_rng(rows), rows, depth)).to(torch.bfloat16).to(DEV)
+        y = quantized.mxfp4_linear(x, operands, None)
+        _check(y[:, at], _rounded(x) if rows > 32 else x.double().cpu().numpy(), w)
+
+
 # ------------------------------------------------------------------ experts
 
 
