@@ -20,6 +20,8 @@ tensors raise: this package has no CPU path.
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as functional
 
@@ -203,7 +205,9 @@ def mxfp4_linear(x: torch.Tensor, operands: Mxfp4Operands, bias: torch.Tensor | 
     few-row kernel's 65536 inputs or 4194240 outputs at few rows, take the dequantized weight."""
     blocks, scales, tiles, rounded = operands
     out_features, groups, _ = blocks.shape
-    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x.dim() == 0:
+        raise LinnetError("mxfp4_linear: x is [..., In]")
+    flat = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])  # -1 says nothing where In is 0
     rows, depth = flat.shape
     dtype = flat.dtype
     if depth != groups * 32:

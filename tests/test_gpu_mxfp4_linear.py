@@ -294,6 +294,22 @@ def test_linear_takes_the_documented_product(dtype: torch.dtype) -> None:
                                rtol=288 * 2.0 ** -24, atol=288 * 2.0 ** -23 * float(np.abs(w).max() * x.abs().max().item() * 288))
 
 
+def test_linear_of_no_inputs_and_no_rows() -> None:
+    bias = torch.randn(24, device=DEV).to(torch.bfloat16)
+    for rounded in (0, 1):
+        none = quantized.mxfp4_operands(torch.empty(24, 0, 16, dtype=torch.uint8, device=DEV),
+                                        torch.empty(24, 0, dtype=torch.uint8, device=DEV), rounded)
+        some = quantized.mxfp4_operands(torch.zeros(24, 2, 16, dtype=torch.uint8, device=DEV),
+                                        torch.zeros(24, 2, dtype=torch.uint8, device=DEV), rounded)
+        for lead in ((), (3,), (2, 3), (4, 5, 2)):
+            y = quantized.mxfp4_linear(torch.empty(*lead, 0, dtype=torch.bfloat16, device=DEV), none, bias)
+            assert y.shape == (*lead, 24) and torch.equal(y, bias.expand(*lead, 24))
+        for lead in ((0,), (0, 3), (3, 0), (2, 0, 3)):
+            assert quantized.mxfp4_linear(torch.empty(*lead, 64, dtype=torch.bfloat16, device=DEV), some, bias).shape == (*lead, 24)
+        with pytest.raises(LinnetError, match="mxfp4_linear: x"):
+            quantized.mxfp4_linear(torch.zeros((), dtype=torch.bfloat16, device=DEV), some, None)
+
+
 @pytest.mark.parametrize(("out", "depth"), [(70, 65536), (70, 65568), (4194304, 32)])
 def test_linear_of_the_widest_layers(out: int, depth: int) -> None:
     """x is rounded past a few rows at any width, and unrounded up to those."""
