@@ -856,7 +856,7 @@ def expert_route(logits: torch.Tensor, top: int, bias: torch.Tensor | None = Non
         if bias.dtype != torch.float32 or bias.shape != (count,):
             raise LinnetError(f"expert_route: bias is [{count}] float32, got {tuple(bias.shape)} {bias.dtype}")
         bias = bias.contiguous()
-    flat = logits if len(shape) == 2 else logits.reshape(-1, count)
+    flat = logits if len(shape) == 2 else logits.reshape(math.prod(lead), count)
     stride, step = flat.stride()
     if step != 1 and count > 1:
         flat = flat.contiguous()

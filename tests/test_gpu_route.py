@@ -98,6 +98,15 @@ def test_groups_of_one(count: int, score: str) -> None:
         _same(got, logits, top, b, score=score, groups=count, group_top=top)
 
 
+def test_no_experts_and_no_rows() -> None:
+    for lead in ((), (2,), (2, 3)):
+        with pytest.raises(LinnetError, match="0 experts"):
+            kernels.expert_route(torch.empty(*lead, 0, device=DEV), 1)
+    for lead in ((0,), (0, 2), (2, 0), (2, 0, 3)):
+        experts, weights = kernels.expert_route(torch.empty(*lead, 8, device=DEV), 3)
+        assert experts.shape == weights.shape == (*lead, 3)
+
+
 def test_neighbours_in_the_last_bit() -> None:
     """Choices one f32 step apart, as logits and through the bias: 64 bits tell them apart."""
     g = torch.Generator().manual_seed(6)
