@@ -366,6 +366,44 @@ def test_experts_mm(rows: int, chosen: int, count: int, out: int, depth: int, dt
         assert not y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)].any()
 
 
+# Workgroups that are resident at a time, a CU, by the rows of a tile. (Tiles of 64 rows are taken only where those
+# of 128 leave CUs idle, at most 160 of them by the average of an expert's pairs: fewer than 1024 of 64.)
+RESIDENT = {32: 3, 128: 2, 256: 1}
+
+
+@pytest.mark.parametrize("kind", ["spread", "ends"])
+@pytest.mark.parametrize(("bm", "bn", "rows", "chosen", "count", "out", "depth"), [
+    (32, 128, 40, 4, 16, 13549, 96), (32, 128, 60, 4, 16, 12801, 544), (128, 128, 400, 2, 16, 8301, 288),
+    (128, 128, 500, 2, 16, 8197, 512), (256, 256, 600, 2, 8, 17003, 160), (256, 256, 700, 2, 8, 16900, 32)])
+def test_experts_mm_of_several_tiles_a_workgroup(bm: int, bn: int, rows: int, chosen: int, count: int, out: int, depth: int,
+                                                 kind: str) -> None:
+    """More tiles than workgroups at a time, two and more rounds of them: tiles that are looked up, loaded and stored
+    while others' steps run, of two k-steps and of more."""
+    cus = torch.cuda.get_device_properties(DEV).multi_processor_count
+    rng = np.random.default_rng(rows + count)
+    experts = _experts(rng, kind, rows, chosen, count).astype(np.int64)
+    buckets = np.bincount(np.where((experts < 0) | (experts >= count), count, experts).ravel(), minlength=count + 1)
+    tiles = int((-(-buckets // bm)).sum()) * -(-out // bn)
+    print(f"experts {kind} {rows} x {chosen} of {count} {depth} -> {out}: {tiles} tiles of {bm} x {bn}", flush=True)
+    assert tiles > 2 * RESIDENT[bm] * cus
+    dtype = torch.bfloat16 if kind == "spread" else torch.float16
+    gen = torch.Generator(DEV).manual_seed(rows)
+    blocks = torch.randint(0, 256, (count, out, depth // 32, 16), dtype=torch.uint8, device=DEV, generator=gen)
+    scales = torch.randint(120, 127, (count, out, depth // 32), dtype=torch.uint8, device=DEV, generator=gen)
+    tiles = kernels.mxfp4_scale_tiles(scales, depth)
+    ids = torch.from_numpy(experts).to(DEV)
+    for shared in (True, False):
+        x = torch.from_numpy(_values(rng, rows if shared else rows * chosen, depth)).to(dtype).to(DEV)
+        y = kernels.mxfp4_experts_mm(x, blocks, tiles, ids)
+        values = _rounded(x)
+        for e in range(count):
+            r, k = np.nonzero(experts == e)
+            w = quant.dequantize_mxfp4(blocks[e].cpu().numpy(), scales[e].cpu().numpy())
+            _check(y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)], values[r if shared else r * chosen + k], w)
+        r, k = np.nonzero((experts < 0) | (experts >= count))
+        assert not y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)].any()
+
+
 def test_experts_linear_takes_the_documented_product() -> None:
     rng = np.random.default_rng(11)
     count, out, depth = 6, 96, 160
