@@ -138,7 +138,8 @@ __global__ __launch_bounds__(64 * mx::WAVES) void mxfp4_experts_kernel(
   for (int i = 0; i < ROWS; ++i) {
     const float v = wave_sum(acc[i]);
     const int o = o0 + i;
-    if (lane == 0 && o < out_features) y[static_cast<size_t>(pair) * out_features + o] = E::from_f32(v);
+    // (No weight was read for an expert out of range, but an infinity in x times zero is NaN.)
+    if (lane == 0 && o < out_features) y[static_cast<size_t>(pair) * out_features + o] = valid ? E::from_f32(v) : static_cast<uint16_t>(0);
   }
 }
 

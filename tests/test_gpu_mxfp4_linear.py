@@ -482,6 +482,25 @@ def test_wide_experts_of_far_rows() -> None:
 
 @pytest.mark.parametrize("dtype", list(HALF))
 @pytest.mark.parametrize("rounded", [0, 1])
+@pytest.mark.parametrize(("rows", "chosen", "depth"), [(1, 2, 96), (2, 3, 8192), (2, 3, 8224), (32, 4, 96), (40, 2, 288)])
+def test_choices_of_no_expert_are_zeros_whatever_x_holds(rows: int, chosen: int, depth: int, rounded: int, dtype: torch.dtype) -> None:
+    print(f"no expert rows={rows} chosen={chosen} {depth} rounded={rounded} {dtype}", flush=True)
+    rng = np.random.default_rng(rows + depth)
+    blocks, scales, _ = _weight(rng, 4, 40, depth)
+    operands = quantized.mxfp4_experts_operands(blocks, scales, rounded)
+    experts = rng.integers(0, 4, (rows, chosen))
+    experts[0, 0], experts[-1, -1] = -1, 4
+    x = torch.from_numpy(_values(rng, rows, depth)).to(dtype)
+    x[0, 5], x[-1, depth - 1] = float("inf"), float("nan")
+    y = quantized.mxfp4_experts_linear(x.to(DEV), operands, torch.from_numpy(experts).to(DEV)).cpu()
+    none = torch.from_numpy((experts < 0) | (experts > 3))
+    assert not y[none].any()
+    if rows > 2:
+        assert y[1:-1].isfinite().all() and y[-1][~none[-1]].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("rounded", [0, 1])
 @pytest.mark.parametrize(("rows", "chosen", "depth"), [(1, 1, 288), (2, 3, 2112), (20, 2, 288), (32, 4, 96), (40, 2, 288), (600, 4, 96)])
 def test_experts_scales_that_are_nan(rows: int, chosen: int, depth: int, rounded: int, dtype: torch.dtype) -> None:
     """A block with the scale 255 (as `mxfp4_quantize` marks one that is not finite, its codes 0) makes its output of
