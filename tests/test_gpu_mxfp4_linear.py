@@ -468,6 +468,43 @@ def test_wide_experts_at_decode(rows: int, chosen: int, count: int, out: int, de
     assert not y[torch.from_numpy(r).to(DEV), torch.from_numpy(k).to(DEV)].any()
 
 
+def _halves(rng: np.random.Generator, rows: int, shape: tuple[int, ...]) -> tuple:
+    """x of -2 .. 2 and weights of scale 1: every product is a multiple of 1/2 and every sum of them exact in f32, in any
+    order and with x rounded or not. (x, blocks, scales, weights.)"""
+    x = torch.from_numpy(rng.integers(-2, 3, (rows, shape[-1])).astype(np.float32))
+    blocks = rng.integers(0, 256, (*shape[:-1], shape[-1] // 32, 16)).astype(np.uint8)
+    scales = np.full((*shape[:-1], shape[-1] // 32), 127, dtype=np.uint8)
+    w = torch.from_numpy(quant.dequantize_mxfp4(blocks, scales)).double().to(DEV)
+    return x.to(DEV), torch.from_numpy(blocks).to(DEV), torch.from_numpy(scales).to(DEV), w
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("rows", [1, 5, 20, 33, 300])
+@pytest.mark.parametrize(("out", "depth"), [(70, 96), (65, 2880), (40, 8192), (130, 8224), (70, 46080), (33, 65536), (33, 65568)])
+def test_sums_of_wide_layers_are_exact(out: int, depth: int, rows: int, dtype: torch.dtype) -> None:
+    """Where no sum is rounded, only the output is: each of the inputs counts, once."""
+    print(f"exact {depth} -> {out} rows={rows} {dtype}", flush=True)
+    x, blocks, scales, w = _halves(np.random.default_rng(rows + depth), rows, (3, out, depth))
+    experts = torch.from_numpy(np.random.default_rng(rows).integers(0, 3, (rows, 2))).to(DEV)
+    want = torch.stack([x.double() @ w[e].T for e in range(3)], 1).float().to(dtype)
+    pairs = want.gather(1, experts[..., None].expand(rows, 2, out))
+    for rounded in (0, 1):
+        assert torch.equal(quantized.mxfp4_linear(x.to(dtype), quantized.mxfp4_operands(blocks[0], scales[0], rounded), None), want[:, 0])
+        if depth <= 65536 or (rounded and rows > 32):
+            operands = quantized.mxfp4_experts_operands(blocks, scales, rounded)
+            assert torch.equal(quantized.mxfp4_experts_linear(x.to(dtype), operands, experts), pairs)
+
+
+def test_rows_are_rounded_at_any_width() -> None:
+    """x of 1.2, which rounds to 1 (4.8 in its block's scale goes to 4), times weights of 1."""
+    for depth in (65536, 65568):
+        blocks = torch.full((8, depth // 32, 16), 0x22, dtype=torch.uint8, device=DEV)
+        scales = torch.full((8, depth // 32), 127, dtype=torch.uint8, device=DEV)
+        x = torch.full((33, depth), 1.2, dtype=torch.bfloat16, device=DEV)
+        y = quantized.mxfp4_linear(x, quantized.mxfp4_operands(blocks, scales, 1), None)
+        assert (y == torch.tensor(depth, dtype=torch.bfloat16, device=DEV)).all()
+
+
 def test_wide_experts_of_far_rows() -> None:
     """Rows of x 2^28 elements apart: more than a launch's offsets hold."""
     rng = np.random.default_rng(3)
