@@ -246,7 +246,7 @@ static void launch_grouped_dt(const ExpertArgs& g, int pass, hipStream_t stream)
 // of 256 inputs, whatever the pairs in it, their longest chain first, and the listing in every
 // workgroup.
 // us, pair / grouped: 2880 -> 5760, 32 experts, top 4: 4 tokens 32.4 / 38.8, 8 59.4 / 54.9, 32 227 / 80,
-// 256 1590 / 190; top 1: 16 tokens 32.9 / 43.3; 4096 -> 1536, 128 experts, top 1: 64 tokens 40.2 / 66.0,
+// 256 1590 / 170; top 1: 16 tokens 32.9 / 43.3; 4096 -> 1536, 128 experts, top 1: 64 tokens 40.2 / 66.0,
 // 256 145 / 101; 1024 -> 1024, 32 experts, top 4: 2 tokens 4.6 / 7.6, 16 14.4 / 8.5. Routers that
 // send every token to the same experts are not what is estimated: over a narrow layer the pair
 // kernel's reads of one expert then come from the caches, and the grouped kernel has few workgroups

@@ -17,8 +17,8 @@
 // again, so the rest reads step g + 1's first operands and issues step g + 2's loads, the next
 // tile's near a tile's end, into step g's stage.
 //
-// Bound by the power that MFMAs, LDS and loads share (a 4096 x 8192 -> 28672 call: 400 to 475 us by
-// the card's warmth, 4.1 to 4.8 PFLOP/s at 1.75 GHz; its MFMAs alone 213, its loads alone 218, all but
+// Bound by the power that MFMAs, LDS and loads share (a 4096 x 8192 -> 28672 call: 425 to 455 us by
+// the card and its warmth, 4.2 to 4.5 PFLOP/s at 1.75 GHz; its MFMAs alone 213, its loads alone 218, all but
 // the stores 390), with few tiles by a step's latency (0.4 us of 64-row tiles, 0.6 of 128), with few
 // rows by HBM (32 experts of 2880 -> 5760: 59 us, 4.7 TB/s).
 //

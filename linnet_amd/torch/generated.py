@@ -174,10 +174,11 @@ def _mxfp4_grouped(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, 
     chosen expert of a row reads the row) and `mxfp4_combine_experts` (`x` [R, K, In],
     the products weighed by `weights` [R, K] and summed per row in f32, as the
     reference's helper sums its grouped product, `torch_source.cpp:1705-1735`).
-    The MXFP4 products run on the decode kernel, each (row, slot) pair reading its
-    expert's bytes as stored: the semantics of the grouped path for any number of
-    rows, without its expert-sorted MFMA schedule (each pair reads its expert again,
-    from the caches past the first)."""
+    The MXFP4 products run on the decode kernels with x in 16 bits, the experts' bytes
+    read as stored: the semantics of the grouped path for any number of rows, without
+    its expert-sorted MFMA schedule (an expert is read again for each of its pairs, or
+    for every 8 to 32 of them). `quantized.mxfp4_experts_linear` has that schedule, with
+    x rounded to MXFP4."""
     if not x.is_cuda:
         raise LinnetError("_mxfp4_grouped: linnet_amd runs on the GPU; x is on " + str(x.device))
     rows, chosen = experts.shape

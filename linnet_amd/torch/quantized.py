@@ -14,8 +14,8 @@ On the GPU, in bf16 or f16:
   MFMA (`fp8_mm`, replacing `torch._scaled_mm`; `int8_mm`).
 
 Anywhere else on the GPU (f32 activations, shapes the kernels do not take) the
-weight is dequantized by the HIP kernel and multiplied by `F.linear`. CPU
-tensors raise: this package has no CPU path.
+weight is dequantized by the HIP kernel and multiplied by `F.linear`, which records
+x's gradient; the kernels record none. CPU tensors raise: this package has no CPU path.
 """
 
 from __future__ import annotations
