@@ -454,8 +454,8 @@ LNQ_API LnqStatus lnq_mm8_block(const uint8_t* qx, const uint8_t* weight, const 
  * products are summed in f32 and scaled, the blocks added in f32, the sum rounded
  * once. An expert index outside 0 .. num_experts-1 gives zeros. in % 32 == 0,
  * in <= 65536; past 8192 chosen <= 2048, num_experts <= 65534, out <= 2^24 and a row's
- * choices within 2^29 elements of x. Replaces: torch/kernels.py:94-209 `mxfp4_experts` (the generated
- * `_mxfp4_experts`, src/backend/torch_source.cpp:1579-1600). */
+ * choices within 2^29 elements of x. Replaces: torch/kernels.py:94-209 `mxfp4_experts`
+ * (the generated `_mxfp4_experts`, src/backend/torch_source.cpp:1579-1600). */
 LNQ_API LnqStatus lnq_mxfp4_experts(const void* x, int64_t x_row_stride, int64_t x_slot_stride,
                                     const uint8_t* blocks, const uint8_t* scales,
                                     const int64_t* experts, void* y, int64_t rows, int64_t chosen,
@@ -541,8 +541,8 @@ LNQ_API LnqStatus lnq_mxfp4_experts_mm(const void* x, int64_t x_stride, const ui
  * by the lower index. With groups > 1 (equal runs of experts, at most 64) only the group_top
  * groups with the largest sum of their group_best (1 or 2; 1 where a group is one expert) best
  * choices are chosen from (a group with fewer that may be chosen counts -inf; by the scores' sum
- * without a bias). Weights are the chosen experts'
- * scores, without the bias, over their sum if `renormalize` (0 where that is 0), times `scale`.
+ * without a bias). Weights are the chosen experts' scores, without the bias, over their sum if
+ * `renormalize` (0 where that is 0), times `scale`.
  * An expert with a logit of -inf, or a choice of -inf or NaN, is never chosen; places left over
  * hold -1 and weight 0. A row with a NaN logit (or +inf, for softmax): -1 and NaN throughout.
  * num_experts <= 1024, top <= 64 and at most what the kept groups hold. The reference runs a

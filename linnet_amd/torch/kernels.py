@@ -838,10 +838,11 @@ def expert_route(logits: torch.Tensor, top: int, bias: torch.Tensor | None = Non
     logit's "sigmoid"; the choice goes by score + `bias` ([E] f32; without one by the logits), in
     64 bits, equal ones by the lower index. With `groups` > 1 (equal runs of experts) only the
     `group_top` groups whose `group_best` (1 or 2; 1 where a group is one expert) best choices sum
-    highest are chosen from. The weights are the chosen experts' scores (without the bias), over their sum if `renormalize`,
-    times `scale`. An expert whose logit is -inf, or whose choice is -inf or NaN, is never chosen;
-    a place left over holds -1 with weight 0, which the experts' products take as zeros. A row with
-    a NaN logit (or +inf under softmax) gets -1 and NaN. E <= 1024, top <= 64, groups <= 64."""
+    highest are chosen from. The weights are the chosen experts' scores (without the bias), over
+    their sum if `renormalize`, times `scale`. An expert whose logit is -inf, or whose choice is -inf
+    or NaN, is never chosen; a place left over holds -1 with weight 0, which the experts' products
+    take as zeros. A row with a NaN logit (or +inf under softmax) gets -1 and NaN. E <= 1024, top <=
+    64, groups <= 64."""
     device = _on_gpu("expert_route", logits, bias)
     shape = logits.shape
     if not shape:
