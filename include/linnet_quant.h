@@ -735,6 +735,67 @@ LNQ_API LnqStatus lnq_silu_mul_rows(const void* g, const void* u, void* a, int64
 LNQ_API LnqStatus lnq_silu_mul_tiles(const void* g, const void* u, void* xt, int64_t rows, int64_t width,
                                      int64_t g_stride, int64_t u_stride, void* stream);
 
+/* -------------------------------------------------------- a KV cache in pages (bf16, f16)
+ * Sequences of different lengths over one pool of pages, with any number of new tokens each in
+ * a call. No counterpart in the reference, whose generated module keeps one contiguous cache of
+ * one length (python/linnet/src/linnet/torch/compiled.py:430-503).
+ *
+ * The pool, 16-byte aligned: k_cache [pages, kv_heads, head_dim/8, page, 8] and v_cache [pages,
+ * kv_heads, page/8, head_dim, 8], page 16, 32, 64 or 128, head_dim 64 or 128. Entry e of sequence
+ * s lies in page tables[s, e / page] at place e % page. A batch (int32, device memory): tables
+ * [sequences, width], width * page <= 2^30; lengths [sequences], each sequence's entries with its
+ * new tokens; starts [sequences + 1], ascending from 0: tokens starts[s] .. starts[s + 1] - 1 of the
+ * call are the last entries of sequence s. Tokens from starts[sequences] on belong to none.
+ * Everything in device memory is read with its bounds checked: an entry that its table does not hold, or
+ * in a page outside the pool (an id of -1, say), is not there: it is neither read nor written.
+ */
+
+/* New tokens into the cache: per token and head of q [tokens, heads*head_dim] and k [tokens,
+ * kv_heads*head_dim] (rows q_stride / k_stride / v_stride elements apart: column slices of a joined
+ * projection), y = x * rsqrt(mean(x^2) + eps) * norm (q_norm, k_norm f32 [head_dim]; NULL: y = x), then the
+ * pairs (i, i + half), i < half, by cos / sin f32 [table, half] at the token's position (half a
+ * multiple of 8, at most head_dim / 2; 0: no rotation), in f32 and rounded once; q to q_out, k and v
+ * to the cache. A token's position is positions[token] (int32), or with NULL its entry. One without a row
+ * of the tables gives zeros in q_out and is not stored. Rows of q_out of no sequence become
+ * zeros with `fill`, else stay. Two sequences' new entries must not share a page's place. */
+LNQ_API LnqStatus lnq_paged_append(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                                   int64_t v_stride, const float* cos, const float* sin, int64_t table, int64_t half,
+                                   const int32_t* positions, const float* q_norm, const float* k_norm, float eps,
+                                   void* q_out, int64_t q_out_stride, int32_t fill, void* k_cache, void* v_cache,
+                                   const int32_t* tables, const int32_t* lengths, const int32_t* starts,
+                                   int64_t sequences, int64_t width, int64_t pages, int64_t page, int64_t tokens,
+                                   int64_t heads, int64_t kv_heads, int64_t head_dim, int32_t dtype, void* stream);
+
+/* Attention of the new tokens (already in the cache) over their sequences: out [tokens,
+ * heads*head_dim] = softmax(scale q K^T) V over the entries up to the token's own, with window > 0 the last
+ * `window` of them; sinks (f32 [heads], or NULL) add e^sink to each row's sum. parents (int32
+ * [tokens], or NULL): the new tokens of a sequence are a drafted tree of at most 256 nodes, token i's parent
+ * an earlier one of its sequence's or (any other number) the entry before the draft; a token sees the entries before
+ * the draft, its ancestors and itself (window: of that path). Nodes past the 256th, and rows that see
+ * nothing, give zeros. max_queries: the most new tokens of a sequence, as far as known (`tokens` always
+ * will do); it decides the kernels, not the result's meaning. workspace: 16-byte aligned,
+ * lnq_paged_attention_workspace floats; calls that overlap on one race. scale in [1e-30, 1e30]. */
+LNQ_API LnqStatus lnq_paged_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, void* out,
+                                      int64_t out_stride, int32_t fill, const int32_t* tables, const int32_t* lengths,
+                                      const int32_t* starts, const int32_t* parents, const float* sinks, float* workspace,
+                                      int64_t workspace_floats, int64_t sequences, int64_t width, int64_t pages, int64_t page,
+                                      int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_queries,
+                                      int64_t window, float scale, int32_t dtype, void* stream);
+
+/* Floats of lnq_paged_attention's workspace. */
+LNQ_API LnqStatus lnq_paged_attention_workspace(int64_t sequences, int64_t width, int64_t page, int64_t tokens, int64_t heads,
+                                                int64_t kv_heads, int64_t head_dim, int64_t max_queries, int64_t window,
+                                                int64_t* floats);
+
+/* The accepted path of each sequence's drafted tokens to where the sequence goes on: kept [sequences,
+ * path] int32, a sequence's nodes in ascending order (the path ends at the first number that is no later
+ * node); node kept[s, j]'s K and V move to the place of node j, in `layers` pools layer_step elements
+ * apart, and lengths_out[s] (not `lengths` itself) = the entries before the draft + the path's length. */
+LNQ_API LnqStatus lnq_paged_keep(void* k_cache, void* v_cache, int64_t layers, int64_t layer_step, const int32_t* tables,
+                                 const int32_t* lengths, const int32_t* starts, const int32_t* kept, int64_t path,
+                                 int32_t* lengths_out, int64_t sequences, int64_t width, int64_t pages, int64_t page,
+                                 int64_t tokens, int64_t kv_heads, int64_t head_dim, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -92,6 +92,12 @@ SIGNATURES: dict[str, list[object]] = {
     "lnq_silu_mul": [_p, _p, _p, _i64, _p],
     "lnq_silu_mul_rows": [_p, _p, _p, _i64, _i64, _i64, _i64, _p],
     "lnq_silu_mul_tiles": [_p, _p, _p, _i64, _i64, _i64, _i64, _p],
+    "lnq_paged_append": [_p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _f32, _p, _i64, _i32, _p, _p, _p, _p, _p,
+                         _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _p],
+    "lnq_paged_attention": [_p, _i64, _p, _p, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                            _i64, _i64, _i64, _i64, _f32, _i32, _p],
+    "lnq_paged_attention_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "lnq_paged_keep": [_p, _p, _i64, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p],
 }
 
 _lock = threading.Lock()
