@@ -13,11 +13,12 @@
 // one exchange; and with the entries of an MFMA's rows in the order of `entry_of_row`, a lane's
 // scores are, in its own registers, the operand of the second product: no weight goes through LDS.
 //
-// Two kernels. `few`: sequences of up to 32 rows (decode steps, small drafts). Bound by memory: 4
+// Two ways. `few`: sequences of up to 32 rows (decode steps, small drafts). Bound by memory: 4
 // waves of a workgroup take steps of 32 entries in turn, K and V straight from the pages to registers,
 // a step ahead, and add up through LDS. `many`: tiles of 128 rows, 32 a wave, which share tiles of
 // 64 entries in LDS, loaded a tile ahead. Where the rows are few for the chip, the entries are split over
-// workgroups too, and a last kernel adds the parts in order.
+// workgroups too, and a last kernel adds the parts in order. Which sequence is which is on the device:
+// a call that may have both runs both in one launch.
 #include <math.h>
 
 #include <type_traits>
@@ -34,17 +35,23 @@ constexpr int MANY_STEP = 64;
 constexpr int NODES = 256;       // of a drafted tree
 constexpr int MAX_SPLITS = 256;
 
+// The sums of tiles whose entries are split, for each of the splits and rows: the outputs so far, [splits][rows]
+// [head_dim], and maximum (times log2 e) and sum, [splits][rows][2].
+struct Parts {
+  float *sums, *stats;
+  int64_t rows;
+  int splits;  // at most
+};
+
 struct AttendArgs {
   const uint16_t *q, *k_cache, *v_cache;
   uint16_t* out;
   int64_t q_stride, out_stride;
   const float* sinks;      // [heads] or nullptr
   const int32_t* parents;  // [tokens]: a node's parent among its sequence's new tokens; nullptr: no tree
-  float *parts, *stats;    // [splits][rows][head_dim] sums, [splits][rows][2] maximum (times log2 e) and sum
-  int64_t part_rows;
+  Parts small, large;      // of few rows' sequences and of the others
   Batch batch;
   int heads, kv_heads, group, window;
-  int splits;              // at most, of a tile's entries
   int few_tokens;          // few: new tokens of a sequence that may be split
   int few, few_tile;       // rows of a sequence that `few` takes, and of a tile of it
   float scale2;            // scale * log2 e
@@ -363,24 +370,37 @@ __device__ inline int64_t part_row(const AttendArgs& a, bool few, int s, const S
   return few ? (static_cast<int64_t>(s) * a.few_tokens + i) * a.heads + head : static_cast<int64_t>(q.first + i) * a.heads + head;
 }
 
-// A tile of TILE rows (16, or 32 where sequences may have more) of one KV head of one sequence.
+// LDS of the few-row way: each wave's outputs for the others, and maxima and sums.
+template <int HD, int TILE>
+struct FewLds {
+  static constexpr int OWN = HD * TILE / 64 / 4;  // a wave's share of a lane's outputs
+  f32x4 others[4][3][OWN / 4][64];
+  float stat[4][TILE][2];
+};
+
+// A tree's paths, depths and parents (nothing without a tree).
+template <bool TREE>
+struct TreeLds {
+  uint32_t paths[TREE ? NODES * (NODES / 32) : 1];
+  int depth[TREE ? NODES : 1], up[TREE ? NODES : 1];
+};
+
+// The few-row way: tiles of TILE rows (16, or 32 where sequences may have more) of one KV head of one
+// sequence. q_tile: for its queries, [HD / SUMMED][64], where a lane has no registers left for them.
 template <int DT, int HD, int TILE, bool TREE>
-__global__ __launch_bounds__(256, 2) void paged_few_kernel(AttendArgs a) {
+__device__ inline void few_rows(const AttendArgs& a, int block, FewLds<HD, TILE>& lds, u32x4* q_tile, TreeLds<TREE>& tree) {
   using R = Rows<DT, HD, TILE>;
   using S = Shape<TILE>;
   constexpr int CH = HD / 8, QK = R::QK, NT = R::NT, NK = R::NK, DV = R::DV, REGS = S::REGS, GROUPS = S::GROUPS;
-  constexpr int OWN = DV * REGS / 4;  // a wave's share of a lane's outputs
-  constexpr bool Q_IN_LDS = TILE * HD > 16 * 128;  // a lane has no registers left for them
-  __shared__ f32x4 others[4][3][OWN / 4][64];
-  __shared__ float stat[4][TILE][2];
-  __shared__ u32x4 q_tile[Q_IN_LDS ? QK * 64 : 1];
-  __shared__ uint32_t paths[TREE ? NODES * (NODES / 32) : 1];
-  __shared__ int depth[TREE ? NODES : 1], up[TREE ? NODES : 1];
+  constexpr int OWN = FewLds<HD, TILE>::OWN;
+  constexpr bool Q_IN_LDS = TILE * HD > 16 * 128;
+  auto& others = lds.others;
+  auto& stat = lds.stat;
   const Batch& b = a.batch;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = lane / TILE, col = lane % TILE;
-  const int h = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  const int split = rest % a.splits, s = rest / a.splits;
+  const int h = block % a.kv_heads, rest = block / a.kv_heads;
+  const int split = rest % a.small.splits, s = rest / a.small.splits;
   const int mask = (1 << b.page_bits) - 1;
   if (s == b.sequences) {
     if (!a.fill || split != 0) return;
@@ -395,9 +415,9 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttendArgs a) {
   const int64_t all_rows = static_cast<int64_t>(q.n) * a.group;
   if (q.n == 0 || (all_rows > a.few && !a.every)) return;
   const int rows = static_cast<int>(all_rows);
-  const int splits = q.n <= a.few_tokens ? a.splits : 1;
+  const int splits = q.n <= a.few_tokens ? a.small.splits : 1;
   if (split >= splits) return;
-  if constexpr (TREE) paths_of(a, q, paths, depth, up, 256);
+  if constexpr (TREE) paths_of(a, q, tree.paths, tree.depth, tree.up, 256);
   const int limit = min(q.length, capacity(b));  // entries that may be there
   const float slack = 8.f / a.scale2;
 
@@ -407,7 +427,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttendArgs a) {
     if (split >= range.used) continue;
     const int begin = range.lo + split * range.chunk, end = min(range.hi, begin + range.chunk);
     const int r = min(r0 + col, rows - 1), i = r / a.group, head = h * a.group + r % a.group;
-    const Row row = row_of<TREE>(a, q, i, paths, depth);
+    const Row row = row_of<TREE>(a, q, i, tree.paths, tree.depth);
     // All rows see entries sure_low .. sure_last.
     const int sure_last = TREE ? q.base - 1 : q.base + i0;
     const int sure_low = a.window > 0 ? q.base + (TREE ? q.n - 1 : i1) - a.window + 1 : 0;
@@ -570,20 +590,29 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttendArgs a) {
         for (int g = 0; g < OWN / 4; ++g)
           *reinterpret_cast<u32x2*>(to + dim_of(g)) = u32x2{pack2<DT>(total[g][0] * n, total[g][1] * n), pack2<DT>(total[g][2] * n, total[g][3] * n)};
       } else {
-        const int64_t at = split * a.part_rows + part_row(a, true, s, q, i, head);
+        const int64_t at = split * a.small.rows + part_row(a, true, s, q, i, head);
 #pragma unroll
-        for (int g = 0; g < OWN / 4; ++g) *reinterpret_cast<f32x4*>(a.parts + at * HD + dim_of(g)) = total[g];
-        if (wave == 0 && group == 0) a.stats[2 * at] = m, a.stats[2 * at + 1] = sum;
+        for (int g = 0; g < OWN / 4; ++g) *reinterpret_cast<f32x4*>(a.small.sums + at * HD + dim_of(g)) = total[g];
+        if (wave == 0 && group == 0) a.small.stats[2 * at] = m, a.small.stats[2 * at + 1] = sum;
       }
     }
     __syncthreads();  // `stat`, `others` and the queries are the next tile's
   }
 }
 
+template <int DT, int HD, int TILE, bool TREE>
+__global__ __launch_bounds__(256, 2) void paged_few_kernel(AttendArgs a) {
+  __shared__ FewLds<HD, TILE> lds;
+  __shared__ u32x4 q_tile[HD * TILE * 2 / 16];
+  __shared__ TreeLds<TREE> tree;
+  few_rows<DT, HD, TILE, TREE>(a, blockIdx.x, lds, q_tile, tree);
+}
+
 __device__ inline int many_slot(const AttendArgs& a, int s) {
   return static_cast<int>(static_cast<int64_t>(clamp_to(a.batch.starts[s], 0, a.batch.tokens)) * a.group / MANY) + s;
 }
 
+// The many-row way, for the tiles of `slots` slots; past their workgroups, the sequences of few rows.
 template <int DT, int HD, bool TREE>
 __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int slots) {
   using R = Rows<DT, HD, 32>;
@@ -592,15 +621,20 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   // Two tiles, K: [CH][64 entries] and V: [8 eights of entries][HD]. (Two arrays: of one, the compiler
   // has every read wait for the loads in flight into the other half.)
   __shared__ u32x4 tile0[2 * UNITS], tile1[2 * UNITS];
-  __shared__ uint32_t paths[TREE ? NODES * (NODES / 32) : 1];
-  __shared__ int depth[TREE ? NODES : 1], up[TREE ? NODES : 1];
+  __shared__ TreeLds<TREE> tree;
   __shared__ uint32_t odd_waves[4];
+  const int tiles = slots * a.kv_heads * a.large.splits;
+  if (static_cast<int>(blockIdx.x) >= tiles) {
+    static_assert(sizeof(FewLds<HD, 16>) <= sizeof(tile0), "the few-row way's LDS");
+    few_rows<DT, HD, 16, TREE>(a, blockIdx.x - tiles, *reinterpret_cast<FewLds<HD, 16>*>(tile0), tile1, tree);
+    return;
+  }
   const Batch& b = a.batch;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, col = lane & 31;
   const int h = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
   // The last tiles first: of a prompt they see the most.
-  const int split = rest % a.splits, slot = slots - 1 - rest / a.splits;
+  const int split = rest % a.large.splits, slot = slots - 1 - rest / a.large.splits;
   const int s = find_sequence(b.sequences, slot, [&](int i) { return many_slot(a, i); });
   const Sequence q = sequence_of(b, s);
   const int rows = static_cast<int>(static_cast<int64_t>(q.n) * a.group);
@@ -608,10 +642,10 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   if (rows <= a.few || local < 0 || local >= (rows + MANY - 1) / MANY) return;
   const int r0 = local * MANY;
   const int i0 = r0 / a.group, i1 = (min(r0 + MANY, rows) - 1) / a.group;
-  const Range range = range_of(a, q, i0, i1, a.splits, MANY_STEP);
+  const Range range = range_of(a, q, i0, i1, a.large.splits, MANY_STEP);
   if (split >= range.used) return;
   const int begin = range.lo + split * range.chunk, end = min(range.hi, begin + range.chunk);
-  if constexpr (TREE) paths_of(a, q, paths, depth, up, 256);
+  if constexpr (TREE) paths_of(a, q, tree.paths, tree.depth, tree.up, 256);
   const int limit = min(min(q.length, capacity(b)), end);
   const int mask = (1 << b.page_bits) - 1;
   const float slack = 8.f / a.scale2;
@@ -620,7 +654,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   const int w0 = r0 + 32 * wave;
   const bool busy = w0 < rows;
   const int r = min(w0 + col, rows - 1), i = r / a.group, head = h * a.group + r % a.group;
-  const Row row = row_of<TREE>(a, q, i, paths, depth);
+  const Row row = row_of<TREE>(a, q, i, tree.paths, tree.depth);
   const int wa = min(w0, rows - 1) / a.group, wz = min(w0 + 31, rows - 1) / a.group;
   const int sure_last = TREE ? q.base - 1 : q.base + wa, sure_low = a.window > 0 ? q.base + (TREE ? q.n - 1 : wz) - a.window + 1 : 0;
   const int any_last = TREE ? q.length - 1 : q.base + wz, any_low = a.window > 0 ? q.base + (TREE ? 0 : wa) - a.window + 1 : 0;
@@ -762,30 +796,37 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
         *reinterpret_cast<u32x4*>(to + 32 * d + 8 * (g + half)) = u32x4{x[0], x[1], y[0], y[1]};
       }
   } else {
-    const int64_t at = split * a.part_rows + part_row(a, false, s, q, i, head);
+    const int64_t at = split * a.large.rows + part_row(a, false, s, q, i, head);
 #pragma unroll
     for (int d = 0; d < DV; ++d)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(a.parts + at * HD + 32 * d + 8 * g + 4 * half) =
+        *reinterpret_cast<f32x4*>(a.large.sums + at * HD + 32 * d + 8 * g + 4 * half) =
             f32x4{st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]};
-    if (half == 0) a.stats[2 * at] = m, a.stats[2 * at + 1] = l;
+    if (half == 0) a.large.stats[2 * at] = m, a.large.stats[2 * at + 1] = l;
   }
 }
 
-// A row's parts added in order. A workgroup takes one row of one head: of `few` sequences the i-th new
-// token of each, else a token of the batch.
-template <int DT, int HD, bool SMALL>
-__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a) {
-  constexpr int SETS = 256 / HD;
-  __shared__ float weight[MAX_SPLITS];
-  __shared__ float sums[SETS][HD];
+// Parts added in order: a row of one head to a wave, or with many splits to a workgroup (WIDE), whose waves
+// take the splits in turn. First the few-row sequences' rows (their i-th new tokens), then the batch's tokens.
+template <int DT, int HD, bool WIDE>
+__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a, int64_t small_rows, int64_t rows) {
+  constexpr int WAVES = WIDE ? 4 : 1;  // of a row
+  constexpr int D = HD / 64;           // dimensions a lane
+  constexpr int AHEAD = 8;             // splits loaded together
+  __shared__ float weight[WIDE ? MAX_SPLITS : 4 * 64];
+  __shared__ float sums[WIDE ? 3 : 1][HD];
   const Batch& b = a.batch;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int head = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t at_row = WIDE ? blockIdx.x : blockIdx.x * int64_t{4} + wave;
+  if (at_row >= rows) return;
+  const bool small = at_row < small_rows;
+  const Parts& part = small ? a.small : a.large;
+  const int64_t local = small ? at_row : at_row - small_rows;
+  const int head = static_cast<int>(local % a.heads), rest = static_cast<int>(local / a.heads);
   int s, i;
   Sequence q;
-  if constexpr (SMALL) {
+  if (small) {
     s = rest / a.few_tokens;
     q = sequence_of(b, s);
     i = rest % a.few_tokens;
@@ -797,40 +838,60 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a) {
     if (i < 0 || i >= q.n || static_cast<int64_t>(q.n) * a.group <= a.few) return;
   }
   // The tile that the row was computed in.
-  const int per = SMALL ? a.few_tile : MANY;
-  const int64_t rows = static_cast<int64_t>(q.n) * a.group;
+  const int per = small ? a.few_tile : MANY;
+  const int64_t all = static_cast<int64_t>(q.n) * a.group;
   const int64_t r0 = (static_cast<int64_t>(i) * a.group + head % a.group) / per * per;
-  const int i0 = static_cast<int>(r0 / a.group), i1 = static_cast<int>((min(r0 + per, rows) - 1) / a.group);
-  const Range range = range_of(a, q, i0, i1, a.splits, SMALL ? FEW_STEP : MANY_STEP);
+  const int i0 = static_cast<int>(r0 / a.group), i1 = static_cast<int>((min(r0 + per, all) - 1) / a.group);
+  const Range range = range_of(a, q, i0, i1, part.splits, small ? FEW_STEP : MANY_STEP);
   if (range.used == 1) return;
-  const int64_t at = part_row(a, SMALL, s, q, i, head);
+  const int64_t at = part_row(a, small, s, q, i, head);
+  float* const weights = WIDE ? weight : weight + 64 * wave;
   float m = -INFINITY;
-  for (int c = lane; c < range.used; c += 64) m = fmaxf(m, a.stats[2 * (c * a.part_rows + at)]);
+  for (int c = lane; c < range.used; c += 64) m = fmaxf(m, part.stats[2 * (c * part.rows + at)]);
   m = wave_max(m);
   float l = 0.f;
   for (int c = lane; c < range.used; c += 64) {
-    const float mc = a.stats[2 * (c * a.part_rows + at)];
+    const float mc = part.stats[2 * (c * part.rows + at)];
     const float w = mc == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mc - m);
-    l = fmaf(a.stats[2 * (c * a.part_rows + at) + 1], w, l);
-    if (tid < 64) weight[c] = w;
+    l = fmaf(part.stats[2 * (c * part.rows + at) + 1], w, l);
+    if (!WIDE || wave == 0) weights[c] = w;
   }
   l = wave_sum(l);
-  __syncthreads();
-  const int d = tid % HD, set = tid / HD;
-  const float* const from = a.parts + at * HD + d;
-  float o = 0.f;
-#pragma unroll 4
-  for (int c = set; c < range.used; c += SETS) {
-    const float w = weight[c];
-    o += w == 0.f ? 0.f : w * from[c * a.part_rows * HD];
-  }
-  sums[set][d] = o;
-  __syncthreads();
-  if (set != 0) return;
+  if constexpr (WIDE) __syncthreads();
+  const float* const from = part.sums + at * HD + lane * D;
+  float o[D] = {};
+  for (int c0 = WIDE ? wave : 0; c0 < range.used; c0 += WAVES * AHEAD) {
+    float x[AHEAD][D];
 #pragma unroll
-  for (int n = 1; n < SETS; ++n) o += sums[n][d];
-  using E = Elem<DT>;
-  a.out[(q.first + i) * a.out_stride + static_cast<int64_t>(head) * HD + d] = E::from_f32(o * norm_of(m, l, a.sinks, head));
+    for (int n = 0; n < AHEAD; ++n) {
+      const int c = min(c0 + WAVES * n, range.used - 1);  // (past the last: read again, and not used)
+#pragma unroll
+      for (int d = 0; d < D; ++d) x[n][d] = from[c * part.rows * HD + d];
+    }
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) {
+      const int c = c0 + WAVES * n;
+      const float w = c < range.used ? weights[c] : 0.f;
+#pragma unroll
+      for (int d = 0; d < D; ++d) o[d] += w == 0.f ? 0.f : w * x[n][d];
+    }
+  }
+  if constexpr (WIDE) {
+    if (wave > 0) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) sums[wave - 1][lane * D + d] = o[d];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int n = 0; n < 3; ++n)
+#pragma unroll
+      for (int d = 0; d < D; ++d) o[d] += sums[n][lane * D + d];
+  }
+  const float n = norm_of(m, l, a.sinks, head);
+  uint16_t* const to = a.out + (q.first + i) * a.out_stride + static_cast<int64_t>(head) * HD + lane * D;
+  if constexpr (D == 2) *reinterpret_cast<uint32_t*>(to) = pack2<DT>(o[0] * n, o[D - 1] * n);
+  else *to = static_cast<uint16_t>(pack2<DT>(o[0] * n, 0.f));
 }
 
 // ------------------------------------------------------------------ the host's side
@@ -853,10 +914,10 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
   most = most > tokens ? tokens : most;
   most = most < 1 ? 1 : most;
   p.many = most * group > FEW;
-  p.few = p.many && group <= 16 ? 16 : FEW;
+  p.few = p.many ? 16 : FEW;
   p.few_tokens = p.few / group < 1 ? 1 : p.few / group;
   if (!p.many && most < p.few_tokens) p.few_tokens = most;
-  p.few_tile = p.few_tokens * group <= 16 ? 16 : 32;
+  p.few_tile = p.many || p.few_tokens * group <= 16 ? 16 : 32;
   // Entries a tile may see, at most.
   int64_t seen = width * page;
   if (window > 0 && window + most + FEW_STEP < seen) seen = window + most + FEW_STEP;
@@ -871,6 +932,7 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
     const int64_t top = up_to(seen, FEW_STEP);
     p.few_splits = bounded(want, top < MAX_SPLITS ? top : MAX_SPLITS);
   }
+  if (p.many && group > p.few) p.few_splits = 1;  // (no sequence has so few rows)
   p.many_splits = 1;
   if (p.many) {
     p.slots = tokens * group / MANY + sequences;
@@ -887,30 +949,30 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
 
 template <int DT, int HD, bool TREE>
 static LnqStatus attend(AttendArgs a, const Plan& p, float* work, hipStream_t st) {
-  const int64_t heads = a.heads, kv_heads = a.kv_heads, sequences = a.batch.sequences;
+  const int64_t sequences = a.batch.sequences;
   const dim3 block(256);
-  a.parts = work;
-  a.stats = work + p.few_rows * p.few_splits * HD;
-  a.part_rows = p.few_rows;
-  a.splits = static_cast<int>(p.few_splits);
+  a.small = {work, work + p.few_rows * p.few_splits * HD, p.few_rows, static_cast<int>(p.few_splits)};
+  float* const more = work + p.few_floats;
+  a.large = {more, more + p.many_rows * p.many_splits * HD, p.many_rows, static_cast<int>(p.many_splits)};
   a.every = !p.many;
+  a.few = p.few, a.few_tile = p.few_tile;
   a.few_tokens = static_cast<int>(p.few_tokens);
-  a.few = p.few;
-  a.few_tile = p.few_tile;
-  const unsigned few = static_cast<unsigned>((sequences + (a.fill ? 1 : 0)) * kv_heads * p.few_splits);
-  if (few > 0 && p.few_tile == 16) hipLaunchKernelGGL((paged_few_kernel<DT, HD, 16, TREE>), dim3(few), block, 0, st, a);
-  else if (few > 0) hipLaunchKernelGGL((paged_few_kernel<DT, HD, 32, TREE>), dim3(few), block, 0, st, a);
-  if (p.few_splits > 1 && sequences > 0)
-    hipLaunchKernelGGL((paged_join_kernel<DT, HD, true>), dim3(static_cast<unsigned>(sequences * p.few_tokens * heads)), block, 0, st, a);
-  if (p.many && sequences > 0) {
-    a.parts = work + p.few_floats;
-    a.stats = a.parts + p.many_rows * p.many_splits * HD;
-    a.part_rows = p.many_rows;
-    a.splits = static_cast<int>(p.many_splits);
-    hipLaunchKernelGGL((paged_many_kernel<DT, HD, TREE>), dim3(static_cast<unsigned>(p.slots * kv_heads * p.many_splits)), block, 0, st, a,
-                       static_cast<int>(p.slots));
-    if (p.many_splits > 1)
-      hipLaunchKernelGGL((paged_join_kernel<DT, HD, false>), dim3(static_cast<unsigned>(a.batch.tokens * heads)), block, 0, st, a);
+  const int64_t few = (sequences + (a.fill ? 1 : 0)) * a.kv_heads * p.few_splits;
+  if (p.many) {
+    const int64_t tiles = p.slots * a.kv_heads * p.many_splits;
+    if (tiles + few > 0)
+      hipLaunchKernelGGL((paged_many_kernel<DT, HD, TREE>), dim3(static_cast<unsigned>(tiles + few)), block, 0, st, a, static_cast<int>(p.slots));
+  } else if (few > 0) {
+    const dim3 grid(static_cast<unsigned>(few));
+    if (p.few_tile == 16) hipLaunchKernelGGL((paged_few_kernel<DT, HD, 16, TREE>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((paged_few_kernel<DT, HD, 32, TREE>), grid, block, 0, st, a);
+  }
+  const int64_t rows = p.few_rows + p.many_rows;
+  if (rows > 0) {
+    if (p.few_splits > 16 || p.many_splits > 16)
+      hipLaunchKernelGGL((paged_join_kernel<DT, HD, true>), dim3(static_cast<unsigned>(rows)), block, 0, st, a, p.few_rows, rows);
+    else
+      hipLaunchKernelGGL((paged_join_kernel<DT, HD, false>), dim3(static_cast<unsigned>(up_to(rows, 4))), block, 0, st, a, p.few_rows, rows);
   }
   return launched("paged_attention");
 }
@@ -931,7 +993,8 @@ static const char* sizes_refused(int64_t sequences, int64_t width, int64_t pages
   if (window < 0 || window > (1 << 30)) return "a window is 0 (none) to 2^30 entries";
   if (tokens * heads > INT32_MAX || sequences * heads * 32 > INT32_MAX) return "too many tokens, sequences or heads";
   const paged::Plan p = paged::plan_of(sequences, width, page, tokens, heads, kv_heads, head_dim, most, window);
-  if ((sequences + 1) * kv_heads * p.few_splits > INT32_MAX || p.slots * kv_heads * p.many_splits > INT32_MAX) return "too many tokens, sequences or heads";
+  if ((sequences + 1) * kv_heads * p.few_splits + p.slots * kv_heads * p.many_splits > INT32_MAX || p.few_rows + p.many_rows > INT32_MAX)
+    return "too many tokens, sequences or heads";
   return nullptr;
 }
 
