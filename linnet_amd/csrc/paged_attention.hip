@@ -82,6 +82,13 @@ __device__ inline uint32_t pack2(float a, float b) {
   return DT == LNQ_BF16 ? pack_bf16x2(a, b) : pack_f16x2(a, b);
 }
 
+// acc + the two values of a dword (as they are after rounding), one instruction.
+template <int DT>
+__device__ inline float add2(uint32_t pair, float acc) {
+  if constexpr (DT == LNQ_BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, Elem<DT>::ONE2), acc, false);
+  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), __builtin_bit_cast(f16x2, Elem<DT>::ONE2), acc, false);
+}
+
 // The entry (of 32) at row m of the first product's n-th tile: a lane's results are then, in the order
 // of its registers, runs of the eight entries 8 (GROUPS s + group) .. + 7, the second product's summed indices.
 template <int TILE>
@@ -318,15 +325,17 @@ struct Rows {
 #pragma unroll
       for (int r = 0; r < S::REGS; ++r) {
         s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, -at));
-        sum += s[n][r];
       }
-    l += sum;
     // Value i of a lane's 8 NK N, in the order of its registers.
     auto at_of = [&](int i) __attribute__((always_inline)) -> float { return s[i / S::REGS][i % S::REGS]; };
 #pragma unroll
     for (int k = 0; k < N * NK; ++k)
 #pragma unroll
-      for (int d = 0; d < 4; ++d) p[k][d] = pack2<DT>(at_of(8 * k + 2 * d), at_of(8 * k + 2 * d + 1));
+      for (int d = 0; d < 4; ++d) {
+        p[k][d] = pack2<DT>(at_of(8 * k + 2 * d), at_of(8 * k + 2 * d + 1));
+        sum = add2<DT>(p[k][d], sum);
+      }
+    l += sum;
   }
 
   // Adds the infinities and NaNs of V to the rows that see them (and to no other, as 0 times them in
@@ -672,25 +681,31 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   const int32_t* const table = b.tables + static_cast<int64_t>(s) * b.width;
   auto page_at = [&](int t) __attribute__((always_inline)) -> int { return table[min(t + lane, end - 1) >> b.page_bits]; };
   auto good = [&](int page) __attribute__((always_inline)) -> bool { return page >= 0 && page < b.pages; };
-  auto load = [&](int id, int t, u32x4* to) __attribute__((always_inline)) {
+  struct Source {
+    const uint16_t* k;  // this lane's entry, dimensions 0 .. 7
+    int page;           // of this lane's entry
+    int t;
+  };
+  auto source_of = [&](int id, int t) __attribute__((always_inline)) -> Source {
     const int page = good(id) ? id : 0;
     const int64_t kp = static_cast<int64_t>(page) * a.kv_heads + h;
-    const uint16_t* const kr = a.k_cache + ((kp * CH << b.page_bits) + ((t + lane) & mask)) * 8;
-#pragma unroll
-    for (int n = 0; n < CH / 4; ++n) {
-      const int c = wave * (CH / 4) + n;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kr + (static_cast<int64_t>(c) << b.page_bits) * 8),
-                                       (__attribute__((address_space(3))) void*)(to + c * 64), 16, 0, 0);
-    }
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int e8 = 2 * wave + n;  // the eight entries 8 e8 ..
-      const int64_t vp = static_cast<int64_t>(__builtin_amdgcn_readlane(page, 8 * e8)) * a.kv_heads + h;
-      const uint16_t* const vr = a.v_cache + (((vp << (b.page_bits - 3)) + (((t + 8 * e8) & mask) >> 3)) * HD + lane) * 8;
-#pragma unroll
-      for (int d = 0; d < HD / 64; ++d)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vr + 64 * 8 * d),
-                                         (__attribute__((address_space(3))) void*)(to + UNITS + e8 * HD + 64 * d), 16, 0, 0);
+    return Source{a.k_cache + ((kp * CH << b.page_bits) + ((t + lane) & mask)) * 8, page, t};
+  };
+  auto to_lds = [&](const uint16_t* from, u32x4* to) __attribute__((always_inline)) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+  };
+  // Load i of this wave's LOADS of a tile.
+  constexpr int K_LOADS = CH / 4, LOADS = 2 * K_LOADS;
+  auto load_one = [&](const Source& x, u32x4* to, int i) __attribute__((always_inline)) {
+    if (i < K_LOADS) {
+      const int c = wave * K_LOADS + i;
+      to_lds(x.k + (static_cast<int64_t>(c) << b.page_bits) * 8, to + c * 64);
+    } else {
+      const int part = wave * K_LOADS + i - K_LOADS;
+      const int e8 = part / (HD / 64), d = part % (HD / 64);  // the eight entries 8 e8 .., 64 dimensions
+      const int64_t vp = static_cast<int64_t>(__builtin_amdgcn_readlane(x.page, 8 * e8)) * a.kv_heads + h;
+      to_lds(a.v_cache + (((vp << (b.page_bits - 3)) + (((x.t + 8 * e8) & mask) >> 3)) * HD + 64 * d + lane) * 8,
+             to + UNITS + e8 * HD + 64 * d);
     }
   };
 
@@ -699,7 +714,9 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   if (begin < end) {
     id = page_at(begin);
     next = page_at(begin + MANY_STEP);
-    load(id, begin, tile0);
+    const Source first = source_of(id, begin);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load_one(first, tile0, i);
   }
   loads_done();
   lds_barrier();
@@ -707,7 +724,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
     const uint64_t valid = __ballot(t + lane < limit && good(id));
     id = next;
     next = page_at(t + 2 * MANY_STEP);
-    if (t + MANY_STEP < end) load(id, t + MANY_STEP, other);
+    const Source source = source_of(id, t + MANY_STEP);
     u32x4* const kt = cur;
     u32x4* const vt = cur + UNITS;
     // Where some row does not see all of the tile, V's entries that are not there become 0 (their
@@ -749,11 +766,16 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
     if (takes) {
       f32x16 sc[2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[n][e] = 0.f;
+      // The next tile's loads go out between these products (past the last tile the last one's again, into
+      // the buffer that is not read): the CU takes 64 bytes of them a cycle, and a wave waits to issue the next.
 #pragma unroll
-        for (int c = 0; c < QK; ++c) sc[n] = mma<DT, 32>(kt[(2 * c + half) * 64 + 32 * n + entry], qx[c], sc[n]);
+      for (int c = 0; c < QK; ++c) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) sc[n] = mma<DT, 32>(kt[(2 * c + half) * 64 + 32 * n + entry], qx[c], sc[n]);
+        load_one(source, other, c);
       }
       if (!sure) {
         look();
@@ -765,6 +787,10 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
       for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int d = 0; d < DV; ++d) st.o[d] = mma<DT, 32>(v_of(k, d), p[k], st.o[d]);
+    }
+    if (!takes) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) load_one(source, other, i);
     }
     loads_done();
     lds_barrier();

@@ -79,29 +79,32 @@ class PagedCache:
         return PagedCache(self.k[i], self.v[i])
 
 
-def _no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise LinnetError(f"{what}: records no gradient, and an input requires one")
+# A call's host time is longer than a decode step's kernels here, so the checks below are the direct forms.
+_INT32, _FLOAT32 = torch.int32, torch.float32
 
 
-def _ints(what: str, name: str, t: torch.Tensor, shape: tuple[int, ...]) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.shape != shape:
-        raise LinnetError(f"{what}: {name} is {list(shape)} int32, got {list(t.shape)} {t.dtype}")
+def _records(what: str) -> None:
+    raise LinnetError(f"{what}: records no gradient, and an input requires one")
+
+
+def _ints(what: str, name: str, t: torch.Tensor, count: int) -> torch.Tensor:
+    if t.dtype is not _INT32 or t.dim() != 1 or t.numel() != count:
+        raise LinnetError(f"{what}: {name} is [{count}] int32, got {list(t.shape)} {t.dtype}")
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _batch(what: str, tables: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor) -> tuple:
-    if tables.dim() != 2 or tables.dtype != torch.int32:
+    if tables.dtype is not _INT32 or tables.dim() != 2:
         raise LinnetError(f"{what}: tables is [sequences, width] int32, got {list(tables.shape)} {tables.dtype}")
     sequences, width = tables.shape
-    return (tables if tables.is_contiguous() else tables.contiguous(), _ints(what, "lengths", lengths, (sequences,)),
-            _ints(what, "starts", starts, (sequences + 1,)), sequences, width)
+    return (tables if tables.is_contiguous() else tables.contiguous(), _ints(what, "lengths", lengths, sequences),
+            _ints(what, "starts", starts, sequences + 1), sequences, width)
 
 
-def _rows(what: str, name: str, t: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, int]:
+def _rows(what: str, name: str, t: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, int, int, int]:
     """`t` [tokens, width] as the kernels read it (rows of contiguous values, whole 16 bytes apart; column slices
-    of a joined projection as they are, anything else copied) and its row stride."""
-    if t.dim() != 2 or t.dtype != dtype:
+    of a joined projection as they are, anything else copied), its row stride, tokens and width."""
+    if t.dtype is not dtype or t.dim() != 2:
         raise LinnetError(f"{what}: {name} is [tokens, width] {dtype} as the cache is, got {list(t.shape)} {t.dtype}")
     rows, width = t.shape
     stride, step = t.stride()
@@ -110,15 +113,18 @@ def _rows(what: str, name: str, t: torch.Tensor, dtype: torch.dtype) -> tuple[to
     if step != 1 or stride % 8 or stride < width or t.data_ptr() % 16:
         t = _aligned(t)
         stride = width
-    return t, stride
+    return t, stride, rows, width
 
 
-def _out(what: str, out: torch.Tensor | None, like: torch.Tensor, width: int) -> torch.Tensor:
-    if out is None:
-        return torch.empty(like.shape[0], width, dtype=like.dtype, device=like.device)
-    if out.dtype != like.dtype or out.shape != (like.shape[0], width) or not out.is_contiguous() or out.data_ptr() % 16:
-        raise LinnetError(f"{what}: out is a contiguous, 16-byte aligned [{like.shape[0]}, {width}] {like.dtype}, got "
-                          f"{list(out.shape)} {out.dtype}")
+def _floats(what: str, name: str, t: torch.Tensor, count: int) -> torch.Tensor:
+    if t.dtype is not _FLOAT32 or t.dim() != 1 or t.numel() != count:
+        raise LinnetError(f"{what}: {name} is [{count}] float32, got {list(t.shape)} {t.dtype}")
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else _aligned(t)
+
+
+def _out(what: str, out: torch.Tensor, rows: int, width: int, dtype: torch.dtype) -> torch.Tensor:
+    if out.dtype is not dtype or out.shape != (rows, width) or not out.is_contiguous() or out.data_ptr() % 16:
+        raise LinnetError(f"{what}: out is a contiguous, 16-byte aligned [{rows}, {width}] {dtype}, got {list(out.shape)} {out.dtype}")
     return out
 
 
@@ -146,47 +152,51 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
     sequence give zeros, or with `out` leave its rows as they were. Two sequences may share pages, but not
     the places of their new entries."""
     pages, page, kv_heads, head_dim, code, _ = _one_layer("paged_append", cache)
-    device = _on_gpu("paged_append", q, k, v, cache.k, tables, lengths, starts, cos, sin, positions, q_norm, k_norm, out)
-    _no_gradient("paged_append", q, k, v, cos, sin, q_norm, k_norm, out)
-    dtype = cache.k.dtype
+    k_cache, v_cache = cache.k, cache.v
+    device = _on_gpu("paged_append", q, k, v, k_cache, tables, lengths, starts, cos, sin, positions, q_norm, k_norm, out)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or any(
+            t is not None and t.requires_grad for t in (cos, sin, q_norm, k_norm, out))):
+        _records("paged_append")
+    dtype = k_cache.dtype
     tables, lengths, starts, sequences, width = _batch("paged_append", tables, lengths, starts)
-    q, q_stride = _rows("paged_append", "q", q, dtype)
-    k, k_stride = _rows("paged_append", "k", k, dtype)
-    v, v_stride = _rows("paged_append", "v", v, dtype)
-    tokens = q.shape[0]
-    heads = q.shape[1] // head_dim
-    if q.shape[1] != heads * head_dim or k.shape != (tokens, kv_heads * head_dim) or v.shape != k.shape:
+    q, q_stride, tokens, columns = _rows("paged_append", "q", q, dtype)
+    k, k_stride, k_rows, k_columns = _rows("paged_append", "k", k, dtype)
+    v, v_stride, v_rows, v_columns = _rows("paged_append", "v", v, dtype)
+    heads = columns // head_dim
+    if columns != heads * head_dim or not k_columns == v_columns == kv_heads * head_dim or not k_rows == v_rows == tokens:
         raise LinnetError(f"paged_append: q is [tokens, heads*{head_dim}], k and v [tokens, {kv_heads * head_dim}], got "
                           f"{list(q.shape)}, {list(k.shape)} and {list(v.shape)}")
     table = half = 0
-    if cos is None or sin is None:
-        if cos is not sin:
-            raise LinnetError("paged_append: cos and sin come together")
-    else:
-        if cos.dim() != 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape:
+    at_cos = at_sin = at_positions = at_q_norm = at_k_norm = None
+    if cos is not None and sin is not None:
+        if cos.dtype is not _FLOAT32 or sin.dtype is not _FLOAT32 or cos.dim() != 2 or cos.shape != sin.shape:
             raise LinnetError(f"paged_append: cos and sin are [positions, half] float32, got {list(cos.shape)} {cos.dtype} and "
                               f"{list(sin.shape)} {sin.dtype}")
         table, half = cos.shape
         if half == 0 or half % 8 or 2 * half > head_dim:
             raise LinnetError(f"paged_append: tables of {half} angles (a multiple of 8, at most {head_dim // 2})")
         cos, sin = _aligned(cos), _aligned(sin)
+        at_cos, at_sin = cos.data_ptr(), sin.data_ptr()
+    elif cos is not sin:
+        raise LinnetError("paged_append: cos and sin come together")
     if positions is not None:
-        positions = _ints("paged_append", "positions", positions, (tokens,))
-    norms = []
-    for norm in (q_norm, k_norm):
-        if norm is not None:
-            if norm.dtype != torch.float32 or norm.shape != (head_dim,):
-                raise LinnetError(f"paged_append: norms are [{head_dim}] float32, got {list(norm.shape)} {norm.dtype}")
-            norm = _aligned(norm)
-        norms.append(norm)
+        positions = _ints("paged_append", "positions", positions, tokens)
+        at_positions = positions.data_ptr()
+    if q_norm is not None:
+        q_norm = _floats("paged_append", "q_norm", q_norm, head_dim)
+        at_q_norm = q_norm.data_ptr()
+    if k_norm is not None:
+        k_norm = _floats("paged_append", "k_norm", k_norm, head_dim)
+        at_k_norm = k_norm.data_ptr()
     fill = out is None
-    out = _out("paged_append", out, q, heads * head_dim)
-    _launch(device, "lnq_paged_append", q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride,
-            None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), table, half,
-            None if positions is None else positions.data_ptr(), None if norms[0] is None else norms[0].data_ptr(),
-            None if norms[1] is None else norms[1].data_ptr(), float(eps), out.data_ptr(), heads * head_dim, fill,
-            cache.k.data_ptr(), cache.v.data_ptr(), tables.data_ptr(), lengths.data_ptr(), starts.data_ptr(), sequences, width,
-            pages, page, tokens, heads, kv_heads, head_dim, code)
+    if fill:
+        out = q.new_empty((tokens, columns))
+    else:
+        out = _out("paged_append", out, tokens, columns, dtype)
+    _launch(device, "lnq_paged_append", q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, at_cos, at_sin, table,
+            half, at_positions, at_q_norm, at_k_norm, eps, out.data_ptr(), columns, fill, k_cache.data_ptr(), v_cache.data_ptr(),
+            tables.data_ptr(), lengths.data_ptr(), starts.data_ptr(), sequences, width, pages, page, tokens, heads, kv_heads, head_dim,
+            code)
     return out
 
 
@@ -201,37 +211,45 @@ def _attend(what: str, q: torch.Tensor, cache: PagedCache, tables: torch.Tensor,
             parents: torch.Tensor | None, max_queries: int | None, scale: float | None, window: int | None,
             sinks: torch.Tensor | None, out: torch.Tensor | None) -> torch.Tensor:
     pages, page, kv_heads, head_dim, code, _ = _one_layer(what, cache)
-    device = _on_gpu(what, q, cache.k, tables, lengths, starts, parents, sinks, out)
-    _no_gradient(what, q, cache.k, cache.v, sinks, out)
+    k_cache = cache.k
+    device = _on_gpu(what, q, k_cache, tables, lengths, starts, parents, sinks, out)
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or cache.v.requires_grad or any(
+            t is not None and t.requires_grad for t in (sinks, out))):
+        _records(what)
+    dtype = k_cache.dtype
     tables, lengths, starts, sequences, width = _batch(what, tables, lengths, starts)
-    q, q_stride = _rows(what, "q", q, cache.k.dtype)
-    tokens, columns = q.shape
+    q, q_stride, tokens, columns = _rows(what, "q", q, dtype)
     heads = columns // head_dim
     if heads == 0 or columns != heads * head_dim or heads % kv_heads:
         raise LinnetError(f"{what}: q is [tokens, heads*{head_dim}], heads a multiple of {kv_heads}, got {list(q.shape)}")
     most = tokens if max_queries is None else int(max_queries)
     if most < 1 and tokens > 0:
         raise LinnetError(f"{what}: max_queries of {most}")
+    at_parents = at_sinks = at_work = None
     if parents is not None:
-        parents = _ints(what, "parents", parents, (tokens,))
+        parents = _ints(what, "parents", parents, tokens)
+        at_parents = parents.data_ptr()
     if sinks is not None:
-        if sinks.dtype != torch.float32 or sinks.shape != (heads,):
-            raise LinnetError(f"{what}: sinks is [{heads}] float32, got {list(sinks.shape)} {sinks.dtype}")
-        sinks = sinks.contiguous()
+        sinks = _floats(what, "sinks", sinks, heads)
+        at_sinks = sinks.data_ptr()
     scale = head_dim**-0.5 if scale is None else float(scale)
     if not 1e-30 <= scale <= 1e30:
         raise LinnetError(f"{what}: the scale is a positive number, not {scale}")
-    window = 0 if window is None else int(window)
+    window = int(window) if window else 0
     fill = out is None
-    out = _out(what, out, q, columns)
+    if fill:
+        out = q.new_empty((tokens, columns))
+    else:
+        out = _out(what, out, tokens, columns, dtype)
     if tokens == 0:
         return out
     floats = _workspace(sequences, width, page, tokens, heads, kv_heads, head_dim, most, window)
-    work = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
-    _launch(device, "lnq_paged_attention", q.data_ptr(), q_stride, cache.k.data_ptr(), cache.v.data_ptr(), out.data_ptr(), columns,
-            fill, tables.data_ptr(), lengths.data_ptr(), starts.data_ptr(), None if parents is None else parents.data_ptr(),
-            None if sinks is None else sinks.data_ptr(), None if work is None else work.data_ptr(), floats, sequences, width, pages,
-            page, tokens, heads, kv_heads, head_dim, most, window, scale, code)
+    if floats:
+        work = q.new_empty((floats,), dtype=_FLOAT32)
+        at_work = work.data_ptr()
+    _launch(device, "lnq_paged_attention", q.data_ptr(), q_stride, k_cache.data_ptr(), cache.v.data_ptr(), out.data_ptr(), columns,
+            fill, tables.data_ptr(), lengths.data_ptr(), starts.data_ptr(), at_parents, at_sinks, at_work, floats, sequences, width,
+            pages, page, tokens, heads, kv_heads, head_dim, most, window, scale, code)
     return out
 
 
@@ -275,7 +293,9 @@ def paged_keep(cache: PagedCache, tables: torch.Tensor, lengths: torch.Tensor, s
     tables, lengths, starts, sequences, width = _batch("paged_keep", tables, lengths, starts)
     if kept.dim() != 2:
         raise LinnetError(f"paged_keep: kept is [sequences, path] int32, got {list(kept.shape)}")
-    kept = _ints("paged_keep", "kept", kept, (sequences, kept.shape[1]))
+    if kept.dtype is not _INT32 or kept.shape[0] != sequences:
+        raise LinnetError(f"paged_keep: kept is [{sequences}, path] int32, got {list(kept.shape)} {kept.dtype}")
+    kept = kept if kept.is_contiguous() else kept.contiguous()
     new = torch.empty_like(lengths)
     if sequences == 0:
         return new

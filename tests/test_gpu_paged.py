@@ -585,7 +585,7 @@ def test_refusals() -> None:
     refused(paged.paged_append, *but(append, 8, lengths), match="starts")
     refused(paged.paged_append, *but(append, 6, tables.long()), match="tables")
     refused(paged.paged_append, *append, positions=lengths, match="positions")
-    refused(paged.paged_append, *append, q_norm=torch.ones(64, device=DEV, dtype=BF16), match="norms")
+    refused(paged.paged_append, *append, q_norm=torch.ones(64, device=DEV, dtype=BF16), match="q_norm")
     refused(paged.paged_append, *append, out=q[:1], match="out")
     refused(paged.paged_append, *but(append, 0, q.cpu()), match="GPU tensors")
     refused(paged.paged_append, *but(append, 5, paged.PagedCache.empty(2, 2, 64, 16, layers=2)), match="one layer")
