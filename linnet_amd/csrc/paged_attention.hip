@@ -621,8 +621,11 @@ __device__ inline int many_slot(const AttendArgs& a, int s) {
   return static_cast<int>(static_cast<int64_t>(clamp_to(a.batch.starts[s], 0, a.batch.tokens)) * a.group / MANY) + s;
 }
 
-// The many-row way, for the tiles of `slots` slots; past their workgroups, the sequences of few rows.
-template <int DT, int HD, bool TREE>
+// The many-row way, for the tiles of `slots` slots; past their workgroups, the sequences of few rows. WIDE:
+// pages of 64 entries and more, a tile of entries in one of them, its addresses scalar ones. (A vector
+// instruction costs a wave's matrix unit half its own time; those of a step that only find addresses are
+// a tenth of it.)
+template <int DT, int HD, bool TREE, bool WIDE>
 __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int slots) {
   using R = Rows<DT, HD, 32>;
   constexpr int CH = HD / 8, QK = R::QK, DV = R::DV;
@@ -682,31 +685,39 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   auto page_at = [&](int t) __attribute__((always_inline)) -> int { return table[min(t + lane, end - 1) >> b.page_bits]; };
   auto good = [&](int page) __attribute__((always_inline)) -> bool { return page >= 0 && page < b.pages; };
   struct Source {
-    const uint16_t* k;  // this lane's entry, dimensions 0 .. 7
-    int page;           // of this lane's entry
+    const uint16_t* k;  // dimensions 0 .. 7 of the tile's first entry, or with !WIDE of this lane's
+    int page;           // of the tile, or of this lane's entry
     int t;
   };
   auto source_of = [&](int id, int t) __attribute__((always_inline)) -> Source {
+    if constexpr (WIDE) id = __builtin_amdgcn_readfirstlane(id);
     const int page = good(id) ? id : 0;
     const int64_t kp = static_cast<int64_t>(page) * a.kv_heads + h;
-    return Source{a.k_cache + ((kp * CH << b.page_bits) + ((t + lane) & mask)) * 8, page, t};
+    return Source{a.k_cache + ((kp * CH << b.page_bits) + ((WIDE ? t : t + lane) & mask)) * 8, page, t};
   };
-  auto to_lds = [&](const uint16_t* from, u32x4* to) __attribute__((always_inline)) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+  auto to_lds = [&](const uint16_t* from, int at, u32x4* to) __attribute__((always_inline)) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(reinterpret_cast<const char*>(from) + static_cast<uint32_t>(at)),
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
   };
   // Load i of this wave's LOADS of a tile.
   constexpr int K_LOADS = CH / 4, LOADS = 2 * K_LOADS;
   auto load_one = [&](const Source& x, u32x4* to, int i) __attribute__((always_inline)) {
     if (i < K_LOADS) {
       const int c = wave * K_LOADS + i;
-      to_lds(x.k + (static_cast<int64_t>(c) << b.page_bits) * 8, to + c * 64);
+      to_lds(x.k + (static_cast<int64_t>(c) << b.page_bits) * 8, WIDE ? lane * 16 : 0, to + c * 64);
     } else {
       const int part = wave * K_LOADS + i - K_LOADS;
       const int e8 = part / (HD / 64), d = part % (HD / 64);  // the eight entries 8 e8 .., 64 dimensions
-      const int64_t vp = static_cast<int64_t>(__builtin_amdgcn_readlane(x.page, 8 * e8)) * a.kv_heads + h;
-      to_lds(a.v_cache + (((vp << (b.page_bits - 3)) + (((x.t + 8 * e8) & mask) >> 3)) * HD + 64 * d + lane) * 8,
+      const int64_t vp = static_cast<int64_t>(WIDE ? x.page : __builtin_amdgcn_readlane(x.page, 8 * e8)) * a.kv_heads + h;
+      to_lds(a.v_cache + (((vp << (b.page_bits - 3)) + (((x.t + 8 * e8) & mask) >> 3)) * HD + 64 * d) * 8, lane * 16,
              to + UNITS + e8 * HD + 64 * d);
     }
+  };
+  // The entries of the tile at t that are there.
+  auto there_of = [&](int id, int t) __attribute__((always_inline)) -> uint64_t {
+    if constexpr (!WIDE) return __ballot(t + lane < limit && good(id));
+    const int many = limit - t;
+    return !good(__builtin_amdgcn_readfirstlane(id)) || many <= 0 ? 0 : many >= 64 ? ~0ull : (1ull << many) - 1;
   };
 
   const int entry = entry_of<32>(0, col);
@@ -721,7 +732,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   loads_done();
   lds_barrier();
   auto step = [&](int t, u32x4* cur, u32x4* other) __attribute__((always_inline)) {
-    const uint64_t valid = __ballot(t + lane < limit && good(id));
+    const uint64_t valid = there_of(id, t);
     id = next;
     next = page_at(t + 2 * MANY_STEP);
     const Source source = source_of(id, t + MANY_STEP);
@@ -833,89 +844,159 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   }
 }
 
-// Parts added in order: a row of one head to a wave, or with many splits to a workgroup (WIDE), whose waves
-// take the splits in turn. First the few-row sequences' rows (their i-th new tokens), then the batch's tokens.
-template <int DT, int HD, bool WIDE>
-__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a, int64_t small_rows, int64_t rows) {
-  constexpr int WAVES = WIDE ? 4 : 1;  // of a row
-  constexpr int D = HD / 64;           // dimensions a lane
-  constexpr int AHEAD = 8;             // splits loaded together
-  __shared__ float weight[WIDE ? MAX_SPLITS : 4 * 64];
-  __shared__ float sums[WIDE ? 3 : 1][HD];
-  const Batch& b = a.batch;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t at_row = WIDE ? blockIdx.x : blockIdx.x * int64_t{4} + wave;
-  if (at_row >= rows) return;
-  const bool small = at_row < small_rows;
-  const Parts& part = small ? a.small : a.large;
-  const int64_t local = small ? at_row : at_row - small_rows;
-  const int head = static_cast<int>(local % a.heads), rest = static_cast<int>(local / a.heads);
-  int s, i;
+// A token whose rows may be in parts: of `small` the i-th new one of a few-row sequence, else one of the batch;
+// n == 0 where it is none.
+struct Joined {
   Sequence q;
-  if (small) {
-    s = rest / a.few_tokens;
-    q = sequence_of(b, s);
-    i = rest % a.few_tokens;
-    if (i >= q.n || q.n > a.few_tokens || (static_cast<int64_t>(q.n) * a.group > a.few && !a.every)) return;
-  } else {
-    s = find_sequence(b.sequences, rest, [&](int n) { return clamp_to(b.starts[n], 0, b.tokens); });
-    q = sequence_of(b, s);
-    i = rest - q.first;
-    if (i < 0 || i >= q.n || static_cast<int64_t>(q.n) * a.group <= a.few) return;
-  }
-  // The tile that the row was computed in.
+  int s, i;
+};
+
+__device__ inline Joined joined_of(const AttendArgs& a, bool small, int at) {
+  const Batch& b = a.batch;
+  Joined j;
+  j.s = small ? at / a.few_tokens : find_sequence(b.sequences, at, [&](int n) { return clamp_to(b.starts[n], 0, b.tokens); });
+  j.q = sequence_of(b, j.s);
+  j.i = small ? at % a.few_tokens : at - j.q.first;
+  const bool few = static_cast<int64_t>(j.q.n) * a.group <= a.few || a.every;
+  if (j.i < 0 || j.i >= j.q.n || few != small || (small && j.q.n > a.few_tokens)) j.q.n = 0;
+  return j;
+}
+
+// The parts of head `head` of it, as its tile was computed.
+__device__ inline Range parts_of(const AttendArgs& a, bool small, const Joined& j, int head) {
   const int per = small ? a.few_tile : MANY;
-  const int64_t all = static_cast<int64_t>(q.n) * a.group;
-  const int64_t r0 = (static_cast<int64_t>(i) * a.group + head % a.group) / per * per;
-  const int i0 = static_cast<int>(r0 / a.group), i1 = static_cast<int>((min(r0 + per, all) - 1) / a.group);
-  const Range range = range_of(a, q, i0, i1, part.splits, small ? FEW_STEP : MANY_STEP);
-  if (range.used == 1) return;
-  const int64_t at = part_row(a, small, s, q, i, head);
-  float* const weights = WIDE ? weight : weight + 64 * wave;
+  const int64_t rows = static_cast<int64_t>(j.q.n) * a.group;
+  const int64_t r0 = (static_cast<int64_t>(j.i) * a.group + head % a.group) / per * per;
+  return range_of(a, j.q, static_cast<int>(r0 / a.group), static_cast<int>((min(r0 + per, rows) - 1) / a.group),
+                  small ? a.small.splits : a.large.splits, small ? FEW_STEP : MANY_STEP);
+}
+
+// The parts of rows added in order: HEADS (1 or 4) heads of a token to a wave, up to 64 / HEADS parts of each. Lane
+// PARTS r + c has part c of head r's maximum and sum; then every lane adds its dimensions of all.
+template <int DT, int HD, int HEADS>
+__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a, int64_t small_tokens, int64_t tokens) {
+  constexpr int PARTS = 64 / HEADS;
+  constexpr int D = HD / 64;         // dimensions a lane
+  constexpr int AHEAD = 16 / HEADS;  // parts of a head loaded together
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int blocks = (a.heads + HEADS - 1) / HEADS;
+  const int64_t at_block = blockIdx.x * int64_t{4} + wave;
+  if (at_block >= tokens * blocks) return;
+  const int64_t token = at_block / blocks;
+  const bool small = token < small_tokens;
+  const Parts& part = small ? a.small : a.large;
+  const Joined j = joined_of(a, small, static_cast<int>(small ? token : token - small_tokens));
+  if (j.q.n == 0) return;
+  const int head0 = static_cast<int>(at_block % blocks) * HEADS;
+  const int head = head0 + lane / PARTS, c = lane % PARTS;
+  const int used = head < a.heads ? parts_of(a, small, j, head).used : 1;
+  const int most = static_cast<int>(wave_max(static_cast<float>(used)));
+  if (most == 1) return;
+  const int64_t at0 = part_row(a, small, j.s, j.q, j.i, head0);
+  float m = -INFINITY, l = 0.f;
+  if (head < a.heads && c < used && used > 1) {
+    const float* const st = part.stats + 2 * (c * part.rows + at0 + lane / PARTS);
+    m = st[0], l = st[1];
+  }
+  float top = m;
+#pragma unroll
+  for (int off = 1; off < PARTS; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  const float w = c >= used ? 0.f : m == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - top);
+  l *= w;
+#pragma unroll
+  for (int off = 1; off < PARTS; off <<= 1) l += __shfl_xor(l, off, 64);
+  const float n = norm_of(top, l, a.sinks, min(head, a.heads - 1));
+  float o[HEADS][D] = {};
+  for (int c0 = 0; c0 < most; c0 += AHEAD) {
+    float x[HEADS][AHEAD][D];
+#pragma unroll
+    for (int r = 0; r < HEADS; ++r)
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        // (Past the last part or head: read again, and not used.)
+        const int64_t at = at0 + min(r, a.heads - 1 - head0) + min(c0 + e, most - 1) * part.rows;
+#pragma unroll
+        for (int d = 0; d < D; ++d) x[r][e][d] = part.sums[at * HD + lane * D + d];
+      }
+#pragma unroll
+    for (int r = 0; r < HEADS; ++r)
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        const int lane_of = PARTS * r + min(c0 + e, PARTS - 1);
+        const float by = c0 + e < most ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), lane_of)) : 0.f;
+#pragma unroll
+        for (int d = 0; d < D; ++d) o[r][d] += by == 0.f ? 0.f : by * x[r][e][d];
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < HEADS; ++r) {
+    if (head0 + r >= a.heads || __builtin_amdgcn_readlane(used, PARTS * r) == 1) continue;
+    const float by = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, n), PARTS * r));
+    uint16_t* const to = a.out + (j.q.first + j.i) * a.out_stride + static_cast<int64_t>(head0 + r) * HD + lane * D;
+    if constexpr (D == 2) *reinterpret_cast<uint32_t*>(to) = pack2<DT>(o[r][0] * by, o[r][D - 1] * by);
+    else *to = static_cast<uint16_t>(pack2<DT>(o[r][0] * by, 0.f));
+  }
+}
+
+// The same of any number of parts: a row to a workgroup, whose waves take the parts in turn.
+template <int DT, int HD>
+__global__ __launch_bounds__(256) void paged_join_wide_kernel(AttendArgs a, int64_t small_tokens, int64_t tokens) {
+  constexpr int D = HD / 64, AHEAD = 8;
+  __shared__ float weights[MAX_SPLITS];
+  __shared__ float sums[3][HD];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t token = blockIdx.x / a.heads;
+  const int head = blockIdx.x % a.heads;
+  if (token >= tokens) return;
+  const bool small = token < small_tokens;
+  const Parts& part = small ? a.small : a.large;
+  const Joined j = joined_of(a, small, static_cast<int>(small ? token : token - small_tokens));
+  if (j.q.n == 0) return;
+  const int used = parts_of(a, small, j, head).used;
+  if (used == 1) return;
+  const int64_t at = part_row(a, small, j.s, j.q, j.i, head);
   float m = -INFINITY;
-  for (int c = lane; c < range.used; c += 64) m = fmaxf(m, part.stats[2 * (c * part.rows + at)]);
+  for (int c = lane; c < used; c += 64) m = fmaxf(m, part.stats[2 * (c * part.rows + at)]);
   m = wave_max(m);
   float l = 0.f;
-  for (int c = lane; c < range.used; c += 64) {
+  for (int c = lane; c < used; c += 64) {
     const float mc = part.stats[2 * (c * part.rows + at)];
     const float w = mc == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mc - m);
     l = fmaf(part.stats[2 * (c * part.rows + at) + 1], w, l);
-    if (!WIDE || wave == 0) weights[c] = w;
+    if (wave == 0) weights[c] = w;
   }
   l = wave_sum(l);
-  if constexpr (WIDE) __syncthreads();
+  __syncthreads();
   const float* const from = part.sums + at * HD + lane * D;
   float o[D] = {};
-  for (int c0 = WIDE ? wave : 0; c0 < range.used; c0 += WAVES * AHEAD) {
+  for (int c0 = wave; c0 < used; c0 += 4 * AHEAD) {
     float x[AHEAD][D];
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) {
-      const int c = min(c0 + WAVES * n, range.used - 1);  // (past the last: read again, and not used)
+      const int c = min(c0 + 4 * n, used - 1);  // (past the last: read again, and not used)
 #pragma unroll
       for (int d = 0; d < D; ++d) x[n][d] = from[c * part.rows * HD + d];
     }
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) {
-      const int c = c0 + WAVES * n;
-      const float w = c < range.used ? weights[c] : 0.f;
+      const int c = c0 + 4 * n;
+      const float w = c < used ? weights[c] : 0.f;
 #pragma unroll
       for (int d = 0; d < D; ++d) o[d] += w == 0.f ? 0.f : w * x[n][d];
     }
   }
-  if constexpr (WIDE) {
-    if (wave > 0) {
+  if (wave > 0) {
 #pragma unroll
-      for (int d = 0; d < D; ++d) sums[wave - 1][lane * D + d] = o[d];
-    }
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int n = 0; n < 3; ++n)
-#pragma unroll
-      for (int d = 0; d < D; ++d) o[d] += sums[n][lane * D + d];
+    for (int d = 0; d < D; ++d) sums[wave - 1][lane * D + d] = o[d];
   }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int n = 0; n < 3; ++n)
+#pragma unroll
+    for (int d = 0; d < D; ++d) o[d] += sums[n][lane * D + d];
   const float n = norm_of(m, l, a.sinks, head);
-  uint16_t* const to = a.out + (q.first + i) * a.out_stride + static_cast<int64_t>(head) * HD + lane * D;
+  uint16_t* const to = a.out + (j.q.first + j.i) * a.out_stride + static_cast<int64_t>(head) * HD + lane * D;
   if constexpr (D == 2) *reinterpret_cast<uint32_t*>(to) = pack2<DT>(o[0] * n, o[D - 1] * n);
   else *to = static_cast<uint16_t>(pack2<DT>(o[0] * n, 0.f));
 }
@@ -952,9 +1033,12 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
     return v < 1 ? int64_t{1} : v;
   };
   {
+    // As many workgroups as the chip holds at once (3 a CU at head_dim 64, 2 at 128), and none of much over 1024
+    // entries where lengths differ. One row of 131000 entries at head_dim 64: 57.0 us with 768 workgroups, 59.9 with
+    // 512 or 1024, 62.3 with 2048; 64 rows of 230000 at 128: 180.6 with parts of 1024, 183.4 of 2048, 184.5 of 512.
     const int64_t base = sequences * kv_heads;
-    int64_t want = up_to(1024, base > 0 ? base : 1);
-    if (want < up_to(seen, 2048)) want = up_to(seen, 2048);
+    int64_t want = up_to(head_dim == 64 ? 768 : 512, base > 0 ? base : 1);
+    if (want < up_to(seen, 1024)) want = up_to(seen, 1024);
     const int64_t top = up_to(seen, FEW_STEP);
     p.few_splits = bounded(want, top < MAX_SPLITS ? top : MAX_SPLITS);
   }
@@ -963,8 +1047,10 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
   if (p.many) {
     p.slots = tokens * group / MANY + sequences;
     const int64_t base = p.slots * kv_heads;
-    const int64_t top = up_to(seen, 256);
-    p.many_splits = bounded(up_to(512, base > 0 ? base : 1), top < 64 ? top : 64);
+    // Twice what the chip holds at once, as the tiles differ: 16 trees of 900 nodes 131 us with 1024 (or 768), 149 with 512;
+    // one of 24 over 1000 entries 14.5 with parts of 64 entries, 17.0 of 256.
+    const int64_t top = up_to(seen, MANY_STEP);
+    p.many_splits = bounded(up_to(1024, base > 0 ? base : 1), top < 64 ? top : 64);
   }
   p.few_rows = p.few_splits > 1 ? sequences * p.few_tokens * heads : 0;
   p.many_rows = p.many_splits > 1 ? tokens * heads : 0;
@@ -986,19 +1072,27 @@ static LnqStatus attend(AttendArgs a, const Plan& p, float* work, hipStream_t st
   const int64_t few = (sequences + (a.fill ? 1 : 0)) * a.kv_heads * p.few_splits;
   if (p.many) {
     const int64_t tiles = p.slots * a.kv_heads * p.many_splits;
-    if (tiles + few > 0)
-      hipLaunchKernelGGL((paged_many_kernel<DT, HD, TREE>), dim3(static_cast<unsigned>(tiles + few)), block, 0, st, a, static_cast<int>(p.slots));
+    const dim3 grid(static_cast<unsigned>(tiles + few));
+    if (tiles + few > 0 && a.batch.page_bits >= 6)
+      hipLaunchKernelGGL((paged_many_kernel<DT, HD, TREE, true>), grid, block, 0, st, a, static_cast<int>(p.slots));
+    else if (tiles + few > 0)
+      hipLaunchKernelGGL((paged_many_kernel<DT, HD, TREE, false>), grid, block, 0, st, a, static_cast<int>(p.slots));
   } else if (few > 0) {
     const dim3 grid(static_cast<unsigned>(few));
     if (p.few_tile == 16) hipLaunchKernelGGL((paged_few_kernel<DT, HD, 16, TREE>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((paged_few_kernel<DT, HD, 32, TREE>), grid, block, 0, st, a);
   }
-  const int64_t rows = p.few_rows + p.many_rows;
-  if (rows > 0) {
-    if (p.few_splits > 16 || p.many_splits > 16)
-      hipLaunchKernelGGL((paged_join_kernel<DT, HD, true>), dim3(static_cast<unsigned>(rows)), block, 0, st, a, p.few_rows, rows);
+  const int64_t small = p.few_splits > 1 ? sequences * p.few_tokens : 0, joined = small + (p.many_splits > 1 ? a.batch.tokens : 0);
+  if (joined > 0) {
+    const int64_t parts = p.few_splits > p.many_splits ? p.few_splits : p.many_splits, rows = joined * a.heads;
+    // 28800 rows of 3 parts: 13 us at four heads a wave, 30 at a row a wave, 75 at a row a workgroup; 768 of 16: 6.9, 4.2 and
+    // 7.2; 32 of 8: 4.6, 4.9 at a row a wave, 4.6.
+    if (rows > 2048 && parts <= 16)
+      hipLaunchKernelGGL((paged_join_kernel<DT, HD, 4>), dim3(static_cast<unsigned>(up_to(joined * up_to(a.heads, 4), 4))), block, 0, st, a, small, joined);
+    else if (rows > 256 && parts <= 64)
+      hipLaunchKernelGGL((paged_join_kernel<DT, HD, 1>), dim3(static_cast<unsigned>(up_to(rows, 4))), block, 0, st, a, small, joined);
     else
-      hipLaunchKernelGGL((paged_join_kernel<DT, HD, false>), dim3(static_cast<unsigned>(up_to(rows, 4))), block, 0, st, a, p.few_rows, rows);
+      hipLaunchKernelGGL((paged_join_wide_kernel<DT, HD>), dim3(static_cast<unsigned>(rows)), block, 0, st, a, small, joined);
   }
   return launched("paged_attention");
 }
