@@ -64,32 +64,32 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
   const Sequence q = sequence_of(b, s);
   const int e0 = ((q.base >> 3) + local) * UNIT;  // the unit's first entry (base may be negative)
   if (e0 >= q.length || q.n == 0) return;
-  const int page = page_of(b, s, e0);  // of the whole unit: pages hold whole units
+  // The page of the whole unit (pages hold whole units): its id is read here and looked at where it is used,
+  // so that the loads below need not wait for it.
+  const bool listed = e0 >= 0 && e0 < capacity(b);
+  int id = -1;
+  if (listed) id = b.tables[static_cast<int64_t>(s) * b.width + (e0 >> b.page_bits)];
   const int place = e0 & ((1 << b.page_bits) - 1);
-
-  // Whether entry e0 + j is a new token whose position has a row of the tables.
+  // The token of entry e0 + j (the nearest one where that is none), and its position if it has a row of the tables.
+  auto token = [&](int j) { return q.first + clamp_to(e0 + j - q.base, 0, q.n - 1); };
+  auto is_new = [&](int j) { return e0 + j >= q.base && e0 + j < q.length; };
   auto position = [&](int j) -> int {
-    const int i = e0 + j - q.base;
-    if (i < 0 || i >= q.n) return -1;
-    const int p = a.positions != nullptr ? a.positions[q.first + i] : e0 + j;
+    if (!is_new(j)) return -1;
+    const int p = a.positions != nullptr ? a.positions[token(j)] : e0 + j;
     return a.half == 0 ? max(p, 0) : p < a.table ? p : -1;
   };
 
   if (head >= a.heads + a.kv_heads) {
-    if (page < 0) return;
     const int h = head - a.heads - a.kv_heads;
     if (2 * lane >= HD) return;
     uint32_t x[UNIT];
     uint32_t there = 0;
 #pragma unroll
-    for (int j = 0; j < UNIT; ++j) {
-      x[j] = 0;
-      if (position(j) >= 0) {
-        there |= 1u << j;
-        x[j] = *reinterpret_cast<const uint32_t*>(a.v + (q.first + e0 + j - q.base) * a.v_stride + h * HD + 2 * lane);
-      }
-    }
-    uint16_t* const to = a.v_cache + ((static_cast<int64_t>(page) * a.kv_heads + h) << b.page_bits) * HD + static_cast<int64_t>(place) * HD +
+    for (int j = 0; j < UNIT; ++j) x[j] = *reinterpret_cast<const uint32_t*>(a.v + token(j) * a.v_stride + h * HD + 2 * lane);
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) there |= position(j) >= 0 ? 1u << j : 0u;
+    if (id < 0 || id >= b.pages) return;
+    uint16_t* const to = a.v_cache + ((static_cast<int64_t>(id) * a.kv_heads + h) << b.page_bits) * HD + static_cast<int64_t>(place) * HD +
                          16 * lane;
     if (there == 0xffu) {
       u32x4 lo, hi;
@@ -111,34 +111,53 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
     return;
   }
 
+  constexpr int ROUNDS = UNIT / TOKENS;  // tokens a lane takes
   const bool is_q = head < a.heads;
   const int h = is_q ? head : head - a.heads;
   const uint16_t* const src = is_q ? a.q : a.k;
   const int64_t stride = is_q ? a.q_stride : a.k_stride;
   const float* const norm = is_q ? a.q_norm : a.k_norm;
   const int c = lane % CH;
-  f32x4 w0 = {1.f, 1.f, 1.f, 1.f}, w1 = w0;
-  if (norm != nullptr) {
-    w0 = *reinterpret_cast<const f32x4*>(norm + 8 * c);
-    w1 = *reinterpret_cast<const f32x4*>(norm + 8 * c + 4);
-  }
   // The lane with the other dimension of this one's pairs, and the pairs' first angle.
   const int turn = a.half / 8;
   const bool first_half = c < turn, turned = c < 2 * turn;
   const int other = (lane & ~(CH - 1)) | (first_half ? c + turn : turned ? c - turn : c);
-  const int angle = 8 * (first_half ? c : c - turn);
+  const int angle = turned ? 8 * (first_half ? c : c - turn) : 0;
+  // Every load before any of them is used (a row that is not there: one that is, and not used).
+  u32x4 raw[ROUNDS];
+  f32x4 cs[ROUNDS][2], sn[ROUNDS][2];
+  int at[ROUNDS];
 #pragma unroll
-  for (int it = 0; it < UNIT / TOKENS; ++it) {
-    const int j = it * TOKENS + lane / CH;
-    const int i = e0 + j - q.base, p = position(j);
-    const bool mine = i >= 0 && i < q.n;
-    u32x4 raw = {0u, 0u, 0u, 0u};
-    if (p >= 0) raw = *reinterpret_cast<const u32x4*>(src + (q.first + i) * stride + h * HD + 8 * c);
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int j = r * TOKENS + lane / CH;
+    at[r] = position(j);
+    raw[r] = *reinterpret_cast<const u32x4*>(src + token(j) * stride + h * HD + 8 * c);
+  }
+  if (a.half > 0 && a.table > 0) {
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int64_t row = static_cast<int64_t>(max(at[r], 0)) * a.half + angle;
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        cs[r][d] = *reinterpret_cast<const f32x4*>(a.cos + row + 4 * d);
+        sn[r][d] = *reinterpret_cast<const f32x4*>(a.sin + row + 4 * d);
+      }
+    }
+  }
+  f32x4 w[2] = {{1.f, 1.f, 1.f, 1.f}, {1.f, 1.f, 1.f, 1.f}};
+  if (norm != nullptr) {
+    w[0] = *reinterpret_cast<const f32x4*>(norm + 8 * c);
+    w[1] = *reinterpret_cast<const f32x4*>(norm + 8 * c + 4);
+  }
+  const bool stored = id >= 0 && id < b.pages;
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int j = r * TOKENS + lane / CH;
     float x[8];
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      x[2 * d] = E::to_f32(static_cast<uint16_t>(raw[d] & 0xffffu));
-      x[2 * d + 1] = E::to_f32(static_cast<uint16_t>(raw[d] >> 16));
+      x[2 * d] = E::to_f32(static_cast<uint16_t>(raw[r][d] & 0xffffu));
+      x[2 * d + 1] = E::to_f32(static_cast<uint16_t>(raw[r][d] >> 16));
     }
     if (norm != nullptr) {
       float sum = chunk_squares(x);
@@ -146,23 +165,16 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
       for (int off = 1; off < CH; off <<= 1) sum += __shfl_xor(sum, off, 64);
       const float by = rsqrtf(sum / static_cast<float>(HD) + a.eps);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        x[d] = x[d] * by * w0[d];
-        x[4 + d] = x[4 + d] * by * w1[d];
-      }
+      for (int d = 0; d < 8; ++d) x[d] = x[d] * by * w[d / 4][d % 4];
     }
     if (a.half > 0) {
       float y[8];
 #pragma unroll
       for (int d = 0; d < 8; ++d) y[d] = __shfl(x[d], other, 64);
-      if (turned && p >= 0) {
-        const float* const cp = a.cos + static_cast<int64_t>(p) * a.half + angle;
-        const float* const sp = a.sin + static_cast<int64_t>(p) * a.half + angle;
-        const f32x4 c0 = *reinterpret_cast<const f32x4*>(cp), c1 = *reinterpret_cast<const f32x4*>(cp + 4);
-        const f32x4 s0 = *reinterpret_cast<const f32x4*>(sp), s1 = *reinterpret_cast<const f32x4*>(sp + 4);
+      if (turned) {
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-          const float cv = d < 4 ? c0[d & 3] : c1[d & 3], sv = d < 4 ? s0[d & 3] : s1[d & 3];
+          const float cv = cs[r][d / 4][d % 4], sv = sn[r][d / 4][d % 4];
           x[d] = first_half ? fmaf(x[d], cv, -(y[d] * sv)) : fmaf(x[d], cv, y[d] * sv);
         }
       }
@@ -173,18 +185,21 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
       out[d] = static_cast<uint32_t>(E::from_f32(x[2 * d])) | (static_cast<uint32_t>(E::from_f32(x[2 * d + 1])) << 16);
     if (is_q) {
       // (A token whose position has no row of the tables: zeros.)
-      if (mine) *reinterpret_cast<u32x4*>(a.q_out + (q.first + i) * a.q_out_stride + h * HD + 8 * c) = p >= 0 ? out : u32x4{0u, 0u, 0u, 0u};
-    } else if (p >= 0 && page >= 0) {
-      const int64_t at = (static_cast<int64_t>(page) * a.kv_heads + h) * CH + c;
-      *reinterpret_cast<u32x4*>(a.k_cache + ((at << b.page_bits) + place + j) * 8) = out;
+      if (is_new(j))
+        *reinterpret_cast<u32x4*>(a.q_out + token(j) * a.q_out_stride + h * HD + 8 * c) = at[r] >= 0 ? out : u32x4{0u, 0u, 0u, 0u};
+    } else if (at[r] >= 0 && stored) {
+      const int64_t to = (static_cast<int64_t>(id) * a.kv_heads + h) * CH + c;
+      *reinterpret_cast<u32x4*>(a.k_cache + ((to << b.page_bits) + place + j) * 8) = out;
     }
   }
 }
 
 // keep: entry base + path[j] of each sequence to base + j, in every layer's cache, for the nodes
 // path[0] < path[1] < .. of an accepted path (to the first entry that is no later node), and the
-// sequence's new length base + their number. A wave takes one KV head of one layer of one sequence, 64 chunks
-// of 16 bytes at a time; as path[j] >= j and ascends, no entry is written before it has been read.
+// sequence's new length base + their number. A wave takes one KV head of one layer of one sequence, eight
+// nodes at a time, all of them read before any is written; as path[j] >= j and ascends, none is written before
+// it has been read. Bound by lines: eight entries of a dimension share 16 bytes, so an entry's V is read
+// and written in all lines of its eight.
 struct KeepArgs {
   uint16_t *k_cache, *v_cache;
   const int32_t* kept;  // [sequences, path]
@@ -223,36 +238,52 @@ __global__ __launch_bounds__(64 * WAVES) void paged_keep_kernel(KeepArgs a) {
   uint16_t* const vc = a.v_cache + layer * a.layer_step;
   const int c = lane % CH;
   const int mask = (1 << b.page_bits) - 1;
-  for (int j0 = 0; j0 < number; j0 += TOKENS) {
-    const int j = j0 + lane / CH;
-    bool move = j < number;
-    int from = 0, to = 0, from_page = -1, to_page = -1;
-    if (move) {
+  constexpr int BATCH = 8, ROUNDS = BATCH / TOKENS;
+  for (int j0 = 0; j0 < number; j0 += BATCH) {
+    // Lane k (of each 8) has node j0 + k: its entry and place to go, in K's pages (in 16-byte pieces from dimension
+    // 0) and V's (in values), or -1 where it stays.
+    const int j = j0 + lane % BATCH;
+    int64_t from_v = -1, to_v = -1, from_k = -1, to_k = -1;
+    if (j < number) {
       const int node = path[j];
-      from = q.base + node;
-      to = q.base + j;
-      if (node != j) {
-        from_page = page_of(b, s, from);
-        to_page = page_of(b, s, to);
+      const int from = q.base + node, to = q.base + j;
+      const int from_page = node != j ? page_of(b, s, from) : -1, to_page = node != j ? page_of(b, s, to) : -1;
+      if (from_page >= 0 && to_page >= 0) {
+        const int64_t fp = static_cast<int64_t>(from_page) * a.kv_heads + h, tp = static_cast<int64_t>(to_page) * a.kv_heads + h;
+        from_k = (fp * CH << b.page_bits) + (from & mask);
+        to_k = (tp * CH << b.page_bits) + (to & mask);
+        from_v = ((fp << (b.page_bits - 3)) + ((from & mask) >> 3)) * HD * 8 + (from & 7);
+        to_v = ((tp << (b.page_bits - 3)) + ((to & mask) >> 3)) * HD * 8 + (to & 7);
       }
     }
-    move = move && from_page >= 0 && to_page >= 0;
-    if (!move) continue;
-    const int64_t from_k = (((static_cast<int64_t>(from_page) * a.kv_heads + h) * CH + c) << b.page_bits) + (from & mask);
-    const int64_t to_k = (((static_cast<int64_t>(to_page) * a.kv_heads + h) * CH + c) << b.page_bits) + (to & mask);
-    auto v_at = [&](int page, int e) {
-      const int64_t eight = ((static_cast<int64_t>(page) * a.kv_heads + h) << (b.page_bits - 3)) + ((e & mask) >> 3);
-      return (eight * HD + 8 * c) * 8 + (e & 7);
-    };
-    const uint16_t* const from_v = vc + v_at(from_page, from);
-    uint16_t* const to_v = vc + v_at(to_page, to);
-    const u32x4 kv = *reinterpret_cast<const u32x4*>(kc + from_k * 8);
-    uint16_t v[8];
+    u32x4 kv[ROUNDS];
+    int64_t k_to[ROUNDS];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) v[d] = from_v[8 * d];
-    *reinterpret_cast<u32x4*>(kc + to_k * 8) = kv;
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int lane_of = r * TOKENS + lane / CH;
+      const int64_t at = __shfl(from_k, lane_of, 64);
+      k_to[r] = __shfl(to_k, lane_of, 64);
+      kv[r] = u32x4{0u, 0u, 0u, 0u};
+      if (at >= 0) kv[r] = *reinterpret_cast<const u32x4*>(kc + (at + (static_cast<int64_t>(c) << b.page_bits)) * 8);
+    }
+    // V: a lane a dimension, so that an instruction reads eight neighbouring lines of one entry.
+    uint16_t v[BATCH][HD / 64];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) to_v[8 * d] = v[d];
+    for (int k = 0; k < BATCH; ++k) {
+      const int64_t at = __shfl(from_v, k, 64);
+#pragma unroll
+      for (int d = 0; d < HD / 64; ++d) v[k][d] = at >= 0 ? vc[at + (64 * d + lane) * 8] : uint16_t{0};
+    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+      if (k_to[r] >= 0) *reinterpret_cast<u32x4*>(kc + (k_to[r] + (static_cast<int64_t>(c) << b.page_bits)) * 8) = kv[r];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int64_t at = __shfl(to_v, k, 64);
+#pragma unroll
+      for (int d = 0; d < HD / 64; ++d)
+        if (at >= 0) vc[at + (64 * d + lane) * 8] = v[k][d];
+    }
   }
 }
 

@@ -165,6 +165,8 @@ ATTENDS = [
     ([300], [300], 3, 1, 128, 128, BF16, 70, False),
     ([257, 1], [700, 1], 40, 1, 64, 32, BF16, 0, False),
     ([100], [100], 28, 4, 128, 16, F16, 1, False),
+    ([300], [420], 7, 7, 64, 16, BF16, 0, True),
+    ([300, 20], [420, 900], 10, 1, 128, 64, F16, 0, False),
 ]
 
 
