@@ -7,8 +7,8 @@
 // written once.
 //
 // Eight entries at an aligned place of a sequence are the unit, as V's layout keeps eight entries
-// of a dimension together: one wave takes one head of one unit. Of q and k a lane holds 8
-// dimensions of a token (16 bytes; the other of a pair comes from the lane that holds it), of v a
+// of a dimension together: one wave takes one head of one unit. Of q and k a lane holds one or two times 8
+// dimensions of a token (16 bytes; the other of a pair is its own or comes from the lane that holds it), of v a
 // lane holds two dimensions of all eight tokens, so that V's 16-byte pieces come out of registers by
 // v_perm. A whole unit is written in whole lines, a partial one (a single token of a decode step)
 // by its entries alone.
@@ -111,32 +111,27 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
     return;
   }
 
-  constexpr int ROUNDS = UNIT / TOKENS;  // tokens a lane takes
+  // Lane 8 j + i takes chunks i, i + 8 of token j: K's lines (eight tokens of a chunk) are written whole, and at
+  // a head of 128 rotated dimensions a pair's two are the lane's own.
+  constexpr int ROUNDS = CH / 8;
   const bool is_q = head < a.heads;
   const int h = is_q ? head : head - a.heads;
-  const uint16_t* const src = is_q ? a.q : a.k;
+  const uint16_t* const src = (is_q ? a.q : a.k) + h * HD;
   const int64_t stride = is_q ? a.q_stride : a.k_stride;
   const float* const norm = is_q ? a.q_norm : a.k_norm;
-  const int c = lane % CH;
-  // The lane with the other dimension of this one's pairs, and the pairs' first angle.
-  const int turn = a.half / 8;
-  const bool first_half = c < turn, turned = c < 2 * turn;
-  const int other = (lane & ~(CH - 1)) | (first_half ? c + turn : turned ? c - turn : c);
-  const int angle = turned ? 8 * (first_half ? c : c - turn) : 0;
+  const int j = lane >> 3, i = lane & 7;
+  const int turn = a.half / 8;  // chunks from a pair's first dimension to its second
+  const int at = position(j);
   // Every load before any of them is used (a row that is not there: one that is, and not used).
   u32x4 raw[ROUNDS];
-  f32x4 cs[ROUNDS][2], sn[ROUNDS][2];
-  int at[ROUNDS];
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
-    const int j = r * TOKENS + lane / CH;
-    at[r] = position(j);
-    raw[r] = *reinterpret_cast<const u32x4*>(src + token(j) * stride + h * HD + 8 * c);
-  }
+  for (int r = 0; r < ROUNDS; ++r) raw[r] = *reinterpret_cast<const u32x4*>(src + token(j) * stride + 8 * (8 * r + i));
+  f32x4 cs[ROUNDS][2], sn[ROUNDS][2];
   if (a.half > 0 && a.table > 0) {
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-      const int64_t row = static_cast<int64_t>(max(at[r], 0)) * a.half + angle;
+      const int c = 8 * r + i;
+      const int64_t row = static_cast<int64_t>(max(at, 0)) * a.half + (c < turn ? 8 * c : c < 2 * turn ? 8 * (c - turn) : 0);
 #pragma unroll
       for (int d = 0; d < 2; ++d) {
         cs[r][d] = *reinterpret_cast<const f32x4*>(a.cos + row + 4 * d);
@@ -144,50 +139,78 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
       }
     }
   }
-  f32x4 w[2] = {{1.f, 1.f, 1.f, 1.f}, {1.f, 1.f, 1.f, 1.f}};
+  f32x4 w[ROUNDS][2];
   if (norm != nullptr) {
-    w[0] = *reinterpret_cast<const f32x4*>(norm + 8 * c);
-    w[1] = *reinterpret_cast<const f32x4*>(norm + 8 * c + 4);
-  }
-  const bool stored = id >= 0 && id < b.pages;
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
-    const int j = r * TOKENS + lane / CH;
-    float x[8];
+    for (int r = 0; r < ROUNDS; ++r)
+#pragma unroll
+      for (int d = 0; d < 2; ++d) w[r][d] = *reinterpret_cast<const f32x4*>(norm + 8 * (8 * r + i) + 4 * d);
+  }
+  float x[ROUNDS][8];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      x[2 * d] = E::to_f32(static_cast<uint16_t>(raw[r][d] & 0xffffu));
-      x[2 * d + 1] = E::to_f32(static_cast<uint16_t>(raw[r][d] >> 16));
+      x[r][2 * d] = E::to_f32(static_cast<uint16_t>(raw[r][d] & 0xffffu));
+      x[r][2 * d + 1] = E::to_f32(static_cast<uint16_t>(raw[r][d] >> 16));
     }
-    if (norm != nullptr) {
-      float sum = chunk_squares(x);
+  if (norm != nullptr) {
+    float sum = chunk_squares(x[0]);
+    if constexpr (ROUNDS == 2) sum += chunk_squares(x[ROUNDS - 1]);
 #pragma unroll
-      for (int off = 1; off < CH; off <<= 1) sum += __shfl_xor(sum, off, 64);
-      const float by = rsqrtf(sum / static_cast<float>(HD) + a.eps);
+    for (int off = 1; off < 8; off <<= 1) sum += __shfl_xor(sum, off, 64);
+    const float by = rsqrtf(sum / static_cast<float>(HD) + a.eps);
 #pragma unroll
-      for (int d = 0; d < 8; ++d) x[d] = x[d] * by * w[d / 4][d % 4];
-    }
-    if (a.half > 0) {
-      float y[8];
+    for (int r = 0; r < ROUNDS; ++r)
 #pragma unroll
-      for (int d = 0; d < 8; ++d) y[d] = __shfl(x[d], other, 64);
-      if (turned) {
+      for (int d = 0; d < 8; ++d) x[r][d] = x[r][d] * by * w[r][d / 4][d % 4];
+  }
+  if (a.half > 0) {
+    float y[ROUNDS][8];  // the pairs' other dimensions
+    if (ROUNDS == 2 && turn == 8) {
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) y[r][d] = x[ROUNDS - 1 - r][d];
+    } else {
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        const int c = 8 * r + i, other = c < turn ? c + turn : c < 2 * turn ? c - turn : c;
+        const int lane_of = (lane & ~7) | (other & 7);
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-          const float cv = cs[r][d / 4][d % 4], sv = sn[r][d / 4][d % 4];
-          x[d] = first_half ? fmaf(x[d], cv, -(y[d] * sv)) : fmaf(x[d], cv, y[d] * sv);
+          y[r][d] = __shfl(x[0][d], lane_of, 64);
+          if constexpr (ROUNDS == 2) {
+            const float high = __shfl(x[ROUNDS - 1][d], lane_of, 64);
+            if (other >= 8) y[r][d] = high;
+          }
         }
       }
     }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int c = 8 * r + i;
+      if (c < 2 * turn) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const float cv = cs[r][d / 4][d % 4], sv = sn[r][d / 4][d % 4];
+          x[r][d] = c < turn ? fmaf(x[r][d], cv, -(y[r][d] * sv)) : fmaf(x[r][d], cv, y[r][d] * sv);
+        }
+      }
+    }
+  }
+  const bool stored = at >= 0 && id >= 0 && id < b.pages;
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
     u32x4 out;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
-      out[d] = static_cast<uint32_t>(E::from_f32(x[2 * d])) | (static_cast<uint32_t>(E::from_f32(x[2 * d + 1])) << 16);
+      out[d] = static_cast<uint32_t>(E::from_f32(x[r][2 * d])) | (static_cast<uint32_t>(E::from_f32(x[r][2 * d + 1])) << 16);
+    const int c = 8 * r + i;
     if (is_q) {
       // (A token whose position has no row of the tables: zeros.)
-      if (is_new(j))
-        *reinterpret_cast<u32x4*>(a.q_out + token(j) * a.q_out_stride + h * HD + 8 * c) = at[r] >= 0 ? out : u32x4{0u, 0u, 0u, 0u};
-    } else if (at[r] >= 0 && stored) {
+      if (is_new(j)) *reinterpret_cast<u32x4*>(a.q_out + token(j) * a.q_out_stride + h * HD + 8 * c) = at >= 0 ? out : u32x4{0u, 0u, 0u, 0u};
+    } else if (stored) {
       const int64_t to = (static_cast<int64_t>(id) * a.kv_heads + h) * CH + c;
       *reinterpret_cast<u32x4*>(a.k_cache + ((to << b.page_bits) + place + j) * 8) = out;
     }
