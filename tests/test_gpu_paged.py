@@ -86,6 +86,8 @@ APPENDS = [
     ([130, 3], [130, 131], 5, 5, 64, 32, F16, 16, False),
     ([33, 64], [200, 64], 3, 1, 128, 128, F16, 0, True),
     ([20, 20], [33, 41], 1, 1, 64, 16, BF16, 8, False),
+    ([900, 1, 61], [905, 30, 61], 11, 4, 128, 64, BF16, 64, True),
+    ([700, 400], [700, 400], 13, 4, 64, 16, F16, 16, False),
     ([1] * 70 + [9] + [0] * 3 + [2] * 70, [5] * 70 + [60] + [0] * 3 + [2] * 70, 2, 1, 64, 16, BF16, 32, False),
 ]
 
