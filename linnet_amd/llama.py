@@ -276,6 +276,47 @@ class Int4Llama:
         self.set_position(x.shape[0])
         return logits
 
+    def paged_cache(self, pages, page=64):
+        """A pool of KV pages for every layer (`paged.PagedCache`), for `paged_step`."""
+        from linnet_amd.torch import paged
+
+        return paged.PagedCache.empty(pages, self.kv_heads, self.hd, page, self.torch.bfloat16, self.pos_t.device,
+                                      layers=len(self.layers))
+
+    def paged_layer(self, i, x, delta, cache, tables, lengths, starts, parents=None, positions=None, max_queries=None):
+        """Layer i of new tokens of several sequences over a paged cache: `layer_fused` with `paged_append` and
+        `paged_attention` (with `parents` `paged_tree_attention`) in place of the decode attention. `cache`: the
+        pool of every layer. x is updated in place; returns the MLP branch's output, not yet added."""
+        from linnet_amd.torch import decode, generated, paged
+
+        p, pool, tiles = self.layers[i], cache.layer(i), self._tiles(x)
+        h = decode.rmsnorm(x, p["n1"], 1e-5, delta, tiles=tiles)
+        q, k, v = generated._int4_split(self.linear(h, p["qkv"]), p["qkv_rows"])
+        q = paged.paged_append(q, k, v, self.cos_tab, self.sin_tab, pool, tables, lengths, starts, positions=positions)
+        if parents is None:
+            att = paged.paged_attention(q, pool, tables, lengths, starts, max_queries=max_queries)
+        else:
+            att = paged.paged_tree_attention(q, pool, tables, lengths, starts, parents, max_queries=max_queries)
+        o = self.linear(att, p["o"])
+        h = decode.rmsnorm(x, p["n2"], 1e-5, o, tiles=tiles)
+        g, u = generated._int4_split(self.linear(h, p["gate_up"]), p["gate_up_rows"])
+        return self.linear(decode.silu_mul(g, u, tiles=tiles), p["down"])
+
+    def paged_step(self, x, cache, tables, lengths, starts, parents=None, positions=None, max_queries=None, rows=None):
+        """New tokens x [tokens, hidden] (bf16) of several sequences through every layer over a paged cache
+        (`paged_cache`; `tables`, `lengths`, `starts` as `linnet_amd.torch.paged` has them): prompts, chunks of
+        them and single tokens in one call, or with `parents` drafted trees (with `positions`, each node's entry
+        were it alone with its ancestors; `paged.paged_keep(cache, ...)` then moves an accepted path). The model's
+        rotary tables hold its capacity's positions (`ctx` and `spare`). Returns the logits of `rows` (an index tensor:
+        each sequence's last token, say), or of all tokens."""
+        x = x.clone()  # the residual stream is updated in place
+        delta = None
+        for i in range(len(self.layers)):
+            delta = self.paged_layer(i, x, delta, cache, tables, lengths, starts, parents, positions, max_queries)
+        if rows is not None:
+            x, delta = x[rows], delta[rows]
+        return self.head_fused(x, delta)
+
     def _folds(self, x):
         return self.fused and self.fold and x.shape[0] == 1
 
