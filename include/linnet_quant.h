@@ -757,7 +757,7 @@ LNQ_API LnqStatus lnq_silu_mul_tiles(const void* g, const void* u, void* xt, int
  * multiple of 8, at most head_dim / 2; 0: no rotation), in f32 and rounded once; q to q_out, k and v
  * to the cache. A token's position is positions[token] (int32), or with NULL its entry. One without a row
  * of the tables gives zeros in q_out and is not stored. Rows of q_out of no sequence become
- * zeros with `fill`, else stay. Two sequences' new entries must not share a page's place. */
+ * zeros with `fill`, else stay. q_out may be q, at its stride. Two sequences' new entries must not share a page's place. */
 LNQ_API LnqStatus lnq_paged_append(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                                    int64_t v_stride, const float* cos, const float* sin, int64_t table, int64_t half,
                                    const int32_t* positions, const float* q_norm, const float* k_norm, float eps,
@@ -774,7 +774,8 @@ LNQ_API LnqStatus lnq_paged_append(const void* q, int64_t q_stride, const void* 
  * the draft, its ancestors and itself (window: of that path). Nodes past the 256th, and rows that see
  * nothing, give zeros. max_queries: the most new tokens of a sequence, as far as known (`tokens` always
  * will do); it decides the kernels, not the result's meaning. workspace: 16-byte aligned,
- * lnq_paged_attention_workspace floats; calls that overlap on one race. scale in [1e-30, 1e30]. */
+ * lnq_paged_attention_workspace floats; calls that overlap on one race. scale in [1e-9, 1e9]. Infinities and NaNs of a value reach the rows that see its entry and
+ * no other. out shares no memory with the inputs. */
 LNQ_API LnqStatus lnq_paged_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, void* out,
                                       int64_t out_stride, int32_t fill, const int32_t* tables, const int32_t* lengths,
                                       const int32_t* starts, const int32_t* parents, const float* sinks, float* workspace,

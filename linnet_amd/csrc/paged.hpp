@@ -90,6 +90,9 @@ inline const char* refused(const BatchCheck& c) {
   return nullptr;
 }
 
+// Workgroups of 256 a launch takes at most (its threads are counted in 32 bits).
+constexpr int64_t MOST_WORKGROUPS = (int64_t{1} << 24) - 1;
+
 inline int bits_of(int64_t page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
 
 }  // namespace paged

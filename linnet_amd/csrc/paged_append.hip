@@ -346,7 +346,7 @@ LNQ_API LnqStatus lnq_paged_append(const void* q, int64_t q_stride, const void* 
   // at one and 42.1 at four; one token 4.1 and 4.9 against 3.5.
   const int64_t turned = heads + kv_heads, each = units * (turned + kv_heads) > 8192 ? 2 : 1;
   const int64_t groups = ((turned + each - 1) / each + kv_heads + paged::WAVES - 1) / paged::WAVES;
-  LNQ_REQUIRE(units * groups <= INT32_MAX, "lnq_paged_append: too large");
+  LNQ_REQUIRE(units * groups <= paged::MOST_WORKGROUPS, "lnq_paged_append: too large (fewer tokens a call)");
   if (tokens == 0) {
     clear_error();
     return LNQ_OK;
@@ -394,7 +394,7 @@ LNQ_API LnqStatus lnq_paged_keep(void* k_cache, void* v_cache, int64_t layers, i
   const int64_t one = pages * kv_heads * page * head_dim;
   LNQ_REQUIRE(layers == 1 || (layer_step >= one && layer_step % 8 == 0), "lnq_paged_keep: layers overlap");
   const int64_t waves = sequences * layers * kv_heads, blocks = (waves + paged::WAVES - 1) / paged::WAVES;
-  LNQ_REQUIRE(layers * kv_heads <= INT32_MAX && blocks <= INT32_MAX, "lnq_paged_keep: too large");
+  LNQ_REQUIRE(layers * kv_heads <= INT32_MAX && blocks <= paged::MOST_WORKGROUPS, "lnq_paged_keep: too large (fewer layers a call)");
   if (sequences == 0) {
     clear_error();
     return LNQ_OK;

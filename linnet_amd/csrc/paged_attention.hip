@@ -1113,7 +1113,10 @@ static const char* sizes_refused(int64_t sequences, int64_t width, int64_t pages
   if (window < 0 || window > (1 << 30)) return "a window is 0 (none) to 2^30 entries";
   if (tokens * heads > INT32_MAX || sequences * heads * 32 > INT32_MAX) return "too many tokens, sequences or heads";
   const paged::Plan p = paged::plan_of(sequences, width, page, tokens, heads, kv_heads, head_dim, most, window);
-  if ((sequences + 1) * kv_heads * p.few_splits + p.slots * kv_heads * p.many_splits > INT32_MAX || p.few_rows + p.many_rows > INT32_MAX)
+  // (A join takes a workgroup a row where there are more than 64 parts, and one for four rows otherwise.)
+  const int64_t parts = p.few_splits > p.many_splits ? p.few_splits : p.many_splits;
+  if ((sequences + 1) * kv_heads * p.few_splits + p.slots * kv_heads * p.many_splits > paged::MOST_WORKGROUPS ||
+      (p.few_rows + p.many_rows) / (parts > 64 ? 1 : 4) >= paged::MOST_WORKGROUPS)
     return "too many tokens, sequences or heads";
   return nullptr;
 }
@@ -1140,7 +1143,7 @@ LNQ_API LnqStatus lnq_paged_attention(const void* q, int64_t q_stride, const voi
   const char* const no = sizes_refused(sequences, width, pages, page, tokens, heads, kv_heads, head_dim, max_queries, window);
   LNQ_REQUIRE(no == nullptr, "lnq_paged_attention: %s", no);
   LNQ_REQUIRE(dtype == LNQ_BF16 || dtype == LNQ_F16, "lnq_paged_attention: dtype %d is not bf16 or f16", dtype);
-  LNQ_REQUIRE(scale >= 1e-30f && scale <= 1e30f, "lnq_paged_attention: the scale is a positive number, not %g", static_cast<double>(scale));
+  LNQ_REQUIRE(scale >= 1e-9f && scale <= 1e9f, "lnq_paged_attention: the scale is a positive number, not %g", static_cast<double>(scale));
   if (tokens == 0) {
     clear_error();
     return LNQ_OK;

@@ -27,7 +27,7 @@ import torch
 
 from .. import _lib
 from ..errors import LinnetError
-from .kernels import _aligned, _code, _launch, _on_gpu
+from .kernels import _aligned, _code, _on_gpu
 
 PAGES = (16, 32, 64, 128)  # entries a page may hold
 TREE_NODES = 256  # of a drafted tree
@@ -79,8 +79,19 @@ class PagedCache:
         return PagedCache(self.k[i], self.v[i])
 
 
-# A call's host time is longer than a decode step's kernels here, so the checks below are the direct forms.
+# A call's host time is longer than a decode step's kernels here (10 us against 4), so the checks below are the
+# direct forms.
 _INT32, _FLOAT32 = torch.int32, torch.float32
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _launch(index: int, name: str, *args: object) -> None:
+    """Calls entry point `name` on the current stream of device `index`, its last argument."""
+    if index == _current_device():
+        _lib.call(name, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _raw_stream(index))
 
 
 def _records(what: str) -> None:
@@ -153,9 +164,13 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
     the places of their new entries."""
     pages, page, kv_heads, head_dim, code, _ = _one_layer("paged_append", cache)
     k_cache, v_cache = cache.k, cache.v
-    device = _on_gpu("paged_append", q, k, v, k_cache, tables, lengths, starts, cos, sin, positions, q_norm, k_norm, out)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or any(
-            t is not None and t.requires_grad for t in (cos, sin, q_norm, k_norm, out))):
+    index = q.get_device()
+    if not (0 <= index == k.get_device() == v.get_device() == k_cache.get_device() == tables.get_device() == lengths.get_device()
+            == starts.get_device()) or any(t is not None and t.get_device() != index for t in (cos, sin, positions, q_norm, k_norm, out)):
+        _on_gpu("paged_append", q, k, v, k_cache, tables, lengths, starts, cos, sin, positions, q_norm, k_norm, out)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_cache.requires_grad
+                                    or v_cache.requires_grad or any(t is not None and t.requires_grad
+                                                                    for t in (cos, sin, q_norm, k_norm, out))):
         _records("paged_append")
     dtype = k_cache.dtype
     tables, lengths, starts, sequences, width = _batch("paged_append", tables, lengths, starts)
@@ -193,7 +208,7 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
         out = q.new_empty((tokens, columns))
     else:
         out = _out("paged_append", out, tokens, columns, dtype)
-    _launch(device, "lnq_paged_append", q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, at_cos, at_sin, table,
+    _launch(index, "lnq_paged_append", q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, at_cos, at_sin, table,
             half, at_positions, at_q_norm, at_k_norm, eps, out.data_ptr(), columns, fill, k_cache.data_ptr(), v_cache.data_ptr(),
             tables.data_ptr(), lengths.data_ptr(), starts.data_ptr(), sequences, width, pages, page, tokens, heads, kv_heads, head_dim,
             code)
@@ -212,7 +227,10 @@ def _attend(what: str, q: torch.Tensor, cache: PagedCache, tables: torch.Tensor,
             sinks: torch.Tensor | None, out: torch.Tensor | None) -> torch.Tensor:
     pages, page, kv_heads, head_dim, code, _ = _one_layer(what, cache)
     k_cache = cache.k
-    device = _on_gpu(what, q, k_cache, tables, lengths, starts, parents, sinks, out)
+    index = q.get_device()
+    if not (0 <= index == k_cache.get_device() == tables.get_device() == lengths.get_device() == starts.get_device()) or any(
+            t is not None and t.get_device() != index for t in (parents, sinks, out)):
+        _on_gpu(what, q, k_cache, tables, lengths, starts, parents, sinks, out)
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or cache.v.requires_grad or any(
             t is not None and t.requires_grad for t in (sinks, out))):
         _records(what)
@@ -233,7 +251,7 @@ def _attend(what: str, q: torch.Tensor, cache: PagedCache, tables: torch.Tensor,
         sinks = _floats(what, "sinks", sinks, heads)
         at_sinks = sinks.data_ptr()
     scale = head_dim**-0.5 if scale is None else float(scale)
-    if not 1e-30 <= scale <= 1e30:
+    if not 1e-9 <= scale <= 1e9:
         raise LinnetError(f"{what}: the scale is a positive number, not {scale}")
     window = int(window) if window else 0
     fill = out is None
@@ -247,7 +265,7 @@ def _attend(what: str, q: torch.Tensor, cache: PagedCache, tables: torch.Tensor,
     if floats:
         work = q.new_empty((floats,), dtype=_FLOAT32)
         at_work = work.data_ptr()
-    _launch(device, "lnq_paged_attention", q.data_ptr(), q_stride, k_cache.data_ptr(), cache.v.data_ptr(), out.data_ptr(), columns,
+    _launch(index, "lnq_paged_attention", q.data_ptr(), q_stride, k_cache.data_ptr(), cache.v.data_ptr(), out.data_ptr(), columns,
             fill, tables.data_ptr(), lengths.data_ptr(), starts.data_ptr(), at_parents, at_sinks, at_work, floats, sequences, width,
             pages, page, tokens, heads, kv_heads, head_dim, most, window, scale, code)
     return out
@@ -259,11 +277,12 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, le
     """Grouped-query attention of the new tokens' queries q [tokens, heads*head_dim] (as `paged_append` returns
     them, their keys and values in the cache): `softmax(scale q K^T) V` over the entries up to each
     token's own, the last `window` of them with one (0 or None: all); scale head_dim^-0.5 unless given. `sinks`
-    (f32 [heads]) add e^sink to each row's sum. Returns [tokens, heads*head_dim] (`out`, if given).
+    (f32 [heads]) add e^sink to each row's sum. Returns [tokens, heads*head_dim] (`out`, if given, which shares no memory
+    with the inputs).
 
     `max_queries`, the most new tokens of a sequence, where the caller knows it, spares the kernels for longer
-    ones: 1 for a decode step. Sequences with more are computed all the same. A row that sees no entry
-    gives zeros; tokens of no sequence give zeros, or with `out` leave its rows as they were."""
+    ones: 1 for a decode step. Sequences with more are computed all the same. A row that sees no entry, or
+    only ones whose score is -inf, gives zeros; infinities and NaNs of a value reach the rows that see its entry and no other; tokens of no sequence give zeros, or with `out` leave its rows as they were."""
     return _attend("paged_attention", q, cache, tables, lengths, starts, None, max_queries, scale, window, sinks, out)
 
 
@@ -289,7 +308,10 @@ def paged_keep(cache: PagedCache, tables: torch.Tensor, lengths: torch.Tensor, s
     place of node j. Returns the new lengths ([sequences] int32): the entries before the draft and the path's. The
     places after those hold what they held."""
     pages, page, kv_heads, head_dim, _, layers = cache._sizes
-    device = _on_gpu("paged_keep", cache.k, tables, lengths, starts, kept)
+    index = cache.k.get_device()
+    _on_gpu("paged_keep", cache.k, tables, lengths, starts, kept)
+    if torch.is_grad_enabled() and (cache.k.requires_grad or cache.v.requires_grad):
+        _records("paged_keep")
     tables, lengths, starts, sequences, width = _batch("paged_keep", tables, lengths, starts)
     if kept.dim() != 2:
         raise LinnetError(f"paged_keep: kept is [sequences, path] int32, got {list(kept.shape)}")
@@ -299,7 +321,7 @@ def paged_keep(cache: PagedCache, tables: torch.Tensor, lengths: torch.Tensor, s
     new = torch.empty_like(lengths)
     if sequences == 0:
         return new
-    _launch(device, "lnq_paged_keep", cache.k.data_ptr(), cache.v.data_ptr(), layers or 1, pages * kv_heads * page * head_dim,
+    _launch(index, "lnq_paged_keep", cache.k.data_ptr(), cache.v.data_ptr(), layers or 1, pages * kv_heads * page * head_dim,
             tables.data_ptr(), lengths.data_ptr(), starts.data_ptr(), kept.data_ptr(), kept.shape[1], new.data_ptr(), sequences,
             width, pages, page, _MOST_TOKENS, kv_heads, head_dim)
     return new

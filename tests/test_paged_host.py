@@ -56,6 +56,7 @@ BATCHES = [(dict(page=24), "16, 32, 64 or 128"), (dict(sequences=-1), "sequences
     (dict(cos=NULL), "null"), (dict(tables=NULL), "null"), (dict(starts=NULL), "null"), (dict(v_cache=NULL), "null"),
     (dict(q=ODD), "aligned"), (dict(k_cache=ODD), "aligned"), (dict(q_stride=516), "whole 16 bytes"), (dict(q_stride=504), "shorter"),
     (dict(k_stride=0), "shorter"), (dict(tokens=1 << 24, heads=65536, sequences=1), "too large"),
+    (dict(tokens=1 << 24, heads=64, q_stride=4096, q_out_stride=4096), "too large"),
 ])
 def test_append_refuses(change: dict, message: str) -> None:
     status, error = _status("lnq_paged_append", *_append(**change))
@@ -69,7 +70,8 @@ def test_append_refuses(change: dict, message: str) -> None:
     (dict(q=NULL), "null"), (dict(out=NULL), "null"), (dict(lengths=NULL), "null"), (dict(k_cache=NULL), "null"),
     (dict(q=ODD), "aligned"), (dict(out=ODD), "aligned"), (dict(v_cache=ODD), "aligned"), (dict(q_stride=516), "whole 16 bytes"),
     (dict(out_stride=0), "shorter"), (dict(workspace_floats=3, width=1000), "floats"), (dict(workspace=NULL, width=1000), "floats"),
-    (dict(tokens=1 << 24, heads=1024), "too many"),
+    (dict(tokens=1 << 24, heads=1024), "too many"), (dict(tokens=1 << 24, sequences=1 << 20, heads=64, kv_heads=64), "too many"),
+    (dict(sequences=1 << 20, width=1 << 15, heads=64, kv_heads=64), "too many"), (dict(scale=1e10), "scale"), (dict(scale=1e-10), "scale"),
 ])
 def test_attention_refuses(change: dict, message: str) -> None:
     status, error = _status("lnq_paged_attention", *_attend(**change))
@@ -79,7 +81,7 @@ def test_attention_refuses(change: dict, message: str) -> None:
 @pytest.mark.parametrize(("change", "message"), BATCHES + [
     (dict(kv_heads=0), "bad shape"), (dict(layers=0), "bad shape"), (dict(path=-1), "bad shape"), (dict(layer_step=64), "overlap"),
     (dict(k_cache=NULL), "null"), (dict(kept=NULL), "null"), (dict(lengths_out=NULL), "null"), (dict(v_cache=ODD), "aligned"),
-    (dict(layers=65536, kv_heads=65536, layer_step=1 << 50), "too large"),
+    (dict(layers=65536, kv_heads=65536, layer_step=1 << 50), "too large"), (dict(layers=1024, sequences=1 << 15), "too large"),
 ])
 def test_keep_refuses(change: dict, message: str) -> None:
     status, error = _status("lnq_paged_keep", *_keep(**change))
