@@ -35,8 +35,17 @@ constexpr int MANY_STEP = 64;
 constexpr int NODES = 256;       // of a drafted tree
 constexpr int MAX_SPLITS = 256;
 
+// f16 weights are kept times 2^7: with the maximum's slack of 2^8 they stay below 2^15 (f16 ends at 2^16), and what
+// rounds to 0 is below 2^-32 of the largest, not 2^-25, of which the tail of a long cache can hold a sizable sum.
+template <int DT>
+constexpr float LIFT = DT == LNQ_F16 ? 7.f : 0.f;
+
+// The maximum of a row's scores in the stored form: times log2 e, less the lift, so that weights are 2^(score - it).
+template <int DT>
+__device__ inline float stored_max(float m, float c) { return m == -INFINITY ? m : fmaf(m, c, -LIFT<DT>); }
+
 // The sums of tiles whose entries are split, for each of the splits and rows: the outputs so far, [splits][rows]
-// [head_dim], and maximum (times log2 e) and sum, [splits][rows][2].
+// [head_dim], and stored_max and sum, [splits][rows][2].
 struct Parts {
   float *sums, *stats;
   int64_t rows;
@@ -318,7 +327,7 @@ struct Rows {
         for (int r = 0; r < S::REGS; ++r) o[d][r] *= by;
       m = now;
     }
-    const float at = m == -INFINITY ? 0.f : m * c;
+    const float at = m == -INFINITY ? 0.f : stored_max<DT>(m, c);
     float sum = 0.f;
 #pragma unroll
     for (int n = 0; n < N * NT; ++n)
@@ -365,7 +374,7 @@ struct Rows {
 // asm statement it would wait for the queries again in each step, and with them for the loads after.)
 __device__ inline void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
-// The factor that normalises a row of maximum m (times log2 e) and sum l.
+// The factor that normalises a row of stored maximum m and sum l.
 __device__ inline float norm_of(float m, float l, const float* sinks, int head) {
   if (l == 0.f) return 0.f;  // the row sees nothing
   if (sinks == nullptr) return 1.f / l;
@@ -559,7 +568,7 @@ __device__ inline void few_rows(const AttendArgs& a, int block, FewLds<HD, TILE>
     // The four waves' rows into one: each scales its outputs to the common maximum, hands each other wave the
     // registers of that one's share, and adds up its own share in the waves' order.
     const float l = sum_across<TILE>(st.l);
-    const float mine = st.m == -INFINITY ? -INFINITY : st.m * a.scale2;
+    const float mine = stored_max<DT>(st.m, a.scale2);
     if (group == 0) stat[wave][col][0] = mine, stat[wave][col][1] = l;
     __syncthreads();
     float m = stat[0][col][0];
@@ -813,7 +822,7 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
 
   if (w0 + col >= rows) return;
   const float l = sum_across<32>(st.l);
-  const float m = st.m == -INFINITY ? -INFINITY : st.m * a.scale2;
+  const float m = stored_max<DT>(st.m, a.scale2);
   if (range.used == 1) {
     const float n = norm_of(m, l, a.sinks, head);
     uint16_t* const to = a.out + (q.first + i) * a.out_stride + static_cast<int64_t>(head) * HD;

@@ -34,7 +34,7 @@ TREE_NODES = 256  # of a drafted tree
 _MOST_TOKENS = 1 << 24  # new tokens of a batch
 
 
-@dataclasses.dataclass(frozen=True)
+@dataclasses.dataclass(frozen=True, eq=False)
 class PagedCache:
     """The pool of one layer, or of several: `k` [(layers,) pages, kv_heads, head_dim/8, page, 8] and `v`
     [(layers,) pages, kv_heads, page/8, head_dim, 8], bf16 or f16, contiguous. Entry e of a sequence
@@ -277,12 +277,13 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, le
     """Grouped-query attention of the new tokens' queries q [tokens, heads*head_dim] (as `paged_append` returns
     them, their keys and values in the cache): `softmax(scale q K^T) V` over the entries up to each
     token's own, the last `window` of them with one (0 or None: all); scale head_dim^-0.5 unless given. `sinks`
-    (f32 [heads]) add e^sink to each row's sum. Returns [tokens, heads*head_dim] (`out`, if given, which shares no memory
-    with the inputs).
+    (f32 [heads]) add e^sink to each row's sum. Returns [tokens, heads*head_dim] (`out`, if given, which shares
+    no memory with the inputs).
 
     `max_queries`, the most new tokens of a sequence, where the caller knows it, spares the kernels for longer
     ones: 1 for a decode step. Sequences with more are computed all the same. A row that sees no entry, or
-    only ones whose score is -inf, gives zeros; infinities and NaNs of a value reach the rows that see its entry and no other; tokens of no sequence give zeros, or with `out` leave its rows as they were."""
+    only ones whose score is -inf, gives zeros; infinities and NaNs of a value reach the rows that see its entry
+    and no other; tokens of no sequence give zeros, or with `out` leave its rows as they were."""
     return _attend("paged_attention", q, cache, tables, lengths, starts, None, max_queries, scale, window, sinks, out)
 
 

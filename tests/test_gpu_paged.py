@@ -607,3 +607,30 @@ def test_refusals() -> None:
         paged.paged_attention(q.float().requires_grad_().to(BF16), *attend[1:])
     empty = paged.paged_attention(q[:0], *attend[1:])
     assert empty.shape == (0, 256)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("sink", [False, True])
+def test_attention_f16_keeps_a_long_tail_of_small_weights(new, sink) -> None:
+    print("tail", new, sink, flush=True)
+    entries, hd, page = 1 << 17, 64, 64
+    pages = entries // page
+    k = torch.zeros(pages, 1, hd // 8, page, 8, dtype=F16, device=DEV)
+    v = torch.ones(pages, 1, page // 8, hd, 8, dtype=F16, device=DEV)
+    k[0, 0, 0, 0, 0] = 1  # entry 0: score 17.75 of value 0; the others 0 of value 1, weights of 2^-25.6 each
+    v[0, 0, 0, :, 0] = 0
+    q = torch.zeros(new, hd, dtype=F16, device=DEV)
+    q[:, 0] = 17.75
+    ints = lambda *n: torch.tensor(n, dtype=torch.int32, device=DEV)  # noqa: E731
+    sinks = torch.tensor([17.75], device=DEV) if sink else None
+    got = paged.paged_attention(q, paged.PagedCache(k, v), torch.arange(pages, dtype=torch.int32, device=DEV)[None], ints(entries),
+                                ints(0, new), scale=1.0, sinks=sinks).double().cpu()
+    seen = torch.arange(entries - new, entries, dtype=torch.float64)  # entries but the first that a row sees
+    tail = seen * torch.tensor(-17.75, dtype=torch.float64).exp()
+    want = (tail / (tail + (2 if sink else 1)))[:, None].expand(-1, hd)
+    # A weight below f16's normal numbers is off by half of 2^-24 / 2^7 of the largest, each one the same; the output
+    # by half a step; sums and exponents in f32 by under 2^-16 of it.
+    tol = entries * 2.0**-32 + want * (2.0**-11 + 2.0**-16)
+    err = (got - want).abs()
+    print(f"largest error {err.max().item():.2e} of {tol.max().item():.2e}", flush=True)
+    assert (err <= tol).all()
