@@ -170,23 +170,36 @@ __device__ inline Row row_of(const AttendArgs& a, const Sequence& q, int i, cons
   return r;
 }
 
-// The paths from each node to the draft's root, bit j for node j, within the window; every thread of
-// the workgroup takes part. A parent that is no earlier node is the entry before the draft.
-__device__ inline void paths_of(const AttendArgs& a, const Sequence& q, uint32_t* paths, int* depth, int* up, int threads) {
-  const int n = min(q.n, NODES), tid = threadIdx.x;
-  for (int i = tid; i < n; i += threads) {
-    const int p = a.parents[q.first + i];
-    up[i] = p >= 0 && p < i ? p : -1;
-  }
-  for (int i = tid; i < n * (NODES / 32); i += threads) paths[i] = 0;
-  __syncthreads();
-  for (int i = tid; i < n; i += threads) {
-    int many = 0;
-    for (int j = i; j >= 0; j = up[j], ++many)
-      if (a.window == 0 || many < a.window) paths[i * (NODES / 32) + (j >> 5)] |= 1u << (j & 31);
+// A tree's parent of this thread's node. (A parent that is no earlier node is the entry before the draft.)
+__device__ inline int parent_of(const AttendArgs& a, const Sequence& q) {
+  const int i = threadIdx.x;
+  if (i >= min(q.n, NODES)) return -1;
+  const int p = a.parents[q.first + i];
+  return p >= 0 && p < i ? p : -1;
+}
+
+// The paths from each node to the draft's root, bit j for node j, within the window, a thread a node (NODES
+// threads, all of which take part).
+__device__ inline void paths_of(const AttendArgs& a, const Sequence& q, int parent, uint32_t* paths, int* depth, int* up) {
+  const int n = min(q.n, NODES), i = threadIdx.x;
+  up[i] = parent;
+  lds_barrier();
+  if (i < n) {
+    const int most = a.window > 0 ? a.window : NODES;
+    uint32_t* const path = paths + i * (NODES / 32);
+#pragma unroll
+    for (int w = 0; w < NODES / 32; ++w) path[w] = 0;
+    int many = 0, word = i >> 5;
+    uint32_t bits = 0;
+    for (int j = i; j >= 0; ++many) {
+      if (j >> 5 != word) path[word] = bits, bits = 0, word = j >> 5;
+      if (many < most) bits |= 1u << (j & 31);
+      j = up[j];
+    }
+    path[word] = bits;
     depth[i] = many - 1;
   }
-  __syncthreads();
+  lds_barrier();
 }
 
 // Of the 32 entries from t, those the row sees, as bits in the order of this lane's registers.
@@ -435,7 +448,7 @@ __device__ inline void few_rows(const AttendArgs& a, int block, FewLds<HD, TILE>
   const int rows = static_cast<int>(all_rows);
   const int splits = q.n <= a.few_tokens ? a.small.splits : 1;
   if (split >= splits) return;
-  if constexpr (TREE) paths_of(a, q, tree.paths, tree.depth, tree.up, 256);
+  if constexpr (TREE) paths_of(a, q, parent_of(a, q), tree.paths, tree.depth, tree.up);
   const int limit = min(q.length, capacity(b));  // entries that may be there
   const float slack = 8.f / a.scale2;
 
@@ -666,7 +679,6 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   const Range range = range_of(a, q, i0, i1, a.large.splits, MANY_STEP);
   if (split >= range.used) return;
   const int begin = range.lo + split * range.chunk, end = min(range.hi, begin + range.chunk);
-  if constexpr (TREE) paths_of(a, q, tree.paths, tree.depth, tree.up, 256);
   const int limit = min(min(q.length, capacity(b)), end);
   const int mask = (1 << b.page_bits) - 1;
   const float slack = 8.f / a.scale2;
@@ -675,7 +687,6 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   const int w0 = r0 + 32 * wave;
   const bool busy = w0 < rows;
   const int r = min(w0 + col, rows - 1), i = r / a.group, head = h * a.group + r % a.group;
-  const Row row = row_of<TREE>(a, q, i, tree.paths, tree.depth);
   const int wa = min(w0, rows - 1) / a.group, wz = min(w0 + 31, rows - 1) / a.group;
   const int sure_last = TREE ? q.base - 1 : q.base + wa, sure_low = a.window > 0 ? q.base + (TREE ? q.n - 1 : wz) - a.window + 1 : 0;
   const int any_last = TREE ? q.length - 1 : q.base + wz, any_low = a.window > 0 ? q.base + (TREE ? 0 : wa) - a.window + 1 : 0;
@@ -730,7 +741,10 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
   };
 
   const int entry = entry_of<32>(0, col);
-  int id = -1, next = -1;
+  int id = -1, next = -1, parent = -1;
+  // (Without a window, a part that ends before the draft needs no paths.)
+  const bool nodes = TREE && (a.window > 0 || end > q.base);
+  if (nodes) parent = parent_of(a, q);
   if (begin < end) {
     id = page_at(begin);
     next = page_at(begin + MANY_STEP);
@@ -738,6 +752,10 @@ __global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int sl
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) load_one(first, tile0, i);
   }
+  if constexpr (TREE) {
+    if (nodes) paths_of(a, q, parent, tree.paths, tree.depth, tree.up);
+  }
+  const Row row = row_of<TREE>(a, q, i, tree.paths, tree.depth);
   loads_done();
   lds_barrier();
   auto step = [&](int t, u32x4* cur, u32x4* other) __attribute__((always_inline)) {
