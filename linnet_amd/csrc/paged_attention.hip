@@ -646,9 +646,10 @@ __device__ inline int many_slot(const AttendArgs& a, int s) {
 // The many-row way, for the tiles of `slots` slots; past their workgroups, the sequences of few rows. WIDE:
 // pages of 64 entries and more, a tile of entries in one of them, its addresses scalar ones. (A vector
 // instruction costs a wave's matrix unit half its own time; those of a step that only find addresses are
-// a tenth of it.)
+// a tenth of it.) Four workgroups a CU at head_dim 64 (for a few registers' spills): 8191 tokens in a window of
+// 128, 53.7 us against 60 with three.
 template <int DT, int HD, bool TREE, bool WIDE>
-__global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a, int slots) {
+__global__ __launch_bounds__(256, HD == 64 && !TREE ? 4 : 2) void paged_many_kernel(AttendArgs a, int slots) {
   using R = Rows<DT, HD, 32>;
   constexpr int CH = HD / 8, QK = R::QK, DV = R::DV;
   constexpr int UNITS = HD * MANY_STEP / 8;  // 16-byte units of K's tile, and of V's
@@ -1052,9 +1053,11 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
   p.few_tokens = p.few / group < 1 ? 1 : p.few / group;
   if (!p.many && most < p.few_tokens) p.few_tokens = most;
   p.few_tile = p.many || p.few_tokens * group <= 16 ? 16 : 32;
-  // Entries a tile may see, at most.
-  int64_t seen = width * page;
-  if (window > 0 && window + most + FEW_STEP < seen) seen = window + most + FEW_STEP;
+  // Entries that a tile of `queries` tokens may see, at most.
+  auto seen_by = [&](int64_t queries) {
+    const int64_t all = width * page, near = window + queries + FEW_STEP;
+    return window > 0 && near < all ? near : all;
+  };
   auto bounded = [](int64_t v, int64_t hi) {
     v = v > hi ? hi : v;
     return v < 1 ? int64_t{1} : v;
@@ -1063,9 +1066,12 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
     // As many workgroups as the chip holds at once (3 a CU at head_dim 64, 2 at 128), and none of much over 1024
     // entries where lengths differ. One row of 131000 entries at head_dim 64: 57.0 us with 768 workgroups, 59.9 with
     // 512 or 1024, 62.3 with 2048; 64 rows of 230000 at 128: 180.6 with parts of 1024, 183.4 of 2048, 184.5 of 512.
-    const int64_t base = sequences * kv_heads;
+    const int64_t base = sequences * kv_heads, seen = seen_by(p.few_tokens);
     int64_t want = up_to(head_dim == 64 ? 768 : 512, base > 0 ? base : 1);
     if (want < up_to(seen, 1024)) want = up_to(seen, 1024);
+    // Parts cost a second kernel: 8 KV heads of 250 entries take 5.9 us whole and 9.2 in parts, of 500 7.4 and 9.3, of 1000
+    // 10.0 and 9.4; 64 of 375 to 750 10.4 and 11.6; 512 of 1000 47.6 and 55.8.
+    if (seen <= (base < 64 ? 512 : 1280)) want = 1;
     const int64_t top = up_to(seen, FEW_STEP);
     p.few_splits = bounded(want, top < MAX_SPLITS ? top : MAX_SPLITS);
   }
@@ -1076,7 +1082,7 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
     const int64_t base = p.slots * kv_heads;
     // Twice what the chip holds at once, as the tiles differ: 16 trees of 900 nodes 131 us with 1024 (or 768), 149 with 512;
     // one of 24 over 1000 entries 14.5 with parts of 64 entries, 17.0 of 256.
-    const int64_t top = up_to(seen, MANY_STEP);
+    const int64_t top = up_to(seen_by(most), MANY_STEP);
     p.many_splits = bounded(up_to(1024, base > 0 ? base : 1), top < 64 ? top : 64);
   }
   p.few_rows = p.few_splits > 1 ? sequences * p.few_tokens * heads : 0;
