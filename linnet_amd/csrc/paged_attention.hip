@@ -913,19 +913,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a, int64_t s
   const int64_t token = at_block / blocks;
   const bool small = token < small_tokens;
   const Parts& part = small ? a.small : a.large;
-  const Joined j = joined_of(a, small, static_cast<int>(small ? token : token - small_tokens));
-  if (j.q.n == 0) return;
   const int head0 = static_cast<int>(at_block % blocks) * HEADS;
   const int head = head0 + lane / PARTS, c = lane % PARTS;
+  const int64_t at0 = (small ? token : token - small_tokens) * a.heads + head0;  // (part_row)
+  // Read before the batch says which of the parts are there: a wave waits once, not twice.
+  const float* const st = part.stats + 2 * (min(c, part.splits - 1) * part.rows + min(at0 + lane / PARTS, part.rows - 1));
+  const float m_read = st[0], l_read = st[1];
+  const Joined j = joined_of(a, small, static_cast<int>(small ? token : token - small_tokens));
+  if (j.q.n == 0) return;
   const int used = head < a.heads ? parts_of(a, small, j, head).used : 1;
   const int most = static_cast<int>(wave_max(static_cast<float>(used)));
   if (most == 1) return;
-  const int64_t at0 = part_row(a, small, j.s, j.q, j.i, head0);
   float m = -INFINITY, l = 0.f;
-  if (head < a.heads && c < used && used > 1) {
-    const float* const st = part.stats + 2 * (c * part.rows + at0 + lane / PARTS);
-    m = st[0], l = st[1];
-  }
+  if (head < a.heads && c < used && used > 1) m = m_read, l = l_read;
   float top = m;
 #pragma unroll
   for (int off = 1; off < PARTS; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
@@ -978,33 +978,50 @@ __global__ __launch_bounds__(256) void paged_join_wide_kernel(AttendArgs a, int6
   if (token >= tokens) return;
   const bool small = token < small_tokens;
   const Parts& part = small ? a.small : a.large;
+  const int64_t at = (small ? token : token - small_tokens) * a.heads + head;  // (part_row)
+  // Statistics and, of few rows (of many it could be traffic for nothing), the first parts are read before the batch
+  // says which of them are there: a wave waits once, not three times.
+  constexpr int STATS = MAX_SPLITS / 64;
+  float ms[STATS], ls[STATS];
+#pragma unroll
+  for (int n = 0; n < STATS; ++n) {
+    const float* const st = part.stats + 2 * (min(lane + 64 * n, part.splits - 1) * part.rows + at);
+    ms[n] = st[0], ls[n] = st[1];
+  }
+  const float* const from = part.sums + at * HD + lane * D;
+  float x[AHEAD][D];
+  auto load = [&](int c0, int last) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) {
+      const int c = min(c0 + 4 * n, last);  // (past the last: read again, and not used)
+#pragma unroll
+      for (int d = 0; d < D; ++d) x[n][d] = from[c * part.rows * HD + d];
+    }
+  };
+  const bool early = gridDim.x <= 256;
+  if (early) load(wave, part.splits - 1);
   const Joined j = joined_of(a, small, static_cast<int>(small ? token : token - small_tokens));
   if (j.q.n == 0) return;
   const int used = parts_of(a, small, j, head).used;
   if (used == 1) return;
-  const int64_t at = part_row(a, small, j.s, j.q, j.i, head);
+  if (!early) load(wave, used - 1);
   float m = -INFINITY;
-  for (int c = lane; c < used; c += 64) m = fmaxf(m, part.stats[2 * (c * part.rows + at)]);
+#pragma unroll
+  for (int n = 0; n < STATS; ++n) m = fmaxf(m, lane + 64 * n < used ? ms[n] : -INFINITY);
   m = wave_max(m);
   float l = 0.f;
-  for (int c = lane; c < used; c += 64) {
-    const float mc = part.stats[2 * (c * part.rows + at)];
-    const float w = mc == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mc - m);
-    l = fmaf(part.stats[2 * (c * part.rows + at) + 1], w, l);
-    if (wave == 0) weights[c] = w;
+#pragma unroll
+  for (int n = 0; n < STATS; ++n) {
+    const int c = lane + 64 * n;
+    const float w = ms[n] == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(ms[n] - m);
+    if (c < used) l = fmaf(ls[n], w, l);
+    if (wave == 0 && c < used) weights[c] = w;
   }
   l = wave_sum(l);
   __syncthreads();
-  const float* const from = part.sums + at * HD + lane * D;
   float o[D] = {};
   for (int c0 = wave; c0 < used; c0 += 4 * AHEAD) {
-    float x[AHEAD][D];
-#pragma unroll
-    for (int n = 0; n < AHEAD; ++n) {
-      const int c = min(c0 + 4 * n, used - 1);  // (past the last: read again, and not used)
-#pragma unroll
-      for (int d = 0; d < D; ++d) x[n][d] = from[c * part.rows * HD + d];
-    }
+    if (c0 != wave) load(c0, used - 1);
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) {
       const int c = c0 + 4 * n;
