@@ -634,3 +634,46 @@ def test_attention_f16_keeps_a_long_tail_of_small_weights(new, sink) -> None:
     err = (got - want).abs()
     print(f"largest error {err.max().item():.2e} of {tol.max().item():.2e}", flush=True)
     assert (err <= tol).all()
+
+
+PARTS = [case for case in ATTENDS if sum(case[0]) <= 70] + [
+    # joined one head of a token a wave, and four
+    ([1] * 41, [40 + 9 * i for i in range(41)], 9, 3, 64, 16, BF16, 0, True),
+    ([1] * 69 + [0, 1], [20 + 11 * i for i in range(69)] + [7, 3], 32, 8, 128, 32, BF16, 0, True),
+    ([2] * 70, [2 + 9 * i for i in range(70)], 18, 6, 64, 16, F16, 0, False),
+]
+
+
+@pytest.mark.parametrize("case", PARTS, ids=lambda case: f"{len(case[0])}-{case[1][0]}-{case[2:]}")
+def test_attention_in_parts(case) -> None:
+    """The same over tables of 4096 entries: the entries are divided by what the tables can hold."""
+    counts, lengths, heads, kvh, hd, page, dtype, window, sinks = case
+    print(case, flush=True)
+    batch = Batch(counts, lengths, kvh, hd, page, dtype, seed=41, width=4096 // page).fill()
+    for most in (None, max(counts)):
+        _attend(batch, heads, window, sinks, max_queries=most)
+
+
+@pytest.mark.parametrize("case", [case for case in TREES if sum(case[0]) <= 140], ids=str)
+def test_tree_attention_in_parts(case) -> None:
+    counts, lengths, heads, kvh, hd, page, dtype, window, sinks = case
+    print(case, flush=True)
+    batch = Batch(counts, lengths, kvh, hd, page, dtype, seed=42, width=4096 // page).fill()
+    for most in (None, max(counts)):
+        _attend(batch, heads, window, sinks, max_queries=most, parents=_random_parents(counts, batch.g))
+
+
+@pytest.mark.parametrize("most", [None, 2])
+def test_attention_in_parts_keeps_infinities_and_nan_to_the_rows_that_see_them(most) -> None:
+    print("odd values in parts", most, flush=True)
+    inf, nan = float("inf"), float("nan")
+    batch = Batch([2, 1], [300, 140], 1, 64, 16, BF16, seed=43, width=256)
+    for e, d, what in ((-1, 5, nan), (-1, 9, -inf), (10, 40, inf), (200, 40, inf), (200, 50, -inf), (20, 50, inf)):
+        batch.values[0][e, 0, d] = what
+    batch.fill()
+    q = (2 * torch.randn(3, 512, generator=batch.g)).to(BF16).to(DEV)
+    got = paged.paged_attention(q, batch.cache, batch.tables, batch.lengths, batch.starts, max_queries=most)
+    want, tol = attention(batch, q)
+    compare(f"most={most}", got, want, torch.where(tol.isfinite(), tol, 0.0))
+    rows = got.view(3, 8, 64)
+    assert rows[:2, :, 40].isinf().all() and rows[:2, :, 50].isnan().all() and rows[0, :, [5, 9]].isfinite().all()
