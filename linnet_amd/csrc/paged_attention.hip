@@ -1086,9 +1086,10 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
     const int64_t base = sequences * kv_heads, seen = seen_by(p.few_tokens);
     int64_t want = up_to(head_dim == 64 ? 768 : 512, base > 0 ? base : 1);
     if (want < up_to(seen, 1024)) want = up_to(seen, 1024);
-    // Parts cost a second kernel: 8 KV heads of 250 entries take 5.9 us whole and 9.2 in parts, of 500 7.4 and 9.3, of 1000
-    // 10.0 and 9.4; 64 of 375 to 750 10.4 and 11.6; 512 of 1000 47.6 and 55.8.
-    if (seen <= (base < 64 ? 512 : 1280)) want = 1;
+    // Parts cost a second kernel, of the GPU's time and of the host's. In a graph, 8 KV heads of 250 entries take 5.9 us whole
+    // and 9.2 in parts, of 500 7.4 and 9.3, of 1000 10.0 and 9.1 (launched one by one 10.1 and 12.8); 64 of 375 to 750
+    // 10.4 and 11.6; 512 of 1000 47.6 and 55.8.
+    if (seen <= (base < 64 ? 1024 : 1280)) want = 1;
     const int64_t top = up_to(seen, FEW_STEP);
     p.few_splits = bounded(want, top < MAX_SPLITS ? top : MAX_SPLITS);
   }
