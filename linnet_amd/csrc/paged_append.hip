@@ -11,7 +11,8 @@
 // dimensions of a token (16 bytes; the other of a pair is its own or comes from the lane that holds it), of v a
 // lane holds two dimensions of all eight tokens, so that V's 16-byte pieces come out of registers by
 // v_perm. A whole unit is written in whole lines, a partial one (a single token of a decode step)
-// by its entries alone.
+// by its entries alone. 8191 tokens of 32 + 8 + 8 heads of 128 (202 MB): 41 us, 4.9 TB/s (58 with 16 lanes a token of K,
+// which writes half lines); one token 3.1 in a graph, a launch and four dependent loads.
 #include "paged.hpp"
 
 namespace lnq {
@@ -230,7 +231,8 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
 // sequence's new length base + their number. A wave takes one KV head of one layer of one sequence, eight
 // nodes at a time, all of them read before any is written; as path[j] >= j and ascends, none is written before
 // it has been read. Bound by lines: eight entries of a dimension share 16 bytes, so an entry's V is read
-// and written in all lines of its eight.
+// and written in all lines of its eight. 48 sequences' paths out of 2700 nodes, 32 layers of 8 KV heads of 128: 62 us (70 to 80
+// with a node at a time, its V sixteen dimensions a lane); one sequence's 4.0.
 struct KeepArgs {
   uint16_t *k_cache, *v_cache;
   const int32_t* kept;  // [sequences, path]
