@@ -677,3 +677,60 @@ def test_attention_in_parts_keeps_infinities_and_nan_to_the_rows_that_see_them(m
     compare(f"most={most}", got, want, torch.where(tol.isfinite(), tol, 0.0))
     rows = got.view(3, 8, 64)
     assert rows[:2, :, 40].isinf().all() and rows[:2, :, 50].isnan().all() and rows[0, :, [5, 9]].isfinite().all()
+
+
+def test_of_thousands_of_sequences() -> None:
+    """More than 64 times 64 sequences, many of them without new tokens: each workgroup finds its own."""
+    print("4200 sequences", flush=True)
+    counts = [(i * 7) % 3 if i % 50 else 0 for i in range(4200)]
+    counts[4100] = 45
+    lengths = [n + (i * 5) % 9 for i, n in enumerate(counts)]
+    _append(Batch(counts, lengths, 1, 64, 16, BF16, seed=44), 1, 8, False)
+    batch = Batch(counts, lengths, 1, 64, 16, BF16, seed=44).fill()
+    for most in (None, 2):
+        _attend(batch, 1, max_queries=most, extra=3)
+
+
+def test_captured_trees_follow_the_batch_on_the_device() -> None:
+    """Append, tree attention and keep in one graph, in two graphs whose replays take turns, against the eager calls'
+    bits while parents, paths and lengths change."""
+    print("captured trees", flush=True)
+    batch = Batch([9, 40, 0], [50, 300, 5], 2, 64, 16, BF16, seed=45, layers=2)
+    g = batch.g
+    batch.cache.k.copy_(torch.randn(batch.cache.k.shape, generator=g)), batch.cache.v.copy_(torch.randn(batch.cache.v.shape, generator=g))
+    cos, sin = torch.rand(400, 32, generator=g).to(DEV), torch.rand(400, 32, generator=g).to(DEV)
+    x = torch.randn(52, 12 * 64, generator=g).to(BF16).to(DEV)
+    positions, parents = torch.zeros(52, dtype=torch.int32, device=DEV), torch.zeros(52, dtype=torch.int32, device=DEV)
+    kept = torch.zeros(3, 6, dtype=torch.int32, device=DEV)
+    lengths, starts = batch.lengths.clone(), batch.starts.clone()
+
+    def step(cache):
+        q, k, v = x.split([8 * 64, 2 * 64, 2 * 64], 1)
+        pool = cache.layer(1)
+        q = paged.paged_append(q, k, v, cos, sin, pool, batch.tables, lengths, starts, positions=positions)
+        out = paged.paged_tree_attention(q, pool, batch.tables, lengths, starts, parents, max_queries=40)
+        return out, paged.paged_keep(cache, batch.tables, lengths, starts, kept)
+
+    copies = [paged.PagedCache(batch.cache.k.clone(), batch.cache.v.clone()) for _ in range(3)]
+    for cache in copies:
+        step(cache)
+    torch.cuda.synchronize()
+    graphs = []
+    for cache in copies[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(cache)
+        graphs.append((graph, outs))
+    for turn in range(4):
+        x.copy_(torch.randn(x.shape, generator=g))
+        positions.copy_(torch.randint(0, 400, (52,), generator=g))
+        parents.copy_(torch.tensor(_random_parents([9, 40, 3], g)))
+        kept.copy_(torch.tensor([[0, 2, 5, 8, -1, -1], [1, 2, 7 + turn, 20, 33, 39], [0, 1, 2, 3, 4, 5]]))
+        want = step(copies[2])
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, outs), cache in zip(graphs, copies):
+            assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+            assert torch.equal(cache.k, copies[2].k) and torch.equal(cache.v, copies[2].v)
+        lengths.copy_(torch.tensor([50 - turn, 299 - 13 * turn, 5]))
