@@ -20,8 +20,8 @@
 // workgroups too, and a last kernel adds the parts in order. Which sequence is which is on the device:
 // a call that may have both runs both in one launch.
 //
-// Measured: 64 sequences of 230000 entries together, 32 heads over 8 of 128 (942 MB), 181 us: 5.2 TB/s. One of 131000 entries
-// at head_dim 64, 8 KV heads, 57 to 60 us. Prompts of 8191 tokens (203 GFLOP) 220 us: 0.92 PFLOP/s, bound by the vector instructions of
+// Measured: 64 sequences of 230000 entries together, 32 heads over 8 of 128 (942 MB), 172 to 181 us: 5.2 to 5.5 TB/s. One of 131000 entries
+// at head_dim 64, 8 KV heads, 57 to 60 us. Prompts of 8191 tokens (203 GFLOP) 225 us: 0.90 PFLOP/s, bound by the vector instructions of
 // the softmax beside the MFMAs (a step of 64 entries takes a wave 32 MFMAs and 126 vector instructions, 32 of them
 // exponentials). 16 trees of 46 to 67 nodes over 70000 entries 130 us; one token over 1024 entries 9.4.
 #include <math.h>
@@ -772,17 +772,23 @@ __global__ __launch_bounds__(256, HD == 64 && !TREE ? 4 : 2) void paged_many_ker
     u32x4* const kt = cur;
     u32x4* const vt = cur + UNITS;
     // Where some row does not see all of the tile, V's entries that are not there become 0 (their
-    // weight is 0, but they may hold anything), and its infinities and NaNs are looked for.
+    // weight is 0, but they may hold anything), and its infinities and NaNs are looked for. (All there: looked for only.
+    // A window of 128 over 8191 tokens at head_dim 64, 56.5 us against 57.8.)
     uint32_t odd = 0;
     if (valid != ~0ull || t + 63 > all_last || t < all_low) {
       uint32_t found = 0;
+      if (valid == ~0ull) {
 #pragma unroll
-      for (int n = 0; n < UNITS / 256; ++n) {
-        const int u = n * 256 + tid;
-        const uint32_t there = static_cast<uint32_t>(valid >> (8 * (u / HD))) & 0xffu;
-        const u32x4 v = and_of(vt[u], masks_of(there));
-        found |= any_odd<DT>(v);
-        if (there != 0xffu) vt[u] = v;
+        for (int n = 0; n < UNITS / 256; ++n) found |= any_odd<DT>(vt[n * 256 + tid]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < UNITS / 256; ++n) {
+          const int u = n * 256 + tid;
+          const uint32_t there = static_cast<uint32_t>(valid >> (8 * (u / HD))) & 0xffu;
+          const u32x4 v = and_of(vt[u], masks_of(there));
+          found |= any_odd<DT>(v);
+          if (there != 0xffu) vt[u] = v;
+        }
       }
       const uint64_t lanes = __ballot(found != 0);
       if (lane == 0) odd_waves[wave] = lanes != 0 ? 1u : 0u;
