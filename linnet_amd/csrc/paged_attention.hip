@@ -21,8 +21,9 @@
 // a call that may have both runs both in one launch.
 //
 // Measured: 64 sequences of 230000 entries together, 32 heads over 8 of 128 (942 MB), 172 to 181 us: 5.2 to 5.5 TB/s. One of 131000 entries
-// at head_dim 64, 8 KV heads, 57 to 60 us. Prompts of 8191 tokens (203 GFLOP) 225 us: 0.90 PFLOP/s, bound by the vector instructions of
-// the softmax beside the MFMAs (a step of 64 entries takes a wave 32 MFMAs and 126 vector instructions, 32 of them
+// at head_dim 64, 8 KV heads, 57 to 60 us. Prompts of 8191 tokens (203 GFLOP) 225 us: 0.90 PFLOP/s, bound by the MFMAs (busy
+// 46% of the time), the softmax's vector instructions, of which they hide about half, and a clock that falls to 2.0
+// GHz under both (a step of 64 entries takes a wave 32 MFMAs and 126 vector instructions, 32 of them
 // exponentials). 16 trees of 46 to 67 nodes over 70000 entries 130 us; one token over 1024 entries 9.4.
 #include <math.h>
 
