@@ -52,8 +52,9 @@ __device__ inline int page_of(const Batch& b, int s, int e) {
 // Work is laid out in slots: a sequence of n tokens has at most n / per + more blocks (of `per`
 // aligned entries, or of rows), and slot_of(start, s) = start / per + more * s leaves that many
 // slots between a sequence's first token and the next one's, so that the grid's size needs the
-// number of tokens alone. The last sequence in [0, count) whose first slot is not past `slot`; the
-// whole wave takes part (64 sequences a look, or 64 samples of them first).
+// number of tokens alone. The last sequence in [0, count) whose first slot is not past `slot`, of one
+// sequence at least (nothing that looks for one is launched without any); the whole wave takes part (64
+// sequences a look, or 64 samples of them first).
 template <class SlotOf>
 __device__ inline int find_sequence(int count, int slot, SlotOf slot_of) {
   if (count <= 1) return 0;

@@ -1077,7 +1077,8 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
   const int64_t group = heads / kv_heads;
   most = most > tokens ? tokens : most;
   most = most < 1 ? 1 : most;
-  p.many = most * group > FEW;
+  // (Without sequences there are no rows but those of no sequence, which the few-row kernel clears.)
+  p.many = sequences > 0 && most * group > FEW;
   p.few = p.many ? 16 : FEW;
   p.few_tokens = p.few / group < 1 ? 1 : p.few / group;
   if (!p.many && most < p.few_tokens) p.few_tokens = most;
@@ -1105,7 +1106,7 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
     const int64_t top = up_to(seen, FEW_STEP);
     p.few_splits = bounded(want, top < MAX_SPLITS ? top : MAX_SPLITS);
   }
-  if (p.many && group > p.few) p.few_splits = 1;  // (no sequence has so few rows)
+  if (sequences == 0 || (p.many && group > p.few)) p.few_splits = 1;  // (no sequence has so few rows)
   p.many_splits = 1;
   if (p.many) {
     p.slots = tokens * group / MANY + sequences;

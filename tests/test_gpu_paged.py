@@ -734,3 +734,26 @@ def test_captured_trees_follow_the_batch_on_the_device() -> None:
             assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
             assert torch.equal(cache.k, copies[2].k) and torch.equal(cache.v, copies[2].v)
         lengths.copy_(torch.tensor([50 - turn, 299 - 13 * turn, 5]))
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize(("tokens", "heads", "kvh", "hd", "page", "width"),
+                         [(50, 4, 2, 64, 16, 8), (64, 4, 2, 64, 16, 0), (300, 4, 2, 128, 64, 2048), (1000, 40, 1, 64, 128, 3), (1, 1, 1, 128, 16, 5)])
+def test_attention_of_no_sequences(tokens, heads, kvh, hd, page, width, tree) -> None:
+    """Tokens of which none has a sequence give zeros, or with `out` leave its rows, whatever the tables could hold."""
+    print("no sequences", tokens, heads, kvh, hd, page, width, tree, flush=True)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    cache = paged.PagedCache.empty(4, kvh, hd, page)
+    tables, lengths, starts = torch.zeros(0, width, **i32), torch.zeros(0, **i32), torch.zeros(1, **i32)
+    parents = torch.full((tokens,), -1, **i32)
+    q = torch.randn(tokens, heads * hd, device=DEV).to(BF16)
+    for most in (None, 1, 33, 200):
+        for window in (0, 20):
+            for out in (None, torch.full_like(q, 3.0)):
+                kinds = dict(max_queries=most, window=window, out=out)
+                if tree:
+                    got = paged.paged_tree_attention(q, cache, tables, lengths, starts, parents, **kinds)
+                else:
+                    got = paged.paged_attention(q, cache, tables, lengths, starts, **kinds)
+                torch.cuda.synchronize()
+                assert torch.equal(got, torch.zeros_like(q) if out is None else torch.full_like(q, 3.0))

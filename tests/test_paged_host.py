@@ -113,6 +113,17 @@ def test_workspace_stays_small() -> None:
     assert _floats(1, 2048, 64, 1, 32, 8, 128, 1, 128) <= 4 * 32 * 130
 
 
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize(("heads", "kv_heads"), [(1, 1), (4, 2), (40, 1), (32, 8), (64, 64)])
+def test_no_sequences_have_no_parts(heads: int, kv_heads: int, head_dim: int) -> None:
+    """Tokens of no sequence are only cleared: whatever the tables could hold, no kernel looks for a sequence of theirs."""
+    for width, page in ((0, 16), (3, 16), (8, 16), (2048, 64), (1 << 23, 128)):
+        for tokens in (1, 16, 50, 64, 300, 8191):
+            for most in (0, 1, 2, 33, tokens, 1 << 20):
+                for window in (0, 1, 128):
+                    assert _floats(0, width, page, tokens, heads, kv_heads, head_dim, most, window) == 0, (width, page, tokens, most, window)
+
+
 CPU = dict(dtype=torch.bfloat16, device="cpu")
 
 
