@@ -465,8 +465,8 @@ __device__ inline void few_rows(const AttendArgs& a, int block, FewLds<HD, TILE>
     const int begin = range.lo + split * range.chunk, end = min(range.hi, begin + range.chunk);
     const int r = min(r0 + col, rows - 1), i = r / a.group, head = h * a.group + r % a.group;
     const Row row = row_of<TREE>(a, q, i, tree.paths, tree.depth);
-    // All rows see entries sure_low .. sure_last.
-    const int sure_last = TREE ? q.base - 1 : q.base + i0;
+    // All rows see entries sure_low .. sure_last (of a tree none where a node past the last one is among them).
+    const int sure_last = TREE ? (i1 < NODES ? q.base - 1 : -1) : q.base + i0;
     const int sure_low = a.window > 0 ? q.base + (TREE ? q.n - 1 : i1) - a.window + 1 : 0;
 
     // A step: 32 entries from t, in one page or two. Its keys' registers take the next step's keys as
@@ -690,14 +690,15 @@ __global__ __launch_bounds__(256, HD == 64 && !TREE ? 4 : 2) void paged_many_ker
   const int mask = (1 << b.page_bits) - 1;
   const float slack = 8.f / a.scale2;
 
-  // This wave's rows, and what all of them and what any of them see (of the workgroup's rows, too).
+  // This wave's rows, and what all of them and what any of them see (of the workgroup's rows, too); nodes of a tree
+  // past the last one see nothing.
   const int w0 = r0 + 32 * wave;
   const bool busy = w0 < rows;
   const int r = min(w0 + col, rows - 1), i = r / a.group, head = h * a.group + r % a.group;
   const int wa = min(w0, rows - 1) / a.group, wz = min(w0 + 31, rows - 1) / a.group;
-  const int sure_last = TREE ? q.base - 1 : q.base + wa, sure_low = a.window > 0 ? q.base + (TREE ? q.n - 1 : wz) - a.window + 1 : 0;
+  const int sure_last = TREE ? (wz < NODES ? q.base - 1 : -1) : q.base + wa, sure_low = a.window > 0 ? q.base + (TREE ? q.n - 1 : wz) - a.window + 1 : 0;
   const int any_last = TREE ? q.length - 1 : q.base + wz, any_low = a.window > 0 ? q.base + (TREE ? 0 : wa) - a.window + 1 : 0;
-  const int all_last = TREE ? q.base - 1 : q.base + i0, all_low = a.window > 0 ? q.base + (TREE ? q.n - 1 : i1) - a.window + 1 : 0;
+  const int all_last = TREE ? (i1 < NODES ? q.base - 1 : -1) : q.base + i0, all_low = a.window > 0 ? q.base + (TREE ? q.n - 1 : i1) - a.window + 1 : 0;
 
   R st;
   st.clear();

@@ -757,3 +757,18 @@ def test_attention_of_no_sequences(tokens, heads, kvh, hd, page, width, tree) ->
                     got = paged.paged_attention(q, cache, tables, lengths, starts, **kinds)
                 torch.cuda.synchronize()
                 assert torch.equal(got, torch.zeros_like(q) if out is None else torch.full_like(q, 3.0))
+
+
+@pytest.mark.parametrize("width", [None, 256])
+@pytest.mark.parametrize(("counts", "lengths", "heads", "kvh", "hd", "window", "sinks"),
+                         [([300], [500], 4, 2, 64, 0, False), ([290, 3, 257], [420, 40, 600], 2, 2, 128, 0, True),
+                          ([300], [2000], 3, 1, 64, 1500, False), ([700, 1], [900, 300], 1, 1, 64, 0, True)])
+def test_tree_nodes_past_the_256th_after_a_context(counts, lengths, heads, kvh, hd, window, sinks, width) -> None:
+    """They see nothing, the entries before the draft neither; the nodes before them what they saw."""
+    print("long drafts", counts, lengths, heads, kvh, hd, window, sinks, width, flush=True)
+    batch = Batch(counts, lengths, kvh, hd, 16, BF16, seed=34, width=width).fill()
+    parents = _random_parents(counts, batch.g)
+    for most in (None, 1):
+        got = _attend(batch, heads, window, sinks, max_queries=most, parents=parents)
+        for first, n in zip(batch.starts_list, counts):
+            assert got[first : first + min(n, 256)].any(-1).all() and not got[first + min(n, 256) : first + n].any()
