@@ -964,9 +964,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a, int64_t s
 #pragma unroll
       for (int e = 0; e < AHEAD; ++e) {
         const int lane_of = PARTS * r + min(c0 + e, PARTS - 1);
-        const float by = c0 + e < most ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), lane_of)) : 0.f;
+        const float by = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), lane_of));
+        // (A part whose weight is 0 is added too: a row that sees an infinity or a NaN in it is no number.)
+        const bool there = c0 + e < __builtin_amdgcn_readlane(used, PARTS * r);
 #pragma unroll
-        for (int d = 0; d < D; ++d) o[r][d] += by == 0.f ? 0.f : by * x[r][e][d];
+        for (int d = 0; d < D; ++d) o[r][d] += there ? by * x[r][e][d] : 0.f;
       }
   }
 #pragma unroll
@@ -1038,9 +1040,9 @@ __global__ __launch_bounds__(256) void paged_join_wide_kernel(AttendArgs a, int6
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) {
       const int c = c0 + 4 * n;
-      const float w = c < used ? weights[c] : 0.f;
+      const float w = weights[min(c, used - 1)];
 #pragma unroll
-      for (int d = 0; d < D; ++d) o[d] += w == 0.f ? 0.f : w * x[n][d];
+      for (int d = 0; d < D; ++d) o[d] += c < used ? w * x[n][d] : 0.f;  // (parts of weight 0 too, as above)
     }
   }
   if (wave > 0) {

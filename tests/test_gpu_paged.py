@@ -772,3 +772,28 @@ def test_tree_nodes_past_the_256th_after_a_context(counts, lengths, heads, kvh, 
         got = _attend(batch, heads, window, sinks, max_queries=most, parents=parents)
         for first, n in zip(batch.starts_list, counts):
             assert got[first : first + min(n, 256)].any(-1).all() and not got[first + min(n, 256) : first + n].any()
+
+
+@pytest.mark.parametrize(("new", "heads", "width"), [(1, 4, 256), (1, 4, 4096), (1, 300, 256), (1, 520, 2048), (1, 5000, 256), (40, 4, 256)])
+def test_odd_values_of_parts_without_weight_reach_their_rows(new, heads, width) -> None:
+    """Infinities and NaNs in parts whose weights are 0 beside another part's: no dimension that has one is a number
+    in the rows that see them, and the others are as without them."""
+    print("odd values in parts without weight", new, heads, width, flush=True)
+    batch = Batch([new, 1], [4000, 1300], 1, 64, 16, BF16, seed=46, width=width)
+    for s, n in ((0, new), (1, 1)):  # scores 300 of the sequence's first new entry, 0 of all before it
+        batch.keys[s].zero_()
+        batch.keys[s][-n, 0, 0] = 20
+    inf, nan = float("inf"), float("nan")
+    for e, d, what in ((10, 5, nan), (700, 6, inf), (1500, 7, -inf)):
+        batch.values[0][e, 0, d] = what
+    batch.fill()
+    q = torch.zeros(new + 1, heads, 64, dtype=BF16, device=DEV)
+    q[:, :, 0] = 15
+    got = paged.paged_attention(q.view(new + 1, -1), batch.cache, batch.tables, batch.lengths, batch.starts, scale=1.0)
+    got = got.view(new + 1, heads, 64).cpu()
+    odd = [5, 6, 7]
+    assert not got[:new, :, odd].isfinite().any()
+    rest = [d for d in range(64) if d not in odd]
+    # The one entry has all of the weight (the others' sum is below 4000 e^-300): its value, exactly, to the first new token.
+    assert torch.equal(got[0][:, rest], batch.values[0][-new, 0, rest].expand(heads, -1))
+    assert got[:, :, rest].isfinite().all() and torch.equal(got[new], batch.values[1][-1, 0].expand(heads, -1))
