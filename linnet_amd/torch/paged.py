@@ -14,7 +14,8 @@ neither read nor written.
 
 The reference keeps one contiguous cache of one length in its generated module
 (`python/linnet/src/linnet/torch/compiled.py:430-503`). Every call enqueues on the current stream and
-returns; the kernels record no gradient, and inputs that require one are refused.
+returns; the kernels record no gradient, and inputs that require one or have a tangent of forward mode
+are refused.
 """
 
 from __future__ import annotations
@@ -24,6 +25,7 @@ import dataclasses
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from ..errors import LinnetError
@@ -96,6 +98,12 @@ def _launch(index: int, name: str, *args: object) -> None:
 
 def _records(what: str) -> None:
     raise LinnetError(f"{what}: records no gradient, and an input requires one")
+
+
+def _tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Refuses duals, whose tangents the kernels would drop (asked only inside a level of forward mode)."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise LinnetError(f"{what}: records no gradient in forward mode, and an input has a tangent")
 
 
 def _ints(what: str, name: str, t: torch.Tensor, count: int) -> torch.Tensor:
@@ -172,6 +180,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
                                     or v_cache.requires_grad or any(t is not None and t.requires_grad
                                                                     for t in (cos, sin, q_norm, k_norm, out))):
         _records("paged_append")
+    if forward_ad._current_level >= 0:
+        _tangents("paged_append", q, k, v, k_cache, v_cache, cos, sin, q_norm, k_norm, out)
     dtype = k_cache.dtype
     tables, lengths, starts, sequences, width = _batch("paged_append", tables, lengths, starts)
     q, q_stride, tokens, columns = _rows("paged_append", "q", q, dtype)
@@ -234,6 +244,8 @@ def _attend(what: str, q: torch.Tensor, cache: PagedCache, tables: torch.Tensor,
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or cache.v.requires_grad or any(
             t is not None and t.requires_grad for t in (sinks, out))):
         _records(what)
+    if forward_ad._current_level >= 0:
+        _tangents(what, q, k_cache, cache.v, sinks, out)
     dtype = k_cache.dtype
     tables, lengths, starts, sequences, width = _batch(what, tables, lengths, starts)
     q, q_stride, tokens, columns = _rows(what, "q", q, dtype)
@@ -313,6 +325,8 @@ def paged_keep(cache: PagedCache, tables: torch.Tensor, lengths: torch.Tensor, s
     _on_gpu("paged_keep", cache.k, tables, lengths, starts, kept)
     if torch.is_grad_enabled() and (cache.k.requires_grad or cache.v.requires_grad):
         _records("paged_keep")
+    if forward_ad._current_level >= 0:
+        _tangents("paged_keep", cache.k, cache.v)
     tables, lengths, starts, sequences, width = _batch("paged_keep", tables, lengths, starts)
     if kept.dim() != 2:
         raise LinnetError(f"paged_keep: kept is [sequences, path] int32, got {list(kept.shape)}")

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from linnet_amd import LinnetError
 from linnet_amd.torch import paged
@@ -797,3 +798,41 @@ def test_odd_values_of_parts_without_weight_reach_their_rows(new, heads, width) 
     # The one entry has all of the weight (the others' sum is below 4000 e^-300): its value, exactly, to the first new token.
     assert torch.equal(got[0][:, rest], batch.values[0][-new, 0, rest].expand(heads, -1))
     assert got[:, :, rest].isfinite().all() and torch.equal(got[new], batch.values[1][-1, 0].expand(heads, -1))
+
+
+def test_duals_of_forward_mode_are_refused() -> None:
+    """No tangent is dropped; inside a level of forward mode, calls without one are as outside of it."""
+    print("duals", flush=True)
+    batch = Batch([2], [5], 2, 64, 16, BF16, seed=66).fill()
+    cache, batch_of = batch.cache, (batch.tables, batch.lengths, batch.starts)
+    q, kv = torch.randn(2, 256, generator=batch.g).to(BF16).to(DEV), torch.randn(2, 128, generator=batch.g).to(BF16).to(DEV)
+    cos, norm, sinks = torch.rand(9, 32, device=DEV), torch.ones(64, device=DEV), torch.zeros(4, device=DEV)
+    parents, kept = torch.tensor([-1, 0], dtype=torch.int32, device=DEV), torch.tensor([[0, 1]], dtype=torch.int32, device=DEV)
+    append = dict(q=q, k=kv, v=kv, cos=cos, sin=cos, q_norm=norm, k_norm=norm)
+
+    def calls():
+        return (paged.paged_append(cache=cache, tables=batch_of[0], lengths=batch_of[1], starts=batch_of[2], **append),
+                paged.paged_attention(q, cache, *batch_of, sinks=sinks), paged.paged_tree_attention(q, cache, *batch_of, parents),
+                paged.paged_keep(cache, *batch_of, kept))
+
+    def refused(call, *args, **kinds):
+        with torch.no_grad(), pytest.raises(LinnetError, match="tangent"):
+            call(*args, **kinds)
+
+    want = calls()
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        assert all(torch.equal(a, b) for a, b in zip(calls(), want))
+        for name in append:
+            refused(paged.paged_append, cache=cache, tables=batch_of[0], lengths=batch_of[1], starts=batch_of[2],
+                    **(append | {name: dual(append[name])}))
+        refused(paged.paged_append, cache=cache, tables=batch_of[0], lengths=batch_of[1], starts=batch_of[2], out=dual(q.clone()), **append)
+        for call, more in ((paged.paged_attention, ()), (paged.paged_tree_attention, (parents,))):
+            refused(call, dual(q), cache, *batch_of, *more)
+            refused(call, q, cache, *batch_of, *more, sinks=dual(sinks))
+            refused(call, q, cache, *batch_of, *more, out=dual(q.clone()))
+        for pool in (paged.PagedCache(dual(cache.k), cache.v), paged.PagedCache(cache.k, dual(cache.v))):
+            refused(paged.paged_append, cache=pool, tables=batch_of[0], lengths=batch_of[1], starts=batch_of[2], **append)
+            refused(paged.paged_attention, q, pool, *batch_of)
+            refused(paged.paged_keep, pool, *batch_of, kept)
+    refused(torch.func.jvp, lambda x: paged.paged_attention(x, cache, *batch_of), (q,), (q,))
