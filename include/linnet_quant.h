@@ -783,7 +783,8 @@ LNQ_API LnqStatus lnq_paged_attention(const void* q, int64_t q_stride, const voi
                                       int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_queries,
                                       int64_t window, float scale, int32_t dtype, void* stream);
 
-/* Floats of lnq_paged_attention's workspace. */
+/* Floats of lnq_paged_attention's workspace: of a call whose entries may be split, parts of every sequence by what its
+ * table could hold (width * page entries or the window), whatever its length; at most 2^28. */
 LNQ_API LnqStatus lnq_paged_attention_workspace(int64_t sequences, int64_t width, int64_t page, int64_t tokens, int64_t heads,
                                                 int64_t kv_heads, int64_t head_dim, int64_t max_queries, int64_t window,
                                                 int64_t* floats);

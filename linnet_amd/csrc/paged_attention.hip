@@ -40,6 +40,10 @@ constexpr int FEW_STEP = 128;    // entries a workgroup of the few-row kernel ta
 constexpr int MANY_STEP = 64;
 constexpr int NODES = 256;       // of a drafted tree
 constexpr int MAX_SPLITS = 256;
+// Of a workspace, 1 GiB. Parts are as many as the tables could fill, for every sequence: without a bound, 512 sequences with
+// a chunk among them under tables of 131072 entries (32 heads of 128, parts of four tokens each) take 4.4 GB and at
+// 1800 to 5400 entries 2584 us, with it 1809 (2669 and 1904 where one sequence has 131000); the largest batches 140 GB.
+constexpr int64_t MOST_FLOATS = int64_t{1} << 28;
 
 // f16 weights are kept times 2^7: with the maximum's slack of 2^8 they stay below 2^15 (f16 ends at 2^16), and what
 // rounds to 0 is below 2^-32 of the largest, not 2^-25, of which the tail of a long cache can hold a sizable sum.
@@ -1119,10 +1123,13 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
     const int64_t top = up_to(seen_by(most), MANY_STEP);
     p.many_splits = bounded(up_to(1024, base > 0 ? base : 1), top < 64 ? top : 64);
   }
-  p.few_rows = p.few_splits > 1 ? sequences * p.few_tokens * heads : 0;
   p.many_rows = p.many_splits > 1 ? tokens * heads : 0;
+  const int64_t many_floats = p.many_rows * p.many_splits * (head_dim + 2);  // (below 2^26: rows that are few for the chip)
+  const int64_t one_part = sequences * p.few_tokens * heads * (head_dim + 2);
+  if (p.few_splits * one_part > MOST_FLOATS - 4 - many_floats) p.few_splits = bounded((MOST_FLOATS - 4 - many_floats) / one_part, MAX_SPLITS);
+  p.few_rows = p.few_splits > 1 ? sequences * p.few_tokens * heads : 0;
   p.few_floats = (p.few_rows * p.few_splits * (head_dim + 2) + 3) / 4 * 4;
-  p.floats = p.few_floats + p.many_rows * p.many_splits * (head_dim + 2);
+  p.floats = p.few_floats + many_floats;
   return p;
 }
 

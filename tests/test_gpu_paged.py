@@ -836,3 +836,15 @@ def test_duals_of_forward_mode_are_refused() -> None:
             refused(paged.paged_attention, q, pool, *batch_of)
             refused(paged.paged_keep, pool, *batch_of, kept)
     refused(torch.func.jvp, lambda x: paged.paged_attention(x, cache, *batch_of), (q,), (q,))
+
+
+def test_attention_of_a_workspace_at_its_bound() -> None:
+    """A mixed batch whose tables could hold more parts than the workspace has room for."""
+    print("workspace at its bound", flush=True)
+    counts, lengths = [1] * 128, [1 + (37 * i) % 200 for i in range(128)]
+    counts[40], counts[70], counts[71] = 20, 3, 16
+    for s, n in ((40, 300), (70, 1900), (71, 700), (90, 2600)):
+        lengths[s] = n
+    batch = Batch(counts, lengths, 16, 64, 128, BF16, seed=47, width=1024).fill()
+    assert paged._workspace(128, 1024, 128, batch.tokens, 16, 16, 64, batch.tokens, 0) == 124 * 128 * 16 * 16 * 66  # 128 parts: 2^28 and more
+    _attend(batch, 16, sinks=True)

@@ -4,6 +4,7 @@ refuse, and the workspace's size."""
 from __future__ import annotations
 
 import ctypes
+import itertools
 
 import pytest
 import torch
@@ -122,6 +123,23 @@ def test_no_sequences_have_no_parts(heads: int, kv_heads: int, head_dim: int) ->
             for most in (0, 1, 2, 33, tokens, 1 << 20):
                 for window in (0, 1, 128):
                     assert _floats(0, width, page, tokens, heads, kv_heads, head_dim, most, window) == 0, (width, page, tokens, most, window)
+
+
+def test_workspace_has_a_bound() -> None:
+    """No batch that is taken needs more than 1 GiB, however wide its tables."""
+    floats, taken = ctypes.c_int64(-1), 0
+    call = _lib.load().lnq_paged_attention_workspace
+    for head_dim, page, width in itertools.product((64, 128), (16, 128), (1, 10, 64, 1024, 8192, 1 << 23)):
+        for sequences in [3, 700] + [1 << i for i in range(21)]:
+            for kv_heads, group in itertools.product((1, 2, 8, 64, 4096), (1, 2, 4, 8, 16, 17, 32, 40)):
+                for most, window in ((1, 0), (2, 0), (16, 0), (33, 0), (2000, 0), (2000, 5000)):
+                    sizes = (sequences, width, page, sequences + most, kv_heads * group, kv_heads, head_dim, most, window)
+                    if call(*sizes, ctypes.byref(floats)) == _lib.LNQ_OK:
+                        taken += 1
+                        assert 0 <= floats.value <= 1 << 28, sizes
+    assert taken > 10000
+    # What lies within the bound is divided as it would be without one.
+    assert _floats(256, 2048, 64, 256, 32, 8, 128, 1) == 128 * 256 * 32 * 130
 
 
 CPU = dict(dtype=torch.bfloat16, device="cpu")
