@@ -775,7 +775,8 @@ LNQ_API LnqStatus lnq_paged_append(const void* q, int64_t q_stride, const void* 
  * nothing, give zeros. max_queries: the most new tokens of a sequence, as far as known (`tokens` always
  * will do); it decides the kernels, not the result's meaning. workspace: 16-byte aligned,
  * lnq_paged_attention_workspace floats; calls that overlap on one race. scale in [1e-9, 1e9]. Infinities and
- * NaNs of a value reach the rows that see its entry and no other. out shares no memory with the inputs. */
+ * NaNs of a value reach the rows that see its entry and no other (an infinity as it is, or as NaN where its weight beside
+ * the row's others is 0). out shares no memory with the inputs. */
 LNQ_API LnqStatus lnq_paged_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, void* out,
                                       int64_t out_stride, int32_t fill, const int32_t* tables, const int32_t* lengths,
                                       const int32_t* starts, const int32_t* parents, const float* sinks, float* workspace,

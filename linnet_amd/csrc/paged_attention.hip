@@ -1103,6 +1103,8 @@ static Plan plan_of(int64_t sequences, int64_t width, int64_t page, int64_t toke
     // As many workgroups as the chip holds at once (3 a CU at head_dim 64, 2 at 128), and none of much over 1024
     // entries where lengths differ. One row of 131000 entries at head_dim 64: 57.0 us with 768 workgroups, 59.9 with
     // 512 or 1024, 62.3 with 2048; 64 rows of 230000 at 128: 180.6 with parts of 1024, 183.4 of 2048, 184.5 of 512.
+    // (By what the tables can hold. Under tables much wider than the lengths parts are shorter, at least FEW_STEP: 64 sequences of
+    // 1800 to 5400 entries under 131072 each 291 to 303 us, under 5440 each 172.)
     const int64_t base = sequences * kv_heads, seen = seen_by(p.few_tokens);
     int64_t want = up_to(head_dim == 64 ? 768 : 512, base > 0 ? base : 1);
     if (want < up_to(seen, 1024)) want = up_to(seen, 1024);

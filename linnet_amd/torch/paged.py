@@ -295,7 +295,12 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, tables: torch.Tensor, le
     `max_queries`, the most new tokens of a sequence, where the caller knows it, spares the kernels for longer
     ones: 1 for a decode step. Sequences with more are computed all the same. A row that sees no entry, or
     only ones whose score is -inf, gives zeros; infinities and NaNs of a value reach the rows that see its entry
-    and no other; tokens of no sequence give zeros, or with `out` leave its rows as they were."""
+    and no other (an infinity as it is, or as NaN where its weight beside the row's others is 0); tokens of no
+    sequence give zeros, or with `out` leave its rows as they were.
+
+    Long contexts of few rows are split over the chip by what the tables can hold. Tables much wider than the
+    sequences (131072 entries for some thousands) make a decode step slower and its workspace larger, up to 1 GiB:
+    pass the columns that are in use (`tables[:, :n]`, contiguous; in a captured step one of a few widths)."""
     return _attend("paged_attention", q, cache, tables, lengths, starts, None, max_queries, scale, window, sinks, out)
 
 
